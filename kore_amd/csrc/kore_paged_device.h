@@ -1,0 +1,63 @@
+// kore_paged_device.h - device helpers shared by the rotary, append and
+// paged-attention kernels.  Internal to libkore_paged.so.
+#pragma once
+
+#include "kore_paged_kernels.h"
+
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+
+namespace kore_paged_gpu {
+namespace {
+
+typedef _Float16 half_t;
+typedef __bf16 bhalf_t;
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(half_t x) { return (float)x; }
+__device__ __forceinline__ float to_f32(bhalf_t x) { return (float)x; }
+
+// N elements from an address that is aligned to N elements (VEC), or to one.
+template <int N, class T>
+__device__ __forceinline__ void load_n(const T *p, T (&x)[N], bool vec) {
+    typedef T vec_t __attribute__((ext_vector_type(N)));
+    if (vec) {
+        const vec_t v = *reinterpret_cast<const vec_t *>(p);
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = v[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = p[i];
+    }
+}
+template <int N, class T>
+__device__ __forceinline__ void store_n(T *p, const T (&x)[N], bool vec) {
+    typedef T vec_t __attribute__((ext_vector_type(N)));
+    if (vec) {
+        vec_t v;
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = x[i];
+        *reinterpret_cast<vec_t *>(p) = v;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) p[i] = x[i];
+    }
+}
+
+// Number of sequences that end at or before row (q_start ascending), counted by
+// a whole wave, 64 table entries at a time: the row's sequence, or n_seq where
+// the row lies behind the last one.  The loads of one wave do not depend on each
+// other, as those of a binary search would.
+__device__ __forceinline__ int seq_of_row(const Batch &b, int row) {
+    const int lane = threadIdx.x & 63;
+    int n = 0;
+    for (int s0 = 0; s0 < b.n_seq; s0 += 64) {
+        const int s = s0 + lane;
+        const bool before = s < b.n_seq && b.q_start[s + 1] <= row;
+        n += __popcll(__ballot(before));
+    }
+    return n;
+}
+
+}  // namespace
+}  // namespace kore_paged_gpu
