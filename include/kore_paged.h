@@ -72,7 +72,7 @@ typedef struct kore_paged_batch {
     const int *q_start;          /* device [n_seq + 1] */
     const int *kv_len;           /* device [n_seq] */
     const int *pages;            /* device [n_seq][pages_stride] */
-    int pages_stride;            /* entries of a sequence's row of the table */
+    int pages_stride;            /* entries of a sequence's row of the table; 2^30 positions at most */
     int max_q;                   /* the most new rows that a sequence has, or 0 (unknown): picks the kernel, any
                                     value gives the same result but for rounding */
 } kore_paged_batch;

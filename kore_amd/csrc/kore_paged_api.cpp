@@ -228,8 +228,8 @@ int check_batch(kore_paged *h, int layer, const kore_paged_batch *b, int type) {
         return fail(h, KORE_PAGED_E_INVALID, "negative n_seq, n_tok or max_q");
     if (b->n_seq == 0 || b->n_tok == 0) return KORE_PAGED_OK;
     if (!b->q_start || !b->kv_len || !b->pages) return fail(h, KORE_PAGED_E_INVALID, "null q_start, kv_len or pages");
-    if (b->pages_stride <= 0 || b->pages_stride > INT_MAX / h->cfg.page_size)
-        return fail(h, KORE_PAGED_E_INVALID, "pages_stride %d outside 1..%d", b->pages_stride, INT_MAX / h->cfg.page_size);
+    if (b->pages_stride <= 0 || b->pages_stride > kMaxKeys / h->cfg.page_size)
+        return fail(h, KORE_PAGED_E_INVALID, "pages_stride %d outside 1..%d", b->pages_stride, kMaxKeys / h->cfg.page_size);
     if ((int64_t)b->n_tok * h->cfg.n_head > (1 << 28) || b->n_seq > 1 << 20)
         return fail(h, KORE_PAGED_E_UNSUPPORTED, "n_tok %d x %d heads or n_seq %d is too large", b->n_tok, h->cfg.n_head,
                     b->n_seq);

@@ -1,0 +1,296 @@
+// kore_paged_attend.h - what the paged-attention kernels share: how the work of
+// a batch is cut into workgroups, the 16-bit parts of fp32 values, the online
+// softmax.  Internal to libkore_paged.so.
+//
+// The work.  The new rows of a sequence and the n_head / n_head_kv = rep q-heads
+// of a kv-head are one list, row r being token r / rep and head r % rep, cut into
+// tiles of a kernel's TILE rows: every q-head of a tile reads the same K and V.
+// A tile's keys are cut into splits of len keys, the same len for the whole
+// batch, and a workgroup takes one (sequence, tile, split, kv-head).  What a
+// sequence has is read from device memory, so every workgroup finds its place
+// itself: its waves scan the sequences 64 at a time.
+#pragma once
+
+#include "kore_paged_device.h"
+
+namespace kore_paged_gpu {
+
+// How a launch cuts its work; every field is the host's.
+struct Cut {
+    int rep;         // q-heads of a kv-head
+    int target;      // workgroups to aim at, in tiles x keys; 0: nothing is split
+    int min_len;     // a split's fewest keys
+};
+
+namespace {
+
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef half_t half4 __attribute__((ext_vector_type(4)));
+typedef half_t half8 __attribute__((ext_vector_type(8)));
+typedef bhalf_t bhalf4 __attribute__((ext_vector_type(4)));
+typedef bhalf_t bhalf8 __attribute__((ext_vector_type(8)));
+typedef short short4_t __attribute__((ext_vector_type(4)));
+typedef short short8_t __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) short4_t lds_short4;
+
+constexpr float kNone = -INFINITY;
+
+// Lane l's and lane l ^ 16's, or l ^ 32's, value.  (The results are copied to
+// integers before the bit casts: this hipcc compiles a bit cast of an element of
+// the returned vector as its first element for either index.)
+__device__ __forceinline__ float max16(float x) {
+    const unsigned b = __builtin_bit_cast(unsigned, x);
+    const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+    const unsigned r0 = r[0], r1 = r[1];
+    return fmaxf(__builtin_bit_cast(float, r0), __builtin_bit_cast(float, r1));
+}
+__device__ __forceinline__ float max32(float x) {
+    const unsigned b = __builtin_bit_cast(unsigned, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    const unsigned r0 = r[0], r1 = r[1];
+    return fmaxf(__builtin_bit_cast(float, r0), __builtin_bit_cast(float, r1));
+}
+__device__ __forceinline__ float sum16(float x) {
+    const unsigned b = __builtin_bit_cast(unsigned, x);
+    const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+    const unsigned r0 = r[0], r1 = r[1];
+    return __builtin_bit_cast(float, r0) + __builtin_bit_cast(float, r1);
+}
+__device__ __forceinline__ float sum32(float x) {
+    const unsigned b = __builtin_bit_cast(unsigned, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    const unsigned r0 = r[0], r1 = r[1];
+    return __builtin_bit_cast(float, r0) + __builtin_bit_cast(float, r1);
+}
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// ---- the cut -----------------------------------------------------------------
+
+// A sequence's share of the cut.
+struct Share {
+    int tiles;      // of its rows, each for every kv-head
+    int keys;       // that a tile can span
+};
+
+template <int TILE>
+__device__ __forceinline__ Share share_of(const Batch &b, int s, int rep, int cap, int window, int &q0, int &n, int &kv) {
+    q0 = min(max(b.q_start[s], 0), b.n_tok);
+    n = min(max(b.q_start[s + 1], q0), b.n_tok) - q0;
+    kv = max(b.kv_len[s], 0);
+    Share r;
+    r.tiles = (n * rep + TILE - 1) / TILE;
+    // the rows of a tile span (TILE - 1) / rep + 2 tokens at most, and its first key is rounded down by up to 63
+    const int held = max(0, min(kv, cap)), wide = (TILE - 1) / rep + 65;
+    r.keys = window < held - wide ? window + wide : held;
+    return r;
+}
+
+// A workgroup's place, equal in every lane.
+struct Place {
+    int seq, tile, split, n_split, head;
+    int q0, n, kv;      // of the sequence: first row, rows, positions
+    int len;            // keys of a split
+    int first;          // number of the tile's first split among the launch's places
+};
+
+__device__ __forceinline__ int prefix_sum(int x) {   // inclusive, over the wave
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int y = __shfl_up(x, d);
+        if (lane >= d) x += y;
+    }
+    return x;
+}
+
+// The place of number `id`, false where there is none.  Numbers run over the
+// sequences, then a sequence's tiles from the last (which has the most keys),
+// then its splits, then the kv-heads.  by_tile: one number for all splits of a
+// tile (the merge).
+template <int TILE>
+__device__ __forceinline__ bool place_of(const Batch &b, const Cut &c, int id, int nkv, int cap, int window, bool by_tile,
+                                         Place &p) {
+    const int lane = threadIdx.x & 63;
+    int len = INT_MAX;
+    if (c.target) {
+        // so that all splits are at most target (of len keys) and one more for each tile
+        float w = 0;
+        for (int s0 = 0; s0 < b.n_seq; s0 += 64) {
+            const int s = s0 + lane;
+            int q0, n, kv;
+            const Share r = s < b.n_seq ? share_of<TILE>(b, s, c.rep, cap, window, q0, n, kv) : Share{0, 0};
+            w += (float)r.tiles * (float)r.keys;
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) w += __shfl_xor(w, d);
+        const float each = ceilf(w * (float)nkv / (float)c.target);
+        len = max(c.min_len, ((int)fminf(each, 1e9f) + 63) & ~63);
+    }
+    int at = 0, splits_at = 0;
+    for (int s0 = 0; s0 < b.n_seq; s0 += 64) {
+        const int s = s0 + lane;
+        int q0 = 0, n = 0, kv = 0;
+        const Share r = s < b.n_seq ? share_of<TILE>(b, s, c.rep, cap, window, q0, n, kv) : Share{0, 0};
+        const int n_split = max(1, r.keys / len + (r.keys % len != 0));
+        const int all = r.tiles * n_split * nkv, mine = by_tile ? r.tiles * nkv : all;
+        const int upto = prefix_sum(mine), splits_upto = by_tile ? prefix_sum(all) : upto;
+        const unsigned long long past = __ballot(at + upto > id);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            const auto of = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
+            p.seq = s0 + l;
+            p.n_split = of(n_split);
+            p.q0 = of(q0);
+            p.n = of(n);
+            p.kv = of(kv);
+            p.len = len;
+            int i = id - at - of(upto) + of(mine);
+            p.head = i % nkv;
+            i /= nkv;
+            p.split = by_tile ? 0 : i % p.n_split;
+            if (!by_tile) i /= p.n_split;
+            p.tile = of(r.tiles) - 1 - i;
+            p.first = splits_at + of(splits_upto) - of(all) + i * p.n_split * nkv + p.head;
+            return true;
+        }
+        at += __builtin_amdgcn_readlane(upto, 63);
+        splits_at += __builtin_amdgcn_readlane(splits_upto, 63);
+    }
+    return false;
+}
+
+// The keys of a place: [lo, hi) of its split; all rows of the tile see those in
+// [all_lo, all_hi).
+struct Keys {
+    int lo, hi, all_lo, all_hi;
+};
+
+template <int TILE>
+__device__ __forceinline__ Keys keys_of(const Place &p, int rep, int cap, int window) {
+    const int t0 = p.tile * TILE / rep, t1 = min(p.n - 1, (p.tile * TILE + TILE - 1) / rep);
+    const int p0 = p.kv - p.n + t0, p1 = p.kv - p.n + t1;   // positions of the first and last row
+    Keys k;
+    const int first = window <= p0 ? (p0 - window + 1) & ~63 : 0, end = min(p1 + 1, cap);
+    k.lo = first;
+    k.hi = end;
+    if (p.n_split > 1) {
+        const long long a = first + (long long)p.split * p.len, z = a + p.len;
+        k.lo = (int)min(a, (long long)INT_MAX - 64);
+        k.hi = (int)min(z, (long long)end);
+    }
+    k.all_lo = window <= p1 ? p1 - window + 1 : 0;
+    k.all_hi = min(p0 + 1, cap);
+    return k;
+}
+
+// ---- 16-bit parts ------------------------------------------------------------
+
+// The bits of x cut to 16 (bf16, towards zero).
+__device__ __forceinline__ float bf16_cut(float x) {
+    return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, x) & 0xffff0000u);
+}
+__device__ __forceinline__ bool finite(float x) {
+    return (__builtin_bit_cast(unsigned, x) & 0x7f800000u) != 0x7f800000u;
+}
+
+template <class C> struct Mma;   // the 16-bit matrix instructions of a type
+
+template <> struct Mma<half_t> {
+    typedef half8 vec8;
+    static __device__ __forceinline__ floatx4 mul16(half8 a, half8 b, floatx4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ floatx16 mul32(half8 a, half8 b, floatx16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+    // Weights reach 2^14 (kLag and kBias below), so that those of 2^-20 of a row's largest are no subnormals.
+    static constexpr float kBias = 6.0f;
+};
+template <> struct Mma<bhalf_t> {
+    typedef bhalf8 vec8;
+    static __device__ __forceinline__ floatx4 mul16(bhalf8 a, bhalf8 b, floatx4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ floatx16 mul32(bhalf8 a, bhalf8 b, floatx16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+    static constexpr float kBias = 0.0f;
+};
+
+// Parts that hold an fp32 value: two of fp16 (22 bits of a value near its row's
+// largest), three of bf16 (24 bits).
+template <class A, class C> struct Parts { static constexpr int q = 1, p = 1; };
+template <> struct Parts<float, half_t> { static constexpr int q = 2, p = 2; };
+template <> struct Parts<float, bhalf_t> { static constexpr int q = 3, p = 3; };
+
+// The parts of one q value.  All have its sign and none is 0 where q is not, so
+// that an infinity of K gives every product the same sign: an infinite score, as
+// in exact arithmetic, not NaN.  (A part set to its least value adds 2^-30 of the
+// value, or, for fp16, 2^-37 of the row's largest.)
+template <int N>
+__device__ __forceinline__ void split_q(float x, bhalf_t (&part)[N]) {
+    const float h = bf16_cut(x);
+    part[0] = (bhalf_t)h;
+    if constexpr (N == 3) {
+        const float r = finite(x) ? x - h : x, m = bf16_cut(r), l = finite(x) ? r - m : x, least = bf16_cut(h * 0x1p-30f);
+        part[1] = (bhalf_t)(m == 0.f ? least : m);
+        part[2] = (bhalf_t)(l == 0.f ? least : bf16_cut(l));
+    }
+}
+template <int N>
+__device__ __forceinline__ void split_q(float x, half_t (&part)[N]) {
+    const auto cut = __builtin_amdgcn_cvt_pkrtz(x, x);
+    const half_t least = (half_t)__builtin_copysignf(0x1p-24f, x);
+    half_t h = (half_t)cut[0];
+    const half_t l = (half_t)(x - (float)h);
+    if (x != 0.f && (float)h == 0.f) h = least;
+    part[0] = h;
+    if constexpr (N == 2) part[1] = x != 0.f && (float)l == 0.f ? least : l;
+}
+
+// Parts of a weight, each the nearest.
+template <int N, class C>
+__device__ __forceinline__ void split_p(float x, C (&part)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        part[i] = (C)x;
+        if (i + 1 < N) x -= (float)part[i];
+    }
+}
+
+// A power of two that brings |x| <= big to 2^13 .. 2^14 (1 where there is none),
+// and its inverse.
+__device__ __forceinline__ void unit_of(float big, float &to, float &back) {
+    const int e = (int)((__builtin_bit_cast(unsigned, big) >> 23) & 255);
+    if (e == 0 || e == 255) {   // 0 or a subnormal, or not finite
+        to = back = 1.f;
+        if (e == 0 && big != 0.f) { to = 0x1p120f; back = 0x1p-120f; }
+        return;
+    }
+    const int up = min(max(140 - e, -126), 126);   // 2^up * 2^(e - 127) = 2^13
+    to = __builtin_bit_cast(float, (unsigned)(127 + up) << 23);
+    back = __builtin_bit_cast(float, (unsigned)(127 - up) << 23);
+}
+
+// ---- the softmax ---------------------------------------------------------------
+
+// exp(scale q.k) = 2^(dot * (hi + lo)), hi + lo = scale log2(e) to 48 bits; a row's
+// weights are 2^(that - ref).  The reference follows the row's largest score: it
+// moves when that passes it by kLag, so that the accumulators are rescaled rarely.
+constexpr float kLag = 8.0f;
+
+struct ScaleLog2 {
+    float hi, lo;
+};
+
+// 4 elements of a transposed block of LDS: lane i of 16 gives the address of
+// elements 4 (i % 4) .. + 3 of row i / 4, and gets element i of the four rows
+// (checked on the GPU).
+template <class V4>
+__device__ __forceinline__ V4 read_transposed(const void *lds) {
+    return __builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)lds));
+}
+
+}  // namespace
+}  // namespace kore_paged_gpu

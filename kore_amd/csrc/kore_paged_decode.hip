@@ -1,0 +1,634 @@
+// kore_paged_decode.hip - paged attention of few rows (a decode step), and the
+// merge of split tiles (gfx950).
+//
+// A tile is 16 rows: the q-heads of one token's kv-head, or of a few tokens.  K and
+// V are read once for them, so at 16 flops a cache value the kernel is bound by
+// HBM; 16 waves' worth of loads in flight per CU are what carries it.  A workgroup
+// is four waves that take blocks of keys in turn, each with its own softmax state,
+// merged through LDS at the end; the next block's K and V are requested before the
+// current one is computed.
+#include "kore_paged_attend.h"
+
+#include <algorithm>
+
+namespace kore_paged_gpu {
+namespace {
+
+constexpr int kThreads = 256, kWaves = 4, kRows = 16;
+
+struct DecodeArgs {
+    AttendArgs a;
+    Cut cut;
+    ScaleLog2 sl;
+    float *part_o, *part_ml;
+};
+
+// What a lane knows of its row (column l % 16 of the products).
+struct Row {
+    int lo, hi;      // sees keys [lo, hi)
+    bool real;
+    int token, head;
+};
+
+__device__ __forceinline__ Row row_of(const Place &p, int r, int rep, int cap, int window) {
+    Row x;
+    x.real = r < p.n * rep;
+    x.token = r / rep;
+    x.head = p.head * rep + (r - x.token * rep);
+    const int pos = p.kv - p.n + x.token;
+    x.lo = window <= pos ? pos - window + 1 : 0;
+    x.hi = x.real ? min(pos + 1, cap) : 0;
+    return x;
+}
+
+// The pages of a wave's 16-key groups, 64 at a time in the lanes of a register and
+// the next 64 in another, requested long before they are needed.
+struct PageRun {
+    int now, ahead;
+    // group: this lane's
+    static __device__ __forceinline__ int load(const AttendArgs &a, const int *table, int group, int hi) {
+        const int key = group * 16, at = key >> a.page_shift;
+        int p = -1;
+        if (key >= 0 && key < hi && at < a.b.pages_stride) p = table[at];   // (a number past the keys may wrap)
+        return p < a.n_pages ? p : -1;   // negative: none
+    }
+    __device__ __forceinline__ int get(int i) const { return __builtin_amdgcn_readlane(now, i); }
+};
+
+// The four waves' states (ref, sum, and o as [dim / 4][row] float4) into out, or
+// into the split's partial.
+template <class A, int HDP>
+__device__ __forceinline__ void finish(const DecodeArgs &d, const Place &p, const float4 (*o)[HDP / 4][kRows],
+                                       const float2 (*ml)[kRows]) {
+    const AttendArgs &a = d.a;
+    __syncthreads();
+    const int rep = d.cut.rep;
+    for (int i = threadIdx.x; i < HDP / 4 * kRows; i += kThreads) {
+        const int row = i % kRows, d4 = i / kRows;
+        float m = kNone, l = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) m = fmaxf(m, ml[w][row].x);
+        const float base = m == kNone ? 0.f : m;
+        float4 s = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float2 e = ml[w][row];
+            const float f = exp2_(e.x - base);
+            const float4 v = o[w][d4][row];
+            l = fmaf(e.y, f, l);
+            s.x = fmaf(v.x, f, s.x);
+            s.y = fmaf(v.y, f, s.y);
+            s.z = fmaf(v.z, f, s.z);
+            s.w = fmaf(v.w, f, s.w);
+        }
+        if (p.n_split > 1) {
+            const size_t id = blockIdx.x;
+            reinterpret_cast<float4 *>(d.part_o)[(id * (HDP / 4) + d4) * kRows + row] = s;
+            if (d4 == 0) reinterpret_cast<float2 *>(d.part_ml)[id * kRows + row] = make_float2(m, l);
+            continue;
+        }
+        const int r = p.tile * kRows + row;
+        if (r >= p.n * rep || 4 * d4 >= a.hd) continue;
+        const int token = r / rep, head = p.head * rep + r - token * rep;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        A *out = (A *)a.out + (size_t)(p.q0 + token) * a.out_stride + (size_t)head * a.hd + 4 * d4;
+        const A v[4] = {(A)(s.x * inv), (A)(s.y * inv), (A)(s.z * inv), (A)(s.w * inv)};
+        store_n<4>(out, v, ((uintptr_t)out & (4 * sizeof(A) - 1)) == 0);
+    }
+}
+
+// A tile's rescale where a score passes the reference by kLag (or is the first).
+template <int N>
+__device__ __forceinline__ void follow(float top, float &ref, float &sum, float bias, floatx4 (&o)[N]) {
+    const bool moves = top - bias > ref + kLag || (ref == kNone && top > kNone);
+    if (__any(moves)) {
+        const float next = moves ? top - bias : ref;
+        const float f = moves ? exp2_(ref - next) : 1.f;
+        sum *= f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) o[i] *= f;
+        ref = next;
+    }
+}
+
+// ---- 16-bit caches -----------------------------------------------------------
+//
+// A block is 32 keys.  S^T = K Q^T on 16x16x32 MFMA: lane (m, g) = (l % 16, l / 16)
+// loads 16-byte pieces of K's row m, 64 contiguous bytes for the four g, straight
+// into the A operand.  The product leaves a lane the scores of row n = l % 16 and
+// keys 4 g + i of either 16, which, rounded, are the B operand of O^T += V^T P^T in a
+// k order of its own; V^T's operand in that order comes out of LDS by transposed
+// reads (rows padded by 32 bytes: the 8 rows that half a wave reads lie on different
+// banks).  No lane ever needs another's score but for the maximum and the sum.
+template <class A, class C, int HDP>
+__global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode16_kernel(DecodeArgs d) {
+    constexpr int QP = Parts<A, C>::q, PP = Parts<A, C>::p;
+    constexpr int KS = HDP / 32, DT = HDP / 16, VR = HDP / 16;   // k-steps, dim tiles, V registers of 16 bytes
+    constexpr int kPitch = HDP + 16;                             // of a V row in LDS, elements
+    constexpr int kBlock = 32;
+    typedef typename Mma<C>::vec8 vec8;
+    typedef C vec4 __attribute__((ext_vector_type(4)));
+    constexpr size_t kVBytes = sizeof(C) * kWaves * kBlock * kPitch, kOBytes = sizeof(float) * kWaves * HDP * kRows;
+    __shared__ __attribute__((aligned(16))) unsigned char shared[kVBytes > kOBytes ? kVBytes : kOBytes];
+    __shared__ float2 ml[kWaves][kRows];
+    const AttendArgs &a = d.a;
+    const int cap = a.b.pages_stride << a.page_shift, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Place p;
+    if (!place_of<kRows>(a.b, d.cut, blockIdx.x, a.n_head_kv, cap, a.window, false, p)) return;
+    const Keys k = keys_of<kRows>(p, d.cut.rep, cap, a.window);
+    const int col = lane & 15, g = lane >> 4;
+    const Row row = row_of(p, p.tile * kRows + col, d.cut.rep, cap, a.window);
+    const int *table = a.b.pages + (size_t)p.seq * a.b.pages_stride;
+    const int slot_mask = (1 << a.page_shift) - 1;
+    const bool padded = a.hd != HDP;
+
+    // page groups of this wave: block j's two are lanes 2 (j % 32), + 1
+    const int first_block = k.lo / kBlock + wave;
+    const auto pages_from = [&](int j) {
+        return PageRun::load(a, table, (first_block + kWaves * (j + (lane >> 1))) * 2 + (lane & 1), k.hi);
+    };
+    const int n_block = k.lo < k.hi ? max(0, ((k.hi + kBlock - 1) / kBlock - first_block + kWaves - 1) / kWaves) : 0;
+    PageRun run;
+    run.now = pages_from(0);
+    run.ahead = -1;
+
+    // Q: B operand, lane (n, g) has dims 32 t + 8 g .. + 7 of its row
+    vec8 q[QP][KS];
+    float unit = 1.f;
+    {
+        float x[KS][8];
+        const A *src = (const A *)a.q + (size_t)(row.real ? p.q0 + row.token : 0) * a.q_stride + (size_t)(row.real ? row.head : 0) * a.hd;
+        float big = 0;
+#pragma unroll
+        for (int t = 0; t < KS; ++t) {
+            const int dim = 32 * t + 8 * g;
+            A v[8];
+            const bool in = row.real && dim < a.hd;
+            if (in) load_n<8>(src + dim, v, ((uintptr_t)src & (8 * sizeof(A) - 1)) == 0);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[t][i] = in ? to_f32(v[i]) : 0.f;
+                big = fmaxf(big, fabsf(x[t][i]));
+            }
+        }
+        float to = 1.f;
+        if (QP == 2) unit_of(max32(max16(big)), to, unit);
+#pragma unroll
+        for (int t = 0; t < KS; ++t)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if constexpr (QP == 1) {
+                    q[0][t][i] = (C)x[t][i];
+                } else {
+                    C part[QP];
+                    split_q<QP>(x[t][i] * to, part);
+#pragma unroll
+                    for (int j = 0; j < QP; ++j) q[j][t][i] = part[j];
+                }
+            }
+    }
+    const float s_hi = d.sl.hi * unit, s_lo = d.sl.lo * unit;
+
+    // A 16-key group lies in one page: a base that is the wave's, and a lane's offset
+    // that does not change.  A group without a page reads page 0.
+    const auto base_of = [&](const void *pool, int page, int key) {
+        return (const C *)pool + ((((size_t)max(page, 0) * a.n_head_kv + p.head) << a.page_shift) + (key & slot_mask)) * a.hd;
+    };
+    constexpr int kPerRow = HDP / 8, kRowsPer = 64 / kPerRow;   // 16-byte pieces of a V row; rows a load covers
+    const int v_row = lane / kPerRow, v_dim = 8 * (lane % kPerRow);
+    int k_off[KS];
+#pragma unroll
+    for (int t = 0; t < KS; ++t) k_off[t] = col * a.hd + (padded ? min(32 * t + 8 * g, a.hd - 8) : 32 * t + 8 * g);
+    const int v_off = v_row * a.hd + (padded ? min(v_dim, a.hd - 8) : v_dim);
+    vec8 kr[2][KS], vr[VR];
+    int p0 = 0, p1 = 0;   // pages of the block whose K and V are in flight
+    const auto load_k = [&](int key0) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            const C *src = base_of(a.k_pool, m ? p1 : p0, key0 + 16 * m);
+#pragma unroll
+            for (int t = 0; t < KS; ++t) kr[m][t] = *reinterpret_cast<const vec8 *>(src + k_off[t]);
+        }
+    };
+    const auto load_v = [&](int key0) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            const C *src = base_of(a.v_pool, m ? p1 : p0, key0 + 16 * m);
+#pragma unroll
+            for (int r = 0; r < VR / 2; ++r) vr[m * (VR / 2) + r] = *reinterpret_cast<const vec8 *>(src + (v_off + kRowsPer * r * a.hd));
+        }
+    };
+
+    floatx4 o[DT];
+#pragma unroll
+    for (int i = 0; i < DT; ++i) o[i] = floatx4{0, 0, 0, 0};
+    float ref = kNone, sum = 0;
+    C *const v_lds = reinterpret_cast<C *>(shared) + wave * kBlock * kPitch;
+    // V^T's operand: lane (m, g) needs dim 16 i + m of keys 4 g .. + 3 of either 16
+    const C *const v_from = v_lds + (4 * g + (col >> 2)) * kPitch + 4 * (col & 3);
+    const auto v_operand = [&](int i) {
+        const vec4 x = read_transposed<vec4>(v_from + 16 * i), y = read_transposed<vec4>(v_from + 16 * kPitch + 16 * i);
+        return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+
+    if (n_block) {
+        p0 = run.get(0);
+        p1 = run.get(1);
+        load_k(first_block * kBlock);
+        load_v(first_block * kBlock);
+        run.ahead = pages_from(32);
+    }
+    for (int j = 0; j < n_block; ++j) {
+        const int key0 = (first_block + kWaves * j) * kBlock;
+        const bool has0 = p0 >= 0, has1 = p1 >= 0;
+        const bool whole = key0 >= k.all_lo && key0 + kBlock <= min(k.all_hi, k.hi) && has0 && has1;
+        // pages of the next block
+        const int next = j + 1, next_key = key0 + kWaves * kBlock;
+        if ((next & 31) == 0) {
+            run.now = run.ahead;
+            run.ahead = pages_from(next + 32);
+        }
+        p0 = run.get(2 * (next & 31));
+        p1 = run.get(2 * (next & 31) + 1);
+
+        if (padded) {
+#pragma unroll
+            for (int t = 0; t < KS; ++t)
+                if (32 * t + 8 * g >= a.hd) {
+                    kr[0][t] = vec8{};
+                    kr[1][t] = vec8{};
+                }
+        }
+        floatx4 s[2];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            s[m] = floatx4{0, 0, 0, 0};
+#pragma unroll
+            for (int t = 0; t < KS; ++t)
+#pragma unroll
+                for (int x = 0; x < QP; ++x) s[m] = Mma<C>::mul16(kr[m][t], q[x][t], s[m]);
+        }
+        if (next < n_block) load_k(next_key);
+
+        bool odd = false;   // an infinity or NaN of V that some row sees and another does not
+        if (!whole) {
+#pragma unroll
+            for (int r = 0; r < VR; ++r) {
+                const int key = key0 + kRowsPer * r + v_row;
+                // V of positions that no row sees may hold anything
+                if (!(key < k.hi && (kRowsPer * r >= 16 ? has1 : has0))) vr[r] = vec8{};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) odd |= !finite(to_f32(vr[r][i]));
+            }
+            odd = __any(odd);
+        }
+#pragma unroll
+        for (int r = 0; r < VR; ++r) *reinterpret_cast<vec8 *>(v_lds + (kRowsPer * r + v_row) * kPitch + v_dim) = vr[r];
+        if (next < n_block) load_v(next_key);
+
+        if (!whole) {
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int key = key0 + 16 * m + 4 * g + i;
+                    if (!(key >= row.lo && key < min(row.hi, k.hi) && (m ? has1 : has0))) s[m][i] = kNone;
+                }
+        }
+        float top = kNone;
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, s[m][i]);
+        top = max32(max16(top)) * s_hi;
+        follow(top, ref, sum, Mma<C>::kBias, o);
+        const float base = ref == kNone ? 0.f : ref;
+        vec8 w[PP];
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float e = PP > 1 ? fmaf(s[m][i], s_hi, fmaf(s[m][i], s_lo, -base)) : fmaf(s[m][i], s_hi, -base);
+                const float x = s[m][i] == kNone ? 0.f : exp2_(e);
+                C part[PP];
+                split_p<PP>(x, part);
+                // one rounded weight is also what is summed: what rounding adds to all of a row's weights divides out
+                sum += PP > 1 ? x : to_f32(part[0]);
+#pragma unroll
+                for (int y = 0; y < PP; ++y) w[y][4 * m + i] = part[y];
+            }
+        if (!odd) {
+#pragma unroll
+            for (int i = 0; i < DT; ++i) {
+                const vec8 v = v_operand(i);
+#pragma unroll
+                for (int y = 0; y < PP; ++y) o[i] = Mma<C>::mul16(v, w[y], o[i]);
+            }
+        } else {
+            // key by key, each added only to the rows that see it
+            for (int e = 0; e < kBlock; ++e) {
+                const int key = key0 + e, mine = 4 * (e >> 4) + (e & 3);
+                const bool sees = key >= row.lo && key < row.hi, here = ((e >> 2) & 3) == g;
+#pragma unroll
+                for (int i = 0; i < DT; ++i) {
+                    vec8 v = v_operand(i);
+#pragma unroll
+                    for (int x = 0; x < 8; ++x)
+                        if (!here || x != mine) v[x] = (C)0.f;
+                    floatx4 t = floatx4{0, 0, 0, 0};
+#pragma unroll
+                    for (int y = 0; y < PP; ++y) t = Mma<C>::mul16(v, w[y], t);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        if (sees) o[i][x] += t[x];
+                }
+            }
+        }
+    }
+
+    sum = sum32(sum16(sum));
+    __syncthreads();   // V's rows give way to the states
+    float4(*const states)[HDP / 4][kRows] = reinterpret_cast<float4(*)[HDP / 4][kRows]>(shared);
+#pragma unroll
+    for (int i = 0; i < DT; ++i) states[wave][4 * i + g][col] = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
+    if (g == 0) ml[wave][col] = make_float2(ref, sum);
+    finish<A, HDP>(d, p, states, ml);
+}
+
+// ---- fp32 caches ---------------------------------------------------------------
+//
+// A block is 16 keys, both products on 16x16x4 fp32 MFMA (exact products, fp32 sums).
+// Lane (m, g) loads K's row m, dims 16 u + 4 g + e: e picks the instruction, g is its
+// k.  The scores of keys 4 g + i are its k order of the second product, whose V
+// operand, lane (m, g): V[4 g + i][64 j + 4 m + e], comes straight from memory too.
+template <int HDP>
+__global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode32_kernel(DecodeArgs d) {
+    constexpr int KU = HDP / 16, DJ = HDP / 64, kBlock = 16;
+    __shared__ float4 states[kWaves][HDP / 4][kRows];
+    __shared__ float2 ml[kWaves][kRows];
+    const AttendArgs &a = d.a;
+    const int cap = a.b.pages_stride << a.page_shift, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Place p;
+    if (!place_of<kRows>(a.b, d.cut, blockIdx.x, a.n_head_kv, cap, a.window, false, p)) return;
+    const Keys k = keys_of<kRows>(p, d.cut.rep, cap, a.window);
+    const int col = lane & 15, g = lane >> 4;
+    const Row row = row_of(p, p.tile * kRows + col, d.cut.rep, cap, a.window);
+    const int *table = a.b.pages + (size_t)p.seq * a.b.pages_stride;
+    const int slot_mask = (1 << a.page_shift) - 1;
+    const bool padded = a.hd != HDP;
+
+    // block j's page is lane j % 64
+    const int first_block = k.lo / kBlock + wave;
+    const auto pages_from = [&](int j) { return PageRun::load(a, table, first_block + kWaves * (j + lane), k.hi); };
+    const int n_block = k.lo < k.hi ? max(0, ((k.hi + kBlock - 1) / kBlock - first_block + kWaves - 1) / kWaves) : 0;
+    PageRun run;
+    run.now = pages_from(0);
+    run.ahead = -1;
+
+    floatx4 q[KU];
+    {
+        const float *src = (const float *)a.q + (size_t)(row.real ? p.q0 + row.token : 0) * a.q_stride + (size_t)(row.real ? row.head : 0) * a.hd;
+        const bool vec = ((uintptr_t)src & 15) == 0;
+#pragma unroll
+        for (int u = 0; u < KU; ++u) {
+            const int dim = 16 * u + 4 * g;
+            float v[4] = {0, 0, 0, 0};
+            if (row.real && dim < a.hd) load_n<4>(src + dim, v, vec);
+            q[u] = floatx4{v[0], v[1], v[2], v[3]};
+        }
+    }
+    const auto base_of = [&](const void *pool, int page, int key) {
+        return (const float *)pool + ((((size_t)max(page, 0) * a.n_head_kv + p.head) << a.page_shift) + (key & slot_mask)) * a.hd;
+    };
+    int k_off[KU], v_off[DJ];
+#pragma unroll
+    for (int u = 0; u < KU; ++u) k_off[u] = col * a.hd + (padded ? min(16 * u + 4 * g, a.hd - 4) : 16 * u + 4 * g);
+#pragma unroll
+    for (int x = 0; x < DJ; ++x) v_off[x] = 4 * g * a.hd + (padded ? min(64 * x + 4 * col, a.hd - 4) : 64 * x + 4 * col);
+    floatx4 kr[KU], vr[4][DJ];
+    int page = 0;
+    const auto load_k = [&](int key0) {
+        const float *src = base_of(a.k_pool, page, key0);
+#pragma unroll
+        for (int u = 0; u < KU; ++u) kr[u] = *reinterpret_cast<const floatx4 *>(src + k_off[u]);
+    };
+    const auto load_v = [&](int key0) {
+        const float *src = base_of(a.v_pool, page, key0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int x = 0; x < DJ; ++x) vr[i][x] = *reinterpret_cast<const floatx4 *>(src + (v_off[x] + i * a.hd));
+    };
+    floatx4 o[4 * DJ];
+#pragma unroll
+    for (int i = 0; i < 4 * DJ; ++i) o[i] = floatx4{0, 0, 0, 0};
+    float ref = kNone, sum = 0;
+
+    if (n_block) {
+        page = run.get(0);
+        load_k(first_block * kBlock);
+        load_v(first_block * kBlock);
+        run.ahead = pages_from(64);
+    }
+    for (int j = 0; j < n_block; ++j) {
+        const int key0 = (first_block + kWaves * j) * kBlock;
+        const bool has = page >= 0, whole = key0 >= k.all_lo && key0 + kBlock <= min(k.all_hi, k.hi) && has;
+        const int next = j + 1, next_key = key0 + kWaves * kBlock;
+        if ((next & 63) == 0) {
+            run.now = run.ahead;
+            run.ahead = pages_from(next + 64);
+        }
+        page = run.get(next & 63);
+
+        if (padded) {
+#pragma unroll
+            for (int u = 0; u < KU; ++u)
+                if (16 * u + 4 * g >= a.hd) kr[u] = floatx4{0, 0, 0, 0};
+        }
+        floatx4 s = floatx4{0, 0, 0, 0}, s2 = floatx4{0, 0, 0, 0};   // two chains
+#pragma unroll
+        for (int u = 0; u < KU; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                s = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[u][e], q[u][e], s, 0, 0, 0);
+                s2 = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[u][e + 1], q[u][e + 1], s2, 0, 0, 0);
+            }
+        s += s2;
+        if (next < n_block) load_k(next_key);
+
+        bool odd = false;
+        if (!whole) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int key = key0 + 4 * g + i;
+                const bool in = key < k.hi && has;
+                if (!(in && key >= row.lo && key < row.hi)) s[i] = kNone;
+#pragma unroll
+                for (int x = 0; x < DJ; ++x) {
+                    if (!in) vr[i][x] = floatx4{0, 0, 0, 0};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) odd |= !finite(vr[i][x][e]);
+                }
+            }
+            odd = __any(odd);
+        }
+        float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+        top = max32(max16(top)) * d.sl.hi;
+        follow(top, ref, sum, 0.f, o);
+        const float base = ref == kNone ? 0.f : ref;
+        float w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[i] = s[i] == kNone ? 0.f : exp2_(fmaf(s[i], d.sl.hi, fmaf(s[i], d.sl.lo, -base)));
+            sum += w[i];
+        }
+        if (!odd) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int x = 0; x < DJ; ++x)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        o[4 * x + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(vr[i][x][e], w[i], o[4 * x + e], 0, 0, 0);
+        } else {
+            // key by key, each added only to the rows that see it
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                for (int y = 0; y < 4; ++y) {
+                    const int key = key0 + 4 * y + i;
+                    const bool sees = key >= row.lo && key < row.hi;
+#pragma unroll
+                    for (int x = 0; x < DJ; ++x)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const floatx4 t = __builtin_amdgcn_mfma_f32_16x16x4f32(g == y ? vr[i][x][e] : 0.f, w[i],
+                                                                                  floatx4{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+                            for (int z = 0; z < 4; ++z)
+                                if (sees) o[4 * x + e][z] += t[z];
+                        }
+                }
+        }
+        if (next < n_block) load_v(next_key);
+    }
+
+    sum = sum32(sum16(sum));
+    // o[4 x + e], lane (n, g), element i: dim 64 x + 4 (4 g + i) + e of row n
+#pragma unroll
+    for (int x = 0; x < DJ; ++x)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            states[wave][16 * x + 4 * g + i][col] = make_float4(o[4 * x][i], o[4 * x + 1][i], o[4 * x + 2][i], o[4 * x + 3][i]);
+    if (g == 0) ml[wave][col] = make_float2(ref, sum);
+    finish<float, HDP>(d, p, states, ml);
+}
+
+// ---- the merge of splits ---------------------------------------------------------
+//
+// A workgroup takes four dims of a tile and kv-head: TILE rows by 256 / TILE lanes
+// over the splits, each its own running maximum, joined through LDS.  (Few tiles may
+// have hundreds of splits, so the dims are what there is to spread.)
+template <class A, int TILE>
+__global__ __launch_bounds__(kThreads) void merge_kernel(DecodeArgs d, int hd4) {
+    constexpr int kLanes = kThreads / TILE;
+    __shared__ float4 so[kLanes][TILE];
+    __shared__ float2 sm[kLanes][TILE];
+    const AttendArgs &a = d.a;
+    const int cap = a.b.pages_stride << a.page_shift, d4 = blockIdx.y;
+    Place p;
+    if (!place_of<TILE>(a.b, d.cut, blockIdx.x, a.n_head_kv, cap, a.window, true, p) || p.n_split <= 1) return;
+    const int row = threadIdx.x % TILE, part = threadIdx.x / TILE;
+    const float4 *po = reinterpret_cast<const float4 *>(d.part_o);
+    const float2 *pm = reinterpret_cast<const float2 *>(d.part_ml);
+    float m = kNone, l = 0;
+    float4 s = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+    for (int i = part; i < p.n_split; i += kLanes) {
+        const size_t id = (size_t)p.first + (size_t)i * a.n_head_kv;
+        const float2 e = pm[id * TILE + row];
+        const float4 v = po[(id * hd4 + d4) * TILE + row];
+        const float next = fmaxf(m, e.x), base = next == kNone ? 0.f : next;
+        const float f = exp2_(m - base), h = exp2_(e.x - base);
+        l = fmaf(e.y, h, l * f);
+        s = make_float4(fmaf(v.x, h, s.x * f), fmaf(v.y, h, s.y * f), fmaf(v.z, h, s.z * f), fmaf(v.w, h, s.w * f));
+        m = next;
+    }
+    so[part][row] = s;
+    sm[part][row] = make_float2(m, l);
+    __syncthreads();
+    const int r = p.tile * TILE + row;
+    if (part != 0 || r >= p.n * d.cut.rep) return;
+#pragma unroll
+    for (int i = 1; i < kLanes; ++i) m = fmaxf(m, sm[i][row].x);
+    const float base = m == kNone ? 0.f : m;
+    l = 0;
+    s = make_float4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < kLanes; ++i) {
+        const float2 e = sm[i][row];
+        const float4 v = so[i][row];
+        const float f = exp2_(e.x - base);
+        l = fmaf(e.y, f, l);
+        s = make_float4(fmaf(v.x, f, s.x), fmaf(v.y, f, s.y), fmaf(v.z, f, s.z), fmaf(v.w, f, s.w));
+    }
+    const int token = r / d.cut.rep, head = p.head * d.cut.rep + r - token * d.cut.rep;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    A *out = (A *)a.out + (size_t)(p.q0 + token) * a.out_stride + (size_t)head * a.hd + 4 * d4;
+    const A v[4] = {(A)(s.x * inv), (A)(s.y * inv), (A)(s.z * inv), (A)(s.w * inv)};
+    store_n<4>(out, v, ((uintptr_t)out & (4 * sizeof(A) - 1)) == 0);
+}
+
+constexpr int kMinLen = 64;         // keys: a block for each of two waves
+constexpr int kPerCu = 2;           // workgroups that fit a CU
+constexpr int kMaxTiles = 1024;     // over this many (tile, kv-head)s nothing is split
+
+int padded_dim(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
+
+}  // namespace
+
+size_t attend_workspace_bytes(int n_head, int n_head_kv, int hd, int num_cu) {
+    const size_t places = (size_t)kMaxTiles + (size_t)kPerCu * num_cu;
+    return places * kRows * ((size_t)padded_dim(hd) + 2) * sizeof(float);
+}
+
+hipError_t launch_attend(const AttendArgs &a, hipStream_t s) {
+    DecodeArgs d{};
+    d.a = a;
+    d.cut.rep = a.n_head / a.n_head_kv;
+    const long long tiles = ((long long)a.b.n_tok * d.cut.rep / kRows + std::min(a.b.n_seq, a.b.n_tok)) * a.n_head_kv;
+    const int places = kPerCu * a.num_cu;
+    d.cut.target = tiles > kMaxTiles ? 0 : (int)std::max<long long>(places - tiles, places / 2);
+    d.cut.min_len = kMinLen;
+    const double sl = (double)a.scale * 1.4426950408889634074;
+    d.sl.hi = (float)sl;
+    d.sl.lo = (float)(sl - (double)d.sl.hi);
+    const int hdp = padded_dim(a.hd);
+    d.part_o = a.part;
+    d.part_ml = a.part + (size_t)(tiles + d.cut.target) * kRows * hdp;
+    const dim3 grid((unsigned)(tiles + d.cut.target));
+#define KORE_DIMS(LAUNCH)            \
+    do {                             \
+        if (hdp == 64) LAUNCH(64);   \
+        else if (hdp == 128) LAUNCH(128); \
+        else LAUNCH(256);            \
+    } while (0)
+#define KORE_FF(H) decode32_kernel<H><<<grid, kThreads, 0, s>>>(d)
+#define KORE_FH(H) decode16_kernel<float, half_t, H><<<grid, kThreads, 0, s>>>(d)
+#define KORE_FB(H) decode16_kernel<float, bhalf_t, H><<<grid, kThreads, 0, s>>>(d)
+#define KORE_HH(H) decode16_kernel<half_t, half_t, H><<<grid, kThreads, 0, s>>>(d)
+#define KORE_BB(H) decode16_kernel<bhalf_t, bhalf_t, H><<<grid, kThreads, 0, s>>>(d)
+    if (a.cache_type == kF32) KORE_DIMS(KORE_FF);
+    else if (a.type == kF32 && a.cache_type == kF16) KORE_DIMS(KORE_FH);
+    else if (a.type == kF32) KORE_DIMS(KORE_FB);
+    else if (a.type == kF16) KORE_DIMS(KORE_HH);
+    else KORE_DIMS(KORE_BB);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !d.cut.target) return e;
+    const dim3 merge((unsigned)tiles, (unsigned)(a.hd / 4));
+    if (a.type == kF32) merge_kernel<float, kRows><<<merge, kThreads, 0, s>>>(d, hdp / 4);
+    else if (a.type == kF16) merge_kernel<half_t, kRows><<<merge, kThreads, 0, s>>>(d, hdp / 4);
+    else merge_kernel<bhalf_t, kRows><<<merge, kThreads, 0, s>>>(d, hdp / 4);
+    return hipGetLastError();
+}
+
+}  // namespace kore_paged_gpu

@@ -4,8 +4,7 @@
 
 #include "kore_paged_kernels.h"
 
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
+#include <climits>
 
 namespace kore_paged_gpu {
 namespace {
@@ -17,7 +16,7 @@ __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(half_t x) { return (float)x; }
 __device__ __forceinline__ float to_f32(bhalf_t x) { return (float)x; }
 
-// N elements from an address that is aligned to N elements (VEC), or to one.
+// N elements from an address that is aligned to N elements (vec), or to one.
 template <int N, class T>
 __device__ __forceinline__ void load_n(const T *p, T (&x)[N], bool vec) {
     typedef T vec_t __attribute__((ext_vector_type(N)));

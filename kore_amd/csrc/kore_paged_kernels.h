@@ -12,6 +12,7 @@ namespace kore_paged_gpu {
 constexpr int kMaxHeadDim = 256;        // of the paged cache
 constexpr int kMaxRopeHeadDim = 1024;   // of the rotary call
 constexpr int kMaxRot = 512;
+constexpr int kMaxKeys = 1 << 30;       // positions of a sequence's row of the page table
 
 enum Type { kF32 = 0, kF16 = 1, kBF16 = 2 };
 inline int type_bytes(int t) { return t == kF32 ? 4 : 2; }
