@@ -22,6 +22,25 @@ struct Cut {
     int min_len;     // a split's fewest keys
 };
 
+// exp(scale q.k) = 2^(dot * (hi + lo)), hi + lo = scale log2(e) to 47 bits, both over
+// 0, so that a score of -inf (one that is masked) needs no test: both terms are -inf.
+struct ScaleLog2 {
+    float hi, lo;
+};
+
+// A launch over tiles; part_o [place][dim / 4][row] float4 and part_ml [place][row]
+// (reference, sum) hold split tiles.
+struct TileArgs {
+    AttendArgs a;
+    Cut cut;
+    ScaleLog2 sl;
+    float *part_o, *part_ml;
+};
+
+constexpr int kChunkRows = 128;   // of a tile of kore_paged_chunk.hip
+inline int padded_dim(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
+hipError_t launch_chunk(const TileArgs &d, int places, hipStream_t s);
+
 namespace {
 
 typedef float floatx4 __attribute__((ext_vector_type(4)));
@@ -275,13 +294,55 @@ __device__ __forceinline__ void unit_of(float big, float &to, float &back) {
 
 // ---- the softmax ---------------------------------------------------------------
 
-// exp(scale q.k) = 2^(dot * (hi + lo)), hi + lo = scale log2(e) to 48 bits; a row's
-// weights are 2^(that - ref).  The reference follows the row's largest score: it
-// moves when that passes it by kLag, so that the accumulators are rescaled rarely.
+// A row's weights are 2^(dot scale log2(e) - ref).  The reference follows the row's
+// largest score: it moves when that passes it by kLag, so that the accumulators are
+// rescaled rarely.
 constexpr float kLag = 8.0f;
 
-struct ScaleLog2 {
-    float hi, lo;
+// A tile's rescale where a score passes the reference by kLag (or is the first).
+template <class V, int N>
+__device__ __forceinline__ void follow(float top, float &ref, float &sum, float bias, V (&o)[N]) {
+    const bool moves = top - bias > ref + kLag || (ref == kNone && top > kNone);
+    if (__any(moves)) {
+        const float next = moves ? top - bias : ref;
+        const float f = moves ? exp2_(ref - next) : 1.f;
+        sum *= f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) o[i] *= f;
+        ref = next;
+    }
+}
+
+// What a lane knows of its row (column l % 16 of the products).
+struct Row {
+    int lo, hi;      // sees keys [lo, hi)
+    bool real;
+    int token, head;
+};
+
+__device__ __forceinline__ Row row_of(const Place &p, int r, int rep, int cap, int window) {
+    Row x;
+    x.real = r < p.n * rep;
+    x.token = r / rep;
+    x.head = p.head * rep + (r - x.token * rep);
+    const int pos = p.kv - p.n + x.token;
+    x.lo = window <= pos ? pos - window + 1 : 0;
+    x.hi = x.real ? min(pos + 1, cap) : 0;
+    return x;
+}
+
+// The pages of a wave's 16-key groups, 64 at a time in the lanes of a register and
+// the next 64 in another, requested long before they are needed.
+struct PageRun {
+    int now, ahead;
+    // group: this lane's
+    static __device__ __forceinline__ int load(const AttendArgs &a, const int *table, int group, int hi) {
+        const int key = group * 16, at = key >> a.page_shift;
+        int p = -1;
+        if (key >= 0 && key < hi && at < a.b.pages_stride) p = table[at];   // (a number past the keys may wrap)
+        return p < a.n_pages ? p : -1;   // negative: none
+    }
+    __device__ __forceinline__ int get(int i) const { return __builtin_amdgcn_readlane(now, i); }
 };
 
 // 4 elements of a transposed block of LDS: lane i of 16 gives the address of

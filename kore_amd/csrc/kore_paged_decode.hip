@@ -10,55 +10,17 @@
 #include "kore_paged_attend.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace kore_paged_gpu {
 namespace {
 
 constexpr int kThreads = 256, kWaves = 4, kRows = 16;
 
-struct DecodeArgs {
-    AttendArgs a;
-    Cut cut;
-    ScaleLog2 sl;
-    float *part_o, *part_ml;
-};
-
-// What a lane knows of its row (column l % 16 of the products).
-struct Row {
-    int lo, hi;      // sees keys [lo, hi)
-    bool real;
-    int token, head;
-};
-
-__device__ __forceinline__ Row row_of(const Place &p, int r, int rep, int cap, int window) {
-    Row x;
-    x.real = r < p.n * rep;
-    x.token = r / rep;
-    x.head = p.head * rep + (r - x.token * rep);
-    const int pos = p.kv - p.n + x.token;
-    x.lo = window <= pos ? pos - window + 1 : 0;
-    x.hi = x.real ? min(pos + 1, cap) : 0;
-    return x;
-}
-
-// The pages of a wave's 16-key groups, 64 at a time in the lanes of a register and
-// the next 64 in another, requested long before they are needed.
-struct PageRun {
-    int now, ahead;
-    // group: this lane's
-    static __device__ __forceinline__ int load(const AttendArgs &a, const int *table, int group, int hi) {
-        const int key = group * 16, at = key >> a.page_shift;
-        int p = -1;
-        if (key >= 0 && key < hi && at < a.b.pages_stride) p = table[at];   // (a number past the keys may wrap)
-        return p < a.n_pages ? p : -1;   // negative: none
-    }
-    __device__ __forceinline__ int get(int i) const { return __builtin_amdgcn_readlane(now, i); }
-};
-
 // The four waves' states (ref, sum, and o as [dim / 4][row] float4) into out, or
 // into the split's partial.
 template <class A, int HDP>
-__device__ __forceinline__ void finish(const DecodeArgs &d, const Place &p, const float4 (*o)[HDP / 4][kRows],
+__device__ __forceinline__ void finish(const TileArgs &d, const Place &p, const float4 (*o)[HDP / 4][kRows],
                                        const float2 (*ml)[kRows]) {
     const AttendArgs &a = d.a;
     __syncthreads();
@@ -97,20 +59,6 @@ __device__ __forceinline__ void finish(const DecodeArgs &d, const Place &p, cons
     }
 }
 
-// A tile's rescale where a score passes the reference by kLag (or is the first).
-template <int N>
-__device__ __forceinline__ void follow(float top, float &ref, float &sum, float bias, floatx4 (&o)[N]) {
-    const bool moves = top - bias > ref + kLag || (ref == kNone && top > kNone);
-    if (__any(moves)) {
-        const float next = moves ? top - bias : ref;
-        const float f = moves ? exp2_(ref - next) : 1.f;
-        sum *= f;
-#pragma unroll
-        for (int i = 0; i < N; ++i) o[i] *= f;
-        ref = next;
-    }
-}
-
 // ---- 16-bit caches -----------------------------------------------------------
 //
 // A block is 32 keys.  S^T = K Q^T on 16x16x32 MFMA: lane (m, g) = (l % 16, l / 16)
@@ -121,7 +69,7 @@ __device__ __forceinline__ void follow(float top, float &ref, float &sum, float 
 // reads (rows padded by 32 bytes: the 8 rows that half a wave reads lie on different
 // banks).  No lane ever needs another's score but for the maximum and the sum.
 template <class A, class C, int HDP>
-__global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode16_kernel(DecodeArgs d) {
+__global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode16_kernel(TileArgs d) {
     constexpr int QP = Parts<A, C>::q, PP = Parts<A, C>::p;
     constexpr int KS = HDP / 32, DT = HDP / 16, VR = HDP / 16;   // k-steps, dim tiles, V registers of 16 bytes
     constexpr int kPitch = HDP + 16;                             // of a V row in LDS, elements
@@ -187,7 +135,7 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode16_kernel(
                 }
             }
     }
-    const float s_hi = d.sl.hi * unit, s_lo = d.sl.lo * unit;
+    const float s_hi = d.sl.hi * unit, s_lo = fmaxf(d.sl.lo * unit, 0x1p-126f);
 
     // A 16-key group lies in one page: a base that is the wave's, and a lane's offset
     // that does not change.  A group without a page reads page 0.
@@ -309,7 +257,7 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode16_kernel(
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float e = PP > 1 ? fmaf(s[m][i], s_hi, fmaf(s[m][i], s_lo, -base)) : fmaf(s[m][i], s_hi, -base);
-                const float x = s[m][i] == kNone ? 0.f : exp2_(e);
+                const float x = exp2_(e);
                 C part[PP];
                 split_p<PP>(x, part);
                 // one rounded weight is also what is summed: what rounding adds to all of a row's weights divides out
@@ -362,7 +310,7 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode16_kernel(
 // k.  The scores of keys 4 g + i are its k order of the second product, whose V
 // operand, lane (m, g): V[4 g + i][64 j + 4 m + e], comes straight from memory too.
 template <int HDP>
-__global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode32_kernel(DecodeArgs d) {
+__global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode32_kernel(TileArgs d) {
     constexpr int KU = HDP / 16, DJ = HDP / 64, kBlock = 16;
     __shared__ float4 states[kWaves][HDP / 4][kRows];
     __shared__ float2 ml[kWaves][kRows];
@@ -479,7 +427,7 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode32_kernel(
         float w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            w[i] = s[i] == kNone ? 0.f : exp2_(fmaf(s[i], d.sl.hi, fmaf(s[i], d.sl.lo, -base)));
+            w[i] = exp2_(fmaf(s[i], d.sl.hi, fmaf(s[i], d.sl.lo, -base)));
             sum += w[i];
         }
         if (!odd) {
@@ -529,7 +477,7 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode32_kernel(
 // over the splits, each its own running maximum, joined through LDS.  (Few tiles may
 // have hundreds of splits, so the dims are what there is to spread.)
 template <class A, int TILE>
-__global__ __launch_bounds__(kThreads) void merge_kernel(DecodeArgs d, int hd4) {
+__global__ __launch_bounds__(kThreads) void merge_kernel(TileArgs d, int hd4) {
     constexpr int kLanes = kThreads / TILE;
     __shared__ float4 so[kLanes][TILE];
     __shared__ float2 sm[kLanes][TILE];
@@ -578,56 +526,79 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(DecodeArgs d, int hd4) 
     store_n<4>(out, v, ((uintptr_t)out & (4 * sizeof(A) - 1)) == 0);
 }
 
-constexpr int kMinLen = 64;         // keys: a block for each of two waves
-constexpr int kPerCu = 2;           // workgroups that fit a CU
-constexpr int kMaxTiles = 1024;     // over this many (tile, kv-head)s nothing is split
+hipError_t launch_decode(const TileArgs &d, int places, hipStream_t s) {
+    const int hdp = padded_dim(d.a.hd);
+    const dim3 grid((unsigned)places);
+#define KORE_DECODE(...)                                                 \
+    do {                                                                 \
+        if (hdp == 64) KORE_DECODE_(64, __VA_ARGS__);                    \
+        else if (hdp == 128) KORE_DECODE_(128, __VA_ARGS__);             \
+        else KORE_DECODE_(256, __VA_ARGS__);                             \
+    } while (0)
+#define KORE_DECODE_(H, A, C) decode16_kernel<A, C, H><<<grid, kThreads, 0, s>>>(d)
+    if (d.a.cache_type == kF32) {
+        if (hdp == 64) decode32_kernel<64><<<grid, kThreads, 0, s>>>(d);
+        else if (hdp == 128) decode32_kernel<128><<<grid, kThreads, 0, s>>>(d);
+        else decode32_kernel<256><<<grid, kThreads, 0, s>>>(d);
+    } else if (d.a.type == kF32 && d.a.cache_type == kF16) KORE_DECODE(float, half_t);
+    else if (d.a.type == kF32) KORE_DECODE(float, bhalf_t);
+    else if (d.a.type == kF16) KORE_DECODE(half_t, half_t);
+    else KORE_DECODE(bhalf_t, bhalf_t);
+#undef KORE_DECODE_
+#undef KORE_DECODE
+    return hipGetLastError();
+}
 
-int padded_dim(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
+constexpr int kMinLen = 64, kChunkMinLen = 256;   // a split's fewest keys
+constexpr int kPerCu = 2;                           // workgroups of a CU
+constexpr int kMaxTiles = 1024;                     // over this many (tile, kv-head)s of 16 rows nothing is split
+
+int chunk_places(int hd, int num_cu) { return (hd <= 128 ? 2 : 1) * num_cu; }
 
 }  // namespace
 
 size_t attend_workspace_bytes(int n_head, int n_head_kv, int hd, int num_cu) {
-    const size_t places = (size_t)kMaxTiles + (size_t)kPerCu * num_cu;
-    return places * kRows * ((size_t)padded_dim(hd) + 2) * sizeof(float);
+    const size_t rows = ((size_t)kMaxTiles + (size_t)kPerCu * num_cu) * kRows, chunk_rows = (size_t)chunk_places(hd, num_cu) * kChunkRows;
+    return std::max(rows, chunk_rows) * ((size_t)padded_dim(hd) + 2) * sizeof(float);
 }
 
 hipError_t launch_attend(const AttendArgs &a, hipStream_t s) {
-    DecodeArgs d{};
+    TileArgs d{};
     d.a = a;
     d.cut.rep = a.n_head / a.n_head_kv;
-    const long long tiles = ((long long)a.b.n_tok * d.cut.rep / kRows + std::min(a.b.n_seq, a.b.n_tok)) * a.n_head_kv;
-    const int places = kPerCu * a.num_cu;
-    d.cut.target = tiles > kMaxTiles ? 0 : (int)std::max<long long>(places - tiles, places / 2);
-    d.cut.min_len = kMinLen;
+    const int max_q = a.max_q ? a.max_q : (a.b.n_tok + a.b.n_seq - 1) / a.b.n_seq;
+    const bool chunk = (long long)max_q * d.cut.rep > kRows;
+    const int rows = chunk ? kChunkRows : kRows;
+    // the most (tile, kv-head)s that n_tok rows of n_seq sequences can be
+    const long long tiles = ((long long)a.b.n_tok * d.cut.rep / rows + std::min(a.b.n_seq, a.b.n_tok)) * a.n_head_kv;
+    if (chunk) {
+        const int places = chunk_places(a.hd, a.num_cu);
+        d.cut.target = 4 * tiles > 3 * places ? 0 : (int)(places - tiles);
+        d.cut.min_len = kChunkMinLen;
+    } else {
+        const int places = kPerCu * a.num_cu;
+        d.cut.target = tiles > kMaxTiles ? 0 : (int)std::max<long long>(places - tiles, places / 2);
+        d.cut.min_len = kMinLen;
+    }
     const double sl = (double)a.scale * 1.4426950408889634074;
-    d.sl.hi = (float)sl;
+    d.sl.hi = std::nextafter((float)sl, 0.f);
     d.sl.lo = (float)(sl - (double)d.sl.hi);
     const int hdp = padded_dim(a.hd);
     d.part_o = a.part;
-    d.part_ml = a.part + (size_t)(tiles + d.cut.target) * kRows * hdp;
-    const dim3 grid((unsigned)(tiles + d.cut.target));
-#define KORE_DIMS(LAUNCH)            \
-    do {                             \
-        if (hdp == 64) LAUNCH(64);   \
-        else if (hdp == 128) LAUNCH(128); \
-        else LAUNCH(256);            \
-    } while (0)
-#define KORE_FF(H) decode32_kernel<H><<<grid, kThreads, 0, s>>>(d)
-#define KORE_FH(H) decode16_kernel<float, half_t, H><<<grid, kThreads, 0, s>>>(d)
-#define KORE_FB(H) decode16_kernel<float, bhalf_t, H><<<grid, kThreads, 0, s>>>(d)
-#define KORE_HH(H) decode16_kernel<half_t, half_t, H><<<grid, kThreads, 0, s>>>(d)
-#define KORE_BB(H) decode16_kernel<bhalf_t, bhalf_t, H><<<grid, kThreads, 0, s>>>(d)
-    if (a.cache_type == kF32) KORE_DIMS(KORE_FF);
-    else if (a.type == kF32 && a.cache_type == kF16) KORE_DIMS(KORE_FH);
-    else if (a.type == kF32) KORE_DIMS(KORE_FB);
-    else if (a.type == kF16) KORE_DIMS(KORE_HH);
-    else KORE_DIMS(KORE_BB);
-    hipError_t e = hipGetLastError();
+    d.part_ml = a.part + (size_t)(tiles + d.cut.target) * rows * hdp;
+    const unsigned places = (unsigned)(tiles + d.cut.target);
+    const hipError_t e = chunk ? launch_chunk(d, (int)places, s) : launch_decode(d, (int)places, s);
     if (e != hipSuccess || !d.cut.target) return e;
     const dim3 merge((unsigned)tiles, (unsigned)(a.hd / 4));
-    if (a.type == kF32) merge_kernel<float, kRows><<<merge, kThreads, 0, s>>>(d, hdp / 4);
-    else if (a.type == kF16) merge_kernel<half_t, kRows><<<merge, kThreads, 0, s>>>(d, hdp / 4);
-    else merge_kernel<bhalf_t, kRows><<<merge, kThreads, 0, s>>>(d, hdp / 4);
+#define KORE_MERGE(A)                                                                    \
+    do {                                                                                 \
+        if (chunk) merge_kernel<A, kChunkRows><<<merge, kThreads, 0, s>>>(d, hdp / 4);   \
+        else merge_kernel<A, kRows><<<merge, kThreads, 0, s>>>(d, hdp / 4);              \
+    } while (0)
+    if (a.type == kF32) KORE_MERGE(float);
+    else if (a.type == kF16) KORE_MERGE(half_t);
+    else KORE_MERGE(bhalf_t);
+#undef KORE_MERGE
     return hipGetLastError();
 }
 
