@@ -84,6 +84,26 @@ __device__ __forceinline__ float sum32(float x) {
 }
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// The sum of eight weights, two an instruction, onto s (products with 1: exact; one
+// rounding each).
+__device__ __forceinline__ float sum_weights(half8 w, float s) {
+    typedef half_t half2_t __attribute__((ext_vector_type(2)));
+    const half2_t one = {(half_t)1.f, (half_t)1.f};
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) s = __builtin_amdgcn_fdot2(half2_t{w[i], w[i + 1]}, one, s, false);
+    return s;
+}
+__device__ __forceinline__ float sum_weights(bhalf8 w, float s) {
+    typedef bhalf_t bhalf2_t __attribute__((ext_vector_type(2)));
+    const bhalf2_t one = {(bhalf_t)1.f, (bhalf_t)1.f};
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) s = __builtin_amdgcn_fdot2_f32_bf16(bhalf2_t{w[i], w[i + 1]}, one, s, false);
+    return s;
+}
+
+// A value that is equal in all lanes, in a scalar register.
+__device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 // ---- the cut -----------------------------------------------------------------
 
 // A sequence's share of the cut.
@@ -158,19 +178,19 @@ __device__ __forceinline__ bool place_of(const Batch &b, const Cut &c, int id, i
         if (past) {
             const int l = __builtin_ctzll(past);
             const auto of = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
-            p.seq = s0 + l;
+            p.seq = scalar(s0 + l);
             p.n_split = of(n_split);
             p.q0 = of(q0);
             p.n = of(n);
             p.kv = of(kv);
-            p.len = len;
+            p.len = scalar(len);
             int i = id - at - of(upto) + of(mine);
-            p.head = i % nkv;
-            i /= nkv;
-            p.split = by_tile ? 0 : i % p.n_split;
-            if (!by_tile) i /= p.n_split;
-            p.tile = of(r.tiles) - 1 - i;
-            p.first = splits_at + of(splits_upto) - of(all) + i * p.n_split * nkv + p.head;
+            p.head = scalar(i % nkv);
+            i = scalar(i / nkv);
+            p.split = by_tile ? 0 : scalar(i % p.n_split);
+            if (!by_tile) i = scalar(i / p.n_split);
+            p.tile = scalar(of(r.tiles) - 1 - i);
+            p.first = scalar(splits_at + of(splits_upto) - of(all) + i * p.n_split * nkv + p.head);
             return true;
         }
         at += __builtin_amdgcn_readlane(upto, 63);
@@ -187,7 +207,7 @@ struct Keys {
 
 template <int TILE>
 __device__ __forceinline__ Keys keys_of(const Place &p, int rep, int cap, int window) {
-    const int t0 = p.tile * TILE / rep, t1 = min(p.n - 1, (p.tile * TILE + TILE - 1) / rep);
+    const int t0 = scalar(p.tile * TILE / rep), t1 = min(p.n - 1, scalar((p.tile * TILE + TILE - 1) / rep));
     const int p0 = p.kv - p.n + t0, p1 = p.kv - p.n + t1;   // positions of the first and last row
     Keys k;
     const int first = window <= p0 ? (p0 - window + 1) & ~63 : 0, end = min(p1 + 1, cap);
@@ -198,8 +218,10 @@ __device__ __forceinline__ Keys keys_of(const Place &p, int rep, int cap, int wi
         k.lo = (int)min(a, (long long)INT_MAX - 64);
         k.hi = (int)min(z, (long long)end);
     }
-    k.all_lo = window <= p1 ? p1 - window + 1 : 0;
-    k.all_hi = min(p0 + 1, cap);
+    k.lo = scalar(k.lo);
+    k.hi = scalar(k.hi);
+    k.all_lo = scalar(window <= p1 ? p1 - window + 1 : 0);
+    k.all_hi = scalar(min(p0 + 1, cap));
     return k;
 }
 

@@ -73,11 +73,15 @@ __global__ __launch_bounds__(kThreads, (Shape<A, S, HDP>::per_cu)) void chunk_ke
     int see_lo, see_hi, all_lo, all_hi;
     {
         const int r0 = p.tile * kRows + wave * 32, r1 = min(r0 + 31, p.n * rep - 1);
-        const int p0 = p.kv - p.n + r0 / rep, p1 = p.kv - p.n + max(r1, 0) / rep;
+        const int p0 = p.kv - p.n + scalar(r0 / rep), p1 = p.kv - p.n + scalar(max(r1, 0) / rep);
         see_lo = a.window <= p0 ? p0 - a.window + 1 : 0;
         see_hi = r0 <= r1 ? min(p1 + 1, k.hi) : 0;
         all_lo = a.window <= p1 ? p1 - a.window + 1 : 0;
         all_hi = min(p0 + 1, k.hi);
+        see_lo = scalar(see_lo);
+        see_hi = scalar(see_hi);
+        all_lo = scalar(all_lo);
+        all_hi = scalar(all_hi);
     }
 
     const int n_step = k.lo < k.hi ? (k.hi - k.lo + kKeys - 1) / kKeys : 0;
@@ -127,7 +131,7 @@ __global__ __launch_bounds__(kThreads, (Shape<A, S, HDP>::per_cu)) void chunk_ke
 
     // A thread's share of a step: pieces of 8 dims, kWaveRows rows of a wave side by side
     const int my_row = lane / kPieces, my_dim = 8 * (lane % kPieces);
-    const int off = my_row * a.hd + (padded ? min(my_dim, a.hd - 8) : my_dim);
+    const unsigned off = my_row * a.hd + (padded ? min(my_dim, a.hd - 8) : my_dim);
     const bool no_dim = padded && my_dim >= a.hd;
     raw8 kr[kLoads], vr[kLoads];
     int loaded = 0;                      // step whose K and V are in flight
@@ -246,6 +250,15 @@ __global__ __launch_bounds__(kThreads, (Shape<A, S, HDP>::per_cu)) void chunk_ke
                             if (KP == 1 || y + z < KP) s[m] = Mma<C>::mul32(x, q[z][t], s[m]);
                     }
             }
+            // K's operands are requested kAhead products early
+            constexpr int kReads = MT * KS * KP, kAhead = 6, kPer = KP == 3 ? 2 : QP;
+            __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+            for (int i = 0; i < kReads - kAhead; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, kPer, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, kAhead * kPer, 0);
         }
         if (kBuffers == 2 && step + 1 < n_step) {
             store(buffer ^ 1);
@@ -279,11 +292,15 @@ __global__ __launch_bounds__(kThreads, (Shape<A, S, HDP>::per_cu)) void chunk_ke
                     const float x = exp2_(e);
                     C part[PP];
                     split_p<PP>(x, part);
-                    // one rounded weight is also what is summed: what rounding adds to all of a row's weights divides out
-                    part_sum += PP > 1 ? x : to_f32(part[0]);
+                    if (PP > 1) part_sum += x;
 #pragma unroll
                     for (int y = 0; y < PP; ++y) w[m][i / 8][y][i % 8] = part[y];
                 }
+            // one rounded weight is also what is summed: what rounding adds to all of a row's weights divides out
+            if constexpr (PP == 1) {
+#pragma unroll
+                for (int m = 0; m < MT; ++m) part_sum = sum_weights(w[m][1][0], sum_weights(w[m][0][0], part_sum));
+            }
             sum += part_sum;
             // O^T += V^T P^T, k order as the scores came: V^T's operand, lane (m, half), has keys 16 t + 4 half + 0..3 and
             // those 8 further of dim 32 i + m

@@ -144,10 +144,10 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode16_kernel(
     };
     constexpr int kPerRow = HDP / 8, kRowsPer = 64 / kPerRow;   // 16-byte pieces of a V row; rows a load covers
     const int v_row = lane / kPerRow, v_dim = 8 * (lane % kPerRow);
-    int k_off[KS];
+    unsigned k_off[KS];
 #pragma unroll
     for (int t = 0; t < KS; ++t) k_off[t] = col * a.hd + (padded ? min(32 * t + 8 * g, a.hd - 8) : 32 * t + 8 * g);
-    const int v_off = v_row * a.hd + (padded ? min(v_dim, a.hd - 8) : v_dim);
+    const unsigned v_off = v_row * a.hd + (padded ? min(v_dim, a.hd - 8) : v_dim);
     vec8 kr[2][KS], vr[VR];
     int p0 = 0, p1 = 0;   // pages of the block whose K and V are in flight
     const auto load_k = [&](int key0) {
@@ -348,7 +348,7 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode32_kernel(
     const auto base_of = [&](const void *pool, int page, int key) {
         return (const float *)pool + ((((size_t)max(page, 0) * a.n_head_kv + p.head) << a.page_shift) + (key & slot_mask)) * a.hd;
     };
-    int k_off[KU], v_off[DJ];
+    unsigned k_off[KU], v_off[DJ];
 #pragma unroll
     for (int u = 0; u < KU; ++u) k_off[u] = col * a.hd + (padded ? min(16 * u + 4 * g, a.hd - 4) : 16 * u + 4 * g);
 #pragma unroll
