@@ -20,6 +20,7 @@ struct Cut {
     int rep;         // q-heads of a kv-head
     int target;      // workgroups to aim at, in tiles x keys; 0: nothing is split
     int min_len;     // a split's fewest keys
+    int fold;        // places from this number on are taken from the last; 0: in order
 };
 
 // exp(scale q.k) = 2^(dot * (hi + lo)), hi + lo = scale log2(e) to 47 bits, both over
@@ -133,14 +134,25 @@ struct Place {
     int first;          // number of the tile's first split among the launch's places
 };
 
-__device__ __forceinline__ int prefix_sum(int x) {   // inclusive, over the wave
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int y = __shfl_up(x, d);
-        if (lane >= d) x += y;
-    }
+// Inclusive sums over the wave in six DPP steps (four within rows of 16, then from
+// row to row); the last lane's is the whole.
+template <class T, int CTRL, int ROWS>
+__device__ __forceinline__ T from_lane(T x) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, ROWS, 0xf, false));
+}
+template <class T>
+__device__ __forceinline__ T prefix_sum(T x) {
+    x += from_lane<T, 0x111, 0xf>(x);
+    x += from_lane<T, 0x112, 0xf>(x);
+    x += from_lane<T, 0x114, 0xf>(x);
+    x += from_lane<T, 0x118, 0xf>(x);
+    x += from_lane<T, 0x142, 0xa>(x);
+    x += from_lane<T, 0x143, 0xc>(x);
     return x;
+}
+template <class T>
+__device__ __forceinline__ T last_lane(T x) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
 }
 
 // The place of number `id`, false where there is none.  Numbers run over the
@@ -161,9 +173,7 @@ __device__ __forceinline__ bool place_of(const Batch &b, const Cut &c, int id, i
             const Share r = s < b.n_seq ? share_of<TILE>(b, s, c.rep, cap, window, q0, n, kv) : Share{0, 0};
             w += (float)r.tiles * (float)r.keys;
         }
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) w += __shfl_xor(w, d);
-        const float each = ceilf(w * (float)nkv / (float)c.target);
+        const float each = ceilf(last_lane(prefix_sum(w)) * (float)nkv / (float)c.target);
         len = max(c.min_len, ((int)fminf(each, 1e9f) + 63) & ~63);
     }
     int at = 0, splits_at = 0;
@@ -174,6 +184,10 @@ __device__ __forceinline__ bool place_of(const Batch &b, const Cut &c, int id, i
         const int n_split = max(1, r.keys / len + (r.keys % len != 0));
         const int all = r.tiles * n_split * nkv, mine = by_tile ? r.tiles * nkv : all;
         const int upto = prefix_sum(mine), splits_upto = by_tile ? prefix_sum(all) : upto;
+        if (c.fold && s0 == 0 && b.n_seq <= 64 && id >= c.fold) {
+            id = last_lane(upto) - 1 - (id - c.fold);
+            if (id < c.fold) return false;
+        }
         const unsigned long long past = __ballot(at + upto > id);
         if (past) {
             const int l = __builtin_ctzll(past);
@@ -193,8 +207,8 @@ __device__ __forceinline__ bool place_of(const Batch &b, const Cut &c, int id, i
             p.first = scalar(splits_at + of(splits_upto) - of(all) + i * p.n_split * nkv + p.head);
             return true;
         }
-        at += __builtin_amdgcn_readlane(upto, 63);
-        splits_at += __builtin_amdgcn_readlane(splits_upto, 63);
+        at += last_lane(upto);
+        splits_at += last_lane(splits_upto);
     }
     return false;
 }

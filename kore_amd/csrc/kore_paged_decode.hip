@@ -473,57 +473,81 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode32_kernel(
 
 // ---- the merge of splits ---------------------------------------------------------
 //
-// A workgroup takes four dims of a tile and kv-head: TILE rows by 256 / TILE lanes
-// over the splits, each its own running maximum, joined through LDS.  (Few tiles may
-// have hundreds of splits, so the dims are what there is to spread.)
+// TILE rows by 256 / TILE lanes, which are laid over the tile's splits and, what is left
+// of them, over the dims, four a lane.  A lane has eight splits' loads in flight and a
+// running reference; the lanes' states meet in LDS.  gridDim.y workgroups share a
+// tile's dims.  (Few tiles may have hundreds of splits, many tiles two each.)
 template <class A, int TILE>
 __global__ __launch_bounds__(kThreads) void merge_kernel(TileArgs d, int hd4) {
-    constexpr int kLanes = kThreads / TILE;
+    constexpr int kLanes = kThreads / TILE, kFlight = 8;
     __shared__ float4 so[kLanes][TILE];
     __shared__ float2 sm[kLanes][TILE];
     const AttendArgs &a = d.a;
-    const int cap = a.b.pages_stride << a.page_shift, d4 = blockIdx.y;
+    const int cap = a.b.pages_stride << a.page_shift;
     Place p;
     if (!place_of<TILE>(a.b, d.cut, blockIdx.x, a.n_head_kv, cap, a.window, true, p) || p.n_split <= 1) return;
-    const int row = threadIdx.x % TILE, part = threadIdx.x / TILE;
-    const float4 *po = reinterpret_cast<const float4 *>(d.part_o);
-    const float2 *pm = reinterpret_cast<const float2 *>(d.part_ml);
-    float m = kNone, l = 0;
-    float4 s = make_float4(0, 0, 0, 0);
-#pragma unroll 4
-    for (int i = part; i < p.n_split; i += kLanes) {
-        const size_t id = (size_t)p.first + (size_t)i * a.n_head_kv;
-        const float2 e = pm[id * TILE + row];
-        const float4 v = po[(id * hd4 + d4) * TILE + row];
-        const float next = fmaxf(m, e.x), base = next == kNone ? 0.f : next;
-        const float f = exp2_(m - base), h = exp2_(e.x - base);
-        l = fmaf(e.y, h, l * f);
-        s = make_float4(fmaf(v.x, h, s.x * f), fmaf(v.y, h, s.y * f), fmaf(v.z, h, s.z * f), fmaf(v.w, h, s.w * f));
-        m = next;
-    }
-    so[part][row] = s;
-    sm[part][row] = make_float2(m, l);
-    __syncthreads();
-    const int r = p.tile * TILE + row;
-    if (part != 0 || r >= p.n * d.cut.rep) return;
+    int parts = 1;
+    while (parts < kLanes && parts < p.n_split) parts *= 2;
+    const int row = threadIdx.x % TILE, lane = threadIdx.x / TILE, part = lane & (parts - 1), wide = kLanes / parts;
+    const size_t step = (size_t)a.n_head_kv * TILE;
+    const float2 *const pm = reinterpret_cast<const float2 *>(d.part_ml) + (size_t)p.first * TILE + row;
+    const int r = p.tile * TILE + row, token = r / d.cut.rep, head = p.head * d.cut.rep + r - token * d.cut.rep;
+    A *const out = (A *)a.out + (size_t)(p.q0 + token) * a.out_stride + (size_t)head * a.hd;
+    const bool vec = ((uintptr_t)out & (4 * sizeof(A) - 1)) == 0;
+    for (int d0 = blockIdx.y * wide; 4 * d0 < a.hd; d0 += gridDim.y * wide) {
+        const int d4 = d0 + lane / parts;
+        const bool real = 4 * d4 < a.hd;
+        const float4 *const po = reinterpret_cast<const float4 *>(d.part_o) + ((size_t)p.first * hd4 + d4) * TILE + row;
+        float m = kNone, l = 0;
+        float4 s = make_float4(0, 0, 0, 0);
+        for (int i = part; real && i < p.n_split; i += kFlight * parts) {
+            float2 e[kFlight];
+            float4 v[kFlight];
 #pragma unroll
-    for (int i = 1; i < kLanes; ++i) m = fmaxf(m, sm[i][row].x);
-    const float base = m == kNone ? 0.f : m;
-    l = 0;
-    s = make_float4(0, 0, 0, 0);
+            for (int x = 0; x < kFlight; ++x) {
+                const int n = i + x * parts;
+                e[x] = make_float2(kNone, 0.f);
+                v[x] = make_float4(0, 0, 0, 0);
+                if (n < p.n_split) {
+                    e[x] = pm[n * step];
+                    v[x] = po[n * step * hd4];
+                }
+            }
+            float next = m;
 #pragma unroll
-    for (int i = 0; i < kLanes; ++i) {
-        const float2 e = sm[i][row];
-        const float4 v = so[i][row];
-        const float f = exp2_(e.x - base);
-        l = fmaf(e.y, f, l);
-        s = make_float4(fmaf(v.x, f, s.x), fmaf(v.y, f, s.y), fmaf(v.z, f, s.z), fmaf(v.w, f, s.w));
+            for (int x = 0; x < kFlight; ++x) next = fmaxf(next, e[x].x);
+            const float base = next == kNone ? 0.f : next, f = exp2_(m - base);
+            l *= f;
+            s = make_float4(s.x * f, s.y * f, s.z * f, s.w * f);
+#pragma unroll
+            for (int x = 0; x < kFlight; ++x) {
+                const float g = exp2_(e[x].x - base);
+                l = fmaf(e[x].y, g, l);
+                s = make_float4(fmaf(v[x].x, g, s.x), fmaf(v[x].y, g, s.y), fmaf(v[x].z, g, s.z), fmaf(v[x].w, g, s.w));
+            }
+            m = next;
+        }
+        so[lane][row] = s;
+        sm[lane][row] = make_float2(m, l);
+        __syncthreads();
+        if (real && part == 0 && r < p.n * d.cut.rep) {
+            for (int i = 1; i < parts; ++i) m = fmaxf(m, sm[lane + i][row].x);
+            const float base = m == kNone ? 0.f : m;
+            l = 0;
+            s = make_float4(0, 0, 0, 0);
+            for (int i = 0; i < parts; ++i) {
+                const float2 e = sm[lane + i][row];
+                const float4 v = so[lane + i][row];
+                const float g = exp2_(e.x - base);
+                l = fmaf(e.y, g, l);
+                s = make_float4(fmaf(v.x, g, s.x), fmaf(v.y, g, s.y), fmaf(v.z, g, s.z), fmaf(v.w, g, s.w));
+            }
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const A w[4] = {(A)(s.x * inv), (A)(s.y * inv), (A)(s.z * inv), (A)(s.w * inv)};
+            store_n<4>(out + 4 * d4, w, vec);
+        }
+        __syncthreads();
     }
-    const int token = r / d.cut.rep, head = p.head * d.cut.rep + r - token * d.cut.rep;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    A *out = (A *)a.out + (size_t)(p.q0 + token) * a.out_stride + (size_t)head * a.hd + 4 * d4;
-    const A v[4] = {(A)(s.x * inv), (A)(s.y * inv), (A)(s.z * inv), (A)(s.w * inv)};
-    store_n<4>(out, v, ((uintptr_t)out & (4 * sizeof(A) - 1)) == 0);
 }
 
 hipError_t launch_decode(const TileArgs &d, int places, hipStream_t s) {
@@ -575,6 +599,7 @@ hipError_t launch_attend(const AttendArgs &a, hipStream_t s) {
         const int places = chunk_places(a.hd, a.num_cu);
         d.cut.target = 4 * tiles > 3 * places ? 0 : (int)(places - tiles);
         d.cut.min_len = kChunkMinLen;
+        if (!d.cut.target) d.cut.fold = a.num_cu;
     } else {
         const int places = kPerCu * a.num_cu;
         d.cut.target = tiles > kMaxTiles ? 0 : (int)std::max<long long>(places - tiles, places / 2);
@@ -589,7 +614,8 @@ hipError_t launch_attend(const AttendArgs &a, hipStream_t s) {
     const unsigned places = (unsigned)(tiles + d.cut.target);
     const hipError_t e = chunk ? launch_chunk(d, (int)places, s) : launch_decode(d, (int)places, s);
     if (e != hipSuccess || !d.cut.target) return e;
-    const dim3 merge((unsigned)tiles, (unsigned)(a.hd / 4));
+    // some four workgroups a CU, where there are dims enough
+    const dim3 merge((unsigned)tiles, (unsigned)std::clamp<long long>(8 * a.num_cu / tiles, 1, a.hd / 4));
 #define KORE_MERGE(A)                                                                    \
     do {                                                                                 \
         if (chunk) merge_kernel<A, kChunkRows><<<merge, kThreads, 0, s>>>(d, hdp / 4);   \
