@@ -340,6 +340,8 @@ int kore_paged_create(kore_paged_t *out, const kore_paged_config *cfg) {
     if (c.head_dim % 8 != 0 || c.head_dim > kMaxHeadDim)
         return FAIL0(KORE_PAGED_E_UNSUPPORTED, "no gfx950 kernel for head_dim %d (supported: multiples of 8 up to %d)",
                      c.head_dim, kMaxHeadDim);
+    if ((double)c.n_head_kv * c.page_size * c.head_dim * type_bytes(c.cache_type) >= 4294967296.0)
+        return FAIL0(KORE_PAGED_E_UNSUPPORTED, "a page of one layer takes 4 GiB or more");
     if (c.n_head > 1 << 16) return FAIL0(KORE_PAGED_E_UNSUPPORTED, "n_head %d is too large", c.n_head);
     if ((c.k_pool == nullptr) != (c.v_pool == nullptr)) return FAIL0(KORE_PAGED_E_INVALID, "one pool of two is given");
     if ((uintptr_t)c.k_pool % 16 || (uintptr_t)c.v_pool % 16)

@@ -20,7 +20,6 @@ struct Cut {
     int rep;         // q-heads of a kv-head
     int target;      // workgroups to aim at, in tiles x keys; 0: nothing is split
     int min_len;     // a split's fewest keys
-    int fold;        // places from this number on are taken from the last; 0: in order
 };
 
 // exp(scale q.k) = 2^(dot * (hi + lo)), hi + lo = scale log2(e) to 47 bits, both over
@@ -184,10 +183,6 @@ __device__ __forceinline__ bool place_of(const Batch &b, const Cut &c, int id, i
         const int n_split = max(1, r.keys / len + (r.keys % len != 0));
         const int all = r.tiles * n_split * nkv, mine = by_tile ? r.tiles * nkv : all;
         const int upto = prefix_sum(mine), splits_upto = by_tile ? prefix_sum(all) : upto;
-        if (c.fold && s0 == 0 && b.n_seq <= 64 && id >= c.fold) {
-            id = last_lane(upto) - 1 - (id - c.fold);
-            if (id < c.fold) return false;
-        }
         const unsigned long long past = __ballot(at + upto > id);
         if (past) {
             const int l = __builtin_ctzll(past);
@@ -197,7 +192,8 @@ __device__ __forceinline__ bool place_of(const Batch &b, const Cut &c, int id, i
             p.q0 = of(q0);
             p.n = of(n);
             p.kv = of(kv);
-            p.len = scalar(len);
+            // the sequence's splits of equal length, in whole steps of 64 keys
+            p.len = scalar(((of(r.keys) + p.n_split - 1) / p.n_split + 63) & ~63);
             int i = id - at - of(upto) + of(mine);
             p.head = scalar(i % nkv);
             i = scalar(i / nkv);

@@ -3,13 +3,18 @@
 // A tile is 128 rows of a kv-head's (token, q-head) list, 32 for each of four waves,
 // and passes over its keys 64 (or 32) at a time through LDS: the flops of a key,
 // 512 head_dim for its 4 head_dim bytes, put the kernel between the matrix cores and
-// the vector units that make the weights.
+// the vector units that make the weights.  Two such teams of waves share a CU as one
+// workgroup, each with every other step of the keys, and join their sums through LDS at
+// the end: what a step waits for is a wave's own chain of loads, products and weights,
+// so a tile takes half as long as with one team, and the long tiles of a causal chunk
+// are what the launch waits for (7B, 2048 rows: 56 us with the same waves in two
+// workgroups of four).
 #include "kore_paged_attend.h"
 
 namespace kore_paged_gpu {
 namespace {
 
-constexpr int kThreads = 256, kWaves = 4, kRows = kChunkRows;
+constexpr int kWaves = 4, kRows = kChunkRows;   // of a team
 
 // How a (row type, cache type) is computed: fp32 caches in three bf16 parts of
 // everything, whose products of parts i and j with i + j < 3 hold 24 bits.
@@ -22,13 +27,13 @@ template <> struct Form<float, float> {
     static constexpr int qp = 3, kp = 3, pp = 3;
 };
 
-// What a tile's shape asks of LDS and registers: keys of a step; buffers; workgroups
-// of a CU.
+// What a tile's shape asks of LDS and registers: keys of a step; buffers; teams of a
+// workgroup (a CU holds one workgroup).
 template <class A, class S, int HDP> struct Shape {
     static constexpr bool parts = Form<A, S>::qp > 1;
     static constexpr int keys = parts ? 32 : 64;
     static constexpr int buffers = HDP <= 128 && Form<A, S>::kp == 1 ? 2 : 1;
-    static constexpr int per_cu = HDP <= 128 ? 2 : 1;
+    static constexpr int teams = HDP <= 128 ? 2 : 1, threads = 64 * kWaves * teams;
 };
 
 // Three bf16 parts of an fp32 value of the cache; an infinity or NaN is all in the first.
@@ -41,25 +46,31 @@ __device__ __forceinline__ void split_kv(float x, bhalf_t (&part)[3]) {
 }
 
 template <class A, class S, int HDP>
-__global__ __launch_bounds__(kThreads, (Shape<A, S, HDP>::per_cu)) void chunk_kernel(TileArgs d) {
+__global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(TileArgs d) {
     typedef typename Form<A, S>::C C;
     typedef typename Mma<C>::vec8 vec8;
     typedef C vec4 __attribute__((ext_vector_type(4)));
     constexpr int QP = Form<A, S>::qp, KP = Form<A, S>::kp, PP = Form<A, S>::pp;
-    constexpr int kKeys = Shape<A, S, HDP>::keys, kBuffers = Shape<A, S, HDP>::buffers;
+    constexpr int kKeys = Shape<A, S, HDP>::keys, kBuffers = Shape<A, S, HDP>::buffers, kTeams = Shape<A, S, HDP>::teams;
     constexpr int KS = HDP / 16, DT = HDP / 32, MT = kKeys / 32;         // k-steps, dim tiles, key tiles
     // Rows of LDS: 16 rows' 16-byte pieces of K, and four rows' 64 bytes of V, lie on
     // different banks
     constexpr int kKPitch = HDP + 8, kVPitch = HDP + 32, kPlane = kKeys * (kKPitch + kVPitch);
     constexpr int kPieces = HDP / 8, kWaveRows = 64 / kPieces, kStepRows = kWaves * kWaveRows, kLoads = kKeys / kStepRows;
     typedef S raw8 __attribute__((ext_vector_type(8)));
-    __shared__ __attribute__((aligned(16))) C tile[kBuffers][KP * kPlane];
+    __shared__ __attribute__((aligned(16))) C tiles[kTeams][kBuffers][KP * kPlane];
     // of V's pieces in steps that the tile's rows do not all see: which of 8 dims are +inf, or -inf (a NaN: both)
-    __shared__ unsigned kinds[kBuffers][2][kKeys][HDP / 32];
-    __shared__ int odd_of[kBuffers][kWaves];
+    __shared__ unsigned all_kinds[kTeams][kBuffers][2][kKeys][HDP / 32];
+    __shared__ int all_odd[kTeams][kBuffers][kWaves];
+    __shared__ float2 team_ml[kWaves][32];   // (reference, sum) of the second team's rows
+    static_assert(kTeams == 1 || sizeof tiles >= kWaves * (HDP / 2) * 64 * sizeof(float), "the teams' sums meet in the tiles' place");
     const AttendArgs &a = d.a;
     const int rep = d.cut.rep;
-    const int cap = a.b.pages_stride << a.page_shift, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int cap = a.b.pages_stride << a.page_shift, lane = threadIdx.x & 63;
+    const int wave = scalar(threadIdx.x >> 6) % kWaves, team = scalar(threadIdx.x >> 6) / kWaves;
+    auto &tile = tiles[team];
+    auto &kinds = all_kinds[team];
+    auto &odd_of = all_odd[team];
     Place p;
     if (!place_of<kRows>(a.b, d.cut, blockIdx.x, a.n_head_kv, cap, a.window, false, p)) return;
     const Keys k = keys_of<kRows>(p, rep, cap, a.window);
@@ -84,13 +95,18 @@ __global__ __launch_bounds__(kThreads, (Shape<A, S, HDP>::per_cu)) void chunk_ke
         all_hi = scalar(all_hi);
     }
 
-    const int n_step = k.lo < k.hi ? (k.hi - k.lo + kKeys - 1) / kKeys : 0;
+    // The team's steps are number team, team + kTeams, ... of the keys; a workgroup runs as many of both
+    const int all_steps = k.lo < k.hi ? (k.hi - k.lo + kKeys - 1) / kKeys : 0;
+    const int n_run = (all_steps + kTeams - 1) / kTeams, n_step = (all_steps - team + kTeams - 1) / kTeams;
     constexpr int kGroups = kKeys / 16;
-    // group i of the keys is lane i % 64
-    const auto pages_from = [&](int group) { return PageRun::load(a, table, k.lo / 16 + group + lane, k.hi); };
+    const auto key_of = [&](int step) { return k.lo + (step * kTeams + team) * kKeys; };
+    // 16-key group i of the steps' keys is lane i % 64
+    const auto pages_from = [&](int step) {
+        return PageRun::load(a, table, key_of(step + lane / kGroups) / 16 + lane % kGroups, k.hi);
+    };
     PageRun run;
     run.now = pages_from(0);
-    run.ahead = pages_from(64);
+    run.ahead = pages_from(64 / kGroups);
 
     // Q: B operand, lane (n, half) has dims 16 t + 8 half .. + 7 of its row
     vec8 q[QP][KS];
@@ -131,35 +147,52 @@ __global__ __launch_bounds__(kThreads, (Shape<A, S, HDP>::per_cu)) void chunk_ke
 
     // A thread's share of a step: pieces of 8 dims, kWaveRows rows of a wave side by side
     const int my_row = lane / kPieces, my_dim = 8 * (lane % kPieces);
-    const unsigned off = my_row * a.hd + (padded ? min(my_dim, a.hd - 8) : my_dim);
     const bool no_dim = padded && my_dim >= a.hd;
+    const unsigned row_bytes = a.hd * sizeof(S), off = my_row * row_bytes + (padded ? min(my_dim, a.hd - 8) : my_dim) * (unsigned)sizeof(S);
+    const unsigned first_row = wave * kWaveRows;
+    unsigned offs[kLoads];   // from the step's first key
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) offs[i] = off + (i * kStepRows + first_row) * row_bytes;
+    const unsigned page_bytes = ((unsigned)a.n_head_kv << a.page_shift) * row_bytes;   // (under 2^32: the host's check)
+    const size_t head_bytes = ((size_t)p.head << a.page_shift) * row_bytes;
+    const char *const k_head = (const char *)a.k_pool + head_bytes, *const v_head = (const char *)a.v_pool + head_bytes;
     raw8 kr[kLoads], vr[kLoads];
     int loaded = 0;                      // step whose K and V are in flight
     unsigned has_next = 0, has_now = 0;  // whether its groups have pages, a bit each
-    const auto load = [&](int step) {
-        const int group = step * kGroups;
-        if (group && (group & 63) == 0) {
-            run.now = run.ahead;
-            run.ahead = pages_from(group + 64);
-        }
+    bool mixed_now = false;              // whether the tile's rows differ in what they see of the step in LDS
+    // P groups lie in one page; those without one read page 0.
+    const auto load_groups = [&]<int P>(int step) {
+        const int group = step * kGroups, key = key_of(step);
+        size_t base[kGroups / P];
         has_next = 0;
 #pragma unroll
-        for (int i = 0; i < kGroups; ++i) has_next |= (run.get((group + i) & 63) >= 0 ? 1u : 0u) << i;
+        for (int b = 0; b < kGroups / P; ++b) {
+            const int page = run.get((group + b * P) & 63);
+            has_next |= page >= 0 ? ((1u << P) - 1) << (b * P) : 0;
+            base[b] = (size_t)(unsigned)max(page, 0) * page_bytes + (size_t)(int)((((key + 16 * P * b) & slot_mask) - 16 * P * b) * (int)row_bytes);
+        }
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const int first = i * kStepRows + wave * kWaveRows;   // of the rows of this wave
-            const int page = run.get((group + first / 16) & 63), key = k.lo + step * kKeys + first;
-            const size_t base = ((((size_t)max(page, 0) * a.n_head_kv + p.head) << a.page_shift) + (key & slot_mask)) * a.hd;
-            kr[i] = *reinterpret_cast<const raw8 *>((const S *)a.k_pool + base + off);
-            vr[i] = *reinterpret_cast<const raw8 *>((const S *)a.v_pool + base + off);
+            const size_t at = base[kGroups == P ? 0 : (i * kStepRows + first_row) / (16 * P)];
+            kr[i] = *reinterpret_cast<const raw8 *>(k_head + at + offs[i]);
+            vr[i] = *reinterpret_cast<const raw8 *>(v_head + at + offs[i]);
         }
+    };
+    const auto load = [&](int step) {
+        if (step && (step * kGroups & 63) == 0) {
+            run.now = run.ahead;
+            run.ahead = pages_from(step + 64 / kGroups);
+        }
+        if (a.page_shift >= (kKeys == 64 ? 6 : 5)) load_groups.template operator()<kGroups>(step);
+        else if (kKeys == 64 && a.page_shift == 5) load_groups.template operator()<kGroups == 4 ? 2 : 1>(step);
+        else load_groups.template operator()<1>(step);
         loaded = step;
     };
     // The loaded step into a buffer.  Where the tile's rows differ in what they see, V of
     // positions that none sees is 0, and infinities and NaN are 0 too and noted apart: a
     // product with a weight of 0 would hand them to every row.
     const auto store = [&](int buffer) {
-        const int key0 = k.lo + loaded * kKeys;
+        const int key0 = key_of(loaded);
         C *const ks = tile[buffer], *const vs = ks + kKeys * kKPitch;
         const bool whole = key0 >= k.all_lo && key0 + kKeys <= min(k.all_hi, k.hi) && has_next == (1u << kGroups) - 1;
         bool odd = false;
@@ -180,7 +213,7 @@ __global__ __launch_bounds__(kThreads, (Shape<A, S, HDP>::per_cu)) void chunk_ke
                 }
                 unsigned char *const at = reinterpret_cast<unsigned char *>(kinds[buffer][0][first + my_row]) + my_dim / 8;
                 at[0] = (unsigned char)up;
-                at[sizeof(kinds[0][0])] = (unsigned char)down;
+                at[sizeof all_kinds[0][0][0]] = (unsigned char)down;
                 odd |= (up | down) != 0;
             }
             odd = __any(odd);
@@ -213,6 +246,7 @@ __global__ __launch_bounds__(kThreads, (Shape<A, S, HDP>::per_cu)) void chunk_ke
             }
         }
         has_now = has_next;
+        mixed_now = !whole;
     };
 
     floatx16 o[DT];
@@ -225,12 +259,13 @@ __global__ __launch_bounds__(kThreads, (Shape<A, S, HDP>::per_cu)) void chunk_ke
         store(0);
         if (n_step > 1) load(1);
     }
-    for (int step = 0; step < n_step; ++step) {
-        const int buffer = kBuffers == 2 ? step & 1 : 0, key0 = k.lo + step * kKeys;
+    for (int step = 0; step < n_run; ++step) {
+        const int buffer = kBuffers == 2 ? step & 1 : 0, key0 = key_of(step);
         __syncthreads();
         const unsigned has = has_now;
+        const bool mixed = mixed_now;
         const C *const ks = tile[buffer], *const vs = ks + kKeys * kKPitch;
-        const bool any = key0 < see_hi && key0 + kKeys > see_lo;
+        const bool any = key0 < see_hi && key0 + kKeys > see_lo && step < n_step;
         const bool whole = key0 >= all_lo && key0 + kKeys <= all_hi && has == (1u << kGroups) - 1;
 
         // S^T = K Q^T: lane (n, half) gets its row's scores of keys 32 m + 8 (i / 4) + 4 half + i % 4
@@ -321,7 +356,7 @@ __global__ __launch_bounds__(kThreads, (Shape<A, S, HDP>::per_cu)) void chunk_ke
                         for (int y = 0; y < PP; ++y)
                             if (KP == 1 || x + y < KP) o[i] = Mma<C>::mul32(v, w[t / 2][t & 1][y], o[i]);
                     }
-            if (odd_of[buffer][0] | odd_of[buffer][1] | odd_of[buffer][2] | odd_of[buffer][3]) {
+            if (mixed && (odd_of[buffer][0] | odd_of[buffer][1] | odd_of[buffer][2] | odd_of[buffer][3])) {
                 for (int e = 0; e < kKeys; ++e) {
                     const bool sees = key0 + e >= row.lo && key0 + e < min(row.hi, k.hi);
 #pragma unroll
@@ -338,14 +373,44 @@ __global__ __launch_bounds__(kThreads, (Shape<A, S, HDP>::per_cu)) void chunk_ke
                 }
             }
         }
-        if (kBuffers == 1 && step + 1 < n_step) {
+        if (kBuffers == 1 && step + 1 < n_run) {
             __syncthreads();
-            store(0);
-            if (step + 2 < n_step) load(step + 2);
+            if (step + 1 < n_step) {
+                store(0);
+                if (step + 2 < n_step) load(step + 2);
+            }
         }
     }
 
     sum = sum32(sum);
+    if constexpr (kTeams == 2) {
+        float4 *const meet = reinterpret_cast<float4 *>(tiles) + wave * (HDP / 8) * 64 + lane;
+        __syncthreads();
+        if (team == 1) {
+#pragma unroll
+            for (int i = 0; i < DT; ++i)
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    meet[(4 * i + x) * 64] = make_float4(o[i][4 * x], o[i][4 * x + 1], o[i][4 * x + 2], o[i][4 * x + 3]);
+            if (half == 0) team_ml[wave][col] = make_float2(ref, sum);
+        }
+        __syncthreads();
+        if (team == 1) return;
+        const float2 e = team_ml[wave][col];
+        const float m = fmaxf(ref, e.x), base = m == kNone ? 0.f : m, f = exp2_(ref - base), g = exp2_(e.x - base);
+        ref = m;
+        sum = fmaf(e.y, g, sum * f);
+#pragma unroll
+        for (int i = 0; i < DT; ++i)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const float4 v = meet[(4 * i + x) * 64];
+                o[i][4 * x] = fmaf(v.x, g, o[i][4 * x] * f);
+                o[i][4 * x + 1] = fmaf(v.y, g, o[i][4 * x + 1] * f);
+                o[i][4 * x + 2] = fmaf(v.z, g, o[i][4 * x + 2] * f);
+                o[i][4 * x + 3] = fmaf(v.w, g, o[i][4 * x + 3] * f);
+            }
+    }
     const int r = wave * 32 + col;
     if (p.n_split > 1) {
         const size_t id = blockIdx.x;
@@ -379,9 +444,9 @@ hipError_t launch_chunk(const TileArgs &d, int places, hipStream_t s) {
     const dim3 grid((unsigned)places);
 #define KORE_CHUNK(A, S)                                                        \
     do {                                                                        \
-        if (hdp == 64) chunk_kernel<A, S, 64><<<grid, kThreads, 0, s>>>(d);     \
-        else if (hdp == 128) chunk_kernel<A, S, 128><<<grid, kThreads, 0, s>>>(d); \
-        else chunk_kernel<A, S, 256><<<grid, kThreads, 0, s>>>(d);              \
+        if (hdp == 64) chunk_kernel<A, S, 64><<<grid, Shape<A, S, 64>::threads, 0, s>>>(d);     \
+        else if (hdp == 128) chunk_kernel<A, S, 128><<<grid, Shape<A, S, 128>::threads, 0, s>>>(d); \
+        else chunk_kernel<A, S, 256><<<grid, Shape<A, S, 256>::threads, 0, s>>>(d);              \
     } while (0)
     if (d.a.cache_type == kF32) KORE_CHUNK(float, float);
     else if (d.a.type == kF32 && d.a.cache_type == kF16) KORE_CHUNK(float, half_t);

@@ -577,12 +577,10 @@ constexpr int kMinLen = 64, kChunkMinLen = 256;   // a split's fewest keys
 constexpr int kPerCu = 2;                           // workgroups of a CU
 constexpr int kMaxTiles = 1024;                     // over this many (tile, kv-head)s of 16 rows nothing is split
 
-int chunk_places(int hd, int num_cu) { return (hd <= 128 ? 2 : 1) * num_cu; }
-
 }  // namespace
 
 size_t attend_workspace_bytes(int n_head, int n_head_kv, int hd, int num_cu) {
-    const size_t rows = ((size_t)kMaxTiles + (size_t)kPerCu * num_cu) * kRows, chunk_rows = (size_t)chunk_places(hd, num_cu) * kChunkRows;
+    const size_t rows = ((size_t)kMaxTiles + (size_t)kPerCu * num_cu) * kRows, chunk_rows = (size_t)num_cu * kChunkRows;
     return std::max(rows, chunk_rows) * ((size_t)padded_dim(hd) + 2) * sizeof(float);
 }
 
@@ -596,10 +594,9 @@ hipError_t launch_attend(const AttendArgs &a, hipStream_t s) {
     // the most (tile, kv-head)s that n_tok rows of n_seq sequences can be
     const long long tiles = ((long long)a.b.n_tok * d.cut.rep / rows + std::min(a.b.n_seq, a.b.n_tok)) * a.n_head_kv;
     if (chunk) {
-        const int places = chunk_places(a.hd, a.num_cu);
+        const int places = a.num_cu;
         d.cut.target = 4 * tiles > 3 * places ? 0 : (int)(places - tiles);
         d.cut.min_len = kChunkMinLen;
-        if (!d.cut.target) d.cut.fold = a.num_cu;
     } else {
         const int places = kPerCu * a.num_cu;
         d.cut.target = tiles > kMaxTiles ? 0 : (int)std::max<long long>(places - tiles, places / 2);
