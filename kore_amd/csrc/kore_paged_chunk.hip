@@ -27,22 +27,53 @@ template <> struct Form<float, float> {
     static constexpr int qp = 3, kp = 3, pp = 3;
 };
 
-// What a tile's shape asks of LDS and registers: keys of a step; buffers; teams of a
+// What a tile's shape asks of LDS and registers: keys of a step; teams of a
 // workgroup (a CU holds one workgroup).
 template <class A, class S, int HDP> struct Shape {
     static constexpr bool parts = Form<A, S>::qp > 1;
     static constexpr int keys = parts ? 32 : 64;
-    static constexpr int buffers = HDP <= 128 && Form<A, S>::kp == 1 ? 2 : 1;
     static constexpr int teams = HDP <= 128 ? 2 : 1, threads = 64 * kWaves * teams;
 };
 
-// Three bf16 parts of an fp32 value of the cache; an infinity or NaN is all in the first.
-__device__ __forceinline__ void split_kv(float x, bhalf_t (&part)[3]) {
-    const float h = bf16_cut(x), r = x - h, m = bf16_cut(r), l = r - m;
-    const bool f = finite(x);
-    part[0] = f ? (bhalf_t)h : (bhalf_t)x;
-    part[1] = f ? (bhalf_t)m : (bhalf_t)0.f;
-    part[2] = f ? (bhalf_t)l : (bhalf_t)0.f;
+// Eight values as one, two or three 16-bit parts.  Three bf16 parts are cut, not
+// rounded: 24 bits in all, two values' upper halves an instruction.
+__device__ __forceinline__ unsigned upper_halves(float a, float b) {
+    return __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, b), __builtin_bit_cast(unsigned, a), 0x07060302);
+}
+__device__ __forceinline__ void cut3(const float (&x)[8], bhalf8 (&part)[3], float &rest) {
+    typedef unsigned uint4_t __attribute__((ext_vector_type(4)));
+    uint4_t u[3];
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        float r[2], l[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            r[j] = x[i + j] - bf16_cut(x[i + j]);
+            l[j] = r[j] - bf16_cut(r[j]);
+            rest += l[j];
+        }
+        u[0][i / 2] = upper_halves(x[i], x[i + 1]);
+        u[1][i / 2] = upper_halves(r[0], r[1]);
+        u[2][i / 2] = upper_halves(l[0], l[1]);
+    }
+#pragma unroll
+    for (int j = 0; j < 3; ++j) part[j] = __builtin_bit_cast(bhalf8, u[j]);
+}
+// Eight weights as N parts of C.
+template <int N, class C, class V>
+__device__ __forceinline__ void weights(const float (&x)[8], V (&part)[N]) {
+    if constexpr (N == 3) {
+        float rest = 0;
+        cut3(x, part, rest);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            C y[N];
+            split_p<N>(x[i], y);
+#pragma unroll
+            for (int j = 0; j < N; ++j) part[j][i] = y[j];
+        }
+    }
 }
 
 template <class A, class S, int HDP>
@@ -51,24 +82,25 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
     typedef typename Mma<C>::vec8 vec8;
     typedef C vec4 __attribute__((ext_vector_type(4)));
     constexpr int QP = Form<A, S>::qp, KP = Form<A, S>::kp, PP = Form<A, S>::pp;
-    constexpr int kKeys = Shape<A, S, HDP>::keys, kBuffers = Shape<A, S, HDP>::buffers, kTeams = Shape<A, S, HDP>::teams;
+    constexpr int kKeys = Shape<A, S, HDP>::keys, kTeams = Shape<A, S, HDP>::teams;
     constexpr int KS = HDP / 16, DT = HDP / 32, MT = kKeys / 32;         // k-steps, dim tiles, key tiles
     // Rows of LDS: 16 rows' 16-byte pieces of K, and four rows' 64 bytes of V, lie on
     // different banks
-    constexpr int kKPitch = HDP + 8, kVPitch = HDP + 32, kPlane = kKeys * (kKPitch + kVPitch);
+    constexpr int kKPitch = HDP + 8, kVPitch = HDP + 32;
     constexpr int kPieces = HDP / 8, kWaveRows = 64 / kPieces, kStepRows = kWaves * kWaveRows, kLoads = kKeys / kStepRows;
     typedef S raw8 __attribute__((ext_vector_type(8)));
-    __shared__ __attribute__((aligned(16))) C tiles[kTeams][kBuffers][KP * kPlane];
+    __shared__ __attribute__((aligned(16))) C k_tiles[kTeams][KP][kKeys * kKPitch], v_tiles[kTeams][KP][kKeys * kVPitch];
     // of V's pieces in steps that the tile's rows do not all see: which of 8 dims are +inf, or -inf (a NaN: both)
-    __shared__ unsigned all_kinds[kTeams][kBuffers][2][kKeys][HDP / 32];
-    __shared__ int all_odd[kTeams][kBuffers][kWaves];
+    __shared__ unsigned all_kinds[kTeams][2][kKeys][HDP / 32];
+    __shared__ int all_odd[kTeams][kWaves];
+    __shared__ float4 team_o[kTeams == 2 ? kWaves * HDP / 16 * 64 : 1];   // half of the second team's sums
     __shared__ float2 team_ml[kWaves][32];   // (reference, sum) of the second team's rows
-    static_assert(kTeams == 1 || sizeof tiles >= kWaves * (HDP / 2) * 64 * sizeof(float), "the teams' sums meet in the tiles' place");
     const AttendArgs &a = d.a;
     const int rep = d.cut.rep;
     const int cap = a.b.pages_stride << a.page_shift, lane = threadIdx.x & 63;
     const int wave = scalar(threadIdx.x >> 6) % kWaves, team = scalar(threadIdx.x >> 6) / kWaves;
-    auto &tile = tiles[team];
+    auto &k_tile = k_tiles[team];
+    auto &v_tile = v_tiles[team];
     auto &kinds = all_kinds[team];
     auto &odd_of = all_odd[team];
     Place p;
@@ -157,50 +189,76 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
     const size_t head_bytes = ((size_t)p.head << a.page_shift) * row_bytes;
     const char *const k_head = (const char *)a.k_pool + head_bytes, *const v_head = (const char *)a.v_pool + head_bytes;
     raw8 kr[kLoads], vr[kLoads];
-    int loaded = 0;                      // step whose K and V are in flight
-    unsigned has_next = 0, has_now = 0;  // whether its groups have pages, a bit each
-    bool mixed_now = false;              // whether the tile's rows differ in what they see of the step in LDS
+    // Whether a step's groups have pages, a bit each: of the step in LDS, the next and the one after
+    unsigned has = 0, has_1 = 0, has_2 = 0;
+    constexpr unsigned kAll = (1u << kGroups) - 1;
     // P groups lie in one page; those without one read page 0.
-    const auto load_groups = [&]<int P>(int step) {
+    const auto load_groups = [&]<int P>(int step, const char *pool, raw8 (&x)[kLoads]) {
         const int group = step * kGroups, key = key_of(step);
         size_t base[kGroups / P];
-        has_next = 0;
+        unsigned bits = 0;
 #pragma unroll
         for (int b = 0; b < kGroups / P; ++b) {
             const int page = run.get((group + b * P) & 63);
-            has_next |= page >= 0 ? ((1u << P) - 1) << (b * P) : 0;
+            bits |= page >= 0 ? ((1u << P) - 1) << (b * P) : 0;
             base[b] = (size_t)(unsigned)max(page, 0) * page_bytes + (size_t)(int)((((key + 16 * P * b) & slot_mask) - 16 * P * b) * (int)row_bytes);
         }
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const size_t at = base[kGroups == P ? 0 : (i * kStepRows + first_row) / (16 * P)];
-            kr[i] = *reinterpret_cast<const raw8 *>(k_head + at + offs[i]);
-            vr[i] = *reinterpret_cast<const raw8 *>(v_head + at + offs[i]);
-        }
+        for (int i = 0; i < kLoads; ++i)
+            x[i] = *reinterpret_cast<const raw8 *>(pool + base[kGroups == P ? 0 : (i * kStepRows + first_row) / (16 * P)] + offs[i]);
+        return bits;
     };
-    const auto load = [&](int step) {
+    const auto load = [&](int step, const char *pool, raw8 (&x)[kLoads]) {
+        if (a.page_shift >= (kKeys == 64 ? 6 : 5)) return load_groups.template operator()<kGroups>(step, pool, x);
+        if (kKeys == 64 && a.page_shift == 5) return load_groups.template operator()<kGroups == 4 ? 2 : 1>(step, pool, x);
+        return load_groups.template operator()<1>(step, pool, x);
+    };
+    const auto load_k = [&](int step) {   // before the same step's V
         if (step && (step * kGroups & 63) == 0) {
             run.now = run.ahead;
             run.ahead = pages_from(step + 64 / kGroups);
         }
-        if (a.page_shift >= (kKeys == 64 ? 6 : 5)) load_groups.template operator()<kGroups>(step);
-        else if (kKeys == 64 && a.page_shift == 5) load_groups.template operator()<kGroups == 4 ? 2 : 1>(step);
-        else load_groups.template operator()<1>(step);
-        loaded = step;
+        has_2 = load(step, k_head, kr);
     };
-    // The loaded step into a buffer.  Where the tile's rows differ in what they see, V of
-    // positions that none sees is 0, and infinities and NaN are 0 too and noted apart: a
-    // product with a weight of 0 would hand them to every row.
-    const auto store = [&](int buffer) {
-        const int key0 = key_of(loaded);
-        C *const ks = tile[buffer], *const vs = ks + kKeys * kKPitch;
-        const bool whole = key0 >= k.all_lo && key0 + kKeys <= min(k.all_hi, k.hi) && has_next == (1u << kGroups) - 1;
-        bool odd = false;
-        if (!whole) {
+    const auto load_v = [&](int step) { load(step, v_head, vr); };
+    const auto put = [&](C *plane0, int plane, raw8 x, int at) {
+        if constexpr (KP == 1) {
+            *reinterpret_cast<raw8 *>(plane0 + at) = x;
+        } else {
+            float y[8], rest = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = x[e];
+            vec8 part[3];
+            cut3(y, part, rest);
+            if (__any(rest != rest)) {   // an infinity or NaN: all of it in the first part
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (!finite(y[e])) {
+                        part[0][e] = (bhalf_t)y[e];
+                        part[1][e] = part[2][e] = (bhalf_t)0.f;
+                    }
+            }
+#pragma unroll
+            for (int j = 0; j < 3; ++j) *reinterpret_cast<vec8 *>(plane0 + j * plane + at) = part[j];
+        }
+    };
+    const auto store_k = [&] {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            if (no_dim) kr[i] = raw8{};
+            put(k_tile[0], kKeys * kKPitch, kr[i], (i * kStepRows + wave * kWaveRows + my_row) * kKPitch + my_dim);
+        }
+    };
+    // V into LDS.  Where the tile's rows differ in what they see, V of positions that none
+    // sees is 0, and infinities and NaN are 0 too and noted apart: a product with a weight
+    // of 0 would hand them to every row.
+    const auto store_v = [&](int key0, bool mixed) {
+        if (mixed) {
+            bool odd = false;
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
                 const int first = i * kStepRows + wave * kWaveRows;
-                if (!(key0 + first + my_row < k.hi && (has_next >> (first / 16) & 1))) vr[i] = raw8{};
+                if (!(key0 + first + my_row < k.hi && (has >> (first / 16) & 1))) vr[i] = raw8{};
                 unsigned up = 0, down = 0;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
@@ -211,42 +269,17 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
                         vr[i][e] = (S)0.f;
                     }
                 }
-                unsigned char *const at = reinterpret_cast<unsigned char *>(kinds[buffer][0][first + my_row]) + my_dim / 8;
+                unsigned char *const at = reinterpret_cast<unsigned char *>(kinds[0][first + my_row]) + my_dim / 8;
                 at[0] = (unsigned char)up;
-                at[sizeof all_kinds[0][0][0]] = (unsigned char)down;
+                at[sizeof kinds[0]] = (unsigned char)down;
                 odd |= (up | down) != 0;
             }
             odd = __any(odd);
+            if (lane == 0) odd_of[wave] = odd;
         }
-        if (lane == 0) odd_of[buffer][wave] = odd;
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int r = i * kStepRows + wave * kWaveRows + my_row;
-            if (no_dim) kr[i] = raw8{};
-            if constexpr (KP == 1) {
-                *reinterpret_cast<raw8 *>(ks + r * kKPitch + my_dim) = kr[i];
-                *reinterpret_cast<raw8 *>(vs + r * kVPitch + my_dim) = vr[i];
-            } else {
-                vec8 x[3], y[3];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    bhalf_t part[3];
-                    split_kv(kr[i][e], part);
-#pragma unroll
-                    for (int j = 0; j < 3; ++j) x[j][e] = part[j];
-                    split_kv(vr[i][e], part);
-#pragma unroll
-                    for (int j = 0; j < 3; ++j) y[j][e] = part[j];
-                }
-#pragma unroll
-                for (int j = 0; j < 3; ++j) {
-                    *reinterpret_cast<vec8 *>(ks + j * kPlane + r * kKPitch + my_dim) = x[j];
-                    *reinterpret_cast<vec8 *>(vs + j * kPlane + r * kVPitch + my_dim) = y[j];
-                }
-            }
-        }
-        has_now = has_next;
-        mixed_now = !whole;
+        for (int i = 0; i < kLoads; ++i)
+            put(v_tile[0], kKeys * kVPitch, vr[i], (i * kStepRows + wave * kWaveRows + my_row) * kVPitch + my_dim);
     };
 
     floatx16 o[DT];
@@ -254,19 +287,30 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
     for (int i = 0; i < DT; ++i) o[i] = floatx16{};
     float ref = kNone, sum = 0;
 
+    // A step is two phases: V into LDS, the scores and their maximum; K of the next step
+    // into LDS, the weights and their product with V.  Each reads what the phase before
+    // wrote, so K and V need one place each, and the second team runs a phase behind the
+    // first: one is at its scores while the other makes weights.
     if (n_step) {
-        load(0);
-        store(0);
-        if (n_step > 1) load(1);
+        load_k(0);
+        load_v(0);
+        has = has_2;
+        store_k();
+        if (n_step > 1) load_k(1);
+        has_1 = has_2;
     }
+    if (team == 1) __syncthreads();
     for (int step = 0; step < n_run; ++step) {
-        const int buffer = kBuffers == 2 ? step & 1 : 0, key0 = key_of(step);
+        const int key0 = key_of(step);
+        const bool real = step < n_step;
+        const bool mixed = !(key0 >= k.all_lo && key0 + kKeys <= min(k.all_hi, k.hi) && has == kAll);
+        const bool any = key0 < see_hi && key0 + kKeys > see_lo && real;
+        const bool whole = key0 >= all_lo && key0 + kKeys <= all_hi && has == kAll;
         __syncthreads();
-        const unsigned has = has_now;
-        const bool mixed = mixed_now;
-        const C *const ks = tile[buffer], *const vs = ks + kKeys * kKPitch;
-        const bool any = key0 < see_hi && key0 + kKeys > see_lo && step < n_step;
-        const bool whole = key0 >= all_lo && key0 + kKeys <= all_hi && has == (1u << kGroups) - 1;
+        if (real) {
+            store_v(key0, mixed);
+            if (step + 1 < n_step) load_v(step + 1);
+        }
 
         // S^T = K Q^T: lane (n, half) gets its row's scores of keys 32 m + 8 (i / 4) + 4 half + i % 4
         floatx16 s[MT];
@@ -274,12 +318,12 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
                 s[m] = floatx16{};
-                const C *const from = ks + (32 * m + col) * kKPitch + 8 * half;
+                const int from = (32 * m + col) * kKPitch + 8 * half;
 #pragma unroll
                 for (int t = 0; t < KS; ++t)
 #pragma unroll
                     for (int y = 0; y < KP; ++y) {
-                        const vec8 x = *reinterpret_cast<const vec8 *>(from + y * kPlane + 16 * t);
+                        const vec8 x = *reinterpret_cast<const vec8 *>(&k_tile[y][from + 16 * t]);
 #pragma unroll
                         for (int z = 0; z < QP; ++z)
                             if (KP == 1 || y + z < KP) s[m] = Mma<C>::mul32(x, q[z][t], s[m]);
@@ -294,12 +338,6 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
                 __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             }
             __builtin_amdgcn_sched_group_barrier(0x008, kAhead * kPer, 0);
-        }
-        if (kBuffers == 2 && step + 1 < n_step) {
-            store(buffer ^ 1);
-            if (step + 2 < n_step) load(step + 2);
-        }
-        if (any) {
             if (!whole) {
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
@@ -316,32 +354,39 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
                 for (int i = 0; i < 16; ++i) top = fmaxf(top, s[m][i]);
             top = max32(top) * s_hi;
             follow(top, ref, sum, Mma<C>::kBias, o);
+        }
+        __syncthreads();
+        if (step + 1 < n_step) {
+            store_k();
+            if (step + 2 < n_step) load_k(step + 2);
+        }
+        has = has_1;
+        has_1 = has_2;
+        if (any) {
             const float base = ref == kNone ? 0.f : ref;
             vec8 w[MT][2][PP];
             float part_sum = 0;
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float e = PP > 1 ? fmaf(s[m][i], s_hi, fmaf(s[m][i], s_lo, -base)) : fmaf(s[m][i], s_hi, -base);
-                    const float x = exp2_(e);
-                    C part[PP];
-                    split_p<PP>(x, part);
-                    if (PP > 1) part_sum += x;
+                for (int h = 0; h < 2; ++h) {
+                    float x[8];
 #pragma unroll
-                    for (int y = 0; y < PP; ++y) w[m][i / 8][y][i % 8] = part[y];
+                    for (int i = 0; i < 8; ++i) {
+                        const float y = s[m][8 * h + i];
+                        x[i] = exp2_(PP > 1 ? fmaf(y, s_hi, fmaf(y, s_lo, -base)) : fmaf(y, s_hi, -base));
+                        if (PP > 1) part_sum += x[i];
+                    }
+                    weights<PP, C>(x, w[m][h]);
+                    // one rounded weight is also what is summed: what rounding adds to all of a row's weights divides out
+                    if constexpr (PP == 1) part_sum = sum_weights(w[m][h][0], part_sum);
                 }
-            // one rounded weight is also what is summed: what rounding adds to all of a row's weights divides out
-            if constexpr (PP == 1) {
-#pragma unroll
-                for (int m = 0; m < MT; ++m) part_sum = sum_weights(w[m][1][0], sum_weights(w[m][0][0], part_sum));
-            }
             sum += part_sum;
             // O^T += V^T P^T, k order as the scores came: V^T's operand, lane (m, half), has keys 16 t + 4 half + 0..3 and
             // those 8 further of dim 32 i + m
-            const C *const from = vs + (4 * half + (lane & 15) / 4) * kVPitch + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
+            const int from = (4 * half + (lane & 15) / 4) * kVPitch + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
             const auto v_operand = [&](int plane, int t, int i) {
-                const C *at = from + plane * kPlane + 16 * t * kVPitch + 32 * i;
+                const C *at = &v_tile[plane][from + 16 * t * kVPitch + 32 * i];
                 const vec4 x = read_transposed<vec4>(at), y = read_transposed<vec4>(at + 8 * kVPitch);
                 return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
             };
@@ -356,12 +401,12 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
                         for (int y = 0; y < PP; ++y)
                             if (KP == 1 || x + y < KP) o[i] = Mma<C>::mul32(v, w[t / 2][t & 1][y], o[i]);
                     }
-            if (mixed && (odd_of[buffer][0] | odd_of[buffer][1] | odd_of[buffer][2] | odd_of[buffer][3])) {
+            if (mixed && (odd_of[0] | odd_of[1] | odd_of[2] | odd_of[3])) {
                 for (int e = 0; e < kKeys; ++e) {
                     const bool sees = key0 + e >= row.lo && key0 + e < min(row.hi, k.hi);
 #pragma unroll
                     for (int i = 0; i < DT; ++i) {
-                        const unsigned up = sees ? kinds[buffer][0][e][i] >> (4 * half) : 0, down = sees ? kinds[buffer][1][e][i] >> (4 * half) : 0;
+                        const unsigned up = sees ? kinds[0][e][i] >> (4 * half) : 0, down = sees ? kinds[1][e][i] >> (4 * half) : 0;
                         if (!__any((up | down) != 0)) continue;
 #pragma unroll
                         for (int j = 0; j < 16; ++j) {
@@ -373,43 +418,51 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
                 }
             }
         }
-        if (kBuffers == 1 && step + 1 < n_run) {
-            __syncthreads();
-            if (step + 1 < n_step) {
-                store(0);
-                if (step + 2 < n_step) load(step + 2);
-            }
-        }
     }
+    if (kTeams == 2 && team == 0) __syncthreads();
 
     sum = sum32(sum);
     if constexpr (kTeams == 2) {
-        float4 *const meet = reinterpret_cast<float4 *>(tiles) + wave * (HDP / 8) * 64 + lane;
-        __syncthreads();
-        if (team == 1) {
+        // the second team's sums through LDS, half of them at a time
+        float4 *const meet = team_o + wave * (HDP / 16) * 64 + lane;
+        float f = 1.f, g = 0.f;
 #pragma unroll
-            for (int i = 0; i < DT; ++i)
+        for (int part = 0; part < 2; ++part) {
+            if (team == 1) {
 #pragma unroll
-                for (int x = 0; x < 4; ++x)
-                    meet[(4 * i + x) * 64] = make_float4(o[i][4 * x], o[i][4 * x + 1], o[i][4 * x + 2], o[i][4 * x + 3]);
-            if (half == 0) team_ml[wave][col] = make_float2(ref, sum);
-        }
-        __syncthreads();
-        if (team == 1) return;
-        const float2 e = team_ml[wave][col];
-        const float m = fmaxf(ref, e.x), base = m == kNone ? 0.f : m, f = exp2_(ref - base), g = exp2_(e.x - base);
-        ref = m;
-        sum = fmaf(e.y, g, sum * f);
+                for (int i = 0; i < DT / 2; ++i)
 #pragma unroll
-        for (int i = 0; i < DT; ++i)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const float4 v = meet[(4 * i + x) * 64];
-                o[i][4 * x] = fmaf(v.x, g, o[i][4 * x] * f);
-                o[i][4 * x + 1] = fmaf(v.y, g, o[i][4 * x + 1] * f);
-                o[i][4 * x + 2] = fmaf(v.z, g, o[i][4 * x + 2] * f);
-                o[i][4 * x + 3] = fmaf(v.w, g, o[i][4 * x + 3] * f);
+                    for (int x = 0; x < 4; ++x) {
+                        const floatx16 &from = o[part * (DT / 2) + i];
+                        meet[(4 * i + x) * 64] = make_float4(from[4 * x], from[4 * x + 1], from[4 * x + 2], from[4 * x + 3]);
+                    }
+                if (part == 0 && half == 0) team_ml[wave][col] = make_float2(ref, sum);
             }
+            __syncthreads();
+            if (team == 0) {
+                if (part == 0) {
+                    const float2 e = team_ml[wave][col];
+                    const float m = fmaxf(ref, e.x), base = m == kNone ? 0.f : m;
+                    f = exp2_(ref - base);
+                    g = exp2_(e.x - base);
+                    ref = m;
+                    sum = fmaf(e.y, g, sum * f);
+                }
+#pragma unroll
+                for (int i = 0; i < DT / 2; ++i)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const float4 v = meet[(4 * i + x) * 64];
+                        floatx16 &to = o[part * (DT / 2) + i];
+                        to[4 * x] = fmaf(v.x, g, to[4 * x] * f);
+                        to[4 * x + 1] = fmaf(v.y, g, to[4 * x + 1] * f);
+                        to[4 * x + 2] = fmaf(v.z, g, to[4 * x + 2] * f);
+                        to[4 * x + 3] = fmaf(v.w, g, to[4 * x + 3] * f);
+                    }
+            }
+            if (part == 0) __syncthreads();
+        }
+        if (team == 1) return;
     }
     const int r = wave * 32 + col;
     if (p.n_split > 1) {
