@@ -162,24 +162,24 @@ template <int TILE>
 __device__ __forceinline__ bool place_of(const Batch &b, const Cut &c, int id, int nkv, int cap, int window, bool by_tile,
                                          Place &p) {
     const int lane = threadIdx.x & 63;
-    int len = INT_MAX;
+    int len = INT_MAX, q0 = 0, n = 0, kv = 0;
+    const auto share = [&](int s0) {
+        return s0 + lane < b.n_seq ? share_of<TILE>(b, s0 + lane, c.rep, cap, window, q0, n, kv) : Share{0, 0};
+    };
+    Share r = share(0);
     if (c.target) {
         // so that all splits are at most target (of len keys) and one more for each tile
-        float w = 0;
-        for (int s0 = 0; s0 < b.n_seq; s0 += 64) {
-            const int s = s0 + lane;
-            int q0, n, kv;
-            const Share r = s < b.n_seq ? share_of<TILE>(b, s, c.rep, cap, window, q0, n, kv) : Share{0, 0};
-            w += (float)r.tiles * (float)r.keys;
+        float w = (float)r.tiles * (float)r.keys;
+        for (int s0 = 64; s0 < b.n_seq; s0 += 64) {
+            const Share t = share(s0);
+            w += (float)t.tiles * (float)t.keys;
         }
         const float each = ceilf(last_lane(prefix_sum(w)) * (float)nkv / (float)c.target);
         len = max(c.min_len, ((int)fminf(each, 1e9f) + 63) & ~63);
     }
     int at = 0, splits_at = 0;
     for (int s0 = 0; s0 < b.n_seq; s0 += 64) {
-        const int s = s0 + lane;
-        int q0 = 0, n = 0, kv = 0;
-        const Share r = s < b.n_seq ? share_of<TILE>(b, s, c.rep, cap, window, q0, n, kv) : Share{0, 0};
+        if (b.n_seq > 64) r = share(s0);   // (one round of loads where all sequences have a lane)
         const int n_split = max(1, r.keys / len + (r.keys % len != 0));
         const int all = r.tiles * n_split * nkv, mine = by_tile ? r.tiles * nkv : all;
         const int upto = prefix_sum(mine), splits_upto = by_tile ? prefix_sum(all) : upto;

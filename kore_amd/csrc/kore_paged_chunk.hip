@@ -33,6 +33,7 @@ template <class A, class S, int HDP> struct Shape {
     static constexpr bool parts = Form<A, S>::qp > 1;
     static constexpr int keys = parts ? 32 : 64;
     static constexpr int teams = HDP <= 128 ? 2 : 1, threads = 64 * kWaves * teams;
+    static constexpr bool lag = parts && teams == 2;   // the second team a phase behind
 };
 
 // Eight values as one, two or three 16-bit parts.  Three bf16 parts are cut, not
@@ -83,24 +84,31 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
     typedef C vec4 __attribute__((ext_vector_type(4)));
     constexpr int QP = Form<A, S>::qp, KP = Form<A, S>::kp, PP = Form<A, S>::pp;
     constexpr int kKeys = Shape<A, S, HDP>::keys, kTeams = Shape<A, S, HDP>::teams;
+    constexpr bool kLag = Shape<A, S, HDP>::lag;
     constexpr int KS = HDP / 16, DT = HDP / 32, MT = kKeys / 32;         // k-steps, dim tiles, key tiles
     // Rows of LDS: 16 rows' 16-byte pieces of K, and four rows' 64 bytes of V, lie on
     // different banks
     constexpr int kKPitch = HDP + 8, kVPitch = HDP + 32;
     constexpr int kPieces = HDP / 8, kWaveRows = 64 / kPieces, kStepRows = kWaves * kWaveRows, kLoads = kKeys / kStepRows;
     typedef S raw8 __attribute__((ext_vector_type(8)));
-    __shared__ __attribute__((aligned(16))) C k_tiles[kTeams][KP][kKeys * kKPitch], v_tiles[kTeams][KP][kKeys * kVPitch];
+    // A team's step of K and of V, each in KP planes; at the end half of the second team's sums lie there
+    constexpr int kPlane = kKeys * (kKPitch + kVPitch), kTileBytes = kTeams * KP * kPlane * (int)sizeof(C);
+    constexpr int kMeetBytes = kTeams == 2 ? kWaves * HDP / 16 * 64 * 16 : 0;
+    __shared__ __attribute__((aligned(16))) unsigned char tiles[kTileBytes > kMeetBytes ? kTileBytes : kMeetBytes];
+    // The third part of q, where LDS has room: it would cost the loop its spare registers, and a reload of a spilled
+    // one waits for the loads in flight.  (The teams' rows are the same.)
+    constexpr bool kThird = QP == 3 && !(KP == 3 && HDP == 256);
+    constexpr int kQReg = kThird ? 2 : QP;
+    __shared__ vec8 q_third[kThird ? kWaves : 1][KS][64];
     // of V's pieces in steps that the tile's rows do not all see: which of 8 dims are +inf, or -inf (a NaN: both)
     __shared__ unsigned all_kinds[kTeams][2][kKeys][HDP / 32];
     __shared__ int all_odd[kTeams][kWaves];
-    __shared__ float4 team_o[kTeams == 2 ? kWaves * HDP / 16 * 64 : 1];   // half of the second team's sums
     __shared__ float2 team_ml[kWaves][32];   // (reference, sum) of the second team's rows
     const AttendArgs &a = d.a;
     const int rep = d.cut.rep;
     const int cap = a.b.pages_stride << a.page_shift, lane = threadIdx.x & 63;
     const int wave = scalar(threadIdx.x >> 6) % kWaves, team = scalar(threadIdx.x >> 6) / kWaves;
-    auto &k_tile = k_tiles[team];
-    auto &v_tile = v_tiles[team];
+    C *const k_tile = reinterpret_cast<C *>(tiles) + team * (KP * kPlane), *const v_tile = k_tile + KP * kKeys * kKPitch;
     auto &kinds = all_kinds[team];
     auto &odd_of = all_odd[team];
     Place p;
@@ -140,42 +148,54 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
     run.now = pages_from(0);
     run.ahead = pages_from(64 / kGroups);
 
-    // Q: B operand, lane (n, half) has dims 16 t + 8 half .. + 7 of its row
-    vec8 q[QP][KS];
-    float unit = 1.f;
+    // Q: B operand, lane (n, half) has dims 16 t + 8 half .. + 7 of its row.  Requested here,
+    // used when K and V are on their way.
+    A q_row[KS][8];
     {
         const A *src = (const A *)a.q + (size_t)(row.real ? p.q0 + row.token : 0) * a.q_stride + (size_t)(row.real ? row.head : 0) * a.hd;
         const bool vec = ((uintptr_t)src & (8 * sizeof(A) - 1)) == 0;
-        A v[KS][8];
-        float big = 0;
 #pragma unroll
         for (int t = 0; t < KS; ++t) {
             const int dim = 16 * t + 8 * half;
-            const bool in = row.real && dim < a.hd;
-            if (in) load_n<8>(src + dim, v[t], vec);
+            if (row.real && dim < a.hd) load_n<8>(src + dim, q_row[t], vec);
+            else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (!in) v[t][i] = (A)0.f;
-                if (QP == 2) big = fmaxf(big, fabsf(to_f32(v[t][i])));
+                for (int i = 0; i < 8; ++i) q_row[t][i] = (A)0.f;
             }
         }
+    }
+
+    vec8 q[kQReg][KS];
+    float unit = 1.f;
+    const auto make_q = [&] {
         float to = 1.f;
-        if (QP == 2) unit_of(max32(big), to, unit);
+        if constexpr (QP == 2) {
+            float big = 0;
 #pragma unroll
-        for (int t = 0; t < KS; ++t)
+            for (int t = 0; t < KS; ++t)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(q_row[t][i]));
+            unit_of(max32(big), to, unit);
+        }
+#pragma unroll
+        for (int t = 0; t < KS; ++t) {
+            vec8 third = {};
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 if constexpr (QP == 1) {
-                    q[0][t][i] = v[t][i];
+                    q[0][t][i] = q_row[t][i];
                 } else {
                     C part[QP];
-                    split_q<QP>(to_f32(v[t][i]) * to, part);
+                    split_q<QP>(q_row[t][i] * to, part);
 #pragma unroll
-                    for (int j = 0; j < QP; ++j) q[j][t][i] = part[j];
+                    for (int j = 0; j < kQReg; ++j) q[j][t][i] = part[j];
+                    if (kThird) third[i] = part[QP - 1];
                 }
             }
-    }
-    const float s_hi = d.sl.hi * unit, s_lo = fmaxf(d.sl.lo * unit, 0x1p-126f);
+            if (kThird && team == 0) q_third[wave][t][lane] = third;
+        }
+    };
+    if constexpr (QP > 1) make_q();   // (behind the loads its registers cost the loop more than the wait)
 
     // A thread's share of a step: pieces of 8 dims, kWaveRows rows of a wave side by side
     const int my_row = lane / kPieces, my_dim = 8 * (lane % kPieces);
@@ -246,7 +266,7 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             if (no_dim) kr[i] = raw8{};
-            put(k_tile[0], kKeys * kKPitch, kr[i], (i * kStepRows + wave * kWaveRows + my_row) * kKPitch + my_dim);
+            put(k_tile, kKeys * kKPitch, kr[i], (i * kStepRows + wave * kWaveRows + my_row) * kKPitch + my_dim);
         }
     };
     // V into LDS.  Where the tile's rows differ in what they see, V of positions that none
@@ -279,7 +299,7 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
         }
 #pragma unroll
         for (int i = 0; i < kLoads; ++i)
-            put(v_tile[0], kKeys * kVPitch, vr[i], (i * kStepRows + wave * kWaveRows + my_row) * kVPitch + my_dim);
+            put(v_tile, kKeys * kVPitch, vr[i], (i * kStepRows + wave * kWaveRows + my_row) * kVPitch + my_dim);
     };
 
     floatx16 o[DT];
@@ -289,17 +309,23 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
 
     // A step is two phases: V into LDS, the scores and their maximum; K of the next step
     // into LDS, the weights and their product with V.  Each reads what the phase before
-    // wrote, so K and V need one place each, and the second team runs a phase behind the
-    // first: one is at its scores while the other makes weights.
+    // wrote, so K and V need one place each.  With values in parts, whose products are most
+    // of a step, the second team runs a phase behind the first: one is at its scores while
+    // the other makes weights (512 fp32 rows over 32749 bf16 keys: 686 us against 771 side by
+    // side); without, they run side by side (a 2048-row fp16 prompt: 52.7 against 53.9).
     if (n_step) {
         load_k(0);
         load_v(0);
         has = has_2;
+    }
+    if constexpr (QP == 1) make_q();
+    const float s_hi = d.sl.hi * unit, s_lo = fmaxf(d.sl.lo * unit, 0x1p-126f);
+    if (n_step) {
         store_k();
         if (n_step > 1) load_k(1);
         has_1 = has_2;
     }
-    if (team == 1) __syncthreads();
+    if (kLag && team == 1) __syncthreads();
     for (int step = 0; step < n_run; ++step) {
         const int key0 = key_of(step);
         const bool real = step < n_step;
@@ -323,14 +349,14 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
                 for (int t = 0; t < KS; ++t)
 #pragma unroll
                     for (int y = 0; y < KP; ++y) {
-                        const vec8 x = *reinterpret_cast<const vec8 *>(&k_tile[y][from + 16 * t]);
+                        const vec8 x = *reinterpret_cast<const vec8 *>(&k_tile[y * kKeys * kKPitch + from + 16 * t]);
 #pragma unroll
                         for (int z = 0; z < QP; ++z)
-                            if (KP == 1 || y + z < KP) s[m] = Mma<C>::mul32(x, q[z][t], s[m]);
+                            if (KP == 1 || y + z < KP) s[m] = Mma<C>::mul32(x, z < kQReg ? q[z < kQReg ? z : 0][t] : q_third[wave][t][lane], s[m]);
                     }
             }
             // K's operands are requested kAhead products early
-            constexpr int kReads = MT * KS * KP, kAhead = 6, kPer = KP == 3 ? 2 : QP;
+            constexpr int kReads = MT * KS * (KP + kThird), kAhead = 6, kPer = KP == 3 ? 6 / (3 + kThird) : kThird ? 1 : QP;
             __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
             for (int i = 0; i < kReads - kAhead; ++i) {
@@ -386,7 +412,7 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
             // those 8 further of dim 32 i + m
             const int from = (4 * half + (lane & 15) / 4) * kVPitch + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
             const auto v_operand = [&](int plane, int t, int i) {
-                const C *at = &v_tile[plane][from + 16 * t * kVPitch + 32 * i];
+                const C *at = &v_tile[plane * kKeys * kVPitch + from + 16 * t * kVPitch + 32 * i];
                 const vec4 x = read_transposed<vec4>(at), y = read_transposed<vec4>(at + 8 * kVPitch);
                 return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
             };
@@ -419,12 +445,13 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
             }
         }
     }
-    if (kTeams == 2 && team == 0) __syncthreads();
+    if (kLag && team == 0) __syncthreads();
 
     sum = sum32(sum);
     if constexpr (kTeams == 2) {
         // the second team's sums through LDS, half of them at a time
-        float4 *const meet = team_o + wave * (HDP / 16) * 64 + lane;
+        float4 *const meet = reinterpret_cast<float4 *>(tiles) + wave * (HDP / 16) * 64 + lane;
+        __syncthreads();
         float f = 1.f, g = 0.f;
 #pragma unroll
         for (int part = 0; part < 2; ++part) {

@@ -100,43 +100,22 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode16_kernel(
     run.now = pages_from(0);
     run.ahead = -1;
 
-    // Q: B operand, lane (n, g) has dims 32 t + 8 g .. + 7 of its row
-    vec8 q[QP][KS];
-    float unit = 1.f;
+    // Q: B operand, lane (n, g) has dims 32 t + 8 g .. + 7 of its row.  Requested here, used
+    // when K and V are on their way.
+    A q_row[KS][8];
     {
-        float x[KS][8];
         const A *src = (const A *)a.q + (size_t)(row.real ? p.q0 + row.token : 0) * a.q_stride + (size_t)(row.real ? row.head : 0) * a.hd;
-        float big = 0;
+        const bool vec = ((uintptr_t)src & (8 * sizeof(A) - 1)) == 0;
 #pragma unroll
         for (int t = 0; t < KS; ++t) {
             const int dim = 32 * t + 8 * g;
-            A v[8];
-            const bool in = row.real && dim < a.hd;
-            if (in) load_n<8>(src + dim, v, ((uintptr_t)src & (8 * sizeof(A) - 1)) == 0);
+            if (row.real && dim < a.hd) load_n<8>(src + dim, q_row[t], vec);
+            else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[t][i] = in ? to_f32(v[i]) : 0.f;
-                big = fmaxf(big, fabsf(x[t][i]));
+                for (int i = 0; i < 8; ++i) q_row[t][i] = (A)0.f;
             }
         }
-        float to = 1.f;
-        if (QP == 2) unit_of(max32(max16(big)), to, unit);
-#pragma unroll
-        for (int t = 0; t < KS; ++t)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if constexpr (QP == 1) {
-                    q[0][t][i] = (C)x[t][i];
-                } else {
-                    C part[QP];
-                    split_q<QP>(x[t][i] * to, part);
-#pragma unroll
-                    for (int j = 0; j < QP; ++j) q[j][t][i] = part[j];
-                }
-            }
     }
-    const float s_hi = d.sl.hi * unit, s_lo = fmaxf(d.sl.lo * unit, 0x1p-126f);
-
     // A 16-key group lies in one page: a base that is the wave's, and a lane's offset
     // that does not change.  A group without a page reads page 0.
     const auto base_of = [&](const void *pool, int page, int key) {
@@ -186,6 +165,33 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode16_kernel(
         load_v(first_block * kBlock);
         run.ahead = pages_from(32);
     }
+    vec8 q[QP][KS];
+    float unit = 1.f;
+    {
+        float to = 1.f;
+        if constexpr (QP == 2) {
+            float big = 0;
+#pragma unroll
+            for (int t = 0; t < KS; ++t)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(q_row[t][i]));
+            unit_of(max32(max16(big)), to, unit);
+        }
+#pragma unroll
+        for (int t = 0; t < KS; ++t)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if constexpr (QP == 1) {
+                    q[0][t][i] = q_row[t][i];
+                } else {
+                    C part[QP];
+                    split_q<QP>(q_row[t][i] * to, part);
+#pragma unroll
+                    for (int j = 0; j < QP; ++j) q[j][t][i] = part[j];
+                }
+            }
+    }
+    const float s_hi = d.sl.hi * unit, s_lo = fmaxf(d.sl.lo * unit, 0x1p-126f);
     for (int j = 0; j < n_block; ++j) {
         const int key0 = (first_block + kWaves * j) * kBlock;
         const bool has0 = p0 >= 0, has1 = p1 >= 0;
