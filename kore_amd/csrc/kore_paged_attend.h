@@ -15,9 +15,24 @@
 
 namespace kore_paged_gpu {
 
+// Division by a number that a launch fixes: with 2^(s - 1) < d <= 2^s and m =
+// floor(2^(31 + s) / d) + 1, x m / 2^(31 + s) exceeds x / d by less than 1 / d for
+// 0 <= x < 2^31, so its whole part is the quotient.
+struct Divisor {
+    unsigned m;
+    int shift;
+    __host__ __device__ int of(int x) const { return (int)((unsigned long long)(unsigned)x * m >> shift); }
+};
+inline Divisor divisor(int d) {
+    int s = 0;
+    while ((1LL << s) < d) ++s;
+    return Divisor{(unsigned)((1ULL << (31 + s)) / (unsigned)d + 1), 31 + s};
+}
+
 // How a launch cuts its work; every field is the host's.
 struct Cut {
     int rep;         // q-heads of a kv-head
+    Divisor by_rep, by_heads;   // by rep, and by the kv-heads
     int target;      // workgroups to aim at, in tiles x keys; 0: nothing is split
     int min_len;     // a split's fewest keys
 };
@@ -34,6 +49,7 @@ struct TileArgs {
     AttendArgs a;
     Cut cut;
     ScaleLog2 sl;
+    bool q_wide, out_wide;   // q's rows can be read 16 bytes at a time, out's written four values at a time
     float *part_o, *part_ml;
 };
 
@@ -180,7 +196,7 @@ __device__ __forceinline__ bool place_of(const Batch &b, const Cut &c, int id, i
     int at = 0, splits_at = 0;
     for (int s0 = 0; s0 < b.n_seq; s0 += 64) {
         if (b.n_seq > 64) r = share(s0);   // (one round of loads where all sequences have a lane)
-        const int n_split = max(1, r.keys / len + (r.keys % len != 0));
+        const int n_split = c.target ? max(1, (r.keys + len - 1) / len) : 1;
         const int all = r.tiles * n_split * nkv, mine = by_tile ? r.tiles * nkv : all;
         const int upto = prefix_sum(mine), splits_upto = by_tile ? prefix_sum(all) : upto;
         const unsigned long long past = __ballot(at + upto > id);
@@ -193,12 +209,16 @@ __device__ __forceinline__ bool place_of(const Batch &b, const Cut &c, int id, i
             p.n = of(n);
             p.kv = of(kv);
             // the sequence's splits of equal length, in whole steps of 64 keys
-            p.len = scalar(((of(r.keys) + p.n_split - 1) / p.n_split + 63) & ~63);
+            p.len = p.n_split > 1 ? scalar(((of(r.keys) + p.n_split - 1) / p.n_split + 63) & ~63) : INT_MAX;
             int i = id - at - of(upto) + of(mine);
-            p.head = scalar(i % nkv);
-            i = scalar(i / nkv);
-            p.split = by_tile ? 0 : scalar(i % p.n_split);
-            if (!by_tile) i = scalar(i / p.n_split);
+            const int pairs = c.by_heads.of(i);
+            p.head = i - pairs * nkv;
+            i = pairs;
+            p.split = 0;
+            if (!by_tile && p.n_split > 1) {
+                i = scalar(pairs / p.n_split);
+                p.split = pairs - i * p.n_split;
+            }
             p.tile = scalar(of(r.tiles) - 1 - i);
             p.first = scalar(splits_at + of(splits_upto) - of(all) + i * p.n_split * nkv + p.head);
             return true;
@@ -216,8 +236,8 @@ struct Keys {
 };
 
 template <int TILE>
-__device__ __forceinline__ Keys keys_of(const Place &p, int rep, int cap, int window) {
-    const int t0 = scalar(p.tile * TILE / rep), t1 = min(p.n - 1, scalar((p.tile * TILE + TILE - 1) / rep));
+__device__ __forceinline__ Keys keys_of(const Place &p, const Cut &c, int cap, int window) {
+    const int t0 = c.by_rep.of(p.tile * TILE), t1 = min(p.n - 1, c.by_rep.of(p.tile * TILE + TILE - 1));
     const int p0 = p.kv - p.n + t0, p1 = p.kv - p.n + t1;   // positions of the first and last row
     Keys k;
     const int first = window <= p0 ? (p0 - window + 1) & ~63 : 0, end = min(p1 + 1, cap);
@@ -279,14 +299,15 @@ template <> struct Parts<float, bhalf_t> { static constexpr int q = 3, p = 3; };
 // that an infinity of K gives every product the same sign: an infinite score, as
 // in exact arithmetic, not NaN.  (A part set to its least value adds 2^-30 of the
 // value, or, for fp16, 2^-37 of the row's largest.)
+// (An infinite or NaN q makes its row NaN, in parts as in exact arithmetic.)
 template <int N>
 __device__ __forceinline__ void split_q(float x, bhalf_t (&part)[N]) {
-    const float h = bf16_cut(x);
-    part[0] = (bhalf_t)h;
+    const float h = bf16_cut(x), least = h * 0x1p-30f, r = x - h, m = bf16_cut(r), l = r - m;
+    const auto upper = [](float y) { return __builtin_bit_cast(bhalf_t, (unsigned short)(__builtin_bit_cast(unsigned, y) >> 16)); };
+    part[0] = upper(x);
     if constexpr (N == 3) {
-        const float r = finite(x) ? x - h : x, m = bf16_cut(r), l = finite(x) ? r - m : x, least = bf16_cut(h * 0x1p-30f);
-        part[1] = (bhalf_t)(m == 0.f ? least : m);
-        part[2] = (bhalf_t)(l == 0.f ? least : bf16_cut(l));
+        part[1] = upper(m == 0.f ? least : m);
+        part[2] = upper(l == 0.f ? least : l);
     }
 }
 template <int N>
@@ -352,15 +373,50 @@ struct Row {
     int token, head;
 };
 
-__device__ __forceinline__ Row row_of(const Place &p, int r, int rep, int cap, int window) {
+__device__ __forceinline__ Row row_of(const Place &p, int r, const Cut &c, int cap, int window) {
     Row x;
-    x.real = r < p.n * rep;
-    x.token = r / rep;
-    x.head = p.head * rep + (r - x.token * rep);
+    x.real = r < p.n * c.rep;
+    x.token = c.by_rep.of(r);
+    x.head = p.head * c.rep + (r - x.token * c.rep);
     const int pos = p.kv - p.n + x.token;
     x.lo = window <= pos ? pos - window + 1 : 0;
     x.hi = x.real ? min(pos + 1, cap) : 0;
     return x;
+}
+
+// N pieces of a row of q, 8 values each, piece t from dim first + step t: all requested
+// before one is used.  What is not there (a row past the last, dims past the head) is
+// something else of the row, for zero_q to clear when the rest has arrived.
+template <int N, class A>
+__device__ __forceinline__ void load_q(const AttendArgs &a, const Place &p, const Row &row, bool wide, int first, int step,
+                                       A (&x)[N][8]) {
+    const A *const src = (const A *)a.q + (size_t)(row.real ? p.q0 + row.token : p.q0) * a.q_stride +
+                         (size_t)(row.real ? row.head : 0) * a.hd;
+    if (wide) {
+        typedef A piece __attribute__((ext_vector_type(16 / sizeof(A))));
+        constexpr int kPer = 16 / sizeof(A);
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+#pragma unroll
+            for (int i = 0; i < 8; i += kPer) {
+                const piece v = *reinterpret_cast<const piece *>(src + min(first + step * t, a.hd - 8) + i);
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) x[t][i + j] = v[j];
+            }
+    } else {
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[t][i] = src[min(first + step * t, a.hd - 8) + i];
+    }
+}
+template <int N, class A>
+__device__ __forceinline__ void zero_q(const AttendArgs &a, const Row &row, int first, int step, A (&x)[N][8]) {
+#pragma unroll
+    for (int t = 0; t < N; ++t)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (!row.real || first + step * t >= a.hd) x[t][i] = (A)0.f;
 }
 
 // The pages of a wave's 16-key groups, 64 at a time in the lanes of a register and

@@ -113,9 +113,9 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
     auto &odd_of = all_odd[team];
     Place p;
     if (!place_of<kRows>(a.b, d.cut, blockIdx.x, a.n_head_kv, cap, a.window, false, p)) return;
-    const Keys k = keys_of<kRows>(p, rep, cap, a.window);
+    const Keys k = keys_of<kRows>(p, d.cut, cap, a.window);
     const int col = lane & 31, half = lane >> 5;
-    const Row row = row_of(p, p.tile * kRows + wave * 32 + col, rep, cap, a.window);
+    const Row row = row_of(p, p.tile * kRows + wave * 32 + col, d.cut, cap, a.window);
     const int *table = a.b.pages + (size_t)p.seq * a.b.pages_stride;
     const int slot_mask = (1 << a.page_shift) - 1;
     const bool padded = a.hd != HDP;
@@ -124,7 +124,7 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
     int see_lo, see_hi, all_lo, all_hi;
     {
         const int r0 = p.tile * kRows + wave * 32, r1 = min(r0 + 31, p.n * rep - 1);
-        const int p0 = p.kv - p.n + scalar(r0 / rep), p1 = p.kv - p.n + scalar(max(r1, 0) / rep);
+        const int p0 = p.kv - p.n + d.cut.by_rep.of(r0), p1 = p.kv - p.n + d.cut.by_rep.of(max(r1, 0));
         see_lo = a.window <= p0 ? p0 - a.window + 1 : 0;
         see_hi = r0 <= r1 ? min(p1 + 1, k.hi) : 0;
         all_lo = a.window <= p1 ? p1 - a.window + 1 : 0;
@@ -151,23 +151,12 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
     // Q: B operand, lane (n, half) has dims 16 t + 8 half .. + 7 of its row.  Requested here,
     // used when K and V are on their way.
     A q_row[KS][8];
-    {
-        const A *src = (const A *)a.q + (size_t)(row.real ? p.q0 + row.token : 0) * a.q_stride + (size_t)(row.real ? row.head : 0) * a.hd;
-        const bool vec = ((uintptr_t)src & (8 * sizeof(A) - 1)) == 0;
-#pragma unroll
-        for (int t = 0; t < KS; ++t) {
-            const int dim = 16 * t + 8 * half;
-            if (row.real && dim < a.hd) load_n<8>(src + dim, q_row[t], vec);
-            else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) q_row[t][i] = (A)0.f;
-            }
-        }
-    }
+    load_q<KS>(a, p, row, d.q_wide, 8 * half, 16, q_row);
 
     vec8 q[kQReg][KS];
     float unit = 1.f;
     const auto make_q = [&] {
+        zero_q<KS>(a, row, 8 * half, 16, q_row);
         float to = 1.f;
         if constexpr (QP == 2) {
             float big = 0;
@@ -506,14 +495,13 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
     if (!row.real) return;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     A *const out = (A *)a.out + (size_t)(p.q0 + row.token) * a.out_stride + (size_t)row.head * a.hd;
-    const bool vec = ((uintptr_t)out & (4 * sizeof(A) - 1)) == 0;
 #pragma unroll
     for (int i = 0; i < DT; ++i)
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
             const int dim = 32 * i + 8 * x + 4 * half;
             const A v[4] = {(A)(o[i][4 * x] * inv), (A)(o[i][4 * x + 1] * inv), (A)(o[i][4 * x + 2] * inv), (A)(o[i][4 * x + 3] * inv)};
-            if (dim < a.hd) store_n<4>(out + dim, v, vec);
+            if (dim < a.hd) store_n<4>(out + dim, v, d.out_wide);
         }
 }
 

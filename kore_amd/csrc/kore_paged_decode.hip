@@ -51,11 +51,11 @@ __device__ __forceinline__ void finish(const TileArgs &d, const Place &p, const 
         }
         const int r = p.tile * kRows + row;
         if (r >= p.n * rep || 4 * d4 >= a.hd) continue;
-        const int token = r / rep, head = p.head * rep + r - token * rep;
+        const int token = d.cut.by_rep.of(r), head = p.head * rep + r - token * rep;
         const float inv = l == 0.f ? 0.f : 1.f / l;
         A *out = (A *)a.out + (size_t)(p.q0 + token) * a.out_stride + (size_t)head * a.hd + 4 * d4;
         const A v[4] = {(A)(s.x * inv), (A)(s.y * inv), (A)(s.z * inv), (A)(s.w * inv)};
-        store_n<4>(out, v, ((uintptr_t)out & (4 * sizeof(A) - 1)) == 0);
+        store_n<4>(out, v, d.out_wide);
     }
 }
 
@@ -70,7 +70,10 @@ __device__ __forceinline__ void finish(const TileArgs &d, const Place &p, const 
 // banks).  No lane ever needs another's score but for the maximum and the sum.
 template <class A, class C, int HDP>
 __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode16_kernel(TileArgs d) {
-    constexpr int QP = Parts<A, C>::q, PP = Parts<A, C>::p;
+    // 16-bit rows could have their weights in one part; the second costs nothing beside the loads, and leaves the result
+    // no rounding but its own (bf16, one token over 131072 keys: error 1.7e-3 instead of 2.3e-3 of the result)
+    constexpr int QP = Parts<A, C>::q, PP = Parts<A, C>::p == 1 ? 2 : Parts<A, C>::p;
+    constexpr bool kExact = Parts<A, C>::p > 1;   // fp32 rows
     constexpr int KS = HDP / 32, DT = HDP / 16, VR = HDP / 16;   // k-steps, dim tiles, V registers of 16 bytes
     constexpr int kPitch = HDP + 16;                             // of a V row in LDS, elements
     constexpr int kBlock = 32;
@@ -83,9 +86,9 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode16_kernel(
     const int cap = a.b.pages_stride << a.page_shift, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Place p;
     if (!place_of<kRows>(a.b, d.cut, blockIdx.x, a.n_head_kv, cap, a.window, false, p)) return;
-    const Keys k = keys_of<kRows>(p, d.cut.rep, cap, a.window);
+    const Keys k = keys_of<kRows>(p, d.cut, cap, a.window);
     const int col = lane & 15, g = lane >> 4;
-    const Row row = row_of(p, p.tile * kRows + col, d.cut.rep, cap, a.window);
+    const Row row = row_of(p, p.tile * kRows + col, d.cut, cap, a.window);
     const int *table = a.b.pages + (size_t)p.seq * a.b.pages_stride;
     const int slot_mask = (1 << a.page_shift) - 1;
     const bool padded = a.hd != HDP;
@@ -103,19 +106,7 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode16_kernel(
     // Q: B operand, lane (n, g) has dims 32 t + 8 g .. + 7 of its row.  Requested here, used
     // when K and V are on their way.
     A q_row[KS][8];
-    {
-        const A *src = (const A *)a.q + (size_t)(row.real ? p.q0 + row.token : 0) * a.q_stride + (size_t)(row.real ? row.head : 0) * a.hd;
-        const bool vec = ((uintptr_t)src & (8 * sizeof(A) - 1)) == 0;
-#pragma unroll
-        for (int t = 0; t < KS; ++t) {
-            const int dim = 32 * t + 8 * g;
-            if (row.real && dim < a.hd) load_n<8>(src + dim, q_row[t], vec);
-            else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) q_row[t][i] = (A)0.f;
-            }
-        }
-    }
+    load_q<KS>(a, p, row, d.q_wide, 8 * g, 32, q_row);
     // A 16-key group lies in one page: a base that is the wave's, and a lane's offset
     // that does not change.  A group without a page reads page 0.
     const auto base_of = [&](const void *pool, int page, int key) {
@@ -168,6 +159,7 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode16_kernel(
     vec8 q[QP][KS];
     float unit = 1.f;
     {
+        zero_q<KS>(a, row, 8 * g, 32, q_row);
         float to = 1.f;
         if constexpr (QP == 2) {
             float big = 0;
@@ -262,12 +254,11 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode16_kernel(
         for (int m = 0; m < 2; ++m)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float e = PP > 1 ? fmaf(s[m][i], s_hi, fmaf(s[m][i], s_lo, -base)) : fmaf(s[m][i], s_hi, -base);
+                const float e = kExact ? fmaf(s[m][i], s_hi, fmaf(s[m][i], s_lo, -base)) : fmaf(s[m][i], s_hi, -base);
                 const float x = exp2_(e);
                 C part[PP];
                 split_p<PP>(x, part);
-                // one rounded weight is also what is summed: what rounding adds to all of a row's weights divides out
-                sum += PP > 1 ? x : to_f32(part[0]);
+                sum += x;
 #pragma unroll
                 for (int y = 0; y < PP; ++y) w[y][4 * m + i] = part[y];
             }
@@ -324,9 +315,9 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode32_kernel(
     const int cap = a.b.pages_stride << a.page_shift, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Place p;
     if (!place_of<kRows>(a.b, d.cut, blockIdx.x, a.n_head_kv, cap, a.window, false, p)) return;
-    const Keys k = keys_of<kRows>(p, d.cut.rep, cap, a.window);
+    const Keys k = keys_of<kRows>(p, d.cut, cap, a.window);
     const int col = lane & 15, g = lane >> 4;
-    const Row row = row_of(p, p.tile * kRows + col, d.cut.rep, cap, a.window);
+    const Row row = row_of(p, p.tile * kRows + col, d.cut, cap, a.window);
     const int *table = a.b.pages + (size_t)p.seq * a.b.pages_stride;
     const int slot_mask = (1 << a.page_shift) - 1;
     const bool padded = a.hd != HDP;
@@ -341,14 +332,13 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode32_kernel(
 
     floatx4 q[KU];
     {
-        const float *src = (const float *)a.q + (size_t)(row.real ? p.q0 + row.token : 0) * a.q_stride + (size_t)(row.real ? row.head : 0) * a.hd;
-        const bool vec = ((uintptr_t)src & 15) == 0;
+        const float *const src = (const float *)a.q + (size_t)(row.real ? p.q0 + row.token : p.q0) * a.q_stride +
+                                 (size_t)(row.real ? row.head : 0) * a.hd;
 #pragma unroll
         for (int u = 0; u < KU; ++u) {
-            const int dim = 16 * u + 4 * g;
-            float v[4] = {0, 0, 0, 0};
-            if (row.real && dim < a.hd) load_n<4>(src + dim, v, vec);
-            q[u] = floatx4{v[0], v[1], v[2], v[3]};
+            const float *const at = src + min(16 * u + 4 * g, a.hd - 4);
+            if (d.q_wide) q[u] = *reinterpret_cast<const floatx4 *>(at);
+            else q[u] = floatx4{at[0], at[1], at[2], at[3]};
         }
     }
     const auto base_of = [&](const void *pool, int page, int key) {
@@ -384,6 +374,9 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode32_kernel(
         load_v(first_block * kBlock);
         run.ahead = pages_from(64);
     }
+#pragma unroll
+    for (int u = 0; u < KU; ++u)
+        if (!row.real || 16 * u + 4 * g >= a.hd) q[u] = floatx4{0, 0, 0, 0};
     for (int j = 0; j < n_block; ++j) {
         const int key0 = (first_block + kWaves * j) * kBlock;
         const bool has = page >= 0, whole = key0 >= k.all_lo && key0 + kBlock <= min(k.all_hi, k.hi) && has;
@@ -497,9 +490,8 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(TileArgs d, int hd4) {
     const int row = threadIdx.x % TILE, lane = threadIdx.x / TILE, part = lane & (parts - 1), wide = kLanes / parts;
     const size_t step = (size_t)a.n_head_kv * TILE;
     const float2 *const pm = reinterpret_cast<const float2 *>(d.part_ml) + (size_t)p.first * TILE + row;
-    const int r = p.tile * TILE + row, token = r / d.cut.rep, head = p.head * d.cut.rep + r - token * d.cut.rep;
+    const int r = p.tile * TILE + row, token = d.cut.by_rep.of(r), head = p.head * d.cut.rep + r - token * d.cut.rep;
     A *const out = (A *)a.out + (size_t)(p.q0 + token) * a.out_stride + (size_t)head * a.hd;
-    const bool vec = ((uintptr_t)out & (4 * sizeof(A) - 1)) == 0;
     for (int d0 = blockIdx.y * wide; 4 * d0 < a.hd; d0 += gridDim.y * wide) {
         const int d4 = d0 + lane / parts;
         const bool real = 4 * d4 < a.hd;
@@ -550,7 +542,7 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(TileArgs d, int hd4) {
             }
             const float inv = l == 0.f ? 0.f : 1.f / l;
             const A w[4] = {(A)(s.x * inv), (A)(s.y * inv), (A)(s.z * inv), (A)(s.w * inv)};
-            store_n<4>(out + 4 * d4, w, vec);
+            store_n<4>(out + 4 * d4, w, d.out_wide);
         }
         __syncthreads();
     }
@@ -594,8 +586,17 @@ hipError_t launch_attend(const AttendArgs &a, hipStream_t s) {
     TileArgs d{};
     d.a = a;
     d.cut.rep = a.n_head / a.n_head_kv;
+    d.cut.by_rep = divisor(d.cut.rep);
+    d.cut.by_heads = divisor(a.n_head_kv);
+    const int size = type_bytes(a.type);   // (a head is a multiple of 8 values)
+    d.q_wide = (uintptr_t)a.q % 16 == 0 && a.q_stride * size % 16 == 0;
+    d.out_wide = (uintptr_t)a.out % (4 * size) == 0 && a.out_stride % 4 == 0;
     const int max_q = a.max_q ? a.max_q : (a.b.n_tok + a.b.n_seq - 1) / a.b.n_seq;
-    const bool chunk = (long long)max_q * d.cut.rep > kRows;
+    // Tiles of 16 rows read a sequence's keys once each, most of it from L2: up to three of them beat one of 128.  us, 16 /
+    // 128 rows a tile, 28/4/128 at 32768 keys, new rows 2, 6, 9, 18: fp16 20.0 / 26.0, 27.1 / 26.1, 41.8 / 26.2, 52.3 /
+    // 28.3; fp32 rows and cache 31 / 59, 55 / 60, 79 / 61, 122 / 66; 16 sequences of 2048, fp16: 22.9 / 29.7, 29.8 / 30.4,
+    // 29.8 / 30.3, 45.9 / 37.9.
+    const bool chunk = (long long)max_q * d.cut.rep > 3 * kRows;
     const int rows = chunk ? kChunkRows : kRows;
     // the most (tile, kv-head)s that n_tok rows of n_seq sequences can be
     const long long tiles = ((long long)a.b.n_tok * d.cut.rep / rows + std::min(a.b.n_seq, a.b.n_tok)) * a.n_head_kv;
