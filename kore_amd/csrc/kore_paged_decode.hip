@@ -82,6 +82,8 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode16_kernel(
     constexpr size_t kVBytes = sizeof(C) * kWaves * kBlock * kPitch, kOBytes = sizeof(float) * kWaves * HDP * kRows;
     __shared__ __attribute__((aligned(16))) unsigned char shared[kVBytes > kOBytes ? kVBytes : kOBytes];
     __shared__ float2 ml[kWaves][kRows];
+    // of V's pieces in blocks that the tile's rows do not all see: which of 8 dims are +inf, or -inf (a NaN: both)
+    __shared__ unsigned kinds[kWaves][2][kBlock][HDP / 32];
     const AttendArgs &a = d.a;
     const int cap = a.b.pages_stride << a.page_shift, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Place p;
@@ -216,15 +218,29 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode16_kernel(
         }
         if (next < n_block) load_k(next_key);
 
-        bool odd = false;   // an infinity or NaN of V that some row sees and another does not
+        // Where the tile's rows differ in what they see, V of positions that none sees is 0, and
+        // infinities and NaN are 0 too and noted apart: a product with a weight of 0 would hand
+        // them to every row.
+        bool odd = false;
         if (!whole) {
 #pragma unroll
             for (int r = 0; r < VR; ++r) {
-                const int key = key0 + kRowsPer * r + v_row;
-                // V of positions that no row sees may hold anything
-                if (!(key < k.hi && (kRowsPer * r >= 16 ? has1 : has0))) vr[r] = vec8{};
+                const int key = kRowsPer * r + v_row;
+                if (!(key0 + key < k.hi && (kRowsPer * r >= 16 ? has1 : has0))) vr[r] = vec8{};
+                unsigned up = 0, down = 0;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) odd |= !finite(to_f32(vr[r][i]));
+                for (int i = 0; i < 8; ++i) {
+                    const float v = to_f32(vr[r][i]);
+                    if (!finite(v)) {
+                        if (!(v < 0.f)) up |= 1u << i;
+                        if (!(v > 0.f)) down |= 1u << i;
+                        vr[r][i] = (C)0.f;
+                    }
+                }
+                unsigned char *const at = reinterpret_cast<unsigned char *>(kinds[wave][0][key]) + v_dim / 8;
+                at[0] = (unsigned char)up;
+                at[sizeof kinds[0][0]] = (unsigned char)down;
+                odd |= (up | down) != 0;
             }
             odd = __any(odd);
         }
@@ -262,30 +278,25 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode16_kernel(
 #pragma unroll
                 for (int y = 0; y < PP; ++y) w[y][4 * m + i] = part[y];
             }
-        if (!odd) {
 #pragma unroll
-            for (int i = 0; i < DT; ++i) {
-                const vec8 v = v_operand(i);
+        for (int i = 0; i < DT; ++i) {
+            const vec8 v = v_operand(i);
 #pragma unroll
-                for (int y = 0; y < PP; ++y) o[i] = Mma<C>::mul16(v, w[y], o[i]);
-            }
-        } else {
-            // key by key, each added only to the rows that see it
+            for (int y = 0; y < PP; ++y) o[i] = Mma<C>::mul16(v, w[y], o[i]);
+        }
+        if (odd) {
             for (int e = 0; e < kBlock; ++e) {
-                const int key = key0 + e, mine = 4 * (e >> 4) + (e & 3);
-                const bool sees = key >= row.lo && key < row.hi, here = ((e >> 2) & 3) == g;
+                const bool sees = key0 + e >= row.lo && key0 + e < min(row.hi, k.hi);
 #pragma unroll
                 for (int i = 0; i < DT; ++i) {
-                    vec8 v = v_operand(i);
+                    const int from = 16 * (i & 1) + 4 * g;
+                    const unsigned up = sees ? kinds[wave][0][e][i / 2] >> from : 0, down = sees ? kinds[wave][1][e][i / 2] >> from : 0;
+                    if (!__any((up | down) & 15)) continue;
 #pragma unroll
-                    for (int x = 0; x < 8; ++x)
-                        if (!here || x != mine) v[x] = (C)0.f;
-                    floatx4 t = floatx4{0, 0, 0, 0};
-#pragma unroll
-                    for (int y = 0; y < PP; ++y) t = Mma<C>::mul16(v, w[y], t);
-#pragma unroll
-                    for (int x = 0; x < 4; ++x)
-                        if (sees) o[i][x] += t[x];
+                    for (int x = 0; x < 4; ++x) {
+                        if (up >> x & 1) o[i][x] += INFINITY;
+                        if (down >> x & 1) o[i][x] -= INFINITY;
+                    }
                 }
             }
         }
