@@ -43,20 +43,5 @@ __device__ __forceinline__ void store_n(T *p, const T (&x)[N], bool vec) {
     }
 }
 
-// Number of sequences that end at or before row (q_start ascending), counted by
-// a whole wave, 64 table entries at a time: the row's sequence, or n_seq where
-// the row lies behind the last one.  The loads of one wave do not depend on each
-// other, as those of a binary search would.
-__device__ __forceinline__ int seq_of_row(const Batch &b, int row) {
-    const int lane = threadIdx.x & 63;
-    int n = 0;
-    for (int s0 = 0; s0 < b.n_seq; s0 += 64) {
-        const int s = s0 + lane;
-        const bool before = s < b.n_seq && b.q_start[s + 1] <= row;
-        n += __popcll(__ballot(before));
-    }
-    return n;
-}
-
 }  // namespace
 }  // namespace kore_paged_gpu

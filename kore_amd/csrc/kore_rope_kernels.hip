@@ -48,25 +48,30 @@ __device__ __forceinline__ float2 cos_sin(int pos, float freq, double size) {
     return make_float2((float)(size * cc), (float)(size * ss));
 }
 
-// One unit of a head: V pairs, or 2 V dims behind the rotated ones, which are
-// copied.  cs: the row's (cos, sin) of every pair.
+// One unit of a head: V pairs, or 2 V dims behind the rotated ones, which are copied.
+// Where its two halves lie, and the turn; cs: the row's (cos, sin) of every pair.
+template <int V>
+struct Unit {
+    int at0, at1;
+    bool turned;
+    __device__ __forceinline__ Unit(int unit, int rot, bool interleaved) {
+        turned = unit < rot / (2 * V);
+        const bool near = !turned || interleaved;
+        at0 = near ? unit * 2 * V : unit * V;
+        at1 = near ? at0 + V : at0 + rot / 2;
+    }
+};
 template <int V, class T, class O>
-__device__ __forceinline__ void turn_unit(const T *x, O *y, int unit, int rot, bool interleaved, const float2 *cs,
-                                          float sign) {
+__device__ __forceinline__ void turn_unit(const Unit<V> &where, const T (&a)[V], const T (&b)[V], O *y, int unit,
+                                          bool interleaved, const float2 *cs, float sign) {
 #pragma clang fp contract(off)
-    const int n_turn = rot / (2 * V);
-    const bool turned = unit < n_turn, near = !turned || interleaved;
-    const int at0 = near ? unit * 2 * V : unit * V, at1 = near ? at0 + V : at0 + rot / 2;
-    T a[V], b[V];
-    load_n<V>(x + at0, a, true);
-    load_n<V>(x + at1, b, true);
     float u[2 * V], w[2 * V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         u[i] = to_f32(a[i]);
         u[V + i] = to_f32(b[i]);
     }
-    if (!turned) {
+    if (!where.turned) {
 #pragma unroll
         for (int i = 0; i < 2 * V; ++i) w[i] = u[i];
     } else {
@@ -74,10 +79,10 @@ __device__ __forceinline__ void turn_unit(const T *x, O *y, int unit, int rot, b
         for (int i = 0; i < V; ++i) {
             const float2 c = cs[unit * V + i];
             const float sn = sign * c.y;
-            const int p0 = interleaved ? 2 * i : i, p1 = interleaved ? 2 * i + 1 : V + i;
-            const float e = u[p0] * c.x, f = u[p1] * sn, g = u[p0] * sn, h = u[p1] * c.x;
-            w[p0] = e - f;
-            w[p1] = g + h;
+            const float u0 = interleaved ? u[2 * i] : u[i], u1 = interleaved ? u[2 * i + 1] : u[V + i];
+            const float e = u0 * c.x, f = u1 * sn, g = u0 * sn, h = u1 * c.x;
+            w[interleaved ? 2 * i : i] = e - f;
+            w[interleaved ? 2 * i + 1 : V + i] = g + h;
         }
     }
     O r[V], t[V];
@@ -86,8 +91,8 @@ __device__ __forceinline__ void turn_unit(const T *x, O *y, int unit, int rot, b
         r[i] = (O)w[i];
         t[i] = (O)w[V + i];
     }
-    store_n<V>(y + at0, r, true);
-    store_n<V>(y + at1, t, true);
+    store_n<V>(y + where.at0, r, true);
+    store_n<V>(y + where.at1, t, true);
 }
 
 // The (cos, sin) of a block's row, one pair a thread.
@@ -96,55 +101,112 @@ __device__ __forceinline__ void stage_turn(const Turn &t, int pos, float2 *cs) {
     __syncthreads();
 }
 
-// A block takes one row; its threads are laid over (head, unit).
-template <class T, int V>
+// A block takes one row's units, or a gridDim.y-th of them (of few rows, so that a
+// thread has about one); a thread's first kEarly are requested before the turn is
+// computed.
+constexpr int kEarly = 3;
+
+template <class T, int V, bool INTER>
 __global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs a) {
     __shared__ float2 cs[kMaxRot / 2];
     const int row = blockIdx.x;
-    stage_turn(a.turn, a.pos[row], cs);
     const T *x = (const T *)a.x + (size_t)row * a.x_stride;
     T *y = (T *)a.out + (size_t)row * a.out_stride;
-    const int units = a.hd / (2 * V), total = units * a.n_head;
-    for (int i = threadIdx.x; i < total; i += kThreads) {
-        const int head = i / units, unit = i - head * units;
-        turn_unit<V>(x + (size_t)head * a.hd, y + (size_t)head * a.hd, unit, a.turn.rot, a.turn.interleaved, cs,
-                     (float)a.sign);
+    const int units = a.hd / (2 * V), total = units * a.n_head, step = kThreads * gridDim.y;
+    const int first = blockIdx.y * kThreads + threadIdx.x;
+    T va[kEarly][V], vb[kEarly][V];
+    const auto request = [&](int j, int i) {
+        const int head = i / units;
+        const Unit<V> u(i - head * units, a.turn.rot, INTER);
+        load_n<V>(x + (size_t)head * a.hd + u.at0, va[j], true);
+        load_n<V>(x + (size_t)head * a.hd + u.at1, vb[j], true);
+    };
+#pragma unroll
+    for (int j = 0; j < kEarly; ++j)
+        if (first + j * step < total) request(j, first + j * step);
+    stage_turn(a.turn, a.pos[row], cs);
+    for (int i0 = first; i0 < total; i0 += kEarly * step) {
+#pragma unroll
+        for (int j = 0; j < kEarly; ++j) {
+            const int i = i0 + j * step, head = i / units, unit = i - head * units;
+            if (i < total) {
+                if (i0 != first) request(j, i);
+                turn_unit<V>(Unit<V>(unit, a.turn.rot, INTER), va[j], vb[j], y + (size_t)head * a.hd, unit, INTER, cs, (float)a.sign);
+            }
+        }
     }
 }
 
-// A block takes one row: its k heads into the pool, its v heads into the pool,
-// and its q heads (where there are any).
-template <class T, class C, int V>
+// k heads into the pool, v heads into the pool, and q heads (where there are any).
+template <class T, class C, int V, bool INTER>
 __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a) {
     __shared__ float2 cs[kMaxRot / 2];
-    const int row = blockIdx.x;
-    const int seq = seq_of_row(a.b, row);
-    if (seq >= a.b.n_seq || row < a.b.q_start[seq]) return;
-    const int pos = a.b.kv_len[seq] - (a.b.q_start[seq + 1] - row);
+    const int row = blockIdx.x, lane = threadIdx.x & 63;
+    const int units = a.hd / (2 * V), nq = a.q ? a.n_head : 0, total = units * (nq + 2 * a.n_head_kv);
+    const int step = kThreads * gridDim.y, first = blockIdx.y * kThreads + threadIdx.x;
+    T va[kEarly][V], vb[kEarly][V];
+    // head nq + j: k's j, then v's
+    const auto request = [&](int j, int i) {
+        const int head = i / units, kv = head - nq;
+        const bool is_v = kv >= a.n_head_kv;
+        const Unit<V> u(i - head * units, is_v ? 0 : a.turn.rot, INTER);
+        const T *src = head < nq ? (const T *)a.q + (size_t)row * a.q_stride + (size_t)head * a.hd
+                     : is_v ? (const T *)a.v + (size_t)row * a.v_stride + (size_t)(kv - a.n_head_kv) * a.hd
+                            : (const T *)a.k + (size_t)row * a.k_stride + (size_t)kv * a.hd;
+        load_n<V>(src + u.at0, va[j], true);
+        load_n<V>(src + u.at1, vb[j], true);
+    };
+#pragma unroll
+    for (int j = 0; j < kEarly; ++j)
+        if (first + j * step < total) request(j, first + j * step);
+    // the row's sequence, each wave for itself, 64 at a time: one round of loads
+    int seq = -1, pos = 0;
+    for (int s0 = 0; s0 < a.b.n_seq && seq < 0; s0 += 64) {
+        const int s = s0 + lane;
+        int from = 0, to = 0, len = 0;
+        if (s < a.b.n_seq) {
+            from = a.b.q_start[s];
+            to = a.b.q_start[s + 1];
+            len = a.b.kv_len[s];
+        }
+        const unsigned long long here = __ballot(from <= row && row < to);
+        if (here) {
+            const int l = __builtin_ctzll(here);
+            seq = s0 + l;
+            pos = __builtin_amdgcn_readlane(len, l) - (__builtin_amdgcn_readlane(to, l) - row);
+        }
+    }
+    if (seq < 0) return;
     const int at = pos >> a.page_shift;
     const int page = pos >= 0 && at < a.b.pages_stride ? a.b.pages[(size_t)seq * a.b.pages_stride + at] : -1;
-    const bool stored = page >= 0 && page < a.n_pages;
     stage_turn(a.turn, pos, cs);
-    const int units = a.hd / (2 * V), nq = a.q ? a.n_head : 0, total = units * (nq + 2 * a.n_head_kv);
+    const bool stored = page >= 0 && page < a.n_pages;
     const int slot = pos & ((1 << a.page_shift) - 1);
-    for (int i = threadIdx.x; i < total; i += kThreads) {
-        int head = i / units;
-        const int unit = i - head * units;
-        if (head < nq) {
-            turn_unit<V>((const T *)a.q + (size_t)row * a.q_stride + (size_t)head * a.hd,
-                         (T *)a.q_out + (size_t)row * a.q_out_stride + (size_t)head * a.hd, unit, a.turn.rot,
-                         a.turn.interleaved, cs, 1.0f);
-            continue;
+    for (int i0 = first; i0 < total; i0 += kEarly * step) {
+#pragma unroll
+        for (int j = 0; j < kEarly; ++j) {
+            const int i = i0 + j * step, head = i / units, unit = i - head * units;
+            if (i >= total) continue;
+            if (i0 != first) request(j, i);
+            if (head < nq) {
+                turn_unit<V>(Unit<V>(unit, a.turn.rot, INTER), va[j], vb[j],
+                             (T *)a.q_out + (size_t)row * a.q_out_stride + (size_t)head * a.hd, unit, INTER, cs, 1.0f);
+            } else if (stored) {
+                const bool is_v = head - nq >= a.n_head_kv;
+                const int kv = is_v ? head - nq - a.n_head_kv : head - nq;
+                const size_t to = ((((size_t)page * a.n_head_kv + kv) << a.page_shift) + slot) * a.hd;
+                turn_unit<V>(Unit<V>(unit, is_v ? 0 : a.turn.rot, INTER), va[j], vb[j], (C *)(is_v ? a.v_pool : a.k_pool) + to,
+                             unit, INTER, cs, 1.0f);
+            }
         }
-        if (!stored) continue;
-        head -= nq;
-        const bool is_v = head >= a.n_head_kv;
-        if (is_v) head -= a.n_head_kv;
-        const size_t to = ((((size_t)page * a.n_head_kv + head) << a.page_shift) + slot) * a.hd;
-        const T *x = is_v ? (const T *)a.v + (size_t)row * a.v_stride : (const T *)a.k + (size_t)row * a.k_stride;
-        turn_unit<V>(x + (size_t)head * a.hd, (C *)(is_v ? a.v_pool : a.k_pool) + to, unit, is_v ? 0 : a.turn.rot,
-                     a.turn.interleaved, cs, 1.0f);
     }
+}
+
+// Workgroups that share a row: as many as give a thread one unit while the launch has
+// less than four a CU or so.
+dim3 row_grid(int n_tok, int total) {
+    const int most = (total + kThreads - 1) / kThreads;
+    return dim3((unsigned)n_tok, (unsigned)std::clamp(1024 / n_tok, 1, most));
 }
 
 // Four values at once where rows, heads and the two parts of a head start at
@@ -160,10 +222,13 @@ bool aligned(int bytes, P... p) {
 hipError_t launch_rope(const RopeArgs &a, hipStream_t s) {
     const bool v4 = fours(a.turn.rot, a.hd) && a.x_stride % 4 == 0 && a.out_stride % 4 == 0 &&
                     aligned(type_bytes(a.type), a.x, a.out);
-#define KORE_ROPE_CASE(T)                                                             \
-    do {                                                                              \
-        if (v4) rope_kernel<T, 4><<<a.n_tok, kThreads, 0, s>>>(a);                    \
-        else rope_kernel<T, 1><<<a.n_tok, kThreads, 0, s>>>(a);                       \
+    const dim3 grid = row_grid(a.n_tok, a.hd / (v4 ? 8 : 2) * a.n_head);
+#define KORE_ROPE_CASE(T)                                                                         \
+    do {                                                                                          \
+        if (v4 && a.turn.interleaved) rope_kernel<T, 4, true><<<grid, kThreads, 0, s>>>(a);       \
+        else if (v4) rope_kernel<T, 4, false><<<grid, kThreads, 0, s>>>(a);                       \
+        else if (a.turn.interleaved) rope_kernel<T, 1, true><<<grid, kThreads, 0, s>>>(a);        \
+        else rope_kernel<T, 1, false><<<grid, kThreads, 0, s>>>(a);                               \
     } while (0)
     if (a.type == kF32) KORE_ROPE_CASE(float);
     else if (a.type == kF16) KORE_ROPE_CASE(half_t);
@@ -177,10 +242,13 @@ hipError_t launch_append(const AppendArgs &a, hipStream_t s) {
     const bool v4 = fours(a.turn.rot, a.hd) && a.k_stride % 4 == 0 && a.v_stride % 4 == 0 &&
                     (!a.q || (a.q_stride % 4 == 0 && a.q_out_stride % 4 == 0)) &&
                     aligned(tb, a.k, a.v, a.q, a.q_out) && aligned(cb, a.k_pool, a.v_pool);
-#define KORE_APPEND_CASE(T, C)                                                        \
-    do {                                                                              \
-        if (v4) append_kernel<T, C, 4><<<a.b.n_tok, kThreads, 0, s>>>(a);             \
-        else append_kernel<T, C, 1><<<a.b.n_tok, kThreads, 0, s>>>(a);                \
+    const dim3 grid = row_grid(a.b.n_tok, a.hd / (v4 ? 8 : 2) * ((a.q ? a.n_head : 0) + 2 * a.n_head_kv));
+#define KORE_APPEND_CASE(T, C)                                                                    \
+    do {                                                                                          \
+        if (v4 && a.turn.interleaved) append_kernel<T, C, 4, true><<<grid, kThreads, 0, s>>>(a);  \
+        else if (v4) append_kernel<T, C, 4, false><<<grid, kThreads, 0, s>>>(a);                  \
+        else if (a.turn.interleaved) append_kernel<T, C, 1, true><<<grid, kThreads, 0, s>>>(a);   \
+        else append_kernel<T, C, 1, false><<<grid, kThreads, 0, s>>>(a);                          \
     } while (0)
     if (a.type == kF32 && a.cache_type == kF32) KORE_APPEND_CASE(float, float);
     else if (a.type == kF32 && a.cache_type == kF16) KORE_APPEND_CASE(float, half_t);
