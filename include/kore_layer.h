@@ -17,11 +17,12 @@
  * kore_attn.h, kore_qmv.h), so a layer's result agrees with kore's to that
  * tolerance.
  *
- * Link with -lkore_layer -lkore_qmv -lkore_attn.  No CPU fallback. */
+ * Link with -lkore_layer -lkore_qmv -lkore_attn -lkore_paged.  No CPU fallback. */
 #ifndef KORE_LAYER_H
 #define KORE_LAYER_H
 
 #include "kore_attn.h"
+#include "kore_paged.h"
 #include "kore_qmv.h"
 
 #ifdef __cplusplus
@@ -82,6 +83,19 @@ KORE_LAYER_API int kore_layer_decode_dev(kore_layer_t L, const kore_layer_weight
  * rules as kore_layer_decode_dev. */
 KORE_LAYER_API int kore_layer_prefill_dev(kore_layer_t L, const kore_layer_weights *w, kore_attn_t attn, int layer,
                                           int pos0, int n_tok, float *x, void *stream);
+
+/* The same body (forward_batch()'s) over the new rows of several sequences at
+ * once: x (device, [n_tok][n_embd], n_tok 1..64, 16-byte aligned), the rows of
+ * the batch `b`, one a sequence in a decode step, chunks of prompts, or both.
+ * In place of step 2 the rows are rotated and appended to layer `layer` of the
+ * paged cache `kv` (kore_paged_append_dev, with the cache's rotation) and
+ * attend their sequences (kore_paged_attend_dev; workspace as there).  kore
+ * has no counterpart: its engine holds one sequence.  Rows of x that belong to
+ * no sequence hold nothing of use afterwards.  Results hold kore's tolerance
+ * with an fp32 cache; a 16-bit cache adds its own rounding of K and V.  Same
+ * stream and scratch rules as kore_layer_decode_dev. */
+KORE_LAYER_API int kore_layer_paged_dev(kore_layer_t L, const kore_layer_weights *w, kore_paged_t kv, int layer,
+                                        const kore_paged_batch *b, float *x, void *workspace, void *stream);
 
 /* Wait for the layer's own stream. */
 KORE_LAYER_API int kore_layer_sync(kore_layer_t L);

@@ -93,14 +93,20 @@ KORE_LAYER_API void kore_layer_destroy(kore_layer_t L) {
 
 namespace {
 
-// The checks both layer steps make on their arguments.
-int check_call(kore_layer *L, const kore_layer_weights *w, kore_attn_t attn, const float *x) {
-    if (!w || !attn || !x || ((uintptr_t)x & 15)) return fail(L, KORE_LAYER_E_INVALID, "w, attn or x missing or x unaligned");
+// The checks that the layer steps make on their arguments: the weights and x, and
+// the contiguous cache.
+int check_weights(kore_layer *L, const kore_layer_weights *w) {
     if (!w->attn_norm || !w->ffn_norm) return fail(L, KORE_LAYER_E_INVALID, "attn_norm and ffn_norm are required");
     const int64_t E = L->E, FF = L->FF, kvd = L->kvd;
     if (!shape_is(w->wq, E, E) || !shape_is(w->wk, kvd, E) || !shape_is(w->wv, kvd, E) || !shape_is(w->wo, E, E) ||
         !shape_is(w->w_gate, FF, E) || !shape_is(w->w_up, FF, E) || !shape_is(w->w_down, E, FF))
         return fail(L, KORE_LAYER_E_INVALID, "a weight tensor's shape does not match the layer geometry");
+    return KORE_LAYER_OK;
+}
+
+int check_call(kore_layer *L, const kore_layer_weights *w, kore_attn_t attn, const float *x) {
+    if (!w || !attn || !x || ((uintptr_t)x & 15)) return fail(L, KORE_LAYER_E_INVALID, "w, attn or x missing or x unaligned");
+    if (int rc = check_weights(L, w)) return rc;
     kore_attn_info ai{};
     if (kore_attn_get_info(attn, &ai) != KORE_ATTN_OK || ai.n_head != L->n_head || ai.n_head_kv != L->n_head_kv ||
         ai.head_dim != L->head_dim)
@@ -152,12 +158,13 @@ KORE_LAYER_API int kore_layer_decode_dev(kore_layer_t L, const kore_layer_weight
     return KORE_LAYER_OK;
 }
 
-KORE_LAYER_API int kore_layer_prefill_dev(kore_layer_t L, const kore_layer_weights *w, kore_attn_t attn, int layer,
-                                          int pos0, int n_tok, float *x, void *stream) {
-    if (!L) return fail(nullptr, KORE_LAYER_E_INVALID, "layer handle is NULL");
-    if (int rc = check_call(L, w, attn, x)) return rc;
-    if (n_tok < 1 || n_tok > kMaxBatch) return fail(L, KORE_LAYER_E_INVALID, "n_tok must be 1..64 (kore's KORE_BMAX)");
-    void *s = stream ? stream : (void *)L->stream;
+extern "C++" {
+namespace {
+
+// forward_batch()'s body for a layer over n_tok rows x, with `attend` between the
+// q/k/v projections (L->bq, bk, bv) and Wo (L->batt).
+template <class Attend>
+int rows_step(kore_layer *L, const kore_layer_weights *w, int n_tok, float *x, void *s, const Attend &attend) {
     const int64_t E = L->E, FF = L->FF;
     auto qmv_err = [&](kore_qmv_tensor_t t, const char *what) {
         return fail(L, KORE_LAYER_E_STEP, std::string(what) + ": " + kore_qmv_last_error(t));
@@ -189,9 +196,7 @@ KORE_LAYER_API int kore_layer_prefill_dev(kore_layer_t L, const kore_layer_weigh
     float *qkv_out[3] = {L->bq, L->bk, L->bv};
     if (int rc = norm_matmul(w->attn_norm, 3, qkv, &o1, qkv_out, "attn_norm, q/k/v")) return rc;
     // 2. RoPE + append + causal attention of the rows (kore.cpp:1533-1563)
-    if (kore_attn_prefill_dev(attn, layer, pos0, n_tok, L->n_head, L->n_head_kv, L->head_dim, L->bq, L->bk, L->bv,
-                              L->batt, s) != KORE_ATTN_OK)
-        return fail(L, KORE_LAYER_E_STEP, std::string("attention: ") + kore_attn_last_error(attn));
+    if (int rc = attend()) return rc;
     // 3. Wo, x += o (kore.cpp:1566-1570)
     kore_qmv_mv_opts acc{};
     acc.accumulate = 1;
@@ -214,6 +219,50 @@ KORE_LAYER_API int kore_layer_prefill_dev(kore_layer_t L, const kore_layer_weigh
     if (kore_qmv_matmul_batch_group_ex_dev(1, &w->w_down, L->bgate, n_tok, &acc, &x, s) != KORE_QMV_OK)
         return qmv_err(w->w_down, "down");
     return KORE_LAYER_OK;
+}
+
+}  // namespace
+}  // extern "C++"
+
+KORE_LAYER_API int kore_layer_prefill_dev(kore_layer_t L, const kore_layer_weights *w, kore_attn_t attn, int layer,
+                                          int pos0, int n_tok, float *x, void *stream) {
+    if (!L) return fail(nullptr, KORE_LAYER_E_INVALID, "layer handle is NULL");
+    if (int rc = check_call(L, w, attn, x)) return rc;
+    if (n_tok < 1 || n_tok > kMaxBatch) return fail(L, KORE_LAYER_E_INVALID, "n_tok must be 1..64 (kore's KORE_BMAX)");
+    void *s = stream ? stream : (void *)L->stream;
+    return rows_step(L, w, n_tok, x, s, [&] {
+        if (kore_attn_prefill_dev(attn, layer, pos0, n_tok, L->n_head, L->n_head_kv, L->head_dim, L->bq, L->bk, L->bv,
+                                  L->batt, s) != KORE_ATTN_OK)
+            return fail(L, KORE_LAYER_E_STEP, std::string("attention: ") + kore_attn_last_error(attn));
+        return KORE_LAYER_OK;
+    });
+}
+
+KORE_LAYER_API int kore_layer_paged_dev(kore_layer_t L, const kore_layer_weights *w, kore_paged_t kv, int layer,
+                                        const kore_paged_batch *b, float *x, void *workspace, void *stream) {
+    if (!L) return fail(nullptr, KORE_LAYER_E_INVALID, "layer handle is NULL");
+    if (!w || !kv || !b || !x || ((uintptr_t)x & 15))
+        return fail(L, KORE_LAYER_E_INVALID, "w, kv, batch or x missing or x unaligned");
+    if (int rc = check_weights(L, w)) return rc;
+    kore_paged_info pi{};
+    if (kore_paged_get_info(kv, &pi) != KORE_PAGED_OK || pi.config.n_head != L->n_head ||
+        pi.config.n_head_kv != L->n_head_kv || pi.config.head_dim != L->head_dim)
+        return fail(L, KORE_LAYER_E_INVALID, "the paged cache's geometry differs from the layer's");
+    if (b->n_tok < 1 || b->n_tok > kMaxBatch || b->n_seq < 1)
+        return fail(L, KORE_LAYER_E_INVALID, "n_tok must be 1..64 (kore's KORE_BMAX), of one sequence or more");
+    // before anything is launched: what the append and the attention would refuse
+    if (layer < 0 || layer >= pi.config.n_layer || !b->q_start || !b->kv_len || !b->pages || ((uintptr_t)workspace & 15))
+        return fail(L, KORE_LAYER_E_INVALID, "layer outside the cache, a batch array missing or the workspace unaligned");
+    void *s = stream ? stream : (void *)L->stream;
+    const int64_t E = L->E, kvd = L->kvd;
+    return rows_step(L, w, b->n_tok, x, s, [&] {
+        if (kore_paged_append_dev(kv, layer, b, KORE_PAGED_F32, L->bk, kvd, L->bv, kvd, L->bq, E, L->bq, E, s) !=
+                KORE_PAGED_OK ||
+            kore_paged_attend_dev(kv, layer, b, KORE_PAGED_F32, L->bq, E, L->batt, E, 0.0f, 0, workspace, s) !=
+                KORE_PAGED_OK)
+            return fail(L, KORE_LAYER_E_STEP, std::string("paged attention: ") + kore_paged_last_error(kv));
+        return KORE_LAYER_OK;
+    });
 }
 
 KORE_LAYER_API int kore_layer_sync(kore_layer_t L) {

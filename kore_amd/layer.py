@@ -6,6 +6,7 @@ libkore_attn's decode on one stream.
     L = Layer(n_embd, n_ff, n_head, n_head_kv, rms_eps)
     w = LayerWeights.upload(types, mats, attn_norm, ffn_norm, bq, bk, bv, n_embd, n_ff, kv_dim)
     L.decode_dev(w, attn, layer, pos, x_ptr)       # x (device) updated in place
+    L.paged_dev(w, kv, layer, batch, x_ptr)        # rows of several sequences over a paged.PagedKV
 
 No CPU fallback: without the built library or a GPU every call raises.
 """
@@ -17,7 +18,7 @@ import os
 import numpy as np
 
 from . import _lib as _attn_lib
-from . import hip, qmv
+from . import hip, paged, qmv
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libkore_layer.so")
@@ -40,6 +41,7 @@ SYMBOLS = [
     ("kore_layer_destroy", None, [_vp]),
     ("kore_layer_decode_dev", _i, [_vp, C.POINTER(_Weights), _vp, _i, _i, _vp, _i, _vp]),
     ("kore_layer_prefill_dev", _i, [_vp, C.POINTER(_Weights), _vp, _i, _i, _i, _vp, _vp]),
+    ("kore_layer_paged_dev", _i, [_vp, C.POINTER(_Weights), _vp, _i, C.POINTER(paged.BatchStruct), _vp, _vp, _vp]),
     ("kore_layer_sync", _i, [_vp]),
     ("kore_layer_last_error", C.c_char_p, [_vp]),
 ]
@@ -54,6 +56,7 @@ def lib() -> C.CDLL:
             raise _attn_lib.LibraryMissing(f"{LIB_PATH} is not built; run `make -C kore_amd/csrc`")
         _attn_lib.lib()
         qmv.lib()
+        paged.lib()
         L = C.CDLL(LIB_PATH)
         for name, res, args in SYMBOLS:
             fn = getattr(L, name)
@@ -132,6 +135,14 @@ class Layer:
         x (device, [n_tok][n_embd]) updated in place."""
         s = w.struct()
         self._check(lib().kore_layer_prefill_dev(self._h, C.byref(s), attn.handle, layer, pos0, n_tok, x_ptr, stream))
+
+    def paged_dev(self, w: LayerWeights, kv: "paged.PagedKV", layer: int, batch: "paged.Batch", x_ptr: int,
+                  workspace: int | None = None, stream=None) -> None:
+        """forward_batch()'s body for `layer` over the new rows of a batch of sequences, whose K and V go to and come
+        from the paged cache: x (device, [n_tok][n_embd]) updated in place."""
+        s = w.struct()
+        self._check(lib().kore_layer_paged_dev(self._h, C.byref(s), kv.handle, layer, C.byref(batch.struct), x_ptr,
+                                               workspace, stream))
 
     def sync(self):
         self._check(lib().kore_layer_sync(self._h))
