@@ -93,8 +93,10 @@ KORE_PAGED_API int kore_paged_append_dev(kore_paged_t h, int layer, const kore_p
                                          int64_t q_stride, void *q_out, int64_t q_out_stride, void *stream);
 
 /* Attention of the batch's rows over one layer.  q (rotated): [n_tok][n_head *
- * head_dim] of `type` (KORE_PAGED_F32, or the cache's type), out likewise; head
- * j reads kv-head j / (n_head / n_head_kv).  scale 0: 1 / sqrt(head_dim).
+ * head_dim] of `type` (KORE_PAGED_F32, or the cache's type), out likewise (it may
+ * be q itself with the same stride; they do not overlap otherwise); head j reads
+ * kv-head j / (n_head / n_head_kv).  scale: 0 for 1 / sqrt(head_dim), or 1e-30 ..
+ * 1e30.
  * window 0: a row at position p attends 0 .. p; window w > 0: the last w of
  * those.  Partial sums of a split go to `workspace` (device,
  * kore_paged_workspace_bytes() bytes, 16-byte aligned) or, where it is NULL, to

@@ -452,12 +452,14 @@ int kore_paged_attend_dev(kore_paged_t h, int layer, const kore_paged_batch *b, 
     if (int rc = check_stride(h, "q", q_stride, E, b->n_tok)) return rc;
     if (int rc = check_stride(h, "out", out_stride, E, b->n_tok)) return rc;
     if (window < 0) return fail(h, KORE_PAGED_E_INVALID, "negative window");
-    if (!(scale >= 0) || !std::isfinite(scale)) return fail(h, KORE_PAGED_E_INVALID, "scale must be finite, 0 or more");
+    if (scale != 0 && !(scale >= 1e-30f && scale <= 1e30f))
+        return fail(h, KORE_PAGED_E_INVALID, "scale is neither 0 nor within 1e-30 .. 1e30");
     if ((uintptr_t)workspace % 16) return fail(h, KORE_PAGED_E_INVALID, "the workspace is not 16-byte aligned");
     if (b->n_seq == 0 || b->n_tok == 0) return KORE_PAGED_OK;
     if (!q || !out) return fail(h, KORE_PAGED_E_INVALID, "null buffer");
     if (int rc = check_aligned(h, "q", q, type)) return rc;
     if (int rc = check_aligned(h, "out", out, type)) return rc;
+    if (int rc = check_overlap(h, q, q_stride, out, out_stride, E, b->n_tok, type)) return rc;
     OnDevice on(h->device);
     if (int rc = on_device(h, on)) return rc;
     AttendArgs a{};

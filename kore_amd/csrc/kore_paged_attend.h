@@ -37,18 +37,12 @@ struct Cut {
     int min_len;     // a split's fewest keys
 };
 
-// exp(scale q.k) = 2^(dot * (hi + lo)), hi + lo = scale log2(e) to 47 bits, both over
-// 0, so that a score of -inf (one that is masked) needs no test: both terms are -inf.
-struct ScaleLog2 {
-    float hi, lo;
-};
-
 // A launch over tiles; part_o [place][dim / 4][row] float4 and part_ml [place][row]
-// (reference, sum) hold split tiles.
+// (reference, as q.k, and sum) hold split tiles.
 struct TileArgs {
     AttendArgs a;
     Cut cut;
-    ScaleLog2 sl;
+    float scale_log2;        // scale log2(e), over 0
     bool q_wide, out_wide;   // q's rows can be read 16 bytes at a time, out's written four values at a time
     float *part_o, *part_ml;
 };
@@ -286,7 +280,8 @@ template <> struct Mma<bhalf_t> {
     static __device__ __forceinline__ floatx16 mul32(bhalf8 a, bhalf8 b, floatx16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
     }
-    static constexpr float kBias = 0.0f;
+    // Weights reach 1 and no more, so that a V near fp32's largest value overflows no sooner than it must.
+    static constexpr float kBias = -8.0f;
 };
 
 // Parts that hold an fp32 value: two of fp16 (22 bits of a value near its row's
@@ -347,24 +342,31 @@ __device__ __forceinline__ void unit_of(float big, float &to, float &back) {
 
 // ---- the softmax ---------------------------------------------------------------
 
-// A row's weights are 2^(dot scale log2(e) - ref).  The reference follows the row's
-// largest score: it moves when that passes it by kLag, so that the accumulators are
-// rescaled rarely.
+// A row's weights are 2^((score - ref) s + kBias), score and reference in the units of
+// the products, s = scale log2(e) in those.  The difference comes first: it is exact
+// for scores near the reference, whatever their size, and what rounding s costs grows
+// with the distance from it, as the weights fall.  s is over 0, so that a score of
+// -inf (one that is masked) needs no test.  The reference follows the row's largest
+// score: it moves when that passes it by kLag, so that the accumulators are rescaled
+// rarely.
 constexpr float kLag = 8.0f;
 
-// A tile's rescale where a score passes the reference by kLag (or is the first).
+// The rescale, where a score passes the reference by kLag (or is the first).
 template <class V, int N>
-__device__ __forceinline__ void follow(float top, float &ref, float &sum, float bias, V (&o)[N]) {
-    const bool moves = top - bias > ref + kLag || (ref == kNone && top > kNone);
+__device__ __forceinline__ void follow(float top, float &ref, float &sum, float s, V (&o)[N]) {
+    const bool moves = (top - ref) * s > kLag;
     if (__any(moves)) {
-        const float next = moves ? top - bias : ref;
-        const float f = moves ? exp2_(ref - next) : 1.f;
+        const float next = moves ? top : ref;
+        const float f = moves ? exp2_((ref - next) * s) : 1.f;
         sum *= f;
 #pragma unroll
         for (int i = 0; i < N; ++i) o[i] *= f;
         ref = next;
     }
 }
+// What a state with the reference ref counts beside one with a reference of `to`, the
+// largest of all: 0 where there is none.
+__device__ __forceinline__ float share_at(float ref, float to, float s) { return ref == kNone ? 0.f : exp2_((ref - to) * s); }
 
 // What a lane knows of its row (column l % 16 of the products).
 struct Row {

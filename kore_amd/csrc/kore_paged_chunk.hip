@@ -308,7 +308,7 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
         has = has_2;
     }
     if constexpr (QP == 1) make_q();
-    const float s_hi = d.sl.hi * unit, s_lo = fmaxf(d.sl.lo * unit, 0x1p-126f);
+    const float s2 = fmaxf(d.scale_log2 * unit, 0x1p-126f);
     if (n_step) {
         store_k();
         if (n_step > 1) load_k(1);
@@ -367,8 +367,7 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
             for (int m = 0; m < MT; ++m)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) top = fmaxf(top, s[m][i]);
-            top = max32(top) * s_hi;
-            follow(top, ref, sum, Mma<C>::kBias, o);
+            follow(max32(top), ref, sum, s2, o);
         }
         __syncthreads();
         if (step + 1 < n_step) {
@@ -378,7 +377,20 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
         has = has_1;
         has_1 = has_2;
         if (any) {
+            // the difference from the reference first, as the softmax's comment says; 16-bit rows one fma of the score and
+            // the scaled reference, whose rounding is the same for all of a row's weights, unless it would be a power of 2
             const float base = ref == kNone ? 0.f : ref;
+            float minus = Mma<C>::kBias;
+            if constexpr (PP == 1) {
+                if (__any(fabsf(base * s2) > 0x1p22f)) {
+#pragma unroll
+                    for (int m = 0; m < MT; ++m)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) s[m][i] -= base;
+                } else {
+                    minus = fmaf(-base, s2, Mma<C>::kBias);
+                }
+            }
             vec8 w[MT][2][PP];
             float part_sum = 0;
 #pragma unroll
@@ -389,7 +401,7 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const float y = s[m][8 * h + i];
-                        x[i] = exp2_(PP > 1 ? fmaf(y, s_hi, fmaf(y, s_lo, -base)) : fmaf(y, s_hi, -base));
+                        x[i] = exp2_(fmaf(PP > 1 ? y - base : y, s2, minus));
                         if (PP > 1) part_sum += x[i];
                     }
                     weights<PP, C>(x, w[m][h]);
@@ -458,9 +470,9 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
             if (team == 0) {
                 if (part == 0) {
                     const float2 e = team_ml[wave][col];
-                    const float m = fmaxf(ref, e.x), base = m == kNone ? 0.f : m;
-                    f = exp2_(ref - base);
-                    g = exp2_(e.x - base);
+                    const float m = fmaxf(ref, e.x);
+                    f = share_at(ref, m, s2);
+                    g = share_at(e.x, m, s2);
                     ref = m;
                     sum = fmaf(e.y, g, sum * f);
                 }
@@ -489,7 +501,7 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
             for (int x = 0; x < 4; ++x)
                 reinterpret_cast<float4 *>(d.part_o)[(id * (HDP / 4) + 8 * i + 2 * x + half) * kRows + r] =
                     make_float4(o[i][4 * x], o[i][4 * x + 1], o[i][4 * x + 2], o[i][4 * x + 3]);
-        if (half == 0) reinterpret_cast<float2 *>(d.part_ml)[id * kRows + r] = make_float2(ref, sum);
+        if (half == 0) reinterpret_cast<float2 *>(d.part_ml)[id * kRows + r] = make_float2(ref * unit, sum);
         return;
     }
     if (!row.real) return;

@@ -10,7 +10,6 @@
 #include "kore_paged_attend.h"
 
 #include <algorithm>
-#include <cmath>
 
 namespace kore_paged_gpu {
 namespace {
@@ -30,12 +29,11 @@ __device__ __forceinline__ void finish(const TileArgs &d, const Place &p, const 
         float m = kNone, l = 0;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) m = fmaxf(m, ml[w][row].x);
-        const float base = m == kNone ? 0.f : m;
         float4 s = make_float4(0, 0, 0, 0);
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
             const float2 e = ml[w][row];
-            const float f = exp2_(e.x - base);
+            const float f = share_at(e.x, m, d.scale_log2);
             const float4 v = o[w][d4][row];
             l = fmaf(e.y, f, l);
             s.x = fmaf(v.x, f, s.x);
@@ -73,7 +71,6 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode16_kernel(
     // 16-bit rows could have their weights in one part; the second costs nothing beside the loads, and leaves the result
     // no rounding but its own (bf16, one token over 131072 keys: error 1.7e-3 instead of 2.3e-3 of the result)
     constexpr int QP = Parts<A, C>::q, PP = Parts<A, C>::p == 1 ? 2 : Parts<A, C>::p;
-    constexpr bool kExact = Parts<A, C>::p > 1;   // fp32 rows
     constexpr int KS = HDP / 32, DT = HDP / 16, VR = HDP / 16;   // k-steps, dim tiles, V registers of 16 bytes
     constexpr int kPitch = HDP + 16;                             // of a V row in LDS, elements
     constexpr int kBlock = 32;
@@ -185,7 +182,7 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode16_kernel(
                 }
             }
     }
-    const float s_hi = d.sl.hi * unit, s_lo = fmaxf(d.sl.lo * unit, 0x1p-126f);
+    const float s2 = fmaxf(d.scale_log2 * unit, 0x1p-126f);
     for (int j = 0; j < n_block; ++j) {
         const int key0 = (first_block + kWaves * j) * kBlock;
         const bool has0 = p0 >= 0, has1 = p1 >= 0;
@@ -262,16 +259,15 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode16_kernel(
         for (int m = 0; m < 2; ++m)
 #pragma unroll
             for (int i = 0; i < 4; ++i) top = fmaxf(top, s[m][i]);
-        top = max32(max16(top)) * s_hi;
-        follow(top, ref, sum, Mma<C>::kBias, o);
+        top = max32(max16(top));
+        follow(top, ref, sum, s2, o);
         const float base = ref == kNone ? 0.f : ref;
         vec8 w[PP];
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float e = kExact ? fmaf(s[m][i], s_hi, fmaf(s[m][i], s_lo, -base)) : fmaf(s[m][i], s_hi, -base);
-                const float x = exp2_(e);
+                const float x = exp2_(fmaf(s[m][i] - base, s2, Mma<C>::kBias));
                 C part[PP];
                 split_p<PP>(x, part);
                 sum += x;
@@ -307,7 +303,7 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode16_kernel(
     float4(*const states)[HDP / 4][kRows] = reinterpret_cast<float4(*)[HDP / 4][kRows]>(shared);
 #pragma unroll
     for (int i = 0; i < DT; ++i) states[wave][4 * i + g][col] = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
-    if (g == 0) ml[wave][col] = make_float2(ref, sum);
+    if (g == 0) ml[wave][col] = make_float2(ref * unit, sum);
     finish<A, HDP>(d, p, states, ml);
 }
 
@@ -431,13 +427,13 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode32_kernel(
             odd = __any(odd);
         }
         float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-        top = max32(max16(top)) * d.sl.hi;
-        follow(top, ref, sum, 0.f, o);
+        top = max32(max16(top));
+        follow(top, ref, sum, d.scale_log2, o);
         const float base = ref == kNone ? 0.f : ref;
         float w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            w[i] = exp2_(fmaf(s[i], d.sl.hi, fmaf(s[i], d.sl.lo, -base)));
+            w[i] = exp2_(fmaf(s[i] - base, d.scale_log2, Mma<bhalf_t>::kBias));
             sum += w[i];
         }
         if (!odd) {
@@ -525,12 +521,12 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(TileArgs d, int hd4) {
             float next = m;
 #pragma unroll
             for (int x = 0; x < kFlight; ++x) next = fmaxf(next, e[x].x);
-            const float base = next == kNone ? 0.f : next, f = exp2_(m - base);
+            const float f = share_at(m, next, d.scale_log2);
             l *= f;
             s = make_float4(s.x * f, s.y * f, s.z * f, s.w * f);
 #pragma unroll
             for (int x = 0; x < kFlight; ++x) {
-                const float g = exp2_(e[x].x - base);
+                const float g = share_at(e[x].x, next, d.scale_log2);
                 l = fmaf(e[x].y, g, l);
                 s = make_float4(fmaf(v[x].x, g, s.x), fmaf(v[x].y, g, s.y), fmaf(v[x].z, g, s.z), fmaf(v[x].w, g, s.w));
             }
@@ -541,13 +537,12 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(TileArgs d, int hd4) {
         __syncthreads();
         if (real && part == 0 && r < p.n * d.cut.rep) {
             for (int i = 1; i < parts; ++i) m = fmaxf(m, sm[lane + i][row].x);
-            const float base = m == kNone ? 0.f : m;
             l = 0;
             s = make_float4(0, 0, 0, 0);
             for (int i = 0; i < parts; ++i) {
                 const float2 e = sm[lane + i][row];
                 const float4 v = so[lane + i][row];
-                const float g = exp2_(e.x - base);
+                const float g = share_at(e.x, m, d.scale_log2);
                 l = fmaf(e.y, g, l);
                 s = make_float4(fmaf(v.x, g, s.x), fmaf(v.y, g, s.y), fmaf(v.z, g, s.z), fmaf(v.w, g, s.w));
             }
@@ -620,9 +615,7 @@ hipError_t launch_attend(const AttendArgs &a, hipStream_t s) {
         d.cut.target = tiles > kMaxTiles ? 0 : (int)std::max<long long>(places - tiles, places / 2);
         d.cut.min_len = kMinLen;
     }
-    const double sl = (double)a.scale * 1.4426950408889634074;
-    d.sl.hi = std::nextafter((float)sl, 0.f);
-    d.sl.lo = (float)(sl - (double)d.sl.hi);
+    d.scale_log2 = (float)((double)a.scale * 1.4426950408889634074);
     const int hdp = padded_dim(a.hd);
     d.part_o = a.part;
     d.part_ml = a.part + (size_t)(tiles + d.cut.target) * rows * hdp;

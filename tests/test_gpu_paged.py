@@ -226,6 +226,50 @@ def test_large_and_small_scores(dtype, cache):
     check_rows(c, c.rows("out", 6)[0], *c.exact())
 
 
+@pytest.mark.parametrize("dtype,cache", PAIRS)
+def test_out_in_the_place_of_q(dtype, cache):
+    for lens in ([(1, 900), (1, 40)], [(40, 300), (2, 9)]):
+        c = Case(lens, 6, 2, 64, 16, dtype, cache, seed=8, extra_rows=1).up()
+        with c.handle() as kv:
+            c.attend(kv)
+            kv.attend_dev(0, c.batch(), dtype, c.ptr("q"), c.ptr("q"))
+            kv.sync()
+        assert torch.equal(c.d["q"][:c.used], c.d["out"][:c.used]) and torch.equal(c.rows("q", 6)[0][c.used:], c.q[c.used:])
+
+
+@pytest.mark.parametrize("dtype,cache", [p for p in PAIRS if p[1] != "f16"])
+def test_values_near_the_largest(dtype, cache):
+    """V near fp32's largest value: a weighted mean of them is finite, and so is what is summed on the way (V up to 2^120,
+    300 keys of weights up to 1)."""
+    c = Case([(1, 300), (40, 280)], 6, 2, 64, 16, dtype, cache, seed=10)
+    c.v_pool = (c.v_pool.double().clamp(-4, 4) * 2.0 ** 117).to(c.v_pool.dtype)
+    c.up()
+    with c.handle() as kv:
+        for max_q in (1, 100):
+            c.attend(kv, max_q=max_q)
+            got, want, bound = to64(c.rows("out", 6)[0]), *c.exact()
+            assert np.isfinite(got).all() and (np.abs(got - want) <= bound).all()
+
+
+@pytest.mark.parametrize("dtype,cache", [p for p in PAIRS if p[0] == "f32"])
+def test_tiny_and_huge_q(dtype, cache):
+    """Rows of q of 1e-38 (scores of nothing: the mean of V) and of 1e30 against K of 1e-30 beside ordinary ones, with masked
+    keys in the same tiles."""
+    c = Case([(1, 70), (30, 90)], 6, 2, 64, 16, dtype, cache, seed=14)
+    c.q[::3] *= 1e-38
+    c.q[1::3, 2:] *= 1e30
+    if cache != "f16":
+        c.k_pool[0, :, 1] *= 1e-30
+    c.up()
+    with c.handle() as kv:
+        for max_q in (1, 100):
+            c.attend(kv, max_q=max_q)
+            got, want, bound = to64(c.rows("out", 6)[0]), *c.exact()
+            # an fp16 K cannot be that small: those rows' scores of 1e30 leave one key, wherever its score is the largest by far
+            fine = np.isfinite(bound) & (bound < 1)
+            assert np.isfinite(got).all() and (np.abs(got - want)[fine] <= bound[fine]).all() and fine.mean() > 0.5
+
+
 def test_scale():
     c = Case([(1, 50), (30, 60)], 4, 2, 64, 16, "f32", "f32", seed=2).up()
     with c.handle() as kv:
@@ -401,6 +445,7 @@ def test_calls_refuse():
                 (dict(layer=1), "layer 1"), (dict(layer=-1), "layer"), (dict(dtype="bf16"), "type"), (dict(q_stride=255), "stride"),
                 (dict(out_stride=-256), "stride"), (dict(q_stride=1 << 60), "too large"), (dict(window=-1), "window"),
                 (dict(scale=-1.0), "scale"), (dict(scale=math.inf), "scale"), (dict(scale=math.nan), "scale"),
+                (dict(scale=1e-40), "scale"), (dict(scale=1e31), "scale"), (dict(out=c.ptr("q") + 4), "overlap"),
                 (dict(workspace=8), "workspace"), (dict(q=None), "null"), (dict(out=None), "null"),
                 (dict(q=c.ptr("q") + 2), "aligned"), (dict(batch=batch(n_seq=-1)), "negative"), (dict(batch=batch(n_tok=-1)), "negative"),
                 (dict(batch=batch(max_q=-1)), "negative"), (dict(batch=batch(q_start=None)), "null"), (dict(batch=batch(kv_len=None)), "null"),
