@@ -252,9 +252,13 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
         }
     };
     const auto store_k = [&] {
+        if (padded) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i)
+                if (no_dim) kr[i] = raw8{};
+        }
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            if (no_dim) kr[i] = raw8{};
             put(k_tile, kKeys * kKPitch, kr[i], (i * kStepRows + wave * kWaveRows + my_row) * kKPitch + my_dim);
         }
     };
@@ -329,6 +333,7 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
 
         // S^T = K Q^T: lane (n, half) gets its row's scores of keys 32 m + 8 (i / 4) + 4 half + i % 4
         floatx16 s[MT];
+        bool far = false;
         if (any) {
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
@@ -368,6 +373,19 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
 #pragma unroll
                 for (int i = 0; i < 16; ++i) top = fmaxf(top, s[m][i]);
             follow(max32(top), ref, sum, s2, o);
+            // The difference from the reference first, as the softmax's comment says.  16-bit rows: one fma of the score
+            // and the scaled reference, whose rounding is the same for all of a row's weights, while that is no power of 2
+            // to speak of.
+            if constexpr (PP == 1) {
+                const float base = ref == kNone ? 0.f : ref;
+                far = __any(fabsf(base * s2) > 0x1p22f);
+                if (far) {
+#pragma unroll
+                    for (int m = 0; m < MT; ++m)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) s[m][i] -= base;
+                }
+            }
         }
         __syncthreads();
         if (step + 1 < n_step) {
@@ -377,20 +395,8 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
         has = has_1;
         has_1 = has_2;
         if (any) {
-            // the difference from the reference first, as the softmax's comment says; 16-bit rows one fma of the score and
-            // the scaled reference, whose rounding is the same for all of a row's weights, unless it would be a power of 2
             const float base = ref == kNone ? 0.f : ref;
-            float minus = Mma<C>::kBias;
-            if constexpr (PP == 1) {
-                if (__any(fabsf(base * s2) > 0x1p22f)) {
-#pragma unroll
-                    for (int m = 0; m < MT; ++m)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) s[m][i] -= base;
-                } else {
-                    minus = fmaf(-base, s2, Mma<C>::kBias);
-                }
-            }
+            const float minus = PP == 1 && !far ? fmaf(-base, s2, Mma<C>::kBias) : Mma<C>::kBias;
             vec8 w[MT][2][PP];
             float part_sum = 0;
 #pragma unroll
