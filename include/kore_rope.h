@@ -20,7 +20,7 @@
  *            g_i = clamp((i - lo) / max(hi - lo, 0.001), 0, 1):
  *            f_i (1 - g_i) + g_i f_i / factor, and m = 0.1 ln(factor) + 1.
  * freq_factors (host, rot_dim / 2 floats, or NULL) then divides f_i by its
- * entry, as a GGUF file's rope_freqs tensor is applied.
+ * entry, as a GGUF file's rope_freqs tensor is applied.  No f_i may pass 2^20.
  *
  * Conventions are those of kore_attn.h: 0 or a negative code, nothing throws,
  * kore_rope_last_error() has the text.  Part of libkore_paged.so. */
@@ -75,8 +75,8 @@ typedef struct kore_rope *kore_rope_t;
 KORE_PAGED_API int kore_rope_create(kore_rope_t *out, const kore_rope_config *cfg);
 KORE_PAGED_API void kore_rope_destroy(kore_rope_t r);
 
-/* n_tok rows of n_head heads of head_dim values (head_dim even, >= rot_dim, at
- * most 1024): out = the rows of x turned to the positions pos (device, n_tok
+/* n_tok rows (up to 2^23) of n_head heads of head_dim values (head_dim even, >=
+ * rot_dim, at most 1024): out = the rows of x turned to the positions pos (device, n_tok
  * ints >= 0).  Row i of x starts at x + i * x_stride elements (out likewise);
  * within a row the heads are contiguous.  out may be x itself (with the same
  * stride); otherwise the two do not overlap.  transpose != 0 turns the other

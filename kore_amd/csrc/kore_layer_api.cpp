@@ -248,9 +248,11 @@ KORE_LAYER_API int kore_layer_paged_dev(kore_layer_t L, const kore_layer_weights
     if (kore_paged_get_info(kv, &pi) != KORE_PAGED_OK || pi.config.n_head != L->n_head ||
         pi.config.n_head_kv != L->n_head_kv || pi.config.head_dim != L->head_dim)
         return fail(L, KORE_LAYER_E_INVALID, "the paged cache's geometry differs from the layer's");
+    if (pi.device != L->device) return fail(L, KORE_LAYER_E_INVALID, "the paged cache and the layer are on different devices");
     if (b->n_tok < 1 || b->n_tok > kMaxBatch || b->n_seq < 1)
         return fail(L, KORE_LAYER_E_INVALID, "n_tok must be 1..64 (kore's KORE_BMAX), of one sequence or more");
-    // before anything is launched: what the append and the attention would refuse
+    // before anything is launched: what the append and the attention would refuse (what else the append refuses
+    // leaves x and the cache as they were)
     if (layer < 0 || layer >= pi.config.n_layer || !b->q_start || !b->kv_len || !b->pages || ((uintptr_t)workspace & 15))
         return fail(L, KORE_LAYER_E_INVALID, "layer outside the cache, a batch array missing or the workspace unaligned");
     void *s = stream ? stream : (void *)L->stream;

@@ -97,7 +97,37 @@ int fail(H *h, int code, const char *fmt, ...) {
         if (e_ != hipSuccess) return fail((h), KORE_PAGED_E_HIP, "%s: %s", #expr, hipGetErrorString(e_)); \
     } while (0)
 
+constexpr double kMaxFreq = 0x1p20;   // to which the kernels' angles are exact
+
 bool type_ok(int t) { return t == KORE_PAGED_F32 || t == KORE_PAGED_F16 || t == KORE_PAGED_BF16; }
+
+// The frequencies of the header's formulas, in double, and m.
+class Freqs {
+  public:
+    explicit Freqs(const kore_rope_config &c) : c_(c), size_(c.magnitude > 0 ? (double)c.magnitude : 1.0) {
+        if (c.scaling != KORE_ROPE_YARN) return;
+        const auto corr = [&](double beta) {
+            return c.rot_dim * std::log(c.orig_ctx / (beta * 2 * M_PI)) / (2 * std::log((double)c.base));
+        };
+        lo_ = std::max(std::floor(corr(c.beta_fast > 0 ? c.beta_fast : 32.0)), 0.0);
+        hi_ = std::min(std::ceil(corr(c.beta_slow > 0 ? c.beta_slow : 1.0)), (double)c.rot_dim - 1);
+        if (!(c.magnitude > 0)) size_ = 0.1 * std::log((double)c.factor) + 1.0;
+    }
+    double of(int i) const {
+        double f = std::pow((double)c_.base, -2.0 * i / c_.rot_dim);   // kore.cpp:1339
+        if (c_.scaling == KORE_ROPE_LINEAR) f /= c_.factor;
+        if (c_.scaling == KORE_ROPE_YARN) {
+            const double g = std::clamp((i - lo_) / std::max(hi_ - lo_, 0.001), 0.0, 1.0);
+            f = f / c_.factor * g + f * (1 - g);
+        }
+        return c_.freq_factors ? f / c_.freq_factors[i] : f;
+    }
+    double size() const { return size_; }
+
+  private:
+    const kore_rope_config &c_;
+    double size_, lo_ = 0, hi_ = 0;
+};
 
 int check_rope(const kore_rope_config &c) {
     if (c.rot_dim < 2 || c.rot_dim % 2 != 0 || c.rot_dim > kMaxRot)
@@ -124,33 +154,10 @@ int check_rope(const kore_rope_config &c) {
         for (int i = 0; i < c.rot_dim / 2; ++i)
             if (!(c.freq_factors[i] > 0) || !std::isfinite(c.freq_factors[i]))
                 return FAIL0(KORE_PAGED_E_INVALID, "freq_factors[%d] is not positive and finite", i);
+    const Freqs f(c);
+    for (int i = 0; i < c.rot_dim / 2; ++i)
+        if (!(f.of(i) <= kMaxFreq)) return FAIL0(KORE_PAGED_E_INVALID, "frequency %d is over 2^20", i);
     return KORE_PAGED_OK;
-}
-
-// The frequencies of the header's formulas, in double, rounded to float.
-void fill_freqs(const kore_rope_config &c, std::vector<float> &freq, double &size) {
-    const int half = c.rot_dim / 2;
-    double lo = 0, hi = 0;
-    size = c.magnitude > 0 ? (double)c.magnitude : 1.0;
-    if (c.scaling == KORE_ROPE_YARN) {
-        const auto corr = [&](double beta) {
-            return c.rot_dim * std::log(c.orig_ctx / (beta * 2 * M_PI)) / (2 * std::log((double)c.base));
-        };
-        lo = std::max(std::floor(corr(c.beta_fast > 0 ? c.beta_fast : 32.0)), 0.0);
-        hi = std::min(std::ceil(corr(c.beta_slow > 0 ? c.beta_slow : 1.0)), (double)c.rot_dim - 1);
-        if (!(c.magnitude > 0)) size = 0.1 * std::log((double)c.factor) + 1.0;
-    }
-    freq.resize((size_t)half);
-    for (int i = 0; i < half; ++i) {
-        double f = std::pow((double)c.base, -2.0 * i / c.rot_dim);   // kore.cpp:1339
-        if (c.scaling == KORE_ROPE_LINEAR) f /= c.factor;
-        if (c.scaling == KORE_ROPE_YARN) {
-            const double g = std::clamp((i - lo) / std::max(hi - lo, 0.001), 0.0, 1.0);
-            f = f / c.factor * g + f * (1 - g);
-        }
-        if (c.freq_factors) f /= c.freq_factors[i];
-        freq[(size_t)i] = (float)f;
-    }
 }
 
 void release(kore_rope *r) {
@@ -230,9 +237,10 @@ int check_batch(kore_paged *h, int layer, const kore_paged_batch *b, int type) {
     if (!b->q_start || !b->kv_len || !b->pages) return fail(h, KORE_PAGED_E_INVALID, "null q_start, kv_len or pages");
     if (b->pages_stride <= 0 || b->pages_stride > kMaxKeys / h->cfg.page_size)
         return fail(h, KORE_PAGED_E_INVALID, "pages_stride %d outside 1..%d", b->pages_stride, kMaxKeys / h->cfg.page_size);
-    if ((int64_t)b->n_tok * h->cfg.n_head > (1 << 28) || b->n_seq > 1 << 20)
-        return fail(h, KORE_PAGED_E_UNSUPPORTED, "n_tok %d x %d heads or n_seq %d is too large", b->n_tok, h->cfg.n_head,
-                    b->n_seq);
+    if (b->n_tok > kMaxRows || (int64_t)b->n_tok * h->cfg.n_head > kMaxRowHeads ||
+        (int64_t)b->n_seq * h->cfg.n_head_kv > kMaxSeqHeads)
+        return fail(h, KORE_PAGED_E_UNSUPPORTED, "n_tok %d x %d heads or n_seq %d x %d kv-heads is too large", b->n_tok,
+                    h->cfg.n_head, b->n_seq, h->cfg.n_head_kv);
     return KORE_PAGED_OK;
 }
 
@@ -257,7 +265,9 @@ int kore_rope_create(kore_rope_t *out, const kore_rope_config *cfg) {
     kore_rope *r = new (std::nothrow) kore_rope;
     if (!r) return FAIL0(KORE_PAGED_E_NOMEM, "out of host memory");
     try {
-        fill_freqs(*cfg, r->freq, r->size);
+        const Freqs f(*cfg);
+        r->size = f.size();
+        for (int i = 0; i < cfg->rot_dim / 2; ++i) r->freq.push_back((float)f.of(i));
     } catch (const std::exception &) {
         delete r;
         return FAIL0(KORE_PAGED_E_NOMEM, "out of host memory");
@@ -288,6 +298,7 @@ int kore_rope_apply_dev(kore_rope_t r, int type, int n_tok, int n_head, int head
     if (n_tok < 0 || n_head <= 0) return fail(r, KORE_PAGED_E_INVALID, "bad n_tok %d or n_head %d", n_tok, n_head);
     if (head_dim < r->cfg.rot_dim || head_dim % 2 != 0)
         return fail(r, KORE_PAGED_E_INVALID, "head_dim %d is odd or under rot_dim %d", head_dim, r->cfg.rot_dim);
+    if (n_tok > kMaxRows) return fail(r, KORE_PAGED_E_UNSUPPORTED, "n_tok %d is over %d", n_tok, kMaxRows);
     if (head_dim > kMaxRopeHeadDim)
         return fail(r, KORE_PAGED_E_UNSUPPORTED, "head_dim %d over %d", head_dim, kMaxRopeHeadDim);
     if ((int64_t)n_head * head_dim > 1 << 24)

@@ -13,6 +13,9 @@ constexpr int kMaxHeadDim = 256;        // of the paged cache
 constexpr int kMaxRopeHeadDim = 1024;   // of the rotary call
 constexpr int kMaxRot = 512;
 constexpr int kMaxKeys = 1 << 30;       // positions of a sequence's row of the page table
+// A launch has fewer than 2^32 threads: rows of a call (256 threads each); rows x heads and sequences x kv-heads
+// of a batch, which make at most 2^23 + 2^22 tiles of 256 threads, or 2^20 + 2^22 of 512.
+constexpr int kMaxRows = 1 << 23, kMaxRowHeads = 1 << 27, kMaxSeqHeads = 1 << 22;
 
 enum Type { kF32 = 0, kF16 = 1, kBF16 = 2 };
 inline int type_bytes(int t) { return t == kF32 ? 4 : 2; }

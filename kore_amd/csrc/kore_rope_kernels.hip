@@ -13,9 +13,9 @@ namespace {
 constexpr int kThreads = 256;
 
 // m cos(pos f) and m sin(pos f) to within half a float step.  The angle is
-// exact (24 + 31 bits) but for one rounding of its 53rd bit; it is reduced by the
-// nearest multiple k of pi/2 held as the sum of two doubles, each step one fma,
-// so that r is off by some 2^-50 for any int position; then the power series
+// held as two doubles (24 + 31 bits) and reduced by the nearest multiple k of pi/2,
+// itself the sum of two doubles, each step one fma, so that r is off by some 2^-50
+// for any int position and frequencies up to 2^20; then the power series
 // about 0 up to where the next term, (pi/4)^15 / 15! = 2e-14 of the sine, is
 // nothing beside a float's half step of 3e-8.  fp32 arithmetic would lose the
 // angle itself: at position 131072 a float's step is 2^-7.
@@ -24,7 +24,7 @@ __device__ __forceinline__ float2 cos_sin(int pos, float freq, double size) {
     const double a = (double)pos * (double)freq;
     const double k = __builtin_rint(a * 0.63661977236758134308);
     double r = __builtin_fma(-k, kHi, a);
-    r = __builtin_fma(-k, kLo, r);
+    r = __builtin_fma(-k, kLo, r) + __builtin_fma((double)pos, (double)freq, -a);
     const double z = r * r;
     double s = 1.0 / 6227020800.0;
     s = __builtin_fma(s, z, -1.0 / 39916800.0);

@@ -56,6 +56,8 @@ def test_struct_sizes(tmp_path):
     (dict(rot_dim=64, scaling="yarn", factor=2.0, orig_ctx=10, base=1.0), "base"),
     (dict(rot_dim=64, scaling="yarn", factor=2.0, orig_ctx=10, beta_fast=-1.0), "beta"),
     (dict(rot_dim=64, magnitude=-1.0), "magnitude"), (dict(rot_dim=4, freq_factors=[1.0, 0.0]), "freq_factors[1]"),
+    (dict(rot_dim=64, base=1e-30), "frequency"), (dict(rot_dim=64, scaling="linear", factor=1e-38), "frequency 0"),
+    (dict(rot_dim=4, base=1.0, freq_factors=[1.0, 2.0 ** -21]), "frequency 1"),
 ])
 def test_rope_refuses(kw, fragment):
     from kore_amd import rope

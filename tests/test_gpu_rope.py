@@ -131,6 +131,25 @@ def test_transpose_is_the_gradient(layout):
     assert np.abs(back - to64(x)).max() <= 32 * UNIT["f32"] * np.abs(to64(x)).max()
 
 
+@pytest.mark.skipif(np.finfo(np.longdouble).nmant < 63, reason="the oracle's long double holds no more than a double")
+@pytest.mark.parametrize("factor", [1.0, 0.37, 2.0 ** -20])
+def test_angles_past_a_doubles_53_bits(factor):
+    """Positions and frequencies whose product takes up to 55 bits: within the bound of near ones."""
+    from kore_amd import rope
+    rng = np.random.default_rng(6)
+    pos = np.concatenate([[2 ** 31 - 1, 2 ** 31 - 2, 2 ** 30 + 1, 2 ** 29 + 3], rng.integers(2 ** 29, 2 ** 31 - 1, 400)])
+    x = torch.from_numpy(rng.standard_normal((len(pos), 1, 96))).float()
+    cfg = dict(scaling="linear", factor=factor)
+    got = to64(_apply(x, pos, rope.Config(96, **cfg), 1, 96, "f32"))[:, 0]
+    f, _ = rope_freqs(96, **cfg)
+    ang = pos.astype(np.longdouble)[:, None] * f.astype(np.longdouble)   # exact: 31 + 24 bits
+    c, s, x = np.cos(ang), np.sin(ang), to64(x)[:, 0]
+    a, b = x[:, :48], x[:, 48:]
+    want = np.concatenate([a * c - b * s, a * s + b * c], 1)
+    size = np.concatenate([np.abs(a * c) + np.abs(b * s), np.abs(a * s) + np.abs(b * c)], 1)
+    assert (np.abs(got - want) <= rope_bound(want, size, "f32")).all()
+
+
 def test_nothing_and_infinities():
     from kore_amd import rope
     with rope.Rope(rope.Config(8)) as r:
