@@ -27,7 +27,12 @@
  *   Rows that belong to no sequence (behind q_start[n_seq]) are left as they are.
  *   A page number outside 0 .. n_pages - 1 (say -1) is no page, and nothing past
  *   the table's pages_stride entries is: positions there are not stored, and not
- *   attended.  A row with nothing to attend gets zeros.
+ *   attended.  A row with nothing to attend gets zeros, and so does one whose
+ *   attended scores are all -infinity.
+ *   At most 2^23 rows, 2^27 rows x heads and 2^22 sequences x kv-heads a call.
+ *   With a q_start that is not ascending the rows of out (q_out, the slots stored)
+ *   hold nothing of use; nothing else is written, and nothing outside the buffers
+ *   is read.
  * Values of positions that a row does not attend (later ones, those before its
  * window, slots behind the sequence's end) do not reach it, infinities and NaN
  * included.  Pages may be shared by sequences as long as no two rows of one
@@ -36,8 +41,8 @@
  * Arithmetic: products of the cache's values with q and with the softmax's
  * weights are summed in fp32, and the result is rounded once to the rows' type.
  * fp32 rows keep fp32's precision whatever the cache's type (their products run
- * in several 16-bit parts, or on fp32 MFMA); fp16 and bf16 rows round the weights
- * to that type.  A sum is split over workgroups by a rule on the whole batch, in
+ * in several 16-bit parts, or on fp32 MFMA); fp16 and bf16 rows of chunks (many
+ * new rows of a sequence) round the weights to that type.  A sum is split over workgroups by a rule on the whole batch, in
  * a fixed order: the same call gives the same bits, another batch around a
  * sequence may differ in the last ones.
  *

@@ -33,23 +33,24 @@ inline Divisor divisor(int d) {
 struct Cut {
     int rep;         // q-heads of a kv-head
     Divisor by_rep, by_heads;   // by rep, and by the kv-heads
-    int target;      // workgroups to aim at, in tiles x keys; 0: nothing is split
+    int target;      // a split has all work / target, in tiles x keys, or more; 0: nothing is split
     int min_len;     // a split's fewest keys
 };
 
-// A launch over tiles; part_o [place][dim / 4][row] float4 and part_ml [place][row]
-// (reference, as q.k, and sum) hold split tiles.
+// A launch over tiles; part_o [part][dim / 4][row] float4 and part_ml [part][row]
+// (reference, as q.k, and sum) hold the splits of split tiles.
 struct TileArgs {
     AttendArgs a;
     Cut cut;
     float scale_log2;        // scale log2(e), over 0
     bool q_wide, out_wide;   // q's rows can be read 16 bytes at a time, out's written four values at a time
+    int places, parts;       // workgroups; parts that part_o and part_ml have
     float *part_o, *part_ml;
 };
 
 constexpr int kChunkRows = 128;   // of a tile of kore_paged_chunk.hip
 inline int padded_dim(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
-hipError_t launch_chunk(const TileArgs &d, int places, hipStream_t s);
+hipError_t launch_chunk(const TileArgs &d, hipStream_t s);
 
 namespace {
 
@@ -140,7 +141,7 @@ struct Place {
     int seq, tile, split, n_split, head;
     int q0, n, kv;      // of the sequence: first row, rows, positions
     int len;            // keys of a split
-    int first;          // number of the tile's first split among the launch's places
+    int part;           // number of the split (of the tile's first split, where all are one place) among the parts
 };
 
 // Inclusive sums over the wave in six DPP steps (four within rows of 16, then from
@@ -166,8 +167,8 @@ __device__ __forceinline__ T last_lane(T x) {
 
 // The place of number `id`, false where there is none.  Numbers run over the
 // sequences, then a sequence's tiles from the last (which has the most keys),
-// then its splits, then the kv-heads.  by_tile: one number for all splits of a
-// tile (the merge).
+// then its splits, then the kv-heads.  by_tile (the merge): over the split tiles
+// alone, one number for all splits.
 template <int TILE>
 __device__ __forceinline__ bool place_of(const Batch &b, const Cut &c, int id, int nkv, int cap, int window, bool by_tile,
                                          Place &p) {
@@ -178,7 +179,8 @@ __device__ __forceinline__ bool place_of(const Batch &b, const Cut &c, int id, i
     };
     Share r = share(0);
     if (c.target) {
-        // so that all splits are at most target (of len keys) and one more for each tile
+        // so that a tile of keys > len has keys / len + 1 < 2 keys / len splits: all splits are at most target and the
+        // tiles, those of split tiles at most twice target
         float w = (float)r.tiles * (float)r.keys;
         for (int s0 = 64; s0 < b.n_seq; s0 += 64) {
             const Share t = share(s0);
@@ -187,12 +189,13 @@ __device__ __forceinline__ bool place_of(const Batch &b, const Cut &c, int id, i
         const float each = ceilf(last_lane(prefix_sum(w)) * (float)nkv / (float)c.target);
         len = max(c.min_len, ((int)fminf(each, 1e9f) + 63) & ~63);
     }
-    int at = 0, splits_at = 0;
+    int at = 0, part_at = 0;
     for (int s0 = 0; s0 < b.n_seq; s0 += 64) {
         if (b.n_seq > 64) r = share(s0);   // (one round of loads where all sequences have a lane)
         const int n_split = c.target ? max(1, (r.keys + len - 1) / len) : 1;
-        const int all = r.tiles * n_split * nkv, mine = by_tile ? r.tiles * nkv : all;
-        const int upto = prefix_sum(mine), splits_upto = by_tile ? prefix_sum(all) : upto;
+        const int all = r.tiles * n_split * nkv, part = n_split > 1 ? all : 0;
+        const int mine = !by_tile ? all : n_split > 1 ? r.tiles * nkv : 0;
+        const int upto = prefix_sum(mine), part_upto = c.target ? prefix_sum(part) : 0;
         const unsigned long long past = __ballot(at + upto > id);
         if (past) {
             const int l = __builtin_ctzll(past);
@@ -205,6 +208,7 @@ __device__ __forceinline__ bool place_of(const Batch &b, const Cut &c, int id, i
             // the sequence's splits of equal length, in whole steps of 64 keys
             p.len = p.n_split > 1 ? scalar(((of(r.keys) + p.n_split - 1) / p.n_split + 63) & ~63) : INT_MAX;
             int i = id - at - of(upto) + of(mine);
+            if (i < 0 || i >= of(mine)) return false;   // (sums past 2^31, of a q_start that is not ascending)
             const int pairs = c.by_heads.of(i);
             p.head = i - pairs * nkv;
             i = pairs;
@@ -214,11 +218,11 @@ __device__ __forceinline__ bool place_of(const Batch &b, const Cut &c, int id, i
                 p.split = pairs - i * p.n_split;
             }
             p.tile = scalar(of(r.tiles) - 1 - i);
-            p.first = scalar(splits_at + of(splits_upto) - of(all) + i * p.n_split * nkv + p.head);
+            p.part = scalar(part_at + of(part_upto) - of(part) + (i * p.n_split + p.split) * nkv + p.head);
             return true;
         }
         at += last_lane(upto);
-        splits_at += last_lane(splits_upto);
+        part_at += last_lane(part_upto);
     }
     return false;
 }

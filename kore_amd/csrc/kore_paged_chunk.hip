@@ -500,7 +500,8 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
     }
     const int r = wave * 32 + col;
     if (p.n_split > 1) {
-        const size_t id = blockIdx.x;
+        const size_t id = p.part;
+        if (id >= (unsigned)d.parts) return;   // (only where q_start is not ascending)
 #pragma unroll
         for (int i = 0; i < DT; ++i)
 #pragma unroll
@@ -525,9 +526,9 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
 
 }  // namespace
 
-hipError_t launch_chunk(const TileArgs &d, int places, hipStream_t s) {
+hipError_t launch_chunk(const TileArgs &d, hipStream_t s) {
     const int hdp = padded_dim(d.a.hd);
-    const dim3 grid((unsigned)places);
+    const dim3 grid((unsigned)d.places);
 #define KORE_CHUNK(A, S)                                                        \
     do {                                                                        \
         if (hdp == 64) chunk_kernel<A, S, 64><<<grid, Shape<A, S, 64>::threads, 0, s>>>(d);     \

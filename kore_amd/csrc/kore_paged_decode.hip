@@ -42,7 +42,8 @@ __device__ __forceinline__ void finish(const TileArgs &d, const Place &p, const 
             s.w = fmaf(v.w, f, s.w);
         }
         if (p.n_split > 1) {
-            const size_t id = blockIdx.x;
+            const size_t id = p.part;
+            if (id >= (unsigned)d.parts) continue;   // (only where q_start is not ascending)
             reinterpret_cast<float4 *>(d.part_o)[(id * (HDP / 4) + d4) * kRows + row] = s;
             if (d4 == 0) reinterpret_cast<float2 *>(d.part_ml)[id * kRows + row] = make_float2(m, l);
             continue;
@@ -491,18 +492,19 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(TileArgs d, int hd4) {
     const AttendArgs &a = d.a;
     const int cap = a.b.pages_stride << a.page_shift;
     Place p;
-    if (!place_of<TILE>(a.b, d.cut, blockIdx.x, a.n_head_kv, cap, a.window, true, p) || p.n_split <= 1) return;
+    if (!place_of<TILE>(a.b, d.cut, blockIdx.x, a.n_head_kv, cap, a.window, true, p)) return;
+    if ((unsigned)p.part + (unsigned)(p.n_split - 1) * (unsigned)a.n_head_kv >= (unsigned)d.parts) return;   // as there
     int parts = 1;
     while (parts < kLanes && parts < p.n_split) parts *= 2;
     const int row = threadIdx.x % TILE, lane = threadIdx.x / TILE, part = lane & (parts - 1), wide = kLanes / parts;
     const size_t step = (size_t)a.n_head_kv * TILE;
-    const float2 *const pm = reinterpret_cast<const float2 *>(d.part_ml) + (size_t)p.first * TILE + row;
+    const float2 *const pm = reinterpret_cast<const float2 *>(d.part_ml) + (size_t)p.part * TILE + row;
     const int r = p.tile * TILE + row, token = d.cut.by_rep.of(r), head = p.head * d.cut.rep + r - token * d.cut.rep;
     A *const out = (A *)a.out + (size_t)(p.q0 + token) * a.out_stride + (size_t)head * a.hd;
     for (int d0 = blockIdx.y * wide; 4 * d0 < a.hd; d0 += gridDim.y * wide) {
         const int d4 = d0 + lane / parts;
         const bool real = 4 * d4 < a.hd;
-        const float4 *const po = reinterpret_cast<const float4 *>(d.part_o) + ((size_t)p.first * hd4 + d4) * TILE + row;
+        const float4 *const po = reinterpret_cast<const float4 *>(d.part_o) + ((size_t)p.part * hd4 + d4) * TILE + row;
         float m = kNone, l = 0;
         float4 s = make_float4(0, 0, 0, 0);
         for (int i = part; real && i < p.n_split; i += kFlight * parts) {
@@ -554,9 +556,9 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(TileArgs d, int hd4) {
     }
 }
 
-hipError_t launch_decode(const TileArgs &d, int places, hipStream_t s) {
+hipError_t launch_decode(const TileArgs &d, hipStream_t s) {
     const int hdp = padded_dim(d.a.hd);
-    const dim3 grid((unsigned)places);
+    const dim3 grid((unsigned)d.places);
 #define KORE_DECODE(...)                                                 \
     do {                                                                 \
         if (hdp == 64) KORE_DECODE_(64, __VA_ARGS__);                    \
@@ -577,15 +579,13 @@ hipError_t launch_decode(const TileArgs &d, int places, hipStream_t s) {
     return hipGetLastError();
 }
 
-constexpr int kMinLen = 64, kChunkMinLen = 256;   // a split's fewest keys
-constexpr int kPerCu = 2;                           // workgroups of a CU
-constexpr int kMaxTiles = 1024;                     // over this many (tile, kv-head)s of 16 rows nothing is split
+constexpr int kPerCu = 2;                              // workgroups of a CU, of the 16-row kernels
+constexpr int kShort = 1024, kChunkShort = 2048;       // keys that a tile among many is not split for
 
 }  // namespace
 
 size_t attend_workspace_bytes(int n_head, int n_head_kv, int hd, int num_cu) {
-    const size_t rows = ((size_t)kMaxTiles + (size_t)kPerCu * num_cu) * kRows, chunk_rows = (size_t)num_cu * kChunkRows;
-    return std::max(rows, chunk_rows) * ((size_t)padded_dim(hd) + 2) * sizeof(float);
+    return 2 * (size_t)num_cu * kChunkRows * ((size_t)padded_dim(hd) + 2) * sizeof(float);
 }
 
 hipError_t launch_attend(const AttendArgs &a, hipStream_t s) {
@@ -606,24 +606,33 @@ hipError_t launch_attend(const AttendArgs &a, hipStream_t s) {
     const int rows = chunk ? kChunkRows : kRows;
     // the most (tile, kv-head)s that n_tok rows of n_seq sequences can be
     const long long tiles = ((long long)a.b.n_tok * d.cut.rep / rows + std::min(a.b.n_seq, a.b.n_tok)) * a.n_head_kv;
-    if (chunk) {
-        const int places = a.num_cu;
-        d.cut.target = 4 * tiles > 3 * places ? 0 : (int)(places - tiles);
-        d.cut.min_len = kChunkMinLen;
-    } else {
-        const int places = kPerCu * a.num_cu;
-        d.cut.target = tiles > kMaxTiles ? 0 : (int)std::max<long long>(places - tiles, places / 2);
-        d.cut.min_len = kMinLen;
-    }
+    // Few tiles: splits make up the workgroups that the card holds at once.  From half of those on it is the longest tiles
+    // alone that are split, those of some twice the mean (chunks) or over it (16 rows), and none where a tile cannot have
+    // many keys or all are one sequence's: the merge's launch and the partials cost every call.  us, split / not, 28/4/128:
+    //   rows of one sequence over 4096 keys, tiles 34 %, 50 %, 59 % of the CUs: fp16 52.7 / 75.0, 58.0 / 76.3, 80.4 / 76.7;
+    //   fp32 170 / 297, 188 / 300, 308 / 304;
+    //   four prompts of 512 beside a token over 65536: fp16 77 / 1049, fp32 219 / 4493; over 2048: 59 / 56, 197 / 193;
+    //   300 tokens over 1000 keys, one of them over 65536: 187 / 763; none: 115 / 115;
+    //   100 tokens over 300 keys, one over 512, 1024, 2048: 22.2 / 16.7, 22.6 / 20.5, 24.3 / 29.7.
+    const int at_once = chunk ? a.num_cu : kPerCu * a.num_cu;
+    const long long most = std::min((long long)a.b.pages_stride << a.page_shift, (long long)a.window + (rows - 1) / d.cut.rep + 65);
+    // A step of a chunk's two teams, or half a workgroup's blocks: 64 fp32 rows over 512 keys 21.5 us, in splits of 256 keys
+    // 32.6; 64 fp16 rows 15.4, of 64 keys 15.8, of 256 16.8; one token over 512 keys 9.6, of 128 10.1, of 256 11.2.
+    d.cut.min_len = chunk && size == 2 ? 128 : 64;
+    if (2 * tiles <= at_once) d.cut.target = most > d.cut.min_len ? (int)(at_once - tiles) : 0;
+    else if (a.b.n_seq == 1 || most <= (chunk ? kChunkShort : kShort)) d.cut.target = 0;
+    else d.cut.target = (int)(chunk ? std::min<long long>(tiles / 2, at_once) : std::min<long long>(tiles, at_once / 2));
     d.scale_log2 = (float)((double)a.scale * 1.4426950408889634074);
     const int hdp = padded_dim(a.hd);
+    d.places = (int)tiles + d.cut.target;
     d.part_o = a.part;
-    d.part_ml = a.part + (size_t)(tiles + d.cut.target) * rows * hdp;
-    const unsigned places = (unsigned)(tiles + d.cut.target);
-    const hipError_t e = chunk ? launch_chunk(d, (int)places, s) : launch_decode(d, (int)places, s);
+    d.parts = d.cut.target + (int)std::min<long long>(d.cut.target, tiles);
+    d.part_ml = a.part + (size_t)d.parts * rows * hdp;
+    const hipError_t e = chunk ? launch_chunk(d, s) : launch_decode(d, s);
     if (e != hipSuccess || !d.cut.target) return e;
     // some four workgroups a CU, where there are dims enough
-    const dim3 merge((unsigned)tiles, (unsigned)std::clamp<long long>(8 * a.num_cu / tiles, 1, a.hd / 4));
+    const int joined = (int)std::min<long long>(d.cut.target, tiles);   // the most tiles that can be split
+    const dim3 merge((unsigned)joined, (unsigned)std::clamp(8 * a.num_cu / joined, 1, a.hd / 4));
 #define KORE_MERGE(A)                                                                    \
     do {                                                                                 \
         if (chunk) merge_kernel<A, kChunkRows><<<merge, kThreads, 0, s>>>(d, hdp / 4);   \

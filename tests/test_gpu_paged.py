@@ -137,6 +137,24 @@ def test_long_contexts_are_split(dtype, cache):
 
 
 @pytest.mark.parametrize("dtype,cache", PAIRS)
+@pytest.mark.parametrize("new,n_seq,kv", [(1, 75, (1, 120)), (80, 6, (80, 200))])
+def test_a_long_sequence_among_many_tiles(dtype, cache, new, n_seq, kv):
+    """Tiles enough to fill the card, those of two sequences longer than the rest by far: theirs alone are split."""
+    rng = np.random.default_rng(n_seq)
+    lens = [(new, int(rng.integers(*kv))) for _ in range(n_seq)]
+    lens.insert(2, (1, 3001))
+    lens.append((2, 2750))
+    c = Case(lens, 28, 4, 64, 64, dtype, cache, seed=n_seq, extra_rows=1).up()
+    with c.handle() as kv_:
+        ws = torch.full((kv_.workspace_bytes() + 4096,), 9, dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        c.attend(kv_, workspace=ws.data_ptr())
+    got = c.rows("out", 28)[0]
+    assert (got[c.used:] == 77.0).all() and (ws[-4096:] == 9).all()
+    check_rows(c, got, *c.exact())
+
+
+@pytest.mark.parametrize("dtype,cache", PAIRS)
 @pytest.mark.parametrize("nh,nkv,hd,ps,n_seq", [(28, 4, 128, 16, 70), (6, 1, 64, 32, 200)])
 def test_many_sequences(dtype, cache, nh, nkv, hd, ps, n_seq):
     rng = np.random.default_rng(n_seq)
@@ -425,6 +443,63 @@ def test_a_cache_past_32_bits():
     check_rows(c, c.rows("out", 16)[0], *c.exact())
 
 
+# ---- odd batches -----------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,cache", PAIRS)
+@pytest.mark.parametrize("max_q", [1, 64])
+def test_scores_of_minus_infinity(dtype, cache, max_q):
+    """Rows whose every attended score is -inf get zeros; one finite score is all of a row that has it."""
+    c = Case([(3, 40), (20, 300), (1, 900)], 6, 2, 64, 16, dtype, cache, seed=3)
+    c.q[..., 7] = c.q[..., 7].abs() + 0.5
+    c.k_pool[..., 7] = -math.inf
+    page = int(c.pages[1, 2])
+    c.k_pool[0, page, 1, 5, 7] = 0.25   # sequence 1, position 37, kv-head 1
+    c.up()
+    with c.handle() as kv:
+        c.attend(kv, max_q=max_q)
+    got = to64(c.rows("out", 6)[0])
+    v = to64(c.v_pool[0, page, 1, 5])
+    assert (got[:3] == 0).all() and (got[23:] == 0).all() and (got[3:23, :3] == 0).all()
+    # one weight, which divides out but for its parts' rounding, and the result's own
+    assert (np.abs(got[3:23, 3:] - v) <= (UNIT[dtype] + 2.0 ** -20) * np.abs(v)).all()
+
+
+@pytest.mark.parametrize("dtype,cache", PAIRS)
+@pytest.mark.parametrize("max_q", [1, 64])
+def test_a_page_twice_in_a_sequence(dtype, cache, max_q):
+    c = Case([(5, 200), (1, 130)], 6, 2, 64, 16, dtype, cache, seed=4)
+    c.pages[0, 3] = c.pages[0, 9] = c.pages[0, 0]
+    c.pages[1, :4] = c.pages[1, 5]
+    c.up()
+    with c.handle() as kv:
+        c.attend(kv, max_q=max_q)
+    check_rows(c, c.rows("out", 6)[0], *c.exact())
+
+
+@pytest.mark.parametrize("dtype,cache", [("f32", "f32"), ("f32", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("starts", [[0, 40] * 8 + [0], [40, 0] * 8 + [40], [-5, 100, -2 ** 31, 2 ** 31 - 1, 7] * 3 + [40, 40]])
+@pytest.mark.parametrize("max_q", [1, 64])
+def test_q_start_that_is_not_ascending(dtype, cache, starts, max_q):
+    """Nothing of use comes out, and nothing but out, q_out, the slots of the table and the workspace is written."""
+    c = Case([(40, 700)], 6, 2, 64, 16, dtype, cache, seed=5, extra_rows=2, row_pad=8, row_off=8)
+    n_seq = len(starts) - 1
+    c.lens = [(40, 700)] * n_seq
+    c.pages = np.repeat(c.pages, n_seq, 0)
+    c.kv_len = np.repeat(c.kv_len, n_seq, 0)
+    c.starts = np.asarray(starts, np.int32)
+    c.up()
+    spare = [p for p in range(c.n_pages) if p not in set(c.pages[0])]
+    with c.handle() as kv:
+        ws = torch.full((kv.workspace_bytes() + 4096,), 9, dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        c.attend(kv, max_q=max_q, workspace=ws.data_ptr())
+        _append(c, kv)
+    assert (ws[-4096:] == 9).all()
+    assert c.rows("out", 6)[1] and torch.equal(c.d["q"], c.wide(c.q))
+    for pool in ("k_pool", "v_pool"):
+        assert torch.isnan(c.d[pool][0, spare]).all()
+
+
 # ---- refusals ------------------------------------------------------------------------
 
 def test_calls_refuse():
@@ -450,7 +525,8 @@ def test_calls_refuse():
                 (dict(q=c.ptr("q") + 2), "aligned"), (dict(batch=batch(n_seq=-1)), "negative"), (dict(batch=batch(n_tok=-1)), "negative"),
                 (dict(batch=batch(max_q=-1)), "negative"), (dict(batch=batch(q_start=None)), "null"), (dict(batch=batch(kv_len=None)), "null"),
                 (dict(batch=batch(pages=None)), "null"), (dict(batch=batch(pages_stride=0)), "pages_stride"),
-                (dict(batch=batch(pages_stride=1 << 28)), "pages_stride"), (dict(batch=batch(n_tok=1 << 27)), "too large")]:
+                (dict(batch=batch(pages_stride=1 << 28)), "pages_stride"), (dict(batch=batch(n_tok=1 << 27)), "too large"),
+                (dict(batch=batch(n_tok=(1 << 23) + 1)), "too large"), (dict(batch=batch(n_seq=(1 << 21) + 1)), "too large")]:
             with pytest.raises(paged.PagedError) as e:
                 kv.attend_dev(**{**good, **kw})
             assert text in e.value.message, (kw, e.value.message)
@@ -467,7 +543,8 @@ def test_calls_refuse():
         for kw, text in [
                 (dict(n_tok=-1), "n_tok"), (dict(n_head=0), "n_head"), (dict(head_dim=62), "head_dim"), (dict(head_dim=65), "head_dim"),
                 (dict(head_dim=1026), "head_dim"), (dict(x_stride=10), "stride"), (dict(out_stride=10), "stride"), (dict(x=None), "null"),
-                (dict(pos=None), "null"), (dict(out=c.ptr("q") + 4), "overlap"), (dict(out=c.ptr("out") + 3), "aligned")]:
+                (dict(pos=None), "null"), (dict(out=c.ptr("q") + 4), "overlap"), (dict(out=c.ptr("out") + 3), "aligned"),
+                (dict(n_tok=(1 << 23) + 1), "n_tok")]:
             with pytest.raises(rope.PagedError) as e:
                 r.apply_dev(**{**rot, **kw})
             assert text in e.value.message, (kw, e.value.message)
