@@ -16,15 +16,21 @@ namespace {
 
 constexpr int kWaves = 4, kRows = kChunkRows;   // of a team
 
-// How a (row type, cache type) is computed: fp32 caches in three bf16 parts of
-// everything, whose products of parts i and j with i + j < 3 hold 24 bits.
+// How a (row type, cache type) is computed: the type and parts of q and K, and those
+// of the weights and V.  An fp32 cache's K is two fp16 parts, as q, each key in a power
+// of two of its own, and its V three bf16 parts, as the weights; the products of parts
+// i and j with i + j under the cache's number of parts hold 22 and 24 bits.  (K's units
+// leave again with the scores.  V's would have to be the weights': keys of far smaller V
+// would lose bits.)
 template <class A, class S> struct Form {
     typedef S C;
-    static constexpr int qp = Parts<A, S>::q, kp = 1, pp = Parts<A, S>::p;
+    typedef S CV;
+    static constexpr int qp = Parts<A, S>::q, kp = 1, vp = 1, pp = Parts<A, S>::p;
 };
 template <> struct Form<float, float> {
-    typedef bhalf_t C;
-    static constexpr int qp = 3, kp = 3, pp = 3;
+    typedef half_t C;
+    typedef bhalf_t CV;
+    static constexpr int qp = 2, kp = 2, vp = 3, pp = 3;
 };
 
 // What a tile's shape asks of LDS and registers: keys of a step; teams of a
@@ -60,6 +66,18 @@ __device__ __forceinline__ void cut3(const float (&x)[8], bhalf8 (&part)[3], flo
 #pragma unroll
     for (int j = 0; j < 3; ++j) part[j] = __builtin_bit_cast(bhalf8, u[j]);
 }
+// The largest of PIECES neighbouring lanes' values: 8, 16 or 32.
+template <int CTRL>
+__device__ __forceinline__ float max_lane(float x) {
+    return fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, false)));
+}
+template <int PIECES>
+__device__ __forceinline__ float row_max(float x) {
+    if constexpr (PIECES == 32) x = max16(x);
+    if constexpr (PIECES >= 16) x = max_lane<0x140>(x);    // lane 15 - i of 16
+    x = max_lane<0x141>(x);                                 // lane 7 - i of 8
+    return max_lane<0x4e>(max_lane<0xb1>(x));               // lanes i ^ 1, i ^ 2
+}
 // Eight weights as N parts of C.
 template <int N, class C, class V>
 __device__ __forceinline__ void weights(const float (&x)[8], V (&part)[N]) {
@@ -80,9 +98,11 @@ __device__ __forceinline__ void weights(const float (&x)[8], V (&part)[N]) {
 template <class A, class S, int HDP>
 __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(TileArgs d) {
     typedef typename Form<A, S>::C C;
+    typedef typename Form<A, S>::CV CV;
     typedef typename Mma<C>::vec8 vec8;
-    typedef C vec4 __attribute__((ext_vector_type(4)));
-    constexpr int QP = Form<A, S>::qp, KP = Form<A, S>::kp, PP = Form<A, S>::pp;
+    typedef typename Mma<CV>::vec8 vvec8;
+    typedef CV vec4 __attribute__((ext_vector_type(4)));
+    constexpr int QP = Form<A, S>::qp, KP = Form<A, S>::kp, VP = Form<A, S>::vp, PP = Form<A, S>::pp;
     constexpr int kKeys = Shape<A, S, HDP>::keys, kTeams = Shape<A, S, HDP>::teams;
     constexpr bool kLag = Shape<A, S, HDP>::lag;
     constexpr int KS = HDP / 16, DT = HDP / 32, MT = kKeys / 32;         // k-steps, dim tiles, key tiles
@@ -91,24 +111,27 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
     constexpr int kKPitch = HDP + 8, kVPitch = HDP + 32;
     constexpr int kPieces = HDP / 8, kWaveRows = 64 / kPieces, kStepRows = kWaves * kWaveRows, kLoads = kKeys / kStepRows;
     typedef S raw8 __attribute__((ext_vector_type(8)));
-    // A team's step of K and of V, each in KP planes; at the end half of the second team's sums lie there
-    constexpr int kPlane = kKeys * (kKPitch + kVPitch), kTileBytes = kTeams * KP * kPlane * (int)sizeof(C);
+    // A team's step of K and of V, in KP and VP planes; at the end half of the second team's sums lie there
+    constexpr int kStep = kKeys * (KP * kKPitch + VP * kVPitch), kTileBytes = kTeams * kStep * (int)sizeof(C);
     constexpr int kMeetBytes = kTeams == 2 ? kWaves * HDP / 16 * 64 * 16 : 0;
     __shared__ __attribute__((aligned(16))) unsigned char tiles[kTileBytes > kMeetBytes ? kTileBytes : kMeetBytes];
     // The third part of q, where LDS has room: it would cost the loop its spare registers, and a reload of a spilled
     // one waits for the loads in flight.  (The teams' rows are the same.)
-    constexpr bool kThird = QP == 3 && !(KP == 3 && HDP == 256);
+    constexpr bool kThird = QP == 3;
     constexpr int kQReg = kThird ? 2 : QP;
     __shared__ vec8 q_third[kThird ? kWaves : 1][KS][64];
     // of V's pieces in steps that the tile's rows do not all see: which of 8 dims are +inf, or -inf (a NaN: both)
     __shared__ unsigned all_kinds[kTeams][2][kKeys][HDP / 32];
     __shared__ int all_odd[kTeams][kWaves];
+    __shared__ __attribute__((aligned(16))) float all_back[KP == 2 ? kTeams : 1][kKeys];   // K's units
     __shared__ float2 team_ml[kWaves][32];   // (reference, sum) of the second team's rows
     const AttendArgs &a = d.a;
     const int rep = d.cut.rep;
     const int cap = a.b.pages_stride << a.page_shift, lane = threadIdx.x & 63;
     const int wave = scalar(threadIdx.x >> 6) % kWaves, team = scalar(threadIdx.x >> 6) / kWaves;
-    C *const k_tile = reinterpret_cast<C *>(tiles) + team * (KP * kPlane), *const v_tile = k_tile + KP * kKeys * kKPitch;
+    C *const k_tile = reinterpret_cast<C *>(tiles) + team * kStep;
+    CV *const v_tile = reinterpret_cast<CV *>(k_tile + KP * kKeys * kKPitch);
+    float *const k_back = all_back[KP == 2 ? team : 0];
     auto &kinds = all_kinds[team];
     auto &odd_of = all_odd[team];
     Place p;
@@ -230,14 +253,50 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
         has_2 = load(step, k_head, kr);
     };
     const auto load_v = [&](int step) { load(step, v_head, vr); };
-    const auto put = [&](C *plane0, int plane, raw8 x, int at) {
+    const auto put_k = [&](raw8 x, int row) {
+        C *const at = k_tile + row * kKPitch + my_dim;
         if constexpr (KP == 1) {
-            *reinterpret_cast<raw8 *>(plane0 + at) = x;
+            *reinterpret_cast<raw8 *>(at) = x;
+        } else {
+            // two parts, each the nearest, of the row in its unit
+            float big = 0, to, back;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[e]));
+            big = row_max<kPieces>(big);
+            const bool odd = __any(big == INFINITY);
+            if (odd) {   // the unit of the finite ones
+                big = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) big = fmaxf(big, finite(x[e]) ? fabsf(x[e]) : 0.f);
+                big = row_max<kPieces>(big);
+            }
+            unit_of(big, to, back);
+            vec8 hi, lo;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float y = x[e] * to;
+                hi[e] = (C)y;
+                lo[e] = (C)(y - (float)hi[e]);
+            }
+            if (odd) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (!finite(x[e])) lo[e] = (C)0.f;
+            }
+            *reinterpret_cast<vec8 *>(at) = hi;
+            *reinterpret_cast<vec8 *>(at + kKeys * kKPitch) = lo;
+            if (my_dim == 0) k_back[row] = back;
+        }
+    };
+    const auto put_v = [&](raw8 x, int row) {
+        CV *const at = v_tile + row * kVPitch + my_dim;
+        if constexpr (VP == 1) {
+            *reinterpret_cast<raw8 *>(at) = x;
         } else {
             float y[8], rest = 0;
 #pragma unroll
             for (int e = 0; e < 8; ++e) y[e] = x[e];
-            vec8 part[3];
+            vvec8 part[3];
             cut3(y, part, rest);
             if (__any(rest != rest)) {   // an infinity or NaN: all of it in the first part
 #pragma unroll
@@ -248,7 +307,7 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
                     }
             }
 #pragma unroll
-            for (int j = 0; j < 3; ++j) *reinterpret_cast<vec8 *>(plane0 + j * plane + at) = part[j];
+            for (int j = 0; j < 3; ++j) *reinterpret_cast<vvec8 *>(at + j * kKeys * kVPitch) = part[j];
         }
     };
     const auto store_k = [&] {
@@ -258,9 +317,7 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
                 if (no_dim) kr[i] = raw8{};
         }
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            put(k_tile, kKeys * kKPitch, kr[i], (i * kStepRows + wave * kWaveRows + my_row) * kKPitch + my_dim);
-        }
+        for (int i = 0; i < kLoads; ++i) put_k(kr[i], i * kStepRows + wave * kWaveRows + my_row);
     };
     // V into LDS.  Where the tile's rows differ in what they see, V of positions that none
     // sees is 0, and infinities and NaN are 0 too and noted apart: a product with a weight
@@ -291,8 +348,7 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
             if (lane == 0) odd_of[wave] = odd;
         }
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i)
-            put(v_tile, kKeys * kVPitch, vr[i], (i * kStepRows + wave * kWaveRows + my_row) * kVPitch + my_dim);
+        for (int i = 0; i < kLoads; ++i) put_v(vr[i], i * kStepRows + wave * kWaveRows + my_row);
     };
 
     floatx16 o[DT];
@@ -312,6 +368,9 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
         has = has_2;
     }
     if constexpr (QP == 1) make_q();
+    // An fp32 cache's scores leave q's unit with K's.
+    const float q_unit = KP == 2 ? unit : 1.f;
+    if (KP == 2) unit = 1.f;
     const float s2 = fmaxf(d.scale_log2 * unit, 0x1p-126f);
     if (n_step) {
         store_k();
@@ -350,14 +409,26 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
                     }
             }
             // K's operands are requested kAhead products early
-            constexpr int kReads = MT * KS * (KP + kThird), kAhead = 6, kPer = KP == 3 ? 6 / (3 + kThird) : kThird ? 1 : QP;
+            constexpr int kReads = MT * KS * (KP + kThird), kAhead = 6, kPer = KP == 2 ? 3 : kThird ? 1 : QP;
             __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
-            for (int i = 0; i < kReads - kAhead; ++i) {
+            for (int i = 0; i < kReads - kAhead; i += KP) {
                 __builtin_amdgcn_sched_group_barrier(0x008, kPer, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, KP, 0);
             }
-            __builtin_amdgcn_sched_group_barrier(0x008, kAhead * kPer, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, kAhead / KP * kPer, 0);
+            if constexpr (KP == 2) {
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        const float4 b = *reinterpret_cast<const float4 *>(&k_back[32 * m + 2 * i + 4 * half]);
+                        s[m][i] *= b.x * q_unit;
+                        s[m][i + 1] *= b.y * q_unit;
+                        s[m][i + 2] *= b.z * q_unit;
+                        s[m][i + 3] *= b.w * q_unit;
+                    }
+            }
             if (!whole) {
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
@@ -396,8 +467,8 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
         has_1 = has_2;
         if (any) {
             const float base = ref == kNone ? 0.f : ref;
-            const float minus = PP == 1 && !far ? fmaf(-base, s2, Mma<C>::kBias) : Mma<C>::kBias;
-            vec8 w[MT][2][PP];
+            const float minus = PP == 1 && !far ? fmaf(-base, s2, Mma<CV>::kBias) : Mma<CV>::kBias;
+            vvec8 w[MT][2][PP];
             float part_sum = 0;
 #pragma unroll
             for (int m = 0; m < MT; ++m)
@@ -410,7 +481,7 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
                         x[i] = exp2_(fmaf(PP > 1 ? y - base : y, s2, minus));
                         if (PP > 1) part_sum += x[i];
                     }
-                    weights<PP, C>(x, w[m][h]);
+                    weights<PP, CV>(x, w[m][h]);
                     // one rounded weight is also what is summed: what rounding adds to all of a row's weights divides out
                     if constexpr (PP == 1) part_sum = sum_weights(w[m][h][0], part_sum);
                 }
@@ -419,7 +490,7 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
             // those 8 further of dim 32 i + m
             const int from = (4 * half + (lane & 15) / 4) * kVPitch + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
             const auto v_operand = [&](int plane, int t, int i) {
-                const C *at = &v_tile[plane * kKeys * kVPitch + from + 16 * t * kVPitch + 32 * i];
+                const CV *at = &v_tile[plane * kKeys * kVPitch + from + 16 * t * kVPitch + 32 * i];
                 const vec4 x = read_transposed<vec4>(at), y = read_transposed<vec4>(at + 8 * kVPitch);
                 return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
             };
@@ -428,11 +499,11 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
 #pragma unroll
                 for (int i = 0; i < DT; ++i)
 #pragma unroll
-                    for (int x = 0; x < KP; ++x) {
-                        const vec8 v = v_operand(x, t, i);
+                    for (int x = 0; x < VP; ++x) {
+                        const vvec8 v = v_operand(x, t, i);
 #pragma unroll
                         for (int y = 0; y < PP; ++y)
-                            if (KP == 1 || x + y < KP) o[i] = Mma<C>::mul32(v, w[t / 2][t & 1][y], o[i]);
+                            if (VP == 1 || x + y < VP) o[i] = Mma<CV>::mul32(v, w[t / 2][t & 1][y], o[i]);
                     }
             if (mixed && (odd_of[0] | odd_of[1] | odd_of[2] | odd_of[3])) {
                 for (int e = 0; e < kKeys; ++e) {

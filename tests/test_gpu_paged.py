@@ -464,6 +464,28 @@ def test_scores_of_minus_infinity(dtype, cache, max_q):
     assert (np.abs(got[3:23, 3:] - v) <= (UNIT[dtype] + 2.0 ** -20) * np.abs(v)).all()
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("max_q", [1, 64])
+def test_keys_of_every_size(hd, max_q):
+    """An fp32 cache whose keys reach from the smallest subnormal to 2^40, some 0, and a channel 2^12 times the others that q
+    hardly has."""
+    c = Case([(20, 150), (1, 70)], 4, 2, hd, 16, "f32", "f32", seed=hd)
+    rng = np.random.default_rng(hd)
+    for s, (_, kv) in enumerate(c.lens):
+        for p in range(kv):
+            e = [-149, -140, -126, -100, -30, -3, 0, 0, 0][int(rng.integers(0, 9))] if p else 40
+            c.k_pool[0, c.pages[s, p // 16], :, p % 16] *= 2.0 ** e
+    c.k_pool[0, c.pages[0, 3], 0, 4] = 0.0
+    c.k_pool[..., 5] *= 2.0 ** 12
+    c.q[..., 5] *= 2.0 ** -12
+    c.q[3] *= 2.0 ** -40     # a row that the largest key is nothing special to
+    c.q[7] *= 2.0 ** -130
+    c.up()
+    with c.handle() as kv:
+        c.attend(kv, max_q=max_q)
+    check_rows(c, c.rows("out", 4)[0], *c.exact())
+
+
 @pytest.mark.parametrize("dtype,cache", PAIRS)
 @pytest.mark.parametrize("max_q", [1, 64])
 def test_a_page_twice_in_a_sequence(dtype, cache, max_q):
