@@ -330,18 +330,13 @@ __device__ __forceinline__ void split_p(float x, C (&part)[N]) {
     }
 }
 
-// A power of two that brings |x| <= big to 2^13 .. 2^14 (1 where there is none),
-// and its inverse.
+// A power of two that brings |x| <= big to 2^13 .. 2^14 (2^126 at most: big under
+// 2^-112 stays smaller), and its inverse.  big >= 0, no NaN.
 __device__ __forceinline__ void unit_of(float big, float &to, float &back) {
-    const int e = (int)((__builtin_bit_cast(unsigned, big) >> 23) & 255);
-    if (e == 0 || e == 255) {   // 0 or a subnormal, or not finite
-        to = back = 1.f;
-        if (e == 0 && big != 0.f) { to = 0x1p120f; back = 0x1p-120f; }
-        return;
-    }
-    const int up = min(max(140 - e, -126), 126);   // 2^up * 2^(e - 127) = 2^13
-    to = __builtin_bit_cast(float, (unsigned)(127 + up) << 23);
-    back = __builtin_bit_cast(float, (unsigned)(127 - up) << 23);
+    const unsigned e = __builtin_bit_cast(unsigned, big) >> 23;
+    const unsigned up = min(267u - e, 253u);   // 2^(up - 127) 2^(e - 127) = 2^13
+    to = __builtin_bit_cast(float, up << 23);
+    back = __builtin_bit_cast(float, (254u - up) << 23);
 }
 
 // ---- the softmax ---------------------------------------------------------------

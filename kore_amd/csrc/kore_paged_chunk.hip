@@ -47,6 +47,10 @@ template <class A, class S, int HDP> struct Shape {
 __device__ __forceinline__ unsigned upper_halves(float a, float b) {
     return __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, b), __builtin_bit_cast(unsigned, a), 0x07060302);
 }
+__device__ __forceinline__ float dot_ones(unsigned pair, float s) {
+    typedef bhalf_t bhalf2_t __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bhalf2_t, pair), bhalf2_t{(bhalf_t)1.f, (bhalf_t)1.f}, s, false);
+}
 __device__ __forceinline__ void cut3(const float (&x)[8], bhalf8 (&part)[3], float &rest) {
     typedef unsigned uint4_t __attribute__((ext_vector_type(4)));
     uint4_t u[3];
@@ -57,26 +61,28 @@ __device__ __forceinline__ void cut3(const float (&x)[8], bhalf8 (&part)[3], flo
         for (int j = 0; j < 2; ++j) {
             r[j] = x[i + j] - bf16_cut(x[i + j]);
             l[j] = r[j] - bf16_cut(r[j]);
-            rest += l[j];
         }
         u[0][i / 2] = upper_halves(x[i], x[i + 1]);
         u[1][i / 2] = upper_halves(r[0], r[1]);
         u[2][i / 2] = upper_halves(l[0], l[1]);
+        rest = dot_ones(u[2][i / 2], rest);
     }
 #pragma unroll
     for (int j = 0; j < 3; ++j) part[j] = __builtin_bit_cast(bhalf8, u[j]);
 }
-// The largest of PIECES neighbouring lanes' values: 8, 16 or 32.
+// The largest of PIECES neighbouring lanes' values (8, 16 or 32; none under 0, so that their bits compare as integers).
 template <int CTRL>
-__device__ __forceinline__ float max_lane(float x) {
-    return fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, false)));
+__device__ __forceinline__ unsigned max_lane(unsigned x) {
+    return max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true));
 }
 template <int PIECES>
-__device__ __forceinline__ float row_max(float x) {
-    if constexpr (PIECES == 32) x = max16(x);
+__device__ __forceinline__ float row_max(float big) {
+    if constexpr (PIECES == 32) big = max16(big);
+    unsigned x = __builtin_bit_cast(unsigned, big);
     if constexpr (PIECES >= 16) x = max_lane<0x140>(x);    // lane 15 - i of 16
     x = max_lane<0x141>(x);                                 // lane 7 - i of 8
-    return max_lane<0x4e>(max_lane<0xb1>(x));               // lanes i ^ 1, i ^ 2
+    x = max_lane<0x4e>(max_lane<0xb1>(x));                  // lanes i ^ 1, i ^ 2
+    return __builtin_bit_cast(float, x);
 }
 // Eight weights as N parts of C.
 template <int N, class C, class V>
@@ -267,21 +273,28 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
             if (odd) {   // the unit of the finite ones
                 big = 0;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) big = fmaxf(big, finite(x[e]) ? fabsf(x[e]) : 0.f);
+                for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.f);
                 big = row_max<kPieces>(big);
             }
             unit_of(big, to, back);
             vec8 hi, lo;
+            typedef C vec2 __attribute__((ext_vector_type(2)));
+            typedef float float2_t __attribute__((ext_vector_type(2)));
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float y = x[e] * to;
-                hi[e] = (C)y;
-                lo[e] = (C)(y - (float)hi[e]);
+            for (int e = 0; e < 8; e += 2) {
+                const float2_t y = {x[e] * to, x[e + 1] * to};
+                const vec2 h = __builtin_convertvector(y, vec2);
+                const float2_t r = {__builtin_fmaf((float)h[0], -1.f, y[0]), __builtin_fmaf((float)h[1], -1.f, y[1])};
+                const vec2 l = __builtin_convertvector(r, vec2);
+                hi[e] = h[0];
+                hi[e + 1] = h[1];
+                lo[e] = l[0];
+                lo[e + 1] = l[1];
             }
             if (odd) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    if (!finite(x[e])) lo[e] = (C)0.f;
+                    if (!(fabsf(x[e]) < INFINITY)) lo[e] = (C)0.f;
             }
             *reinterpret_cast<vec8 *>(at) = hi;
             *reinterpret_cast<vec8 *>(at + kKeys * kKPitch) = lo;
