@@ -3,10 +3,10 @@
 //
 // A tile is 16 rows: the q-heads of one token's kv-head, or of a few tokens.  K and
 // V are read once for them, so at 16 flops a cache value the kernel is bound by
-// HBM; 16 waves' worth of loads in flight per CU are what carries it.  A workgroup
-// is four waves that take blocks of keys in turn, each with its own softmax state,
-// merged through LDS at the end; the next block's K and V are requested before the
-// current one is computed.
+// HBM; eight waves a CU, each with its next block in flight, are what carries it.  A
+// workgroup is four waves that take blocks of keys in turn, each with its own softmax
+// state, merged through LDS at the end; the next block's K is requested when this
+// one's scores are made, its V when this one's is in LDS (or used).
 #include "kore_paged_attend.h"
 
 #include <algorithm>
@@ -67,6 +67,10 @@ __device__ __forceinline__ void finish(const TileArgs &d, const Place &p, const 
 // k order of its own; V^T's operand in that order comes out of LDS by transposed
 // reads (rows padded by 32 bytes: the 8 rows that half a wave reads lie on different
 // banks).  No lane ever needs another's score but for the maximum and the sum.
+//
+// 32 sequences of 1k to 8k keys, 28/4/128, fp32 rows over an fp16 cache: 63 us for 282
+// MB, 4.5 TB/s (a large copy: 5.1); one bf16 token over 131072 keys of 16/2/128: 29.6
+// us for 134 MB, 4.5 TB/s.
 template <class A, class C, int HDP>
 __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode16_kernel(TileArgs d) {
     // 16-bit rows could have their weights in one part; the second costs nothing beside the loads, and leaves the result
@@ -314,6 +318,10 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode16_kernel(
 // Lane (m, g) loads K's row m, dims 16 u + 4 g + e: e picks the instruction, g is its
 // k.  The scores of keys 4 g + i are its k order of the second product, whose V
 // operand, lane (m, g): V[4 g + i][64 j + 4 m + e], comes straight from memory too.
+//
+// One token over 512 keys of 14/2/64: 6.1 us (a launch's own time is some 2; then three
+// rounds of memory); 24 of uneven length, 28/4/128: 100 us for
+// 455 MB, 4.5 TB/s.
 template <int HDP>
 __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode32_kernel(TileArgs d) {
     constexpr int KU = HDP / 16, DJ = HDP / 64, kBlock = 16;
@@ -483,7 +491,9 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode32_kernel(
 // TILE rows by 256 / TILE lanes, which are laid over the tile's splits and, what is left
 // of them, over the dims, four a lane.  A lane has eight splits' loads in flight and a
 // running reference; the lanes' states meet in LDS.  gridDim.y workgroups share a
-// tile's dims.  (Few tiles may have hundreds of splits, many tiles two each.)
+// tile's dims.  (Few tiles may have hundreds of splits, many tiles two each.)  Bound by
+// its launch and two rounds of memory: 4.7 us for two tiles of eight splits, 7.5 for 128
+// of three, 12.4 for 112 of 128 rows.
 template <class A, int TILE>
 __global__ __launch_bounds__(kThreads) void merge_kernel(TileArgs d, int hd4) {
     constexpr int kLanes = kThreads / TILE, kFlight = 8;
@@ -580,7 +590,7 @@ hipError_t launch_decode(const TileArgs &d, hipStream_t s) {
 }
 
 constexpr int kPerCu = 2;                              // workgroups of a CU, of the 16-row kernels
-constexpr int kShort = 1024, kChunkShort = 2048;       // keys that a tile among many is not split for
+constexpr int kShort = 1280;                           // keys that a tile among many is not split for
 
 }  // namespace
 
@@ -599,9 +609,9 @@ hipError_t launch_attend(const AttendArgs &a, hipStream_t s) {
     d.out_wide = (uintptr_t)a.out % (4 * size) == 0 && a.out_stride % 4 == 0;
     const int max_q = a.max_q ? a.max_q : (a.b.n_tok + a.b.n_seq - 1) / a.b.n_seq;
     // Tiles of 16 rows read a sequence's keys once each, most of it from L2: up to three of them beat one of 128.  us, 16 /
-    // 128 rows a tile, 28/4/128 at 32768 keys, new rows 2, 6, 9, 18: fp16 20.0 / 26.0, 27.1 / 26.1, 41.8 / 26.2, 52.3 /
-    // 28.3; fp32 rows and cache 31 / 59, 55 / 60, 79 / 61, 122 / 66; 16 sequences of 2048, fp16: 22.9 / 29.7, 29.8 / 30.4,
-    // 29.8 / 30.3, 45.9 / 37.9.
+    // 128 rows a tile, 28/4/128 at 32768 keys, new rows 2, 6, 9, 18: fp16 20.7 / 26.6, 27.5 / 26.7, 42.3 / 26.7, 53.3 /
+    // 28.8; fp32 rows and cache 32 / 55, 56 / 57, 80 / 56, 124 / 61; 16 sequences of 2048, fp16: 23.4 / 27.8, 30.9 / 27.9,
+    // 30.0 / 28.3, 47.5 / 36.5.
     const bool chunk = (long long)max_q * d.cut.rep > 3 * kRows;
     const int rows = chunk ? kChunkRows : kRows;
     // the most (tile, kv-head)s that n_tok rows of n_seq sequences can be
@@ -609,18 +619,19 @@ hipError_t launch_attend(const AttendArgs &a, hipStream_t s) {
     // Few tiles: splits make up the workgroups that the card holds at once.  From half of those on it is the longest tiles
     // alone that are split, those of some twice the mean (chunks) or over it (16 rows), and none where a tile cannot have
     // many keys or all are one sequence's: the merge's launch and the partials cost every call.  us, split / not, 28/4/128:
-    //   rows of one sequence over 4096 keys, tiles 34 %, 50 %, 59 % of the CUs: fp16 52.7 / 75.0, 58.0 / 76.3, 80.4 / 76.7;
-    //   fp32 170 / 297, 188 / 300, 308 / 304;
-    //   four prompts of 512 beside a token over 65536: fp16 77 / 1049, fp32 219 / 4493; over 2048: 59 / 56, 197 / 193;
-    //   300 tokens over 1000 keys, one of them over 65536: 187 / 763; none: 115 / 115;
-    //   100 tokens over 300 keys, one over 512, 1024, 2048: 22.2 / 16.7, 22.6 / 20.5, 24.3 / 29.7.
+    //   rows of one sequence over 4096 keys, tiles 34 %, 50 %, 59 % of the CUs: fp16 55 / 80, 60 / 79, 80 / 77; fp32 160 /
+    //   271, 172 / 278, 276 / 272;
+    //   four prompts of 512 beside a token over 1024, 2048, 65536: fp16 44.7 / 41.0, 49.1 / 56.7, 77 / 1041; fp32 122 / 119,
+    //   128 / 179, 208 / 4025;
+    //   100 tokens over 300 keys, one over 1024, 2048, 65536: 23.0 / 20.6, 24.8 / 29.5, 60 / 645;
+    //   300 tokens over 1000 keys, one over 65536: 186 / 776; 300 over 1100: 137 / 124 (the price of being ready for it).
     const int at_once = chunk ? a.num_cu : kPerCu * a.num_cu;
     const long long most = std::min((long long)a.b.pages_stride << a.page_shift, (long long)a.window + (rows - 1) / d.cut.rep + 65);
-    // A step of a chunk's two teams, or half a workgroup's blocks: 64 fp32 rows over 512 keys 21.5 us, in splits of 256 keys
-    // 32.6; 64 fp16 rows 15.4, of 64 keys 15.8, of 256 16.8; one token over 512 keys 9.6, of 128 10.1, of 256 11.2.
+    // A split's fewest keys, of 64, 128 and 256: 64 fp32 rows over 512 keys 22.6, 25.1, 32.4 us; 64 fp16 rows 15.5, 15.3,
+    // 16.8; one token over 512 keys 9.6, 10.1, 11.2.
     d.cut.min_len = chunk && size == 2 ? 128 : 64;
     if (2 * tiles <= at_once) d.cut.target = most > d.cut.min_len ? (int)(at_once - tiles) : 0;
-    else if (a.b.n_seq == 1 || most <= (chunk ? kChunkShort : kShort)) d.cut.target = 0;
+    else if (a.b.n_seq == 1 || most <= kShort) d.cut.target = 0;
     else d.cut.target = (int)(chunk ? std::min<long long>(tiles / 2, at_once) : std::min<long long>(tiles, at_once / 2));
     d.scale_log2 = (float)((double)a.scale * 1.4426950408889634074);
     const int hdp = padded_dim(a.hd);
@@ -630,7 +641,8 @@ hipError_t launch_attend(const AttendArgs &a, hipStream_t s) {
     d.part_ml = a.part + (size_t)d.parts * rows * hdp;
     const hipError_t e = chunk ? launch_chunk(d, s) : launch_decode(d, s);
     if (e != hipSuccess || !d.cut.target) return e;
-    // some four workgroups a CU, where there are dims enough
+    // some eight workgroups a CU, where there are dims enough (32 sequences, fp16 cache: 57.8 us from cache, with one a CU
+    // 78.3, with 32 59.9)
     const int joined = (int)std::min<long long>(d.cut.target, tiles);   // the most tiles that can be split
     const dim3 merge((unsigned)joined, (unsigned)std::clamp(8 * a.num_cu / joined, 1, a.hd / 4));
 #define KORE_MERGE(A)                                                                    \

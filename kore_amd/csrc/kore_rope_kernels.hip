@@ -2,7 +2,10 @@
 // rows to a paged cache (gfx950).
 //
 // Both are bound by memory: 12 flops a pair beside 16 bytes (fp32) of traffic,
-// and a cosine and sine for each pair of a row, shared by its heads.
+// and a cosine and sine for each pair of a row, shared by its heads.  4096 bf16 rows of
+// 36 heads of 96: 11.8 us, 4.8 TB/s (a large copy: 5.1); three prompts' 1777 rows of
+// 28/4/128 into a bf16 cache: 15.1 us, 5.2 TB/s.  Few rows are a launch and three
+// dependent rounds of memory: one row of 32 heads 2.4 us, an append of 16 rows 3.5.
 #include "kore_paged_device.h"
 
 #include <algorithm>
@@ -203,14 +206,16 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a) {
 }
 
 // Workgroups that share a row: as many as give a thread one unit while the launch has
-// less than four a CU or so.
+// less than four a CU or so (us, with them / one a row, 32 heads of 128: 1 row 2.39 /
+// 2.61, 16 rows 3.07 / 3.50, 333 rows 3.90 / 4.23; an append of 16 rows 3.39 / 4.54).
 dim3 row_grid(int n_tok, int total) {
     const int most = (total + kThreads - 1) / kThreads;
     return dim3((unsigned)n_tok, (unsigned)std::clamp(1024 / n_tok, 1, most));
 }
 
 // Four values at once where rows, heads and the two parts of a head start at
-// multiples of four, one otherwise.
+// multiples of four, one otherwise (4096 rows of 36 heads of 96: 12.0 us, one value at a
+// time 16.7).
 bool fours(int rot, int hd) { return rot % 8 == 0 && (hd - rot) % 8 == 0; }
 template <class... P>
 bool aligned(int bytes, P... p) {
