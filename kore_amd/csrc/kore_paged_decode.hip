@@ -4,9 +4,10 @@
 // A tile is 16 rows: the q-heads of one token's kv-head, or of a few tokens.  K and
 // V are read once for them, so at 16 flops a cache value the kernel is bound by
 // HBM; eight waves a CU, each with its next block in flight, are what carries it.  A
-// workgroup is four waves that take blocks of keys in turn, each with its own softmax
-// state, merged through LDS at the end; the next block's K is requested when this
-// one's scores are made, its V when this one's is in LDS (or used).
+// workgroup is W = 4 waves (8 where little is to be read, launch_attend) that take
+// blocks of keys in turn, each with its own softmax state, merged through LDS at the
+// end; the next block's K is requested when this one's scores are made, its V when this
+// one's is in LDS (or used).
 #include "kore_paged_attend.h"
 
 #include <algorithm>
@@ -14,24 +15,24 @@
 namespace kore_paged_gpu {
 namespace {
 
-constexpr int kThreads = 256, kWaves = 4, kRows = 16;
+constexpr int kThreads = 256, kRows = 16;
 
-// The four waves' states (ref, sum, and o as [dim / 4][row] float4) into out, or
+// The W waves' states (ref, sum, and o as [dim / 4][row] float4) into out, or
 // into the split's partial.
-template <class A, int HDP>
+template <class A, int HDP, int W>
 __device__ __forceinline__ void finish(const TileArgs &d, const Place &p, const float4 (*o)[HDP / 4][kRows],
                                        const float2 (*ml)[kRows]) {
     const AttendArgs &a = d.a;
     __syncthreads();
     const int rep = d.cut.rep;
-    for (int i = threadIdx.x; i < HDP / 4 * kRows; i += kThreads) {
+    for (int i = threadIdx.x; i < HDP / 4 * kRows; i += 64 * W) {
         const int row = i % kRows, d4 = i / kRows;
         float m = kNone, l = 0;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) m = fmaxf(m, ml[w][row].x);
+        for (int w = 0; w < W; ++w) m = fmaxf(m, ml[w][row].x);
         float4 s = make_float4(0, 0, 0, 0);
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
+        for (int w = 0; w < W; ++w) {
             const float2 e = ml[w][row];
             const float f = share_at(e.x, m, d.scale_log2);
             const float4 v = o[w][d4][row];
@@ -71,8 +72,8 @@ __device__ __forceinline__ void finish(const TileArgs &d, const Place &p, const 
 // 32 sequences of 1k to 8k keys, 28/4/128, fp32 rows over an fp16 cache: 63 us for 282
 // MB, 4.5 TB/s (a large copy: 5.1); one bf16 token over 131072 keys of 16/2/128: 29.6
 // us for 134 MB, 4.5 TB/s.
-template <class A, class C, int HDP>
-__global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode16_kernel(TileArgs d) {
+template <class A, class C, int HDP, int W>
+__global__ __launch_bounds__(64 * W, HDP <= 128 && W == 4 ? 2 : 1) void decode16_kernel(TileArgs d) {
     // 16-bit rows could have their weights in one part; the second costs nothing beside the loads, and leaves the result
     // no rounding but its own (bf16, one token over 131072 keys: error 1.7e-3 instead of 2.3e-3 of the result)
     constexpr int QP = Parts<A, C>::q, PP = Parts<A, C>::p == 1 ? 2 : Parts<A, C>::p;
@@ -81,11 +82,11 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode16_kernel(
     constexpr int kBlock = 32;
     typedef typename Mma<C>::vec8 vec8;
     typedef C vec4 __attribute__((ext_vector_type(4)));
-    constexpr size_t kVBytes = sizeof(C) * kWaves * kBlock * kPitch, kOBytes = sizeof(float) * kWaves * HDP * kRows;
+    constexpr size_t kVBytes = sizeof(C) * W * kBlock * kPitch, kOBytes = sizeof(float) * W * HDP * kRows;
     __shared__ __attribute__((aligned(16))) unsigned char shared[kVBytes > kOBytes ? kVBytes : kOBytes];
-    __shared__ float2 ml[kWaves][kRows];
+    __shared__ float2 ml[W][kRows];
     // of V's pieces in blocks that the tile's rows do not all see: which of 8 dims are +inf, or -inf (a NaN: both)
-    __shared__ unsigned kinds[kWaves][2][kBlock][HDP / 32];
+    __shared__ unsigned kinds[W][2][kBlock][HDP / 32];
     const AttendArgs &a = d.a;
     const int cap = a.b.pages_stride << a.page_shift, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Place p;
@@ -100,9 +101,9 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode16_kernel(
     // page groups of this wave: block j's two are lanes 2 (j % 32), + 1
     const int first_block = k.lo / kBlock + wave;
     const auto pages_from = [&](int j) {
-        return PageRun::load(a, table, (first_block + kWaves * (j + (lane >> 1))) * 2 + (lane & 1), k.hi);
+        return PageRun::load(a, table, (first_block + W * (j + (lane >> 1))) * 2 + (lane & 1), k.hi);
     };
-    const int n_block = k.lo < k.hi ? max(0, ((k.hi + kBlock - 1) / kBlock - first_block + kWaves - 1) / kWaves) : 0;
+    const int n_block = k.lo < k.hi ? max(0, ((k.hi + kBlock - 1) / kBlock - first_block + W - 1) / W) : 0;
     PageRun run;
     run.now = pages_from(0);
     run.ahead = -1;
@@ -189,11 +190,11 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode16_kernel(
     }
     const float s2 = fmaxf(d.scale_log2 * unit, 0x1p-126f);
     for (int j = 0; j < n_block; ++j) {
-        const int key0 = (first_block + kWaves * j) * kBlock;
+        const int key0 = (first_block + W * j) * kBlock;
         const bool has0 = p0 >= 0, has1 = p1 >= 0;
         const bool whole = key0 >= k.all_lo && key0 + kBlock <= min(k.all_hi, k.hi) && has0 && has1;
         // pages of the next block
-        const int next = j + 1, next_key = key0 + kWaves * kBlock;
+        const int next = j + 1, next_key = key0 + W * kBlock;
         if ((next & 31) == 0) {
             run.now = run.ahead;
             run.ahead = pages_from(next + 32);
@@ -309,7 +310,7 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode16_kernel(
 #pragma unroll
     for (int i = 0; i < DT; ++i) states[wave][4 * i + g][col] = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
     if (g == 0) ml[wave][col] = make_float2(ref * unit, sum);
-    finish<A, HDP>(d, p, states, ml);
+    finish<A, HDP, W>(d, p, states, ml);
 }
 
 // ---- fp32 caches ---------------------------------------------------------------
@@ -322,11 +323,11 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode16_kernel(
 // One token over 512 keys of 14/2/64: 6.1 us (a launch's own time is some 2; then three
 // rounds of memory); 24 of uneven length, 28/4/128: 100 us for
 // 455 MB, 4.5 TB/s.
-template <int HDP>
-__global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode32_kernel(TileArgs d) {
+template <int HDP, int W>
+__global__ __launch_bounds__(64 * W, HDP <= 128 && W == 4 ? 2 : 1) void decode32_kernel(TileArgs d) {
     constexpr int KU = HDP / 16, DJ = HDP / 64, kBlock = 16;
-    __shared__ float4 states[kWaves][HDP / 4][kRows];
-    __shared__ float2 ml[kWaves][kRows];
+    __shared__ float4 states[W][HDP / 4][kRows];
+    __shared__ float2 ml[W][kRows];
     const AttendArgs &a = d.a;
     const int cap = a.b.pages_stride << a.page_shift, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Place p;
@@ -340,8 +341,8 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode32_kernel(
 
     // block j's page is lane j % 64
     const int first_block = k.lo / kBlock + wave;
-    const auto pages_from = [&](int j) { return PageRun::load(a, table, first_block + kWaves * (j + lane), k.hi); };
-    const int n_block = k.lo < k.hi ? max(0, ((k.hi + kBlock - 1) / kBlock - first_block + kWaves - 1) / kWaves) : 0;
+    const auto pages_from = [&](int j) { return PageRun::load(a, table, first_block + W * (j + lane), k.hi); };
+    const int n_block = k.lo < k.hi ? max(0, ((k.hi + kBlock - 1) / kBlock - first_block + W - 1) / W) : 0;
     PageRun run;
     run.now = pages_from(0);
     run.ahead = -1;
@@ -394,9 +395,9 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode32_kernel(
     for (int u = 0; u < KU; ++u)
         if (!row.real || 16 * u + 4 * g >= a.hd) q[u] = floatx4{0, 0, 0, 0};
     for (int j = 0; j < n_block; ++j) {
-        const int key0 = (first_block + kWaves * j) * kBlock;
+        const int key0 = (first_block + W * j) * kBlock;
         const bool has = page >= 0, whole = key0 >= k.all_lo && key0 + kBlock <= min(k.all_hi, k.hi) && has;
-        const int next = j + 1, next_key = key0 + kWaves * kBlock;
+        const int next = j + 1, next_key = key0 + W * kBlock;
         if ((next & 63) == 0) {
             run.now = run.ahead;
             run.ahead = pages_from(next + 64);
@@ -483,7 +484,7 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void decode32_kernel(
         for (int i = 0; i < 4; ++i)
             states[wave][16 * x + 4 * g + i][col] = make_float4(o[4 * x][i], o[4 * x + 1][i], o[4 * x + 2][i], o[4 * x + 3][i]);
     if (g == 0) ml[wave][col] = make_float2(ref, sum);
-    finish<float, HDP>(d, p, states, ml);
+    finish<float, HDP, W>(d, p, states, ml);
 }
 
 // ---- the merge of splits ---------------------------------------------------------
@@ -566,25 +567,23 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(TileArgs d, int hd4) {
     }
 }
 
+template <int W>
 hipError_t launch_decode(const TileArgs &d, hipStream_t s) {
     const int hdp = padded_dim(d.a.hd);
     const dim3 grid((unsigned)d.places);
-#define KORE_DECODE(...)                                                 \
-    do {                                                                 \
-        if (hdp == 64) KORE_DECODE_(64, __VA_ARGS__);                    \
-        else if (hdp == 128) KORE_DECODE_(128, __VA_ARGS__);             \
-        else KORE_DECODE_(256, __VA_ARGS__);                             \
+#define KORE_DECODE(KERNEL, ...)                                                                \
+    do {                                                                                        \
+        if (hdp == 64) KERNEL<__VA_ARGS__ 64, W><<<grid, 64 * W, 0, s>>>(d);                    \
+        else if (hdp == 128) KERNEL<__VA_ARGS__ 128, W><<<grid, 64 * W, 0, s>>>(d);             \
+        else if constexpr (W == 4) KERNEL<__VA_ARGS__ 256, W><<<grid, 64 * W, 0, s>>>(d);       \
     } while (0)
-#define KORE_DECODE_(H, A, C) decode16_kernel<A, C, H><<<grid, kThreads, 0, s>>>(d)
-    if (d.a.cache_type == kF32) {
-        if (hdp == 64) decode32_kernel<64><<<grid, kThreads, 0, s>>>(d);
-        else if (hdp == 128) decode32_kernel<128><<<grid, kThreads, 0, s>>>(d);
-        else decode32_kernel<256><<<grid, kThreads, 0, s>>>(d);
-    } else if (d.a.type == kF32 && d.a.cache_type == kF16) KORE_DECODE(float, half_t);
-    else if (d.a.type == kF32) KORE_DECODE(float, bhalf_t);
-    else if (d.a.type == kF16) KORE_DECODE(half_t, half_t);
-    else KORE_DECODE(bhalf_t, bhalf_t);
-#undef KORE_DECODE_
+#define KORE_COMMA ,
+    if (d.a.cache_type == kF32) KORE_DECODE(decode32_kernel);
+    else if (d.a.type == kF32 && d.a.cache_type == kF16) KORE_DECODE(decode16_kernel, float KORE_COMMA half_t KORE_COMMA);
+    else if (d.a.type == kF32) KORE_DECODE(decode16_kernel, float KORE_COMMA bhalf_t KORE_COMMA);
+    else if (d.a.type == kF16) KORE_DECODE(decode16_kernel, half_t KORE_COMMA half_t KORE_COMMA);
+    else KORE_DECODE(decode16_kernel, bhalf_t KORE_COMMA bhalf_t KORE_COMMA);
+#undef KORE_COMMA
 #undef KORE_DECODE
     return hipGetLastError();
 }
@@ -630,7 +629,15 @@ hipError_t launch_attend(const AttendArgs &a, hipStream_t s) {
     // A split's fewest keys, of 64, 128 and 256: 64 fp32 rows over 512 keys 22.6, 25.1, 32.4 us; 64 fp16 rows 15.5, 15.3,
     // 16.8; one token over 512 keys 9.6, 10.1, 11.2.
     d.cut.min_len = chunk && size == 2 ? 128 : 64;
-    if (2 * tiles <= at_once) d.cut.target = most > d.cut.min_len ? (int)(at_once - tiles) : 0;
+    // Few tiles of 16 rows whose K and V cannot be much stay whole, with twice the waves, and need no merge: up to some 240
+    // KB, and more where there are more tiles to split.  us, split / whole: a token over 256 keys of 14/2/64 fp32 (128 KB)
+    // 9.6 / 7.3, over 512 9.9 / 10.1; of 28/4/128 fp16 over 256 (128 KB) 11.8 / 9.6, 512 12.1 / 10.9, 1024 12.5 / 15.3; 32
+    // tokens of those over 512 15.5 / 12.3, 1024 23.0 / 16.9.  (16 waves for heads of 64: 8.5 and 11.1 in the first case.)
+    const bool few = 2 * tiles <= at_once;
+    const bool wide = !chunk && few && a.hd <= 128 && most > d.cut.min_len &&
+                      2 * most * a.hd * type_bytes(a.cache_type) <= (240 + 2 * tiles) << 10;
+    if (wide) d.cut.target = 0;
+    else if (few) d.cut.target = most > d.cut.min_len ? (int)(at_once - tiles) : 0;
     else if (a.b.n_seq == 1 || most <= kShort) d.cut.target = 0;
     else d.cut.target = (int)(chunk ? std::min<long long>(tiles / 2, at_once) : std::min<long long>(tiles, at_once / 2));
     d.scale_log2 = (float)((double)a.scale * 1.4426950408889634074);
@@ -639,7 +646,7 @@ hipError_t launch_attend(const AttendArgs &a, hipStream_t s) {
     d.part_o = a.part;
     d.parts = d.cut.target + (int)std::min<long long>(d.cut.target, tiles);
     d.part_ml = a.part + (size_t)d.parts * rows * hdp;
-    const hipError_t e = chunk ? launch_chunk(d, s) : launch_decode(d, s);
+    const hipError_t e = chunk ? launch_chunk(d, s) : wide ? launch_decode<8>(d, s) : launch_decode<4>(d, s);
     if (e != hipSuccess || !d.cut.target) return e;
     // some eight workgroups a CU, where there are dims enough (32 sequences, fp16 cache: 57.8 us from cache, with one a CU
     // 78.3, with 32 59.9)

@@ -137,6 +137,22 @@ def test_long_contexts_are_split(dtype, cache):
 
 
 @pytest.mark.parametrize("dtype,cache", PAIRS)
+@pytest.mark.parametrize("nh,nkv,hd", [(14, 2, 64), (28, 4, 128), (33, 3, 96)])
+@pytest.mark.parametrize("window", [0, 50])
+def test_short_tables(dtype, cache, nh, nkv, hd, window):
+    """A few tokens over a table of few pages: tiles in one piece on either side of where splitting begins, some without a key."""
+    for keys in (65, 112, 240, 448, 500, 1000):
+        c = Case([(1, keys), (1, 1), (2, keys // 2), (1, 0), (1, 7)], nh, nkv, hd, 16, dtype, cache, seed=keys, extra_rows=1)
+        c.kv_len[1] = 10 ** 6 if keys == 240 else 1     # past the table: its last positions are all there are
+        c.up()
+        with c.handle() as kv:
+            c.attend(kv, window=window)
+        got = c.rows("out", nh)[0]
+        assert (got[c.used:] == 77.0).all()
+        check_rows(c, got, *c.exact(window=window), "%d keys" % keys)
+
+
+@pytest.mark.parametrize("dtype,cache", PAIRS)
 @pytest.mark.parametrize("new,n_seq,kv", [(1, 75, (1, 120)), (80, 6, (80, 200))])
 def test_a_long_sequence_among_many_tiles(dtype, cache, new, n_seq, kv):
     """Tiles enough to fill the card, those of two sequences longer than the rest by far: theirs alone are split."""
