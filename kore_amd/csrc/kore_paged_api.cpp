@@ -395,7 +395,7 @@ int kore_paged_create(kore_paged_t *out, const kore_paged_config *cfg) {
         if ((e = hipMemsetAsync(h->v_pool, 0, h->pool_bytes(), h->stream)) != hipSuccess) return bail(e, "hipMemset");
         if ((e = hipStreamSynchronize(h->stream)) != hipSuccess) return bail(e, "hipStreamSynchronize");
     }
-    h->part_bytes = attend_workspace_bytes(c.n_head, c.n_head_kv, c.head_dim, h->num_cu);
+    h->part_bytes = attend_workspace_bytes(c.head_dim, h->num_cu);
     if ((e = hipMalloc(&h->part, h->part_bytes)) != hipSuccess) return bail(e, "workspace allocation");
     h->cfg.k_pool = h->k_pool;
     h->cfg.v_pool = h->v_pool;

@@ -388,27 +388,36 @@ __device__ __forceinline__ Row row_of(const Place &p, int r, const Cut &c, int c
 // N pieces of a row of q, 8 values each, piece t from dim first + step t: all requested
 // before one is used.  What is not there (a row past the last, dims past the head) is
 // something else of the row, for zero_q to clear when the rest has arrived.
+template <class A>
+__device__ __forceinline__ const A *q_row_of(const AttendArgs &a, const Place &p, const Row &row) {
+    return (const A *)a.q + (size_t)(row.real ? p.q0 + row.token : p.q0) * a.q_stride + (size_t)(row.real ? row.head : 0) * a.hd;
+}
+template <class A>
+__device__ __forceinline__ void load_piece(const A *src, bool wide, A (&x)[8]) {
+    constexpr int kPer = 16 / sizeof(A);
+    if (wide) {
+        typedef A piece __attribute__((ext_vector_type(kPer)));
+#pragma unroll
+        for (int i = 0; i < 8; i += kPer) {
+            const piece v = *reinterpret_cast<const piece *>(src + i);
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) x[i + j] = v[j];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = src[i];
+    }
+}
 template <int N, class A>
 __device__ __forceinline__ void load_q(const AttendArgs &a, const Place &p, const Row &row, bool wide, int first, int step,
                                        A (&x)[N][8]) {
-    const A *const src = (const A *)a.q + (size_t)(row.real ? p.q0 + row.token : p.q0) * a.q_stride +
-                         (size_t)(row.real ? row.head : 0) * a.hd;
+    const A *const src = q_row_of<A>(a, p, row);
     if (wide) {
-        typedef A piece __attribute__((ext_vector_type(16 / sizeof(A))));
-        constexpr int kPer = 16 / sizeof(A);
 #pragma unroll
-        for (int t = 0; t < N; ++t)
-#pragma unroll
-            for (int i = 0; i < 8; i += kPer) {
-                const piece v = *reinterpret_cast<const piece *>(src + min(first + step * t, a.hd - 8) + i);
-#pragma unroll
-                for (int j = 0; j < kPer; ++j) x[t][i + j] = v[j];
-            }
+        for (int t = 0; t < N; ++t) load_piece(src + min(first + step * t, a.hd - 8), true, x[t]);
     } else {
 #pragma unroll
-        for (int t = 0; t < N; ++t)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[t][i] = src[min(first + step * t, a.hd - 8) + i];
+        for (int t = 0; t < N; ++t) load_piece(src + min(first + step * t, a.hd - 8), false, x[t]);
     }
 }
 template <int N, class A>

@@ -126,7 +126,14 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
     // A team's step of K and of V, in KP and VP planes; at the end half of the second team's sums lie there
     constexpr int kStep = kKeys * (KP * kKPitch + VP * kVPitch), kTileBytes = kTeams * kStep * (int)sizeof(C);
     constexpr int kMeetBytes = kTeams == 2 ? kWaves * HDP / 16 * 64 * 16 : 0;
-    __shared__ __attribute__((aligned(16))) unsigned char tiles[kTileBytes > kMeetBytes ? kTileBytes : kMeetBytes];
+    // before the first step the tile's rows of q lie there: each is read once, by lanes side by side (in the operands'
+    // order a load touches 32 rows, and either team reads all: 28/4/128, 64 fp16 rows over 512 keys 15.4 us instead of 14.7,
+    // fp32 22.5 instead of 21.5, a 2048-row fp16 prompt 57.8 instead of 56.1; at HDP = 256 fp32 rows would not fit beside
+    // q's third part)
+    constexpr bool kStage = kTeams == 2;
+    constexpr int kQPitch = HDP + 16 / (int)sizeof(A), kQBytes = kStage ? kRows * kQPitch * (int)sizeof(A) : 0;
+    constexpr int kMost = kTileBytes > kMeetBytes ? kTileBytes : kMeetBytes;
+    __shared__ __attribute__((aligned(16))) unsigned char tiles[kMost > kQBytes ? kMost : kQBytes];
     // The third part of q, where LDS has room: it would cost the loop its spare registers, and a reload of a spilled
     // one waits for the loads in flight.  (The teams' rows are the same.)
     constexpr bool kThird = QP == 3;
@@ -183,15 +190,59 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
     run.now = pages_from(0);
     run.ahead = pages_from(64 / kGroups);
 
+    // A thread's share of a step (and of q): pieces of 8 dims, kWaveRows rows of a wave side by side
+    const int my_row = lane / kPieces, my_dim = 8 * (lane % kPieces);
+
     // Q: B operand, lane (n, half) has dims 16 t + 8 half .. + 7 of its row.  Requested here,
     // used when K and V are on their way.
     A q_row[KS][8];
-    load_q<KS>(a, p, row, d.q_wide, 8 * half, 16, q_row);
+    constexpr int kQPass = kTeams * kStepRows, kQLoads = kRows / kQPass;
+    A q_piece[kStage ? kQLoads : 1][8];
+    bool q_real[kStage ? kQLoads : 1];
+    const int q_first = (team * kWaves + wave) * kWaveRows + my_row;
+    if constexpr (kStage) {
+        const A *src[kQLoads];
+#pragma unroll
+        for (int i = 0; i < kQLoads; ++i) {
+            const Row r = row_of(p, p.tile * kRows + i * kQPass + q_first, d.cut, cap, a.window);
+            q_real[i] = r.real && my_dim < a.hd;
+            src[i] = q_row_of<A>(a, p, r) + min(my_dim, a.hd - 8);
+        }
+        if (d.q_wide) {
+#pragma unroll
+            for (int i = 0; i < kQLoads; ++i) load_piece(src[i], true, q_piece[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kQLoads; ++i) load_piece(src[i], false, q_piece[i]);
+        }
+    } else {
+        load_q<KS>(a, p, row, d.q_wide, 8 * half, 16, q_row);
+    }
 
     vec8 q[kQReg][KS];
     float unit = 1.f;
     const auto make_q = [&] {
-        zero_q<KS>(a, row, 8 * half, 16, q_row);
+        if constexpr (kStage) {
+            A *const q_tile = reinterpret_cast<A *>(tiles);
+            typedef A piece8 __attribute__((ext_vector_type(8)));
+#pragma unroll
+            for (int i = 0; i < kQLoads; ++i) {
+                piece8 v;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = q_real[i] ? q_piece[i][e] : (A)0.f;
+                *reinterpret_cast<piece8 *>(q_tile + (i * kQPass + q_first) * kQPitch + my_dim) = v;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int t = 0; t < KS; ++t) {
+                const piece8 v = *reinterpret_cast<const piece8 *>(q_tile + (wave * 32 + col) * kQPitch + 16 * t + 8 * half);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) q_row[t][e] = v[e];
+            }
+            __syncthreads();   // K and V take the place
+        } else {
+            zero_q<KS>(a, row, 8 * half, 16, q_row);
+        }
         float to = 1.f;
         if constexpr (QP == 2) {
             float big = 0;
@@ -221,8 +272,6 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
     };
     if constexpr (QP > 1) make_q();   // (behind the loads its registers cost the loop more than the wait)
 
-    // A thread's share of a step: pieces of 8 dims, kWaveRows rows of a wave side by side
-    const int my_row = lane / kPieces, my_dim = 8 * (lane % kPieces);
     const bool no_dim = padded && my_dim >= a.hd;
     const unsigned row_bytes = a.hd * sizeof(S), off = my_row * row_bytes + (padded ? min(my_dim, a.hd - 8) : my_dim) * (unsigned)sizeof(S);
     const unsigned first_row = wave * kWaveRows;

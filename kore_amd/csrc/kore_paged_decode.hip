@@ -593,7 +593,7 @@ constexpr int kShort = 1280;                           // keys that a tile among
 
 }  // namespace
 
-size_t attend_workspace_bytes(int n_head, int n_head_kv, int hd, int num_cu) {
+size_t attend_workspace_bytes(int hd, int num_cu) {
     return 2 * (size_t)num_cu * kChunkRows * ((size_t)padded_dim(hd) + 2) * sizeof(float);
 }
 

@@ -73,6 +73,6 @@ struct AttendArgs {
 hipError_t launch_rope(const RopeArgs &a, hipStream_t s);
 hipError_t launch_append(const AppendArgs &a, hipStream_t s);
 hipError_t launch_attend(const AttendArgs &a, hipStream_t s);
-size_t attend_workspace_bytes(int n_head, int n_head_kv, int hd, int num_cu);
+size_t attend_workspace_bytes(int hd, int num_cu);
 
 }  // namespace kore_paged_gpu
