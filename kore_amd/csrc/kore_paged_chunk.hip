@@ -7,13 +7,13 @@
 // workgroup, each with every other step of the keys, and join their sums through LDS at
 // the end: what a step waits for is a wave's own chain of loads, products and weights,
 // so a tile takes half as long as with one team, and the long tiles of a causal chunk
-// are what the launch waits for (28/4/128, 2048 fp16 rows: 52.5 us; 56 with the same
-// waves in two workgroups of four).
+// are what the launch waits for (28/4/128, 2048 fp16 rows: 51 us; the same waves in two
+// workgroups of four took 56 where this took 51, an earlier pair of variants).
 //
 // us, and TFLOP/s of products made (a large bf16 product: 1207): 2048 fp16 rows of
-// 28/4/128 52.5, 575; 512 fp32 rows over 32749 bf16 keys, three products each, 620,
-// 1150; 2048 fp32 rows over an fp32 cache, three and six, 159 to 180, 750 to 850.  The
-// rest is vector instructions (weights, parts), which matrix instructions of another
+// 28/4/128 51 to 56 over boxes, 540 to 590; 512 fp32 rows over 32749 bf16 keys, three
+// products each, 602 to 620, 1150 to 1190; 2048 fp32 rows over an fp32 cache, three and
+// six, 154 to 180, 750 to 880.  The rest is vector instructions (weights, parts), which matrix instructions of another
 // wave hardly overlap, a workgroup's start, and waits at the team's two barriers a step.
 #include "kore_paged_attend.h"
 
