@@ -126,6 +126,58 @@ def test_a_layer_is_its_calls(cache):
         w.close()
 
 
+def test_a_captured_step_follows_its_batch():
+    """A layer's step captured once and replayed with other rows, lengths and pages, the program's own steps between the
+    replays: the eager step's bits every time.  The captured step has a workspace of its own."""
+    from kore_amd import paged, rope
+    from kore_amd.layer import Layer
+    ws = _weights(1)
+    n_pages, ps, stride, n = 160, 32, 70, 7
+    try:
+        with paged.PagedKV(1, n_pages, ps, NH, NKV, HD, "f32", rope.Config(HD)) as kv, Layer(E, FF, NH, NKV, 1e-6) as L:
+            starts = torch.zeros(4, dtype=torch.int32, device="cuda")
+            kv_len = torch.zeros(3, dtype=torch.int32, device="cuda")
+            pages = torch.full((3, stride), -1, dtype=torch.int32, device="cuda")
+            x = torch.zeros(n, E, device="cuda")
+            work = torch.empty(kv.workspace_bytes(), dtype=torch.uint8, device="cuda")
+            b = paged.Batch(3, n, starts.data_ptr(), kv_len.data_ptr(), pages.data_ptr(), stride, 5)
+            stream = torch.cuda.Stream()
+
+            def fill(i):
+                torch.cuda.synchronize()
+                r = np.random.default_rng(100 + i)
+                starts.copy_(torch.tensor([[0, 1, 2, 7], [0, 5, 6, 7], [0, 0, 4, 5], [0, 2, 4, 7]][i], dtype=torch.int32))
+                kv_len.copy_(torch.tensor([[40, 2000, 5], [2200, 3, 33], [0, 900, 64], [2, 1500, 300]][i], dtype=torch.int32))
+                order = r.permutation(n_pages)[:150].astype(np.int32)
+                t = np.full((3, stride), -1, np.int32)
+                t[0], t[1], t[2, :10] = order[:70], order[70:140], order[140:150]
+                pages.copy_(torch.from_numpy(t))
+                x.copy_(torch.from_numpy(r.standard_normal((n, E)).astype(np.float32)))
+                torch.cuda.synchronize()
+
+            fill(0)
+            L.paged_dev(ws[0], kv, 0, b, x.data_ptr(), stream=stream.cuda_stream)
+            fill(0)
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=stream):
+                L.paged_dev(ws[0], kv, 0, b, x.data_ptr(), workspace=work.data_ptr(),
+                            stream=torch.cuda.current_stream().cuda_stream)
+            for i in (1, 0, 2, 3, 1):
+                fill(i)
+                L.paged_dev(ws[0], kv, 0, b, x.data_ptr(), stream=stream.cuda_stream)
+                stream.synchronize()
+                want = x[:int(starts[3])].clone()   # the rows behind the last sequence hold nothing of use
+                fill(i)
+                g.replay()
+                torch.cuda.synchronize()
+                got = x[:int(starts[3])]
+                assert torch.isfinite(got).all() and torch.equal(got.view(torch.int32), want.view(torch.int32)), i
+            del g
+    finally:
+        for w in ws:
+            w.close()
+
+
 def test_refusals():
     from kore_amd import paged
     from kore_amd.layer import Layer, LayerError
