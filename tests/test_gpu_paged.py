@@ -459,6 +459,34 @@ def test_a_cache_past_32_bits():
     check_rows(c, c.rows("out", 16)[0], *c.exact())
 
 
+@pytest.mark.parametrize("dtype,cache", [("f32", "f32"), ("f32", "bf16"), ("f16", "f16")])
+@pytest.mark.parametrize("lens", [[(1, 90), (1, 1), (1, 400)], [(40, 90), (70, 70)]])
+def test_rows_of_one_wide_buffer(dtype, cache, lens):
+    """q, k, v and out side by side in one buffer's rows, as a fused projection writes them: q rotated in place, out beside it."""
+    from kore_amd import rope
+    c = Case(lens, 6, 2, 64, 16, dtype, cache, seed=12, extra_rows=1).up()
+    E, D = 6 * 64, 2 * 64
+    wide = torch.full((c.n_tok, 2 * E + 2 * D + 8), 33.0, dtype=DTYPE[dtype])
+    wide[:, :E], wide[:, E:E + D], wide[:, E + D:E + 2 * D] = (t.reshape(c.n_tok, -1) for t in (c.q, c.k, c.v))
+    w = wide.cuda()
+    size, step = w.element_size(), w.shape[1]
+    p = [w.data_ptr() + size * at for at in (0, E, E + D, E + 2 * D)]
+    torch.cuda.synchronize()
+    with c.handle(rope.Config(64)) as kv:
+        kv.append_dev(0, c.batch(), dtype, p[1], p[2], p[0], p[0], step, step, step, step)
+        kv.attend_dev(0, c.batch(), dtype, p[0], p[3], step, step)
+        kv.sync()
+    got = w.cpu()
+    assert torch.equal(got[:, E:E + 2 * D], wide[:, E:E + 2 * D]) and (got[:, -8:] == 33.0).all() and torch.equal(got[c.used:], wide[c.used:])
+    c.q = got[:, :E].reshape(c.n_tok, 6, 64)   # rotated
+    c.k_pool, c.v_pool = c.d["k_pool"].cpu(), c.d["v_pool"].cpu()
+    f, m = rope_freqs(64)
+    pos = np.concatenate([np.arange(kv - n, kv) for n, kv in lens])
+    want, bound = rope_rows(wide[:c.used, :E].reshape(-1, 6, 64).double().numpy(), pos, f, m, "half")
+    assert (np.abs(to64(c.q[:c.used]) - want) <= rope_bound(want, bound, dtype)).all()
+    check_rows(c, got[:, E + 2 * D:2 * E + 2 * D].reshape(c.n_tok, 6, 64), *c.exact())
+
+
 # ---- odd batches -----------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype,cache", PAIRS)
