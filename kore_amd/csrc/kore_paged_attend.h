@@ -330,13 +330,19 @@ __device__ __forceinline__ void split_p(float x, C (&part)[N]) {
     }
 }
 
-// A power of two that brings |x| <= big to 2^13 .. 2^14 (2^126 at most: big under
-// 2^-112 stays smaller), and its inverse.  big >= 0, no NaN.
-__device__ __forceinline__ void unit_of(float big, float &to, float &back) {
+// A power of two `to` that brings |x| <= big to 2^13 .. 2^14 (2^126 at most: big under
+// 2^-112 stays smaller), and the exponent of its inverse.  big >= 0, no NaN.
+__device__ __forceinline__ int unit_of(float big, float &to) {
     const unsigned e = __builtin_bit_cast(unsigned, big) >> 23;
     const unsigned up = min(267u - e, 253u);   // 2^(up - 127) 2^(e - 127) = 2^13
     to = __builtin_bit_cast(float, up << 23);
-    back = __builtin_bit_cast(float, (254u - up) << 23);
+    return 127 - (int)up;
+}
+__device__ __forceinline__ float power(int e) { return __builtin_bit_cast(float, (unsigned)(127 + e) << 23); }   // -126 .. 127
+// scale log2(e) of scores in a unit of q: over 0 and finite (a product with it is used
+// with differences of such scores, 0 or 2^-48 at least), so that 0 stays 0.
+__device__ __forceinline__ float scale_of(float scale_log2, float unit) {
+    return fminf(fmaxf(scale_log2 * unit, 0x1p-126f), 0x1p126f);
 }
 
 // ---- the softmax ---------------------------------------------------------------

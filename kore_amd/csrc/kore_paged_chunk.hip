@@ -143,7 +143,7 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
     // of V's pieces in steps that the tile's rows do not all see: which of 8 dims are +inf, or -inf (a NaN: both)
     __shared__ unsigned all_kinds[kTeams][2][kKeys][HDP / 32];
     __shared__ int all_odd[kTeams][kWaves];
-    __shared__ __attribute__((aligned(16))) float all_back[KP == 2 ? kTeams : 1][kKeys];   // K's units
+    __shared__ __attribute__((aligned(16))) int all_back[KP == 2 ? kTeams : 1][kKeys];   // exponents of K's units
     __shared__ float2 team_ml[kWaves][32];   // (reference, sum) of the second team's rows
     const AttendArgs &a = d.a;
     const int rep = d.cut.rep;
@@ -151,7 +151,7 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
     const int wave = scalar(threadIdx.x >> 6) % kWaves, team = scalar(threadIdx.x >> 6) / kWaves;
     C *const k_tile = reinterpret_cast<C *>(tiles) + team * kStep;
     CV *const v_tile = reinterpret_cast<CV *>(k_tile + KP * kKeys * kKPitch);
-    float *const k_back = all_back[KP == 2 ? team : 0];
+    int *const k_back = all_back[KP == 2 ? team : 0];
     auto &kinds = all_kinds[team];
     auto &odd_of = all_odd[team];
     Place p;
@@ -221,7 +221,7 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
     }
 
     vec8 q[kQReg][KS];
-    float unit = 1.f;
+    int q_unit = 0;   // the exponent of q's unit
     const auto make_q = [&] {
         if constexpr (kStage) {
             A *const q_tile = reinterpret_cast<A *>(tiles);
@@ -251,7 +251,7 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
             for (int t = 0; t < KS; ++t)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(q_row[t][i]));
-            unit_of(max32(big), to, unit);
+            q_unit = unit_of(max32(big), to);
         }
 #pragma unroll
         for (int t = 0; t < KS; ++t) {
@@ -321,7 +321,7 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
             *reinterpret_cast<raw8 *>(at) = x;
         } else {
             // two parts, each the nearest, of the row in its unit
-            float big = 0, to, back;
+            float big = 0, to;
 #pragma unroll
             for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[e]));
             big = row_max<kPieces>(big);
@@ -332,7 +332,7 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
                 for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.f);
                 big = row_max<kPieces>(big);
             }
-            unit_of(big, to, back);
+            const int back = unit_of(big, to);
             vec8 hi, lo;
             typedef C vec2 __attribute__((ext_vector_type(2)));
             typedef float float2_t __attribute__((ext_vector_type(2)));
@@ -437,10 +437,10 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
         has = has_2;
     }
     if constexpr (QP == 1) make_q();
-    // An fp32 cache's scores leave q's unit with K's.
-    const float q_unit = KP == 2 ? unit : 1.f;
-    if (KP == 2) unit = 1.f;
-    const float s2 = fmaxf(d.scale_log2 * unit, 0x1p-126f);
+    // An fp32 cache's scores leave q's unit with K's, both at once: either alone may pass fp32's range, or their product
+    // where the score does not.
+    const float unit = KP == 2 ? 1.f : power(q_unit);
+    const float s2 = scale_of(d.scale_log2, unit);
     if (n_step) {
         store_k();
         if (n_step > 1) load_k(1);
@@ -491,11 +491,11 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
                 for (int m = 0; m < MT; ++m)
 #pragma unroll
                     for (int i = 0; i < 16; i += 4) {
-                        const float4 b = *reinterpret_cast<const float4 *>(&k_back[32 * m + 2 * i + 4 * half]);
-                        s[m][i] *= b.x * q_unit;
-                        s[m][i + 1] *= b.y * q_unit;
-                        s[m][i + 2] *= b.z * q_unit;
-                        s[m][i + 3] *= b.w * q_unit;
+                        const int4 b = *reinterpret_cast<const int4 *>(&k_back[32 * m + 2 * i + 4 * half]);
+                        s[m][i] = __builtin_ldexpf(s[m][i], b.x + q_unit);
+                        s[m][i + 1] = __builtin_ldexpf(s[m][i + 1], b.y + q_unit);
+                        s[m][i + 2] = __builtin_ldexpf(s[m][i + 2], b.z + q_unit);
+                        s[m][i + 3] = __builtin_ldexpf(s[m][i + 3], b.w + q_unit);
                     }
             }
             if (!whole) {

@@ -172,7 +172,7 @@ __global__ __launch_bounds__(64 * W, HDP <= 128 && W == 4 ? 2 : 1) void decode16
             for (int t = 0; t < KS; ++t)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(q_row[t][i]));
-            unit_of(max32(max16(big)), to, unit);
+            unit = power(unit_of(max32(max16(big)), to));
         }
 #pragma unroll
         for (int t = 0; t < KS; ++t)
@@ -188,7 +188,7 @@ __global__ __launch_bounds__(64 * W, HDP <= 128 && W == 4 ? 2 : 1) void decode16
                 }
             }
     }
-    const float s2 = fmaxf(d.scale_log2 * unit, 0x1p-126f);
+    const float s2 = scale_of(d.scale_log2, unit);
     for (int j = 0; j < n_block; ++j) {
         const int key0 = (first_block + W * j) * kBlock;
         const bool has0 = p0 >= 0, has1 = p1 >= 0;

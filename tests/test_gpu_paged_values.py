@@ -52,3 +52,28 @@ def test_scores_with_a_common_part(dtype, common, lens, max_q):
                 want, size = w @ V[:, h // 3], w @ np.abs(V[:, h // 3])
                 e = (2 * u + 2.0 ** -13 + 2.0 ** -17 + (len(p) / 8 + 16) * 2.0 ** -24) * size + u * np.abs(want) + 2.0 ** -24
                 assert (np.abs(got[row, h] - want) <= e).all(), (row, h, float((np.abs(got[row, h] - want) / e).max()))
+
+
+# ---- units of q and K ----------------------------------------------------------------
+
+@pytest.mark.parametrize("cache", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("max_q", [1, 64])
+def test_large_values_that_meet_zeros(cache, max_q):
+    """q and K are large, each where the other is 0: scores of 0, the mean of V, whatever the scale."""
+    c = Case([(20, 90), (1, 40)], 4, 2, 64, 16, "f32", cache, seed=7)
+    c.q[:] = 0
+    c.q[..., 3] = 2.0 ** 100
+    c.k_pool = torch.where(torch.isnan(c.k_pool), c.k_pool, torch.zeros_like(c.k_pool))
+    c.k_pool[..., 5] = torch.where(torch.isnan(c.k_pool[..., 5]), c.k_pool[..., 5], torch.full_like(c.k_pool[..., 5], 2.0 ** (15 if cache == "f16" else 100)))
+    c.up()
+    with c.handle() as kv:
+        for scale in (0.0, 1.0, 1e30, 1e-30):
+            c.attend(kv, max_q=max_q, scale=scale)
+            got = to64(c.rows("out", 4)[0])
+            vp = to64(c.v_pool[0])
+            for s, (n, kv_len) in enumerate(c.lens):
+                for i in range(n):
+                    p = np.arange(kv_len - n + i + 1)
+                    V = vp[c.pages[s, p // 16], :, p % 16].repeat(2, 1)
+                    e = (2.0 ** -20 + (len(p) / 8 + 16) * 2.0 ** -24) * np.abs(V).mean(0)
+                    assert (np.abs(got[int(c.starts[s]) + i] - V.mean(0)) <= e).all(), scale
