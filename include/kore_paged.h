@@ -35,8 +35,12 @@
  *   is read.
  * Values of positions that a row does not attend (later ones, those before its
  * window, slots behind the sequence's end) do not reach it, infinities and NaN
- * included.  Pages may be shared by sequences as long as no two rows of one
- * append go to the same slot.
+ * included.  Of those that it attends, an infinity of V whose score is over
+ * -infinity makes its dim of the row infinite, however small the weight (NaN: with
+ * both signs, or a NaN); one whose score is -infinity does nothing.  A row with a
+ * score of NaN or +infinity is NaN.  What a row gets whose q is not finite is not
+ * said; no other row notices.  Pages may be shared by sequences as long as no two
+ * rows of one append go to the same slot.
  *
  * Arithmetic: products of the cache's values with q and with the softmax's
  * weights are summed in fp32, and the result is rounded once to the rows' type.

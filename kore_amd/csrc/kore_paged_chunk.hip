@@ -54,11 +54,7 @@ template <class A, class S, int HDP> struct Shape {
 __device__ __forceinline__ unsigned upper_halves(float a, float b) {
     return __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, b), __builtin_bit_cast(unsigned, a), 0x07060302);
 }
-__device__ __forceinline__ float dot_ones(unsigned pair, float s) {
-    typedef bhalf_t bhalf2_t __attribute__((ext_vector_type(2)));
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bhalf2_t, pair), bhalf2_t{(bhalf_t)1.f, (bhalf_t)1.f}, s, false);
-}
-__device__ __forceinline__ void cut3(const float (&x)[8], bhalf8 (&part)[3], float &rest) {
+__device__ __forceinline__ void cut3(const float (&x)[8], bhalf8 (&part)[3]) {
     typedef unsigned uint4_t __attribute__((ext_vector_type(4)));
     uint4_t u[3];
 #pragma unroll
@@ -72,7 +68,6 @@ __device__ __forceinline__ void cut3(const float (&x)[8], bhalf8 (&part)[3], flo
         u[0][i / 2] = upper_halves(x[i], x[i + 1]);
         u[1][i / 2] = upper_halves(r[0], r[1]);
         u[2][i / 2] = upper_halves(l[0], l[1]);
-        rest = dot_ones(u[2][i / 2], rest);
     }
 #pragma unroll
     for (int j = 0; j < 3; ++j) part[j] = __builtin_bit_cast(bhalf8, u[j]);
@@ -95,8 +90,7 @@ __device__ __forceinline__ float row_max(float big) {
 template <int N, class C, class V>
 __device__ __forceinline__ void weights(const float (&x)[8], V (&part)[N]) {
     if constexpr (N == 3) {
-        float rest = 0;
-        cut3(x, part, rest);
+        cut3(x, part);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -140,9 +134,10 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
     constexpr bool kThird = QP == 3;
     constexpr int kQReg = kThird ? 2 : QP;
     __shared__ vec8 q_third[kThird ? kWaves : 1][KS][64];
-    // of V's pieces in steps that the tile's rows do not all see: which of 8 dims are +inf, or -inf (a NaN: both)
+    // a careful pass's notes, of eight dims each (take_out), and whether a wave has any
     __shared__ unsigned all_kinds[kTeams][2][kKeys][HDP / 32];
     __shared__ int all_odd[kTeams][kWaves];
+    __shared__ bool all_bad[kTeams * kWaves];   // a wave's sums are not all finite
     __shared__ __attribute__((aligned(16))) int all_back[KP == 2 ? kTeams : 1][kKeys];   // exponents of K's units
     __shared__ float2 team_ml[kWaves][32];   // (reference, sum) of the second team's rows
     const AttendArgs &a = d.a;
@@ -362,19 +357,11 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
         if constexpr (VP == 1) {
             *reinterpret_cast<raw8 *>(at) = x;
         } else {
-            float y[8], rest = 0;
+            float y[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) y[e] = x[e];
             vvec8 part[3];
-            cut3(y, part, rest);
-            if (__any(rest != rest)) {   // an infinity or NaN: all of it in the first part
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (!finite(y[e])) {
-                        part[0][e] = (bhalf_t)y[e];
-                        part[1][e] = part[2][e] = (bhalf_t)0.f;
-                    }
-            }
+            cut3(y, part);   // (of an infinity or NaN some are not finite, and so will the sums be)
 #pragma unroll
             for (int j = 0; j < 3; ++j) *reinterpret_cast<vvec8 *>(at + j * kKeys * kVPitch) = part[j];
         }
@@ -388,27 +375,24 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) put_k(kr[i], i * kStepRows + wave * kWaveRows + my_row);
     };
-    // V into LDS.  Where the tile's rows differ in what they see, V of positions that none
-    // sees is 0, and infinities and NaN are 0 too and noted apart: a product with a weight
-    // of 0 would hand them to every row.
-    const auto store_v = [&](int key0, bool mixed) {
+    // V into LDS; of positions that no row of the tile sees it is 0: it may hold anything
+    const auto store_v = [&]<bool CAREFUL>(int key0, bool mixed) {
         if (mixed) {
+            // (a branch: selects cost registers, and 512 fp16 rows over 8192 keys of 16/2/256 170 us instead of 155)
+            asm volatile("");
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int first = i * kStepRows + wave * kWaveRows, key = key0 + first + my_row;
+                if (!(key < k.hi && key >= k.seen_lo && (has >> (first / 16) & 1))) vr[i] = raw8{};
+            }
+        }
+        if constexpr (CAREFUL) {
             bool odd = false;
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                const int first = i * kStepRows + wave * kWaveRows;
-                if (!(key0 + first + my_row < k.hi && (has >> (first / 16) & 1))) vr[i] = raw8{};
-                unsigned up = 0, down = 0;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float v = to_f32(vr[i][e]);
-                    if (!finite(v)) {
-                        if (!(v < 0.f)) up |= 1u << e;
-                        if (!(v > 0.f)) down |= 1u << e;
-                        vr[i][e] = (S)0.f;
-                    }
-                }
-                unsigned char *const at = reinterpret_cast<unsigned char *>(kinds[0][first + my_row]) + my_dim / 8;
+                unsigned up, down;
+                take_out<S>(vr[i], up, down);
+                unsigned char *const at = reinterpret_cast<unsigned char *>(kinds[0][i * kStepRows + wave * kWaveRows + my_row]) + my_dim / 8;
                 at[0] = (unsigned char)up;
                 at[sizeof kinds[0]] = (unsigned char)down;
                 odd |= (up | down) != 0;
@@ -431,176 +415,208 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
     // of a step, the second team runs a phase behind the first: one is at its scores while
     // the other makes weights (512 fp32 rows over 32749 bf16 keys: 686 us against 771 side by
     // side); without, they run side by side (a 2048-row fp16 prompt: 52.7 against 53.9).
-    if (n_step) {
+    const auto start = [&] {   // run holds the first pages
         load_k(0);
         load_v(0);
         has = has_2;
-    }
+    };
+    if (n_step) start();
     if constexpr (QP == 1) make_q();
     // An fp32 cache's scores leave q's unit with K's, both at once: either alone may pass fp32's range, or their product
     // where the score does not.
     const float unit = KP == 2 ? 1.f : power(q_unit);
     const float s2 = scale_of(d.scale_log2, unit);
-    if (n_step) {
-        store_k();
-        if (n_step > 1) load_k(1);
-        has_1 = has_2;
-    }
-    if (kLag && team == 1) __syncthreads();
-    for (int step = 0; step < n_run; ++step) {
-        const int key0 = key_of(step);
-        const bool real = step < n_step;
-        const bool mixed = !(key0 >= k.all_lo && key0 + kKeys <= min(k.all_hi, k.hi) && has == kAll);
-        const bool any = key0 < see_hi && key0 + kKeys > see_lo && real;
-        const bool whole = key0 >= all_lo && key0 + kKeys <= all_hi && has == kAll;
-        __syncthreads();
-        if (real) {
-            store_v(key0, mixed);
-            if (step + 1 < n_step) load_v(step + 1);
+    const auto pass = [&]<bool CAREFUL>() __attribute__((always_inline)) {
+        if (n_step) {
+            store_k();
+            if (n_step > 1) load_k(1);
+            has_1 = has_2;
         }
+        if (kLag && team == 1) __syncthreads();
+        for (int step = 0; step < n_run; ++step) {
+            const int key0 = key_of(step);
+            const bool real = step < n_step;
+            const bool mixed = !(key0 >= k.all_lo && key0 + kKeys <= min(k.all_hi, k.hi) && has == kAll);
+            const bool any = key0 < see_hi && key0 + kKeys > see_lo && real;
+            const bool whole = key0 >= all_lo && key0 + kKeys <= all_hi && has == kAll;
+            __syncthreads();
+            if (real) {
+                store_v.template operator()<CAREFUL>(key0, mixed);
+                if (step + 1 < n_step) load_v(step + 1);
+            }
 
-        // S^T = K Q^T: lane (n, half) gets its row's scores of keys 32 m + 8 (i / 4) + 4 half + i % 4
-        floatx16 s[MT];
-        bool far = false;
-        if (any) {
+            // S^T = K Q^T: lane (n, half) gets its row's scores of keys 32 m + 8 (i / 4) + 4 half + i % 4
+            floatx16 s[MT];
+            bool far = false;
+            if (any) {
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                s[m] = floatx16{};
-                const int from = (32 * m + col) * kKPitch + 8 * half;
+                for (int m = 0; m < MT; ++m) {
+                    s[m] = floatx16{};
+                    const int from = (32 * m + col) * kKPitch + 8 * half;
 #pragma unroll
-                for (int t = 0; t < KS; ++t)
+                    for (int t = 0; t < KS; ++t)
 #pragma unroll
-                    for (int y = 0; y < KP; ++y) {
-                        const vec8 x = *reinterpret_cast<const vec8 *>(&k_tile[y * kKeys * kKPitch + from + 16 * t]);
+                        for (int y = 0; y < KP; ++y) {
+                            const vec8 x = *reinterpret_cast<const vec8 *>(&k_tile[y * kKeys * kKPitch + from + 16 * t]);
 #pragma unroll
-                        for (int z = 0; z < QP; ++z)
-                            if (KP == 1 || y + z < KP) s[m] = Mma<C>::mul32(x, z < kQReg ? q[z < kQReg ? z : 0][t] : q_third[wave][t][lane], s[m]);
-                    }
-            }
-            // K's operands are requested kAhead products early
-            constexpr int kReads = MT * KS * (KP + kThird), kAhead = 6, kPer = KP == 2 ? 3 : kThird ? 1 : QP;
-            __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+                            for (int z = 0; z < QP; ++z)
+                                if (KP == 1 || y + z < KP) s[m] = Mma<C>::mul32(x, z < kQReg ? q[z < kQReg ? z : 0][t] : q_third[wave][t][lane], s[m]);
+                        }
+                }
+                // K's operands are requested kAhead products early
+                constexpr int kReads = MT * KS * (KP + kThird), kAhead = 6, kPer = KP == 2 ? 3 : kThird ? 1 : QP;
+                __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
-            for (int i = 0; i < kReads - kAhead; i += KP) {
-                __builtin_amdgcn_sched_group_barrier(0x008, kPer, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, KP, 0);
-            }
-            __builtin_amdgcn_sched_group_barrier(0x008, kAhead / KP * kPer, 0);
-            if constexpr (KP == 2) {
-#pragma unroll
-                for (int m = 0; m < MT; ++m)
-#pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        const int4 b = *reinterpret_cast<const int4 *>(&k_back[32 * m + 2 * i + 4 * half]);
-                        s[m][i] = __builtin_ldexpf(s[m][i], b.x + q_unit);
-                        s[m][i + 1] = __builtin_ldexpf(s[m][i + 1], b.y + q_unit);
-                        s[m][i + 2] = __builtin_ldexpf(s[m][i + 2], b.z + q_unit);
-                        s[m][i + 3] = __builtin_ldexpf(s[m][i + 3], b.w + q_unit);
-                    }
-            }
-            if (!whole) {
-#pragma unroll
-                for (int m = 0; m < MT; ++m)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int at = 32 * m + 8 * (i / 4) + 4 * half + i % 4, key = key0 + at;
-                        if (!(key >= row.lo && key < min(row.hi, k.hi) && (has >> (2 * m + i / 8) & 1))) s[m][i] = kNone;
-                    }
-            }
-            float top = kNone;
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) top = fmaxf(top, s[m][i]);
-            follow(max32(top), ref, sum, s2, o);
-            // The difference from the reference first, as the softmax's comment says.  16-bit rows: one fma of the score
-            // and the scaled reference while that is under 2^11.  Its rounding, at most 2^-14 in the exponent, is the same
-            // for the weights of one reference and stays between those of two (a row's teams and splits, and before and
-            // after the reference moves): 2^-13.5 of a weight, beside the weights' own half step of 2^-11 (fp16) or 2^-8.
-            // (2048 fp16 rows of 28/4/128: 50.2 us with every reference under 2^11, 51.9 with every one over it.)
-            if constexpr (PP == 1) {
-                const float base = ref == kNone ? 0.f : ref;
-                far = __any(fabsf(base * s2) >= 0x1p11f);
-                if (far) {
+                for (int i = 0; i < kReads - kAhead; i += KP) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, kPer, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, KP, 0);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x008, kAhead / KP * kPer, 0);
+                if constexpr (KP == 2) {
 #pragma unroll
                     for (int m = 0; m < MT; ++m)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) s[m][i] -= base;
+                        for (int i = 0; i < 16; i += 4) {
+                            const int4 b = *reinterpret_cast<const int4 *>(&k_back[32 * m + 2 * i + 4 * half]);
+                            s[m][i] = __builtin_ldexpf(s[m][i], b.x + q_unit);
+                            s[m][i + 1] = __builtin_ldexpf(s[m][i + 1], b.y + q_unit);
+                            s[m][i + 2] = __builtin_ldexpf(s[m][i + 2], b.z + q_unit);
+                            s[m][i + 3] = __builtin_ldexpf(s[m][i + 3], b.w + q_unit);
+                        }
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int m = 0; m < MT; ++m)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int at = 32 * m + 8 * (i / 4) + 4 * half + i % 4, key = key0 + at;
+                            if (!(key >= row.lo && key < min(row.hi, k.hi) && (has >> (2 * m + i / 8) & 1))) s[m][i] = kNone;
+                        }
+                }
+                float top = kNone;
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) top = fmaxf(top, s[m][i]);
+                follow<CAREFUL>(max32(top), ref, sum, s2, o);
+                // The difference from the reference first, as the softmax's comment says.  16-bit rows: one fma of the score
+                // and the scaled reference while that is under 2^11.  Its rounding, at most 2^-14 in the exponent, is the same
+                // for the weights of one reference and stays between those of two (a row's teams and splits, and before and
+                // after the reference moves): 2^-13.5 of a weight, beside the weights' own half step of 2^-11 (fp16) or 2^-8.
+                // (2048 fp16 rows of 28/4/128: 50.2 us with every reference under 2^11, 51.9 with every one over it.)
+                if constexpr (PP == 1) {
+                    const float base = ref == kNone ? 0.f : ref;
+                    far = __any(fabsf(base * s2) >= 0x1p11f);
+                    if (far) {
+#pragma unroll
+                        for (int m = 0; m < MT; ++m)
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) s[m][i] -= base;
+                    }
                 }
             }
-        }
-        __syncthreads();
-        if (step + 1 < n_step) {
-            store_k();
-            if (step + 2 < n_step) load_k(step + 2);
-        }
-        has = has_1;
-        has_1 = has_2;
-        if (any) {
-            const float base = ref == kNone ? 0.f : ref;
-            const float minus = PP == 1 && !far ? fmaf(-base, s2, Mma<CV>::kBias) : Mma<CV>::kBias;
-            vvec8 w[MT][2][PP];
-            float part_sum = 0;
+            __syncthreads();
+            if (step + 1 < n_step) {
+                store_k();
+                if (step + 2 < n_step) load_k(step + 2);
+            }
+            has = has_1;
+            has_1 = has_2;
+            if (any) {
+                if (CAREFUL && (odd_of[0] | odd_of[1] | odd_of[2] | odd_of[3])) {
+                    unsigned has_weight[MT];   // of the step's keys, for the lane's row
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
+                    for (int m = 0; m < MT; ++m) {
+                        has_weight[m] = 0;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float x[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float y = s[m][8 * h + i];
-                        x[i] = exp2_(fmaf(PP > 1 ? y - base : y, s2, minus));
-                        if (PP > 1) part_sum += x[i];
+                        for (int i = 0; i < 16; ++i) has_weight[m] |= (unsigned)(s[m][i] != kNone) << (8 * (i / 4) + 4 * half + i % 4);
+                        has_weight[m] |= __shfl_xor(has_weight[m], 32);
                     }
-                    weights<PP, CV>(x, w[m][h]);
-                    // one rounded weight is also what is summed: what rounding adds to all of a row's weights divides out
-                    if constexpr (PP == 1) part_sum = sum_weights(w[m][h][0], part_sum);
-                }
-            sum += part_sum;
-            // O^T += V^T P^T, k order as the scores came: V^T's operand, lane (m, half), has keys 16 t + 4 half + 0..3 and
-            // those 8 further of dim 32 i + m
-            const int from = (4 * half + (lane & 15) / 4) * kVPitch + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
-            const auto v_operand = [&](int plane, int t, int i) {
-                const CV *at = &v_tile[plane * kKeys * kVPitch + from + 16 * t * kVPitch + 32 * i];
-                const vec4 x = read_transposed<vec4>(at), y = read_transposed<vec4>(at + 8 * kVPitch);
-                return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-            };
+                    for (int e = 0; e < kKeys; ++e) {
+                        const bool gets = (e < 32 ? has_weight[0] : has_weight[MT - 1]) >> (e & 31) & 1;
 #pragma unroll
-            for (int t = 0; t < 2 * MT; ++t)
+                        for (int i = 0; i < DT; ++i) {
+                            const unsigned up = gets ? kinds[0][e][i] >> (4 * half) : 0, down = gets ? kinds[1][e][i] >> (4 * half) : 0;
+                            if (!__any((up | down) != 0)) continue;
 #pragma unroll
-                for (int i = 0; i < DT; ++i)
-#pragma unroll
-                    for (int x = 0; x < VP; ++x) {
-                        const vvec8 v = v_operand(x, t, i);
-#pragma unroll
-                        for (int y = 0; y < PP; ++y)
-                            if (VP == 1 || x + y < VP) o[i] = Mma<CV>::mul32(v, w[t / 2][t & 1][y], o[i]);
-                    }
-            if (mixed && (odd_of[0] | odd_of[1] | odd_of[2] | odd_of[3])) {
-                for (int e = 0; e < kKeys; ++e) {
-                    const bool sees = key0 + e >= row.lo && key0 + e < min(row.hi, k.hi);
-#pragma unroll
-                    for (int i = 0; i < DT; ++i) {
-                        const unsigned up = sees ? kinds[0][e][i] >> (4 * half) : 0, down = sees ? kinds[1][e][i] >> (4 * half) : 0;
-                        if (!__any((up | down) != 0)) continue;
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            const int bit = 8 * (j / 4) + j % 4;
-                            if (up >> bit & 1) o[i][j] += INFINITY;
-                            if (down >> bit & 1) o[i][j] -= INFINITY;
+                            for (int j = 0; j < 16; ++j) {
+                                const int bit = 8 * (j / 4) + j % 4;
+                                if (up >> bit & 1) o[i][j] += INFINITY;
+                                if (down >> bit & 1) o[i][j] -= INFINITY;
+                            }
                         }
                     }
                 }
+                const float base = ref == kNone ? 0.f : ref;
+                const float minus = PP == 1 && !far ? fmaf(-base, s2, Mma<CV>::kBias) : Mma<CV>::kBias;
+                vvec8 w[MT][2][PP];
+                float part_sum = 0;
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float x[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float y = s[m][8 * h + i];
+                            x[i] = exp2_(fmaf(PP > 1 ? y - base : y, s2, minus));
+                            if (PP > 1) part_sum += x[i];
+                        }
+                        weights<PP, CV>(x, w[m][h]);
+                        // one rounded weight is also what is summed: what rounding adds to all of a row's weights divides out
+                        if constexpr (PP == 1) part_sum = sum_weights(w[m][h][0], part_sum);
+                    }
+                sum += part_sum;
+                // O^T += V^T P^T, k order as the scores came: V^T's operand, lane (m, half), has keys 16 t + 4 half + 0..3 and
+                // those 8 further of dim 32 i + m
+                const int from = (4 * half + (lane & 15) / 4) * kVPitch + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
+                const auto v_operand = [&](int plane, int t, int i) {
+                    const CV *at = &v_tile[plane * kKeys * kVPitch + from + 16 * t * kVPitch + 32 * i];
+                    const vec4 x = read_transposed<vec4>(at), y = read_transposed<vec4>(at + 8 * kVPitch);
+                    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+                };
+#pragma unroll
+                for (int t = 0; t < 2 * MT; ++t)
+#pragma unroll
+                    for (int i = 0; i < DT; ++i)
+#pragma unroll
+                        for (int x = 0; x < VP; ++x) {
+                            const vvec8 v = v_operand(x, t, i);
+#pragma unroll
+                            for (int y = 0; y < PP; ++y)
+                                if (VP == 1 || x + y < VP) o[i] = Mma<CV>::mul32(v, w[t / 2][t & 1][y], o[i]);
+                        }
+                // A branch, which ends the block that the compiler schedules: us without / with it, 700 fp32 rows and cache beside
+                // eight tokens 106.4 / 100.9, 512 fp32 rows over 8192 keys of 16/2/256 288 / 275 (bf16), 261 / 247 (fp16); over
+                // 32749 bf16 keys of 28/4/128 600 / 619, 512 fp16 rows of 16/2/256 156 / 172 (it spills), so not there.
+                if constexpr (VP == 3 || (HDP == 256 && QP > 1))
+                    if (mixed) asm volatile("s_nop 0");
             }
         }
+        if (kLag && team == 0) __syncthreads();
+    };
+    pass.template operator()<false>();
+    const bool bad = __any(not_finite(o));
+    if (lane == 0) all_bad[team * kWaves + wave] = bad;
+    __syncthreads();   // (and K and V give way)
+    bool any_bad = false;
+#pragma unroll
+    for (int i = 0; i < kTeams * kWaves; ++i) any_bad |= all_bad[i];
+    if (__builtin_expect(__any(any_bad), 0)) {
+#pragma unroll
+        for (int i = 0; i < DT; ++i) o[i] = floatx16{};
+        ref = kNone;
+        sum = 0;
+        run.now = pages_from(0);
+        run.ahead = pages_from(64 / kGroups);
+        if (n_step) start();
+        pass.template operator()<true>();
+        __syncthreads();
     }
-    if (kLag && team == 0) __syncthreads();
-
     sum = sum32(sum);
     if constexpr (kTeams == 2) {
         // the second team's sums through LDS, half of them at a time
         float4 *const meet = reinterpret_cast<float4 *>(tiles) + wave * (HDP / 16) * 64 + lane;
-        __syncthreads();
         float f = 1.f, g = 0.f;
 #pragma unroll
         for (int part = 0; part < 2; ++part) {

@@ -85,7 +85,7 @@ __global__ __launch_bounds__(64 * W, HDP <= 128 && W == 4 ? 2 : 1) void decode16
     constexpr size_t kVBytes = sizeof(C) * W * kBlock * kPitch, kOBytes = sizeof(float) * W * HDP * kRows;
     __shared__ __attribute__((aligned(16))) unsigned char shared[kVBytes > kOBytes ? kVBytes : kOBytes];
     __shared__ float2 ml[W][kRows];
-    // of V's pieces in blocks that the tile's rows do not all see: which of 8 dims are +inf, or -inf (a NaN: both)
+    // a careful pass's notes, of eight dims each (take_out)
     __shared__ unsigned kinds[W][2][kBlock][HDP / 32];
     const AttendArgs &a = d.a;
     const int cap = a.b.pages_stride << a.page_shift, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -154,13 +154,14 @@ __global__ __launch_bounds__(64 * W, HDP <= 128 && W == 4 ? 2 : 1) void decode16
         return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
     };
 
-    if (n_block) {
+    const auto start = [&] {   // run.now holds the first pages
         p0 = run.get(0);
         p1 = run.get(1);
         load_k(first_block * kBlock);
         load_v(first_block * kBlock);
         run.ahead = pages_from(32);
-    }
+    };
+    if (n_block) start();
     vec8 q[QP][KS];
     float unit = 1.f;
     {
@@ -189,119 +190,133 @@ __global__ __launch_bounds__(64 * W, HDP <= 128 && W == 4 ? 2 : 1) void decode16
             }
     }
     const float s2 = scale_of(d.scale_log2, unit);
-    for (int j = 0; j < n_block; ++j) {
-        const int key0 = (first_block + W * j) * kBlock;
-        const bool has0 = p0 >= 0, has1 = p1 >= 0;
-        const bool whole = key0 >= k.all_lo && key0 + kBlock <= min(k.all_hi, k.hi) && has0 && has1;
-        // pages of the next block
-        const int next = j + 1, next_key = key0 + W * kBlock;
-        if ((next & 31) == 0) {
-            run.now = run.ahead;
-            run.ahead = pages_from(next + 32);
-        }
-        p0 = run.get(2 * (next & 31));
-        p1 = run.get(2 * (next & 31) + 1);
+    const auto pass = [&]<bool CAREFUL>() __attribute__((always_inline)) {
+        for (int j = 0; j < n_block; ++j) {
+            const int key0 = (first_block + W * j) * kBlock;
+            const bool has0 = p0 >= 0, has1 = p1 >= 0;
+            const bool whole = key0 >= k.all_lo && key0 + kBlock <= min(k.all_hi, k.hi) && has0 && has1;
+            // pages of the next block
+            const int next = j + 1, next_key = key0 + W * kBlock;
+            if ((next & 31) == 0) {
+                run.now = run.ahead;
+                run.ahead = pages_from(next + 32);
+            }
+            p0 = run.get(2 * (next & 31));
+            p1 = run.get(2 * (next & 31) + 1);
 
-        if (padded) {
+            if (padded) {
 #pragma unroll
-            for (int t = 0; t < KS; ++t)
-                if (32 * t + 8 * g >= a.hd) {
-                    kr[0][t] = vec8{};
-                    kr[1][t] = vec8{};
+                for (int t = 0; t < KS; ++t)
+                    if (32 * t + 8 * g >= a.hd) {
+                        kr[0][t] = vec8{};
+                        kr[1][t] = vec8{};
+                    }
+            }
+            floatx4 s[2];
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                s[m] = floatx4{0, 0, 0, 0};
+#pragma unroll
+                for (int t = 0; t < KS; ++t)
+#pragma unroll
+                    for (int x = 0; x < QP; ++x) s[m] = Mma<C>::mul16(kr[m][t], q[x][t], s[m]);
+            }
+            if (next < n_block) load_k(next_key);
+
+            // V of positions that no row of the tile sees is 0: it may hold anything
+            if (!whole) {
+#pragma unroll
+                for (int r = 0; r < VR; ++r) {
+                    const int key = key0 + kRowsPer * r + v_row;
+                    if (!(key < k.hi && key >= k.seen_lo && (kRowsPer * r >= 16 ? has1 : has0))) vr[r] = vec8{};
                 }
-        }
-        floatx4 s[2];
+            }
+            bool odd = false;
+            if constexpr (CAREFUL) {
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            s[m] = floatx4{0, 0, 0, 0};
+                for (int r = 0; r < VR; ++r) {
+                    unsigned up, down;
+                    take_out<C>(vr[r], up, down);
+                    unsigned char *const at = reinterpret_cast<unsigned char *>(kinds[wave][0][kRowsPer * r + v_row]) + v_dim / 8;
+                    at[0] = (unsigned char)up;
+                    at[sizeof kinds[0][0]] = (unsigned char)down;
+                    odd |= (up | down) != 0;
+                }
+                odd = __any(odd);
+            }
 #pragma unroll
-            for (int t = 0; t < KS; ++t)
-#pragma unroll
-                for (int x = 0; x < QP; ++x) s[m] = Mma<C>::mul16(kr[m][t], q[x][t], s[m]);
-        }
-        if (next < n_block) load_k(next_key);
+            for (int r = 0; r < VR; ++r) *reinterpret_cast<vec8 *>(v_lds + (kRowsPer * r + v_row) * kPitch + v_dim) = vr[r];
+            if (next < n_block) load_v(next_key);
 
-        // Where the tile's rows differ in what they see, V of positions that none sees is 0, and
-        // infinities and NaN are 0 too and noted apart: a product with a weight of 0 would hand
-        // them to every row.
-        bool odd = false;
-        if (!whole) {
+            if (!whole) {
 #pragma unroll
-            for (int r = 0; r < VR; ++r) {
-                const int key = kRowsPer * r + v_row;
-                if (!(key0 + key < k.hi && (kRowsPer * r >= 16 ? has1 : has0))) vr[r] = vec8{};
-                unsigned up = 0, down = 0;
+                for (int m = 0; m < 2; ++m)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float v = to_f32(vr[r][i]);
-                    if (!finite(v)) {
-                        if (!(v < 0.f)) up |= 1u << i;
-                        if (!(v > 0.f)) down |= 1u << i;
-                        vr[r][i] = (C)0.f;
+                    for (int i = 0; i < 4; ++i) {
+                        const int key = key0 + 16 * m + 4 * g + i;
+                        if (!(key >= row.lo && key < min(row.hi, k.hi) && (m ? has1 : has0))) s[m][i] = kNone;
+                    }
+            }
+            float top = kNone;
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top = fmaxf(top, s[m][i]);
+            top = max32(max16(top));
+            follow<CAREFUL>(top, ref, sum, s2, o);
+            if (CAREFUL && odd) {
+                unsigned has_weight = 0;   // of the block's keys, for the lane's row
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) has_weight |= (unsigned)(s[m][i] != kNone) << (16 * m + 4 * g + i);
+                has_weight |= __shfl_xor(has_weight, 16);
+                has_weight |= __shfl_xor(has_weight, 32);
+                for (int e = 0; e < kBlock; ++e) {
+                    const bool gets = has_weight >> e & 1;
+#pragma unroll
+                    for (int i = 0; i < DT; ++i) {
+                        const int from = 16 * (i & 1) + 4 * g;
+                        const unsigned up = gets ? kinds[wave][0][e][i / 2] >> from : 0, down = gets ? kinds[wave][1][e][i / 2] >> from : 0;
+                        if (!__any((up | down) & 15)) continue;
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            if (up >> x & 1) o[i][x] += INFINITY;
+                            if (down >> x & 1) o[i][x] -= INFINITY;
+                        }
                     }
                 }
-                unsigned char *const at = reinterpret_cast<unsigned char *>(kinds[wave][0][key]) + v_dim / 8;
-                at[0] = (unsigned char)up;
-                at[sizeof kinds[0][0]] = (unsigned char)down;
-                odd |= (up | down) != 0;
             }
-            odd = __any(odd);
-        }
-#pragma unroll
-        for (int r = 0; r < VR; ++r) *reinterpret_cast<vec8 *>(v_lds + (kRowsPer * r + v_row) * kPitch + v_dim) = vr[r];
-        if (next < n_block) load_v(next_key);
-
-        if (!whole) {
+            const float base = ref == kNone ? 0.f : ref;
+            vec8 w[PP];
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int key = key0 + 16 * m + 4 * g + i;
-                    if (!(key >= row.lo && key < min(row.hi, k.hi) && (m ? has1 : has0))) s[m][i] = kNone;
+                    const float x = exp2_(fmaf(s[m][i] - base, s2, Mma<C>::kBias));
+                    C part[PP];
+                    split_p<PP>(x, part);
+                    sum += x;
+#pragma unroll
+                    for (int y = 0; y < PP; ++y) w[y][4 * m + i] = part[y];
                 }
-        }
-        float top = kNone;
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+            for (int i = 0; i < DT; ++i) {
+                const vec8 v = v_operand(i);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) top = fmaxf(top, s[m][i]);
-        top = max32(max16(top));
-        follow(top, ref, sum, s2, o);
-        const float base = ref == kNone ? 0.f : ref;
-        vec8 w[PP];
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float x = exp2_(fmaf(s[m][i] - base, s2, Mma<C>::kBias));
-                C part[PP];
-                split_p<PP>(x, part);
-                sum += x;
-#pragma unroll
-                for (int y = 0; y < PP; ++y) w[y][4 * m + i] = part[y];
-            }
-#pragma unroll
-        for (int i = 0; i < DT; ++i) {
-            const vec8 v = v_operand(i);
-#pragma unroll
-            for (int y = 0; y < PP; ++y) o[i] = Mma<C>::mul16(v, w[y], o[i]);
-        }
-        if (odd) {
-            for (int e = 0; e < kBlock; ++e) {
-                const bool sees = key0 + e >= row.lo && key0 + e < min(row.hi, k.hi);
-#pragma unroll
-                for (int i = 0; i < DT; ++i) {
-                    const int from = 16 * (i & 1) + 4 * g;
-                    const unsigned up = sees ? kinds[wave][0][e][i / 2] >> from : 0, down = sees ? kinds[wave][1][e][i / 2] >> from : 0;
-                    if (!__any((up | down) & 15)) continue;
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        if (up >> x & 1) o[i][x] += INFINITY;
-                        if (down >> x & 1) o[i][x] -= INFINITY;
-                    }
-                }
+                for (int y = 0; y < PP; ++y) o[i] = Mma<C>::mul16(v, w[y], o[i]);
             }
         }
+    };
+    pass.template operator()<false>();
+    if (__builtin_expect(__any(not_finite(o)), 0)) {
+#pragma unroll
+        for (int i = 0; i < DT; ++i) o[i] = floatx4{0, 0, 0, 0};
+        ref = kNone;
+        sum = 0;
+        run.now = pages_from(0);
+        start();
+        pass.template operator()<true>();
     }
 
     sum = sum32(sum16(sum));
@@ -385,68 +400,100 @@ __global__ __launch_bounds__(64 * W, HDP <= 128 && W == 4 ? 2 : 1) void decode32
     for (int i = 0; i < 4 * DJ; ++i) o[i] = floatx4{0, 0, 0, 0};
     float ref = kNone, sum = 0;
 
-    if (n_block) {
+    const auto start = [&] {   // as above
         page = run.get(0);
         load_k(first_block * kBlock);
         load_v(first_block * kBlock);
         run.ahead = pages_from(64);
-    }
+    };
+    if (n_block) start();
 #pragma unroll
     for (int u = 0; u < KU; ++u)
         if (!row.real || 16 * u + 4 * g >= a.hd) q[u] = floatx4{0, 0, 0, 0};
-    for (int j = 0; j < n_block; ++j) {
-        const int key0 = (first_block + W * j) * kBlock;
-        const bool has = page >= 0, whole = key0 >= k.all_lo && key0 + kBlock <= min(k.all_hi, k.hi) && has;
-        const int next = j + 1, next_key = key0 + W * kBlock;
-        if ((next & 63) == 0) {
-            run.now = run.ahead;
-            run.ahead = pages_from(next + 64);
-        }
-        page = run.get(next & 63);
+    const auto pass = [&]<bool CAREFUL>() __attribute__((always_inline)) {
+        for (int j = 0; j < n_block; ++j) {
+            const int key0 = (first_block + W * j) * kBlock;
+            const bool has = page >= 0, whole = key0 >= k.all_lo && key0 + kBlock <= min(k.all_hi, k.hi) && has;
+            const int next = j + 1, next_key = key0 + W * kBlock;
+            if ((next & 63) == 0) {
+                run.now = run.ahead;
+                run.ahead = pages_from(next + 64);
+            }
+            page = run.get(next & 63);
 
-        if (padded) {
+            if (padded) {
+#pragma unroll
+                for (int u = 0; u < KU; ++u)
+                    if (16 * u + 4 * g >= a.hd) kr[u] = floatx4{0, 0, 0, 0};
+            }
+            floatx4 s = floatx4{0, 0, 0, 0}, s2 = floatx4{0, 0, 0, 0};   // two chains
 #pragma unroll
             for (int u = 0; u < KU; ++u)
-                if (16 * u + 4 * g >= a.hd) kr[u] = floatx4{0, 0, 0, 0};
-        }
-        floatx4 s = floatx4{0, 0, 0, 0}, s2 = floatx4{0, 0, 0, 0};   // two chains
 #pragma unroll
-        for (int u = 0; u < KU; ++u)
-#pragma unroll
-            for (int e = 0; e < 4; e += 2) {
-                s = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[u][e], q[u][e], s, 0, 0, 0);
-                s2 = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[u][e + 1], q[u][e + 1], s2, 0, 0, 0);
-            }
-        s += s2;
-        if (next < n_block) load_k(next_key);
+                for (int e = 0; e < 4; e += 2) {
+                    s = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[u][e], q[u][e], s, 0, 0, 0);
+                    s2 = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[u][e + 1], q[u][e + 1], s2, 0, 0, 0);
+                }
+            s += s2;
+            if (next < n_block) load_k(next_key);
 
-        bool odd = false;
-        if (!whole) {
+            if (!whole) {   // V as for 16-bit caches
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int key = key0 + 4 * g + i;
-                const bool in = key < k.hi && has;
-                if (!(in && key >= row.lo && key < row.hi)) s[i] = kNone;
+                for (int i = 0; i < 4; ++i) {
+                    const int key = key0 + 4 * g + i;
+                    const bool in = key < k.hi && key >= k.seen_lo && has;
+                    if (!(in && key >= row.lo && key < row.hi)) s[i] = kNone;
 #pragma unroll
-                for (int x = 0; x < DJ; ++x) {
-                    if (!in) vr[i][x] = floatx4{0, 0, 0, 0};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) odd |= !finite(vr[i][x][e]);
+                    for (int x = 0; x < DJ; ++x)
+                        if (!in) vr[i][x] = floatx4{0, 0, 0, 0};
                 }
             }
-            odd = __any(odd);
-        }
-        float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-        top = max32(max16(top));
-        follow(top, ref, sum, d.scale_log2, o);
-        const float base = ref == kNone ? 0.f : ref;
-        float w[4];
+            float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+            top = max32(max16(top));
+            follow<CAREFUL>(top, ref, sum, d.scale_log2, o);
+            if constexpr (CAREFUL) {
+                unsigned has_weight = 0;   // of the block's keys, for the lane's row
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            w[i] = exp2_(fmaf(s[i] - base, d.scale_log2, Mma<bhalf_t>::kBias));
-            sum += w[i];
-        }
-        if (!odd) {
+                for (int i = 0; i < 4; ++i) has_weight |= (unsigned)(s[i] != kNone) << (4 * g + i);
+                has_weight |= __shfl_xor(has_weight, 16);
+                has_weight |= __shfl_xor(has_weight, 32);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    bool odd = false;
+#pragma unroll
+                    for (int x = 0; x < DJ; ++x)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) odd |= !finite(vr[i][x][e]);
+                    if (!__any(odd)) continue;
+                    // key by key, laid over the rows by a product with 1
+#pragma unroll 1
+                    for (int y = 0; y < 4; ++y) {
+                        const bool gets = has_weight >> (4 * y + i) & 1;
+#pragma unroll
+                        for (int x = 0; x < DJ; ++x)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const floatx4 t = __builtin_amdgcn_mfma_f32_16x16x4f32(g == y && !finite(vr[i][x][e]) ? vr[i][x][e] : 0.f, 1.f,
+                                                                                      floatx4{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+                                for (int z = 0; z < 4; ++z)
+                                    if (gets) o[4 * x + e][z] += t[z];
+                            }
+                    }
+#pragma unroll
+                    for (int x = 0; x < DJ; ++x)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (!finite(vr[i][x][e])) vr[i][x][e] = 0.f;
+                }
+            }
+            const float base = ref == kNone ? 0.f : ref;
+            float w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[i] = exp2_(fmaf(s[i] - base, d.scale_log2, Mma<bhalf_t>::kBias));
+                sum += w[i];
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -454,26 +501,18 @@ __global__ __launch_bounds__(64 * W, HDP <= 128 && W == 4 ? 2 : 1) void decode32
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         o[4 * x + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(vr[i][x][e], w[i], o[4 * x + e], 0, 0, 0);
-        } else {
-            // key by key, each added only to the rows that see it
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                for (int y = 0; y < 4; ++y) {
-                    const int key = key0 + 4 * y + i;
-                    const bool sees = key >= row.lo && key < row.hi;
-#pragma unroll
-                    for (int x = 0; x < DJ; ++x)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const floatx4 t = __builtin_amdgcn_mfma_f32_16x16x4f32(g == y ? vr[i][x][e] : 0.f, w[i],
-                                                                                  floatx4{0, 0, 0, 0}, 0, 0, 0);
-#pragma unroll
-                            for (int z = 0; z < 4; ++z)
-                                if (sees) o[4 * x + e][z] += t[z];
-                        }
-                }
+            if (next < n_block) load_v(next_key);
         }
-        if (next < n_block) load_v(next_key);
+    };
+    pass.template operator()<false>();
+    if (__builtin_expect(__any(not_finite(o)), 0)) {
+#pragma unroll
+        for (int i = 0; i < 4 * DJ; ++i) o[i] = floatx4{0, 0, 0, 0};
+        ref = kNone;
+        sum = 0;
+        run.now = pages_from(0);
+        start();
+        pass.template operator()<true>();
     }
 
     sum = sum32(sum16(sum));

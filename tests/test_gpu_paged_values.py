@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from tests.paged_ref import DTYPE, UNIT, Case, to64
+from tests.paged_ref import DTYPE, PAIRS, UNIT, Case, check_rows, to64
 
 pytestmark = pytest.mark.gpu
 
@@ -52,6 +52,99 @@ def test_scores_with_a_common_part(dtype, common, lens, max_q):
                 want, size = w @ V[:, h // 3], w @ np.abs(V[:, h // 3])
                 e = (2 * u + 2.0 ** -13 + 2.0 ** -17 + (len(p) / 8 + 16) * 2.0 ** -24) * size + u * np.abs(want) + 2.0 ** -24
                 assert (np.abs(got[row, h] - want) <= e).all(), (row, h, float((np.abs(got[row, h] - want) / e).max()))
+
+
+# ---- infinities of V --------------------------------------------------------------
+
+def _by_weight(c, window=0):
+    """(out, bound): keys whose score is -inf have no weight and give nothing; of the others, however small their weight, an
+    infinity or NaN of V reaches its dim.  Finite dims as Case.exact's, with its bound."""
+    kp, vp, q = to64(c.k_pool[0]), to64(c.v_pool[0]), to64(c.q)
+    out = np.zeros((c.n_tok, c.nh, c.hd))
+    bound = np.zeros_like(out)
+    rep = c.nh // c.nkv
+    for s, (n, kv) in enumerate(c.lens):
+        for i in range(n):
+            row = int(c.starts[s]) + i
+            pos = kv - n + i
+            p = np.arange(max(0, pos - window + 1 if window else 0), pos + 1)
+            for h in range(c.nh):
+                K, V = kp[c.pages[s, p // c.ps], h // rep, p % c.ps], vp[c.pages[s, p // c.ps], h // rep, p % c.ps]
+                with np.errstate(invalid="ignore"):
+                    sc = K @ q[row, h] / math.sqrt(c.hd)
+                on = sc > -np.inf
+                if not on.any():
+                    continue
+                K, V, sc = K[on], V[on], sc[on]
+                w = np.exp(sc - sc.max())
+                w /= w.sum()
+                F = np.where(np.isfinite(V), V, 0)
+                out[row, h] = w @ F
+                S = float((np.abs(K[w > 0]) @ np.abs(q[row, h])).max()) / math.sqrt(c.hd)   # (errors of a weight of 0 are none)
+                u = UNIT[c.dtype] if c.dtype != "f32" else 2.0 ** -21
+                e = 2 * S * ((c.hd + 8) * UNIT["f32"] + 2.0 ** -21) + u + (len(p) / 8 + 16) * UNIT["f32"]
+                bound[row, h] = e * (w @ np.abs(F)) + UNIT[c.dtype] * np.abs(out[row, h]) + 2.0 ** -24
+                up, down = ((V == np.inf) | np.isnan(V)).any(0), ((V == -np.inf) | np.isnan(V)).any(0)
+                out[row, h] = np.where(up & down, np.nan, np.where(up, np.inf, np.where(down, -np.inf, out[row, h])))
+    return out, bound
+
+
+@pytest.mark.parametrize("dtype,cache", PAIRS)
+@pytest.mark.parametrize("hd", [64, 96, 256])
+@pytest.mark.parametrize("lens", ["short", "split"])
+@pytest.mark.parametrize("max_q", [1, 64])
+def test_infinities_reach_a_row_by_its_scores_alone(dtype, cache, hd, lens, max_q):
+    """Infinities and NaN of V in keys of ordinary weight, of a weight far under the smallest float (before and behind the
+    largest score of the row, near it and a split away) and of none (a score of -inf): where tiles and splits are cut, and
+    which kernel is taken, changes nothing."""
+    lens = {"short": [(40, 330), (1, 200)], "split": [(3, 2900), (1, 2500)]}[lens]
+    c = Case(lens, 2, 1, hd, 32, dtype, cache, seed=hd)
+    c.q[..., 7] = c.q[..., 7].abs() + 4.0
+    c.k_pool[..., 7] = torch.where(torch.isnan(c.k_pool[..., 7]), c.k_pool[..., 7], torch.zeros_like(c.k_pool[..., 7]))
+
+    def put(s, p, dim, v, k7=None):
+        c.v_pool[0, c.pages[s, p // 32], 0, p % 32, dim] = v
+        if k7 is not None:
+            c.k_pool[0, c.pages[s, p // 32], 0, p % 32, 7] = k7
+
+    far, gone = -8.0 * 2000, -math.inf
+    put(0, 3, 0, math.inf)                      # of ordinary weight: in tiles that all see it
+    put(0, 40, 1, -math.inf)
+    put(0, 41, 2, math.nan)
+    put(0, 50, 3, math.inf)
+    put(0, 150, 3, -math.inf)                   # both in one dim
+    put(0, 9, 4, math.inf, far)                 # weights of 2^-2000 and less
+    put(0, 130, 5, -math.inf, far)
+    put(0, lens[0][1] - 2, 6, math.inf, far)    # that the last rows alone see
+    put(0, 20, 7, math.nan, far)
+    put(0, 10, 8, math.inf, gone)               # no weight
+    put(0, 140, 9, math.nan, gone)
+    put(0, lens[0][1] - 1, 10, -math.inf, gone)
+    for p in range(64):                         # sequence 1: nothing but far keys, then ordinary ones
+        put(1, p, 11, math.inf if p == 5 else 1.0, far)
+    put(1, 199, 12, -math.inf, gone)
+    put(1, 100, 13, math.inf)
+    c.up()
+    with c.handle() as kv:
+        c.attend(kv, max_q=max_q)
+        check_rows(c, c.rows("out", 2)[0], *_by_weight(c))
+        c.attend(kv, max_q=max_q, window=170)
+        check_rows(c, c.rows("out", 2)[0], *_by_weight(c, 170), "window")
+
+
+@pytest.mark.parametrize("dtype,cache", PAIRS)
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("max_q", [1, 64])
+def test_rows_without_weight_get_zeros_beside_infinities(dtype, cache, bad, max_q):
+    """Every attended score is -inf: zeros, whatever V holds, in whole and in split tiles."""
+    c = Case([(3, 40), (20, 300), (1, 3000)], 6, 2, 64, 16, dtype, cache, seed=3)
+    c.q[..., 7] = c.q[..., 7].abs() + 0.5
+    c.k_pool[..., 7] = -math.inf
+    c.v_pool[..., ::5] = bad
+    c.up()
+    with c.handle() as kv:
+        c.attend(kv, max_q=max_q)
+    assert (to64(c.rows("out", 6)[0]) == 0).all()
 
 
 # ---- units of q and K ----------------------------------------------------------------
