@@ -612,9 +612,9 @@ hipError_t launch_decode(const TileArgs &d, hipStream_t s) {
     const dim3 grid((unsigned)d.places);
 #define KORE_DECODE(KERNEL, ...)                                                                \
     do {                                                                                        \
-        if (hdp == 64) KERNEL<__VA_ARGS__ 64, W><<<grid, 64 * W, 0, s>>>(d);                    \
-        else if (hdp == 128) KERNEL<__VA_ARGS__ 128, W><<<grid, 64 * W, 0, s>>>(d);             \
-        else if constexpr (W == 4) KERNEL<__VA_ARGS__ 256, W><<<grid, 64 * W, 0, s>>>(d);       \
+        if (hdp == 64) return launch(KERNEL<__VA_ARGS__ 64, W>, grid, 64 * W, s, d);                    \
+        else if (hdp == 128) return launch(KERNEL<__VA_ARGS__ 128, W>, grid, 64 * W, s, d);             \
+        else if constexpr (W == 4) return launch(KERNEL<__VA_ARGS__ 256, W>, grid, 64 * W, s, d);       \
     } while (0)
 #define KORE_COMMA ,
     if (d.a.cache_type == kF32) KORE_DECODE(decode32_kernel);
@@ -624,7 +624,7 @@ hipError_t launch_decode(const TileArgs &d, hipStream_t s) {
     else KORE_DECODE(decode16_kernel, bhalf_t KORE_COMMA bhalf_t KORE_COMMA);
 #undef KORE_COMMA
 #undef KORE_DECODE
-    return hipGetLastError();
+    return hipErrorInvalidValue;   // (a head of more than 128 in eight waves: launch_attend makes no such call)
 }
 
 constexpr int kPerCu = 2;                              // workgroups of a CU, of the 16-row kernels
@@ -693,14 +693,13 @@ hipError_t launch_attend(const AttendArgs &a, hipStream_t s) {
     const dim3 merge((unsigned)joined, (unsigned)std::clamp(8 * a.num_cu / joined, 1, a.hd / 4));
 #define KORE_MERGE(A)                                                                    \
     do {                                                                                 \
-        if (chunk) merge_kernel<A, kChunkRows><<<merge, kThreads, 0, s>>>(d, hdp / 4);   \
-        else merge_kernel<A, kRows><<<merge, kThreads, 0, s>>>(d, hdp / 4);              \
+        if (chunk) return launch(merge_kernel<A, kChunkRows>, merge, kThreads, s, d, hdp / 4);   \
+        else return launch(merge_kernel<A, kRows>, merge, kThreads, s, d, hdp / 4);              \
     } while (0)
     if (a.type == kF32) KORE_MERGE(float);
     else if (a.type == kF16) KORE_MERGE(half_t);
     else KORE_MERGE(bhalf_t);
 #undef KORE_MERGE
-    return hipGetLastError();
 }
 
 }  // namespace kore_paged_gpu

@@ -230,16 +230,15 @@ hipError_t launch_rope(const RopeArgs &a, hipStream_t s) {
     const dim3 grid = row_grid(a.n_tok, a.hd / (v4 ? 8 : 2) * a.n_head);
 #define KORE_ROPE_CASE(T)                                                                         \
     do {                                                                                          \
-        if (v4 && a.turn.interleaved) rope_kernel<T, 4, true><<<grid, kThreads, 0, s>>>(a);       \
-        else if (v4) rope_kernel<T, 4, false><<<grid, kThreads, 0, s>>>(a);                       \
-        else if (a.turn.interleaved) rope_kernel<T, 1, true><<<grid, kThreads, 0, s>>>(a);        \
-        else rope_kernel<T, 1, false><<<grid, kThreads, 0, s>>>(a);                               \
+        if (v4 && a.turn.interleaved) return launch(rope_kernel<T, 4, true>, grid, kThreads, s, a);       \
+        else if (v4) return launch(rope_kernel<T, 4, false>, grid, kThreads, s, a);                       \
+        else if (a.turn.interleaved) return launch(rope_kernel<T, 1, true>, grid, kThreads, s, a);        \
+        else return launch(rope_kernel<T, 1, false>, grid, kThreads, s, a);                               \
     } while (0)
     if (a.type == kF32) KORE_ROPE_CASE(float);
     else if (a.type == kF16) KORE_ROPE_CASE(half_t);
     else KORE_ROPE_CASE(bhalf_t);
 #undef KORE_ROPE_CASE
-    return hipGetLastError();
 }
 
 hipError_t launch_append(const AppendArgs &a, hipStream_t s) {
@@ -250,10 +249,10 @@ hipError_t launch_append(const AppendArgs &a, hipStream_t s) {
     const dim3 grid = row_grid(a.b.n_tok, a.hd / (v4 ? 8 : 2) * ((a.q ? a.n_head : 0) + 2 * a.n_head_kv));
 #define KORE_APPEND_CASE(T, C)                                                                    \
     do {                                                                                          \
-        if (v4 && a.turn.interleaved) append_kernel<T, C, 4, true><<<grid, kThreads, 0, s>>>(a);  \
-        else if (v4) append_kernel<T, C, 4, false><<<grid, kThreads, 0, s>>>(a);                  \
-        else if (a.turn.interleaved) append_kernel<T, C, 1, true><<<grid, kThreads, 0, s>>>(a);   \
-        else append_kernel<T, C, 1, false><<<grid, kThreads, 0, s>>>(a);                          \
+        if (v4 && a.turn.interleaved) return launch(append_kernel<T, C, 4, true>, grid, kThreads, s, a);  \
+        else if (v4) return launch(append_kernel<T, C, 4, false>, grid, kThreads, s, a);                  \
+        else if (a.turn.interleaved) return launch(append_kernel<T, C, 1, true>, grid, kThreads, s, a);   \
+        else return launch(append_kernel<T, C, 1, false>, grid, kThreads, s, a);                          \
     } while (0)
     if (a.type == kF32 && a.cache_type == kF32) KORE_APPEND_CASE(float, float);
     else if (a.type == kF32 && a.cache_type == kF16) KORE_APPEND_CASE(float, half_t);
@@ -261,7 +260,6 @@ hipError_t launch_append(const AppendArgs &a, hipStream_t s) {
     else if (a.type == kF16) KORE_APPEND_CASE(half_t, half_t);
     else KORE_APPEND_CASE(bhalf_t, bhalf_t);
 #undef KORE_APPEND_CASE
-    return hipGetLastError();
 }
 
 }  // namespace kore_paged_gpu
