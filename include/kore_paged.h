@@ -29,7 +29,8 @@
  *   the table's pages_stride entries is: positions there are not stored, and not
  *   attended.  A row with nothing to attend gets zeros, and so does one whose
  *   attended scores are all -infinity.
- *   At most 2^23 rows, 2^27 rows x heads and 2^22 sequences x kv-heads a call.
+ *   At most 2^23 rows, 2^27 rows x heads, 2^16 sequences and 2^22 sequences x
+ *   kv-heads a call.
  *   With a q_start that is not ascending the rows of out (q_out, the slots stored)
  *   hold nothing of use; nothing else is written, and nothing outside the buffers
  *   is read.

@@ -237,6 +237,8 @@ int check_batch(kore_paged *h, int layer, const kore_paged_batch *b, int type) {
     if (!b->q_start || !b->kv_len || !b->pages) return fail(h, KORE_PAGED_E_INVALID, "null q_start, kv_len or pages");
     if (b->pages_stride <= 0 || b->pages_stride > kMaxKeys / h->cfg.page_size)
         return fail(h, KORE_PAGED_E_INVALID, "pages_stride %d outside 1..%d", b->pages_stride, kMaxKeys / h->cfg.page_size);
+    if (b->n_seq > kMaxSeq)
+        return fail(h, KORE_PAGED_E_UNSUPPORTED, "n_seq %d is too large (over %d)", b->n_seq, kMaxSeq);
     if (b->n_tok > kMaxRows || (int64_t)b->n_tok * h->cfg.n_head > kMaxRowHeads ||
         (int64_t)b->n_seq * h->cfg.n_head_kv > kMaxSeqHeads)
         return fail(h, KORE_PAGED_E_UNSUPPORTED, "n_tok %d x %d heads or n_seq %d x %d kv-heads is too large", b->n_tok,

@@ -16,6 +16,9 @@ constexpr int kMaxKeys = 1 << 30;       // positions of a sequence's row of the 
 // A launch has fewer than 2^32 threads: rows of a call (256 threads each); rows x heads and sequences x kv-heads
 // of a batch, which make at most 2^23 + 2^22 tiles of 256 threads, or 2^20 + 2^22 of 512.
 constexpr int kMaxRows = 1 << 23, kMaxRowHeads = 1 << 27, kMaxSeqHeads = 1 << 22;
+// Every row of an append and every tile of an attention scans the sequences, 64 a round: at 2^16 of them a call takes
+// seconds at its largest, at 2^22 it would hold the device for many minutes.
+constexpr int kMaxSeq = 1 << 16;
 
 enum Type { kF32 = 0, kF16 = 1, kBF16 = 2 };
 inline int type_bytes(int t) { return t == kF32 ? 4 : 2; }

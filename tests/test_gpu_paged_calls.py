@@ -4,7 +4,7 @@ import ctypes as C
 import pytest
 import torch
 
-from tests.paged_ref import Case
+from tests.paged_ref import Case, check_rows
 
 pytestmark = pytest.mark.gpu
 
@@ -32,3 +32,43 @@ def test_an_error_of_another_call_is_not_theirs():
                 L.hipGetLastError()
         kv.sync()
         r.sync()
+
+
+@pytest.mark.parametrize("max_q", [1, 64])
+def test_the_most_sequences(max_q):
+    """2^16 sequences, three of which have rows, the last among them; one more is refused, by either call, with nothing written."""
+    from kore_amd import paged
+    c = Case([(1, 40), (20, 90), (2, 17)], 4, 2, 64, 16, "f32", "f16", seed=2, extra_rows=1).up()
+    n_seq, at = 1 << 16, [0, 40000, (1 << 16) - 1]
+    starts, lens = torch.zeros(n_seq + 2, dtype=torch.int32), torch.full((n_seq + 1,), 33, dtype=torch.int32)
+    pages = torch.full((n_seq + 1, c.stride), -1, dtype=torch.int32)
+    for s, i in enumerate(at):
+        starts[i + 1:] = int(c.starts[s + 1])
+        lens[i] = int(c.kv_len[s])
+        pages[i] = torch.from_numpy(c.pages[s])
+    starts, lens, pages = starts.cuda(), lens.cuda(), pages.cuda()
+    before = {n: t.clone() for n, t in c.d.items()}
+
+    def batch(n):
+        return paged.Batch(n, c.n_tok, starts.data_ptr(), lens.data_ptr(), pages.data_ptr(), c.stride, max_q)
+
+    with c.handle() as kv:
+        for call in (lambda b: kv.attend_dev(0, b, "f32", c.ptr("q"), c.ptr("out")),
+                     lambda b: kv.append_dev(0, b, "f32", c.ptr("k"), c.ptr("v"))):
+            with pytest.raises(paged.PagedError, match="n_seq"):
+                call(batch(n_seq + 1))
+        kv.sync()
+        for n, t in before.items():
+            assert torch.equal(t.view(torch.uint8), c.d[n].view(torch.uint8)), n
+        kv.append_dev(0, batch(n_seq), "f32", c.ptr("k"), c.ptr("v"))
+        kv.attend_dev(0, batch(n_seq), "f32", c.ptr("q"), c.ptr("out"))
+        kv.sync()
+    for s, (n, kv_len) in enumerate(c.lens):
+        for i in range(n):
+            page, slot, row = int(c.pages[s, (kv_len - n + i) // 16]), (kv_len - n + i) % 16, int(c.starts[s]) + i
+            for pool, x in (("k_pool", c.k), ("v_pool", c.v)):
+                assert torch.equal(c.d[pool][0, page, :, slot].cpu(), x[row].half())
+    c.k_pool, c.v_pool = c.d["k_pool"].cpu(), c.d["v_pool"].cpu()
+    got = c.rows("out", 4)[0]
+    assert (got[c.used:] == 77.0).all()
+    check_rows(c, got, *c.exact())
