@@ -208,19 +208,27 @@ int check_aligned(H *h, const char *what, const void *p, int type) {
     return KORE_PAGED_OK;
 }
 
-// x's rows and y's, [n_tok] of n values: the same buffer with the same stride, or no byte in common.
+// x's rows and y's, [n_tok] of xn and yn values: no byte in common.
+template <class H>
+int check_apart(H *h, const char *what, const void *x, int64_t xs, int64_t xn, const void *y, int64_t ys, int64_t yn, int n_tok,
+                int type) {
+    const uintptr_t size = (uintptr_t)type_bytes(type), x0 = (uintptr_t)x, y0 = (uintptr_t)y;
+    const uintptr_t x1 = x0 + ((uintptr_t)(n_tok - 1) * xs + xn) * size, y1 = y0 + ((uintptr_t)(n_tok - 1) * ys + yn) * size;
+    if (x0 < y1 && y0 < x1) {
+        // rows that lie between each other (two parts of one wide row) share no byte
+        const bool first = x0 < y0;
+        const uintptr_t step = (uintptr_t)xs * size, d = (first ? y0 - x0 : x0 - y0) % step;
+        const uintptr_t w = (uintptr_t)(first ? xn : yn) * size, next = (uintptr_t)(first ? yn : xn) * size;
+        if (xs != ys || d < w || d + next > step) return fail(h, KORE_PAGED_E_INVALID, "%s rows overlap", what);
+    }
+    return KORE_PAGED_OK;
+}
+
+// Input rows and output rows of n values: the same buffer with the same stride, or no byte in common.
 template <class H>
 int check_overlap(H *h, const void *x, int64_t xs, const void *y, int64_t ys, int64_t n, int n_tok, int type) {
     if (x == y && xs == ys) return KORE_PAGED_OK;
-    const uintptr_t size = (uintptr_t)type_bytes(type), x0 = (uintptr_t)x, y0 = (uintptr_t)y;
-    const uintptr_t x1 = x0 + ((uintptr_t)(n_tok - 1) * xs + n) * size, y1 = y0 + ((uintptr_t)(n_tok - 1) * ys + n) * size;
-    if (x0 < y1 && y0 < x1) {
-        // rows that lie between each other (two parts of one wide row) share no byte
-        const uintptr_t d = x0 < y0 ? y0 - x0 : x0 - y0, step = (uintptr_t)xs * size, w = (uintptr_t)n * size;
-        const bool between = xs == ys && d % step >= w && d % step + w <= step;
-        if (!between) return fail(h, KORE_PAGED_E_INVALID, "input and output rows overlap");
-    }
-    return KORE_PAGED_OK;
+    return check_apart(h, "input and output", x, xs, n, y, ys, n, n_tok, type);
 }
 
 int check_batch(kore_paged *h, int layer, const kore_paged_batch *b, int type) {
@@ -427,6 +435,8 @@ int kore_paged_append_dev(kore_paged_t h, int layer, const kore_paged_batch *b, 
         if (int rc = check_aligned(h, "q", q, type)) return rc;
         if (int rc = check_aligned(h, "q_out", q_out, type)) return rc;
         if (int rc = check_overlap(h, q, q_stride, q_out, q_out_stride, E, b->n_tok, type)) return rc;
+        if (int rc = check_apart(h, "k and q_out", k, k_stride, kvd, q_out, q_out_stride, E, b->n_tok, type)) return rc;
+        if (int rc = check_apart(h, "v and q_out", v, v_stride, kvd, q_out, q_out_stride, E, b->n_tok, type)) return rc;
     }
     OnDevice on(h->device);
     if (int rc = on_device(h, on)) return rc;

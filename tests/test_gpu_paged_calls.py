@@ -72,3 +72,32 @@ def test_the_most_sequences(max_q):
     got = c.rows("out", 4)[0]
     assert (got[c.used:] == 77.0).all()
     check_rows(c, got, *c.exact())
+
+
+def test_rotated_q_in_the_place_of_k_or_v():
+    """q_out may be q and lie beside k and v in wide rows, but not on any of their bytes: it would be read after it is written."""
+    from kore_amd import paged, rope
+    E, D, n = 4 * 64, 2 * 64, 3
+    c = Case([(n, 40)], 4, 2, 64, 16, "f32", "f16", seed=1).up()
+    wide = torch.randn(n, E + 2 * D + 8, device="cuda")
+    at = [wide.data_ptr() + 4 * x for x in (0, E, E + D, E + 2 * D)]
+    step = wide.shape[1]
+    torch.cuda.synchronize()
+    with c.handle(rope.Config(64)) as kv:
+        def call(q, q_out, k=at[1], v=at[2], qs=step, qo=step, ks=step, vs=step):
+            kv.append_dev(0, c.batch(), "f32", k, v, q=q, q_out=q_out, k_stride=ks, v_stride=vs, q_stride=qs, q_out_stride=qo)
+
+        before = wide.clone()
+        for kw, text in [
+                (dict(q=c.ptr("q"), qs=E, q_out=at[1]), "k and q_out"), (dict(q=c.ptr("q"), qs=E, q_out=at[0] + 4), "k and q_out"),
+                (dict(q=c.ptr("q"), qs=E, q_out=at[2]), "v and q_out"), (dict(q=c.ptr("q"), qs=E, q_out=at[0], qo=E), "k and q_out"),
+                (dict(q=c.ptr("q"), qs=E, q_out=c.ptr("out"), qo=E, k=c.ptr("out"), ks=D), "k and q_out"),
+                (dict(q=c.ptr("q"), qs=E, q_out=c.ptr("out"), qo=E, v=c.ptr("out") + 4 * E, vs=D), "v and q_out")]:
+            with pytest.raises(paged.PagedError, match=text):
+                call(**kw)
+        kv.sync()
+        assert torch.equal(wide, before)
+        call(q=at[0], q_out=at[0])                              # in place, beside k and v
+        call(q=c.ptr("q"), qs=E, q_out=c.ptr("out"), qo=E)      # apart
+        kv.sync()
+    assert torch.equal(wide[:, E:], before[:, E:]) and not torch.equal(wide[:, :E], before[:, :E])
