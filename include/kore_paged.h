@@ -45,10 +45,17 @@
  *
  * Arithmetic: products of the cache's values with q and with the softmax's
  * weights are summed in fp32, and the result is rounded once to the rows' type.
- * fp32 rows keep fp32's precision whatever the cache's type (their products run
- * in several 16-bit parts, or on fp32 MFMA); fp16 and bf16 rows of chunks (many
- * new rows of a sequence) round the weights to that type.  A sum is split over workgroups by a rule on the whole batch, in
- * a fixed order: the same call gives the same bits, another batch around a
+ * What fp32 rows hold of a value on the way:
+ *   batches of few rows (16-row tiles) over an fp32 cache: all 24 bits;
+ *   over a bf16 cache: 24 bits of q and of the weights (three bf16 parts);
+ *   over an fp16 cache: 22 bits of q, relative to its row's largest, and of the
+ *   weights (two fp16 parts);
+ *   chunks over an fp32 cache: 22 bits of q and of K, relative to their rows'
+ *   largest, 24 of V and of the weights.
+ * fp16 and bf16 rows hold q as it is; their weights are two parts of the type in
+ * 16-row tiles and one, rounded to the type, in chunks (many new rows of a
+ * sequence).  A sum is split over workgroups by a rule on the whole batch, in a
+ * fixed order: the same call gives the same bits, another batch around a
  * sequence may differ in the last ones.
  *
  * Conventions are those of kore_attn.h: 0 or a negative KORE_PAGED_E_* code,

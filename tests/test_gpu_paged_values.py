@@ -1,4 +1,5 @@
-"""The paged attention's values at their ends, against plain implementations in 64 bits."""
+"""The paged attention's values at their ends, and the precision that the header states, against plain implementations in
+64 bits."""
 import math
 
 import numpy as np
@@ -170,3 +171,33 @@ def test_large_values_that_meet_zeros(cache, max_q):
                     V = vp[c.pages[s, p // 16], :, p % 16].repeat(2, 1)
                     e = (2.0 ** -20 + (len(p) / 8 + 16) * 2.0 ** -24) * np.abs(V).mean(0)
                     assert (np.abs(got[int(c.starts[s]) + i] - V.mean(0)) <= e).all(), scale
+
+
+# ---- the precision that the header states -------------------------------------------
+
+def _cut(x, bits):
+    """fp32 values cut to their first `bits` bits."""
+    m, e = np.frexp(np.asarray(x, np.float64))
+    return np.ldexp(np.trunc(np.ldexp(m, bits)), e - bits)
+
+
+@pytest.mark.parametrize("cache", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("max_q", [1, 64])
+def test_fp32_rows_root_mean_square(cache, hd, max_q):
+    """fp32 rows of N(0, 1) values: the root mean square error, relative to the outputs'.  With values of independent sign, a
+    score's error is what hd products and sums leave, sqrt(hd) half steps of fp32 at most, and q's and K's parts, half of 2^-21
+    each (22 bits).  An error d of the scores is one of d in the outputs (sum w d v beside sum w v).  The weights' parts, 2^-21
+    at most, the sums' n / 8 + 16 roundings as roots, and the result's own follow.  A q of 16 bits, as two bf16 parts hold, is
+    beyond it: shown on the oracle."""
+    n, kv = 48, 600
+    c = Case([(n, kv)], 4, 2, hd, 32, "f32", cache, seed=hd).up()
+    with c.handle() as h:
+        c.attend(h, max_q=max_q)
+    got = to64(c.rows("out", 4)[0])
+    want, _ = c.exact()
+    rms = lambda x: float(np.sqrt(np.mean(np.square(x))))  # noqa: E731
+    bound = math.sqrt(sum(x * x for x in (math.sqrt(hd) * 2.0 ** -24, 2.0 ** -22, 2.0 ** -22, 2.0 ** -21, math.sqrt(kv / 8 + 16) * 2.0 ** -24, 2.0 ** -24)))
+    assert rms(got - want) <= bound * rms(want), (rms(got - want) / rms(want), bound)
+    c.q = torch.from_numpy(_cut(c.q.numpy(), 16)).float()
+    assert rms(c.exact()[0] - want) > 2 * bound * rms(want)
