@@ -56,12 +56,9 @@ namespace {
 
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
-typedef half_t half4 __attribute__((ext_vector_type(4)));
 typedef half_t half8 __attribute__((ext_vector_type(8)));
-typedef bhalf_t bhalf4 __attribute__((ext_vector_type(4)));
 typedef bhalf_t bhalf8 __attribute__((ext_vector_type(8)));
 typedef short short4_t __attribute__((ext_vector_type(4)));
-typedef short short8_t __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) short4_t lds_short4;
 
 constexpr float kNone = -INFINITY;
@@ -413,6 +410,7 @@ __device__ __forceinline__ void follow(float top, float &ref, float &sum, float 
         ref = next;
     }
 }
+
 // What a lane knows of its row (column l % 16 of the products).
 struct Row {
     int lo, hi;      // sees keys [lo, hi)

@@ -25,18 +25,13 @@ __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(half_t x) { return (float)x; }
 __device__ __forceinline__ float to_f32(bhalf_t x) { return (float)x; }
 
-// N elements from an address that is aligned to N elements (vec), or to one.
+// N elements from an address that is aligned to N elements, and to one such (vec) or to an element.
 template <int N, class T>
-__device__ __forceinline__ void load_n(const T *p, T (&x)[N], bool vec) {
+__device__ __forceinline__ void load_n(const T *p, T (&x)[N]) {
     typedef T vec_t __attribute__((ext_vector_type(N)));
-    if (vec) {
-        const vec_t v = *reinterpret_cast<const vec_t *>(p);
+    const vec_t v = *reinterpret_cast<const vec_t *>(p);
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = v[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = p[i];
-    }
+    for (int i = 0; i < N; ++i) x[i] = v[i];
 }
 template <int N, class T>
 __device__ __forceinline__ void store_n(T *p, const T (&x)[N], bool vec) {

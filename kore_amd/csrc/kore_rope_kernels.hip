@@ -1,7 +1,7 @@
 // kore_rope_kernels.hip - rotary positions of rows, and the append of rotated
 // rows to a paged cache (gfx950).
 //
-// Both are bound by memory: 12 flops a pair beside 16 bytes (fp32) of traffic,
+// Both are bound by memory: 6 flops a pair beside 16 bytes (fp32) of traffic,
 // and a cosine and sine for each pair of a row, shared by its heads.  4096 bf16 rows of
 // 36 heads of 96: 11.8 us, 4.8 TB/s (a large copy: 5.1); three prompts' 1777 rows of
 // 28/4/128 into a bf16 cache: 15.1 us, 5.2 TB/s.  Few rows are a launch and three
@@ -121,8 +121,8 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs a) {
     const auto request = [&](int j, int i) {
         const int head = i / units;
         const Unit<V> u(i - head * units, a.turn.rot, INTER);
-        load_n<V>(x + (size_t)head * a.hd + u.at0, va[j], true);
-        load_n<V>(x + (size_t)head * a.hd + u.at1, vb[j], true);
+        load_n<V>(x + (size_t)head * a.hd + u.at0, va[j]);
+        load_n<V>(x + (size_t)head * a.hd + u.at1, vb[j]);
     };
 #pragma unroll
     for (int j = 0; j < kEarly; ++j)
@@ -156,8 +156,8 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a) {
         const T *src = head < nq ? (const T *)a.q + (size_t)row * a.q_stride + (size_t)head * a.hd
                      : is_v ? (const T *)a.v + (size_t)row * a.v_stride + (size_t)(kv - a.n_head_kv) * a.hd
                             : (const T *)a.k + (size_t)row * a.k_stride + (size_t)kv * a.hd;
-        load_n<V>(src + u.at0, va[j], true);
-        load_n<V>(src + u.at1, vb[j], true);
+        load_n<V>(src + u.at0, va[j]);
+        load_n<V>(src + u.at1, vb[j]);
     };
 #pragma unroll
     for (int j = 0; j < kEarly; ++j)
