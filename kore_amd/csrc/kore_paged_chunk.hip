@@ -448,6 +448,7 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
             // S^T = K Q^T: lane (n, half) gets its row's scores of keys 32 m + 8 (i / 4) + 4 half + i % 4
             floatx16 s[MT];
             bool far = false;
+            unsigned has_weight[MT];   // CAREFUL: of the step's keys, for the lane's row
             if (any) {
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
@@ -499,6 +500,15 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
 #pragma unroll
                     for (int i = 0; i < 16; ++i) top = fmaxf(top, s[m][i]);
                 follow<CAREFUL>(max32(top), ref, sum, s2, o);
+                if constexpr (CAREFUL) {
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) {
+                        has_weight[m] = 0;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) has_weight[m] |= (unsigned)(s[m][i] != kNone) << (8 * (i / 4) + 4 * half + i % 4);
+                        has_weight[m] |= __shfl_xor(has_weight[m], 32);
+                    }
+                }
                 // The difference from the reference first, as the softmax's comment says.  16-bit rows: one fma of the score
                 // and the scaled reference while that is under 2^11.  Its rounding, at most 2^-14 in the exponent, is the same
                 // for the weights of one reference and stays between those of two (a row's teams and splits, and before and
@@ -524,14 +534,6 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
             has_1 = has_2;
             if (any) {
                 if (CAREFUL && (odd_of[0] | odd_of[1] | odd_of[2] | odd_of[3])) {
-                    unsigned has_weight[MT];   // of the step's keys, for the lane's row
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        has_weight[m] = 0;
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) has_weight[m] |= (unsigned)(s[m][i] != kNone) << (8 * (i / 4) + 4 * half + i % 4);
-                        has_weight[m] |= __shfl_xor(has_weight[m], 32);
-                    }
                     for (int e = 0; e < kKeys; ++e) {
                         const bool gets = (e < 32 ? has_weight[0] : has_weight[MT - 1]) >> (e & 31) & 1;
 #pragma unroll
@@ -608,6 +610,10 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
         ref = kNone;
         sum = 0;
         run.now = pages_from(0);
+        // (as if they were others, so that what this pass makes of them is not kept through the first: 512 fp32 rows over 8192
+        // bf16 keys of 16/2/256 287 us without, 283)
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) asm volatile("" : "+v"(offs[i]));
         run.ahead = pages_from(64 / kGroups);
         if (n_step) start();
         pass.template operator()<true>();

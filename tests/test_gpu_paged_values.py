@@ -148,6 +148,35 @@ def test_rows_without_weight_get_zeros_beside_infinities(dtype, cache, bad, max_
     assert (to64(c.rows("out", 6)[0]) == 0).all()
 
 
+@pytest.mark.parametrize("dtype,cache", [p for p in PAIRS if p[1] != "f16"])
+@pytest.mark.parametrize("max_q", [1, 64])
+def test_an_infinity_at_the_other_end_of_the_scores(dtype, cache, max_q):
+    """Scores of +-2^127 (before the scale), further apart than fp32 reaches: the lower keys' infinities count, and nothing else
+    of them."""
+    c = Case([(40, 150), (1, 70)], 2, 1, 64, 16, dtype, cache, seed=6)
+    c.q[:] = 0
+    c.q[..., 0] = 2.0 ** 63
+    for s, (_, kv) in enumerate(c.lens):
+        for p in range(kv):
+            at = (0, c.pages[s, p // 16], 0, p % 16)
+            c.k_pool[at] = 0
+            c.k_pool[at + (0,)] = 2.0 ** 64 if p % 3 == 0 else -2.0 ** 64
+        c.v_pool[0, c.pages[s, 0], 0, 5, 3 + s] = math.inf       # position 5, low
+    c.up()
+    with c.handle() as kv:
+        c.attend(kv, max_q=max_q)
+    got = to64(c.rows("out", 2)[0])
+    for s, (n, kv_len) in enumerate(c.lens):
+        for i in range(n):
+            p = np.arange(0, kv_len - n + i + 1, 3)     # those of the high score share the weight
+            V = to64(c.v_pool[0, c.pages[s, p // 16], 0, p % 16])
+            want, e = V.mean(0), (2 * UNIT[dtype] + 2.0 ** -20 + (len(p) / 8 + 16) * 2.0 ** -24) * np.abs(V).mean(0)
+            row = got[int(c.starts[s]) + i]
+            assert (row[:, 3 + s] == math.inf).all()
+            row[:, 3 + s] = want[3 + s]
+            assert (np.abs(row - want) <= e).all()
+
+
 # ---- units of q and K ----------------------------------------------------------------
 
 @pytest.mark.parametrize("cache", ["f32", "f16", "bf16"])
