@@ -30,6 +30,7 @@
 // fmaf() calls or MFMA instructions.
 #include "kore_attn_kernels.h"
 #include "kore_attn_device.h"
+#include "kore_launch.h"
 
 #include <algorithm>
 #include <cmath>
@@ -37,6 +38,8 @@
 #include <vector>
 
 namespace kore_attn_gpu {
+
+using kore_gpu::launch;
 namespace {
 
 constexpr size_t kLdsPerCu = 160 * 1024;   // gfx950
@@ -1412,8 +1415,9 @@ hipError_t launch_decode_nr(const DecodeArgs &a, const RopeRow &rr, hipStream_t 
         // one per CU; the head_dim-64 instances would fit two by registers
         static const unsigned pad_m =
             dyn_lds_above(reinterpret_cast<const void *>(&decode_multi_kernel<HD, NR>), kLdsPerCu / 2 + 256);
-        hipLaunchKernelGGL((decode_multi_kernel<HD, NR>), grid, dim3(kThreads), pad_m, s, a.q, a.kc, a.vc, a.k, a.v,
-                           a.n_rows, a.rows_per_split, a.new_slot, a.slots, a, rr);
+        if (hipError_t e = launch(decode_multi_kernel<HD, NR>, grid, dim3(kThreads), pad_m, s, a.q, a.kc, a.vc, a.k, a.v,
+                                  a.n_rows, a.rows_per_split, a.new_slot, a.slots, a, rr))
+            return e;
     } else {
         // enough (unused) dynamic LDS that a CU holds exactly the workgroups
         // the grid plans for it: more than half the CU's LDS for one, more
@@ -1425,18 +1429,19 @@ hipError_t launch_decode_nr(const DecodeArgs &a, const RopeRow &rr, hipStream_t 
         }(), [] {
             return dyn_lds_above(reinterpret_cast<const void *>(&decode_split_kernel<HD, NR>), kLdsPerCu / 3 + 256);
         }()};
-        hipLaunchKernelGGL((decode_split_kernel<HD, NR>), grid, dim3(kThreads), pad[a.wg_per_cu == 2 ? 1 : 0], s,
-                           a.q, a.kc, a.vc, a.k, a.v, a.n_rows, a.rows_per_split, a.new_slot, a.slots, a, rr);
+        if (hipError_t e = launch(decode_split_kernel<HD, NR>, grid, dim3(kThreads), pad[a.wg_per_cu == 2 ? 1 : 0], s,
+                                  a.q, a.kc, a.vc, a.k, a.v, a.n_rows, a.rows_per_split, a.new_slot, a.slots, a, rr))
+            return e;
     }
     static_assert(kMaxDecodeSplits <= 8 * 32, "the combine takes at most 32 splits per lane");
     const dim3 cgrid(a.n_head_kv * a.n_rep, HD / 32);
     const float *po = a.part_o, *pml = a.part_ml;
-    if (a.n_split > 128) hipLaunchKernelGGL((decode_combine_kernel<HD, 32>), cgrid, dim3(64), 0, s, po, pml, a.out, a.n_split);
-    else if (a.n_split > 64) hipLaunchKernelGGL((decode_combine_kernel<HD, 16>), cgrid, dim3(64), 0, s, po, pml, a.out, a.n_split);
-    else if (a.n_split > 32) hipLaunchKernelGGL((decode_combine_kernel<HD, 8>), cgrid, dim3(64), 0, s, po, pml, a.out, a.n_split);
-    else if (a.n_split > 16) hipLaunchKernelGGL((decode_combine_kernel<HD, 4>), cgrid, dim3(64), 0, s, po, pml, a.out, a.n_split);
-    else if (a.n_split > 1) hipLaunchKernelGGL((decode_combine_kernel<HD, 2>), cgrid, dim3(64), 0, s, po, pml, a.out, a.n_split);
-    return hipGetLastError();
+    if (a.n_split > 128) return launch(decode_combine_kernel<HD, 32>, cgrid, dim3(64), 0, s, po, pml, a.out, a.n_split);
+    if (a.n_split > 64) return launch(decode_combine_kernel<HD, 16>, cgrid, dim3(64), 0, s, po, pml, a.out, a.n_split);
+    if (a.n_split > 32) return launch(decode_combine_kernel<HD, 8>, cgrid, dim3(64), 0, s, po, pml, a.out, a.n_split);
+    if (a.n_split > 16) return launch(decode_combine_kernel<HD, 4>, cgrid, dim3(64), 0, s, po, pml, a.out, a.n_split);
+    if (a.n_split > 1) return launch(decode_combine_kernel<HD, 2>, cgrid, dim3(64), 0, s, po, pml, a.out, a.n_split);
+    return hipSuccess;
 }
 
 template <int HD>
@@ -1539,8 +1544,7 @@ hipError_t launch_append(const AppendArgs &a, int head_dim, hipStream_t s) {
     constexpr int kTok = 4;
     const dim3 grid((a.n_tok + kTok - 1) / kTok, a.n_head_kv);
     const int threads = head_dim / 2 >= 64 ? 64 : (head_dim / 2 > 0 ? head_dim / 2 : 1);
-    hipLaunchKernelGGL(append_kernel, grid, dim3(threads, kTok), 0, s, a, head_dim);
-    return hipGetLastError();
+    return launch(append_kernel, grid, dim3(threads, kTok), 0, s, a, head_dim);
 }
 
 bool generic_supported(int head_dim) {
@@ -1574,20 +1578,18 @@ hipError_t launch_generic_decode(const GenericArgs &a, const RopeRow &rr, hipStr
     const bool v4 = a.hd % 4 == 0;
     const size_t lds = generic_lds_bytes(a.hd);
     const dim3 grid(a.n_split, a.n_head_kv);
-    if (v4) hipLaunchKernelGGL(generic_decode_kernel<4>, grid, dim3(kThreads), lds, s, a, rr);
-    else hipLaunchKernelGGL(generic_decode_kernel<2>, grid, dim3(kThreads), lds, s, a, rr);
-    if (a.n_split > 1)
-        hipLaunchKernelGGL(generic_combine_kernel, dim3(a.n_head_kv * a.n_rep), dim3(kThreads), 0, s, a.part_o,
-                           a.part_ml, a.out, a.n_split, a.hd);
-    return hipGetLastError();
+    if (hipError_t e = launch(v4 ? generic_decode_kernel<4> : generic_decode_kernel<2>, grid, dim3(kThreads), lds, s, a, rr))
+        return e;
+    if (a.n_split <= 1) return hipSuccess;
+    return launch(generic_combine_kernel, dim3(a.n_head_kv * a.n_rep), dim3(kThreads), 0, s, a.part_o, a.part_ml, a.out,
+                  a.n_split, a.hd);
 }
 
 hipError_t launch_staging(const float *src, float *dst, size_t floats, hipStream_t s) {
     const size_t n4 = floats / 4;
     if (n4 == 0) return hipSuccess;
-    hipLaunchKernelGGL(staging_kernel, dim3((unsigned)std::min<size_t>(512, (n4 + kThreads - 1) / kThreads)), dim3(kThreads),
-                       0, s, reinterpret_cast<const float4 *>(src), reinterpret_cast<float4 *>(dst), n4);
-    return hipGetLastError();
+    return launch(staging_kernel, dim3((unsigned)std::min<size_t>(512, (n4 + kThreads - 1) / kThreads)), dim3(kThreads), 0, s,
+                  reinterpret_cast<const float4 *>(src), reinterpret_cast<float4 *>(dst), n4);
 }
 
 hipError_t launch_synth(const SynthArgs &a, hipStream_t s) {
@@ -1603,8 +1605,7 @@ hipError_t launch_synth(const SynthArgs &a, hipStream_t s) {
     if (n == 0) return hipSuccess;
     size_t blocks = (n + 255) / 256;
     if (blocks > 65536) blocks = 65536;
-    hipLaunchKernelGGL(synth_kernel, dim3((unsigned)blocks), dim3(256), 0, s, a, key, okey);
-    return hipGetLastError();
+    return launch(synth_kernel, dim3((unsigned)blocks), dim3(256), 0, s, a, key, okey);
 }
 
 }  // namespace kore_attn_gpu

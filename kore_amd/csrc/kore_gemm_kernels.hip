@@ -34,6 +34,7 @@
 // bit for bit.  For one device, shape and B the result is deterministic.
 #include "kore_qmv_kernels.h"
 #include "kore_g16_split.h"
+#include "kore_launch.h"
 #include "kore_swiglu.h"
 
 #include <algorithm>
@@ -42,6 +43,8 @@
 #include <mutex>
 
 namespace kore_qmv_gpu {
+
+using kore_gpu::launch;
 namespace {
 
 typedef float floatx4 __attribute__((ext_vector_type(4)));
@@ -998,13 +1001,11 @@ template <int NB, bool Q6>
 hipError_t launch_nb(const GemmArgs &a, hipStream_t s) {
     int occ = 0;
     if (hipError_t e = prepare_nb<NB, Q6>(&occ)) return e;
-    hipLaunchKernelGGL((gemm_kernel<NB, Q6>), dim3(a.workers), dim3(kThreads), lds_bytes(NB), s, a);
-    if (hipError_t e = hipGetLastError()) return e;
+    if (hipError_t e = launch(gemm_kernel<NB, Q6>, dim3(a.workers), dim3(kThreads), lds_bytes(NB), s, a)) return e;
     // every run a whole number of tiles: nothing split
     const int64_t T = (int64_t)a.tiles * a.nblk;
     if (T % a.workers == 0 && (T / a.workers) % a.nblk == 0) return hipSuccess;
-    hipLaunchKernelGGL((gemm_fixup_kernel<NB>), dim3(a.tiles), dim3(kThreads), 0, s, a);
-    return hipGetLastError();
+    return launch(gemm_fixup_kernel<NB>, dim3(a.tiles), dim3(kThreads), 0, s, a);
 }
 
 template <bool Q6>
@@ -1050,24 +1051,19 @@ template <int NT, bool Q6>
 hipError_t launch16_nt(const GemmArgs &a, hipStream_t s) {
     if (!a.presplit) {
         // every activation the units read: 32 per tile of activations, both halves in halves mode
-        hipLaunchKernelGGL(gemm16_prep_kernel, dim3(32 * NT * a.halves), dim3(kPrepThreads), 0, s, a.x, a.x16, a.B,
-                           a.nblk);
-        if (hipError_t e = hipGetLastError()) return e;
+        if (hipError_t e = launch(gemm16_prep_kernel, dim3(32 * NT * a.halves), dim3(kPrepThreads), 0, s, a.x, a.x16, a.B,
+                                  a.nblk))
+            return e;
     }
-    if (NT == 1 && a.halves == 2) hipLaunchKernelGGL((gemm16_kernel<1, Q6, 2>), dim3(a.workers), dim3(kG16Threads), 0, s, a);
-    else hipLaunchKernelGGL((gemm16_kernel<NT, Q6, 1>), dim3(a.workers), dim3(kG16Threads), 0, s, a);
-    if (hipError_t e = hipGetLastError()) return e;
-    if (a.glu) {   // every gate tile: its SwiGLU is written by the pair's fix-up
-        hipLaunchKernelGGL(gemm16_glu_fixup_kernel, dim3(a.m[1].tile0 * a.halves, kG16SlotFloats / 1024),
-                           dim3(kThreads), 0, s, a);
-        return hipGetLastError();
-    }
+    const auto kernel = NT == 1 && a.halves == 2 ? gemm16_kernel<1, Q6, 2> : gemm16_kernel<NT, Q6, 1>;
+    if (hipError_t e = launch(kernel, dim3(a.workers), dim3(kG16Threads), 0, s, a)) return e;
+    if (a.glu)   // every gate tile: its SwiGLU is written by the pair's fix-up
+        return launch(gemm16_glu_fixup_kernel, dim3(a.m[1].tile0 * a.halves, kG16SlotFloats / 1024), dim3(kThreads), 0, s, a);
     const int64_t T = (int64_t)a.tiles * a.halves * a.nblk;
     if (T % a.workers == 0 && (T / a.workers) % a.nblk == 0) return hipSuccess;
     // 16 slices of 1024 partial floats (the slices of a second tile of
     // activations return at once when NT = 1)
-    hipLaunchKernelGGL(gemm16_fixup_kernel, dim3(a.tiles * a.halves, kG16SlotFloats / 1024), dim3(kThreads), 0, s, a);
-    return hipGetLastError();
+    return launch(gemm16_fixup_kernel, dim3(a.tiles * a.halves, kG16SlotFloats / 1024), dim3(kThreads), 0, s, a);
 }
 
 template <bool Q6>

@@ -695,9 +695,9 @@ hipError_t launch_chunk(const TileArgs &d, hipStream_t s) {
     const dim3 grid((unsigned)d.places);
 #define KORE_CHUNK(A, S)                                                        \
     do {                                                                        \
-        if (hdp == 64) return launch(chunk_kernel<A, S, 64>, grid, Shape<A, S, 64>::threads, s, d);     \
-        else if (hdp == 128) return launch(chunk_kernel<A, S, 128>, grid, Shape<A, S, 128>::threads, s, d); \
-        else return launch(chunk_kernel<A, S, 256>, grid, Shape<A, S, 256>::threads, s, d);              \
+        if (hdp == 64) return launch(chunk_kernel<A, S, 64>, grid, Shape<A, S, 64>::threads, 0, s, d);     \
+        else if (hdp == 128) return launch(chunk_kernel<A, S, 128>, grid, Shape<A, S, 128>::threads, 0, s, d); \
+        else return launch(chunk_kernel<A, S, 256>, grid, Shape<A, S, 256>::threads, 0, s, d);              \
     } while (0)
     if (d.a.cache_type == kF32) KORE_CHUNK(float, float);
     else if (d.a.type == kF32 && d.a.cache_type == kF16) KORE_CHUNK(float, half_t);

@@ -612,9 +612,9 @@ hipError_t launch_decode(const TileArgs &d, hipStream_t s) {
     const dim3 grid((unsigned)d.places);
 #define KORE_DECODE(KERNEL, ...)                                                                \
     do {                                                                                        \
-        if (hdp == 64) return launch(KERNEL<__VA_ARGS__ 64, W>, grid, 64 * W, s, d);                    \
-        else if (hdp == 128) return launch(KERNEL<__VA_ARGS__ 128, W>, grid, 64 * W, s, d);             \
-        else if constexpr (W == 4) return launch(KERNEL<__VA_ARGS__ 256, W>, grid, 64 * W, s, d);       \
+        if (hdp == 64) return launch(KERNEL<__VA_ARGS__ 64, W>, grid, 64 * W, 0, s, d);                    \
+        else if (hdp == 128) return launch(KERNEL<__VA_ARGS__ 128, W>, grid, 64 * W, 0, s, d);             \
+        else if constexpr (W == 4) return launch(KERNEL<__VA_ARGS__ 256, W>, grid, 64 * W, 0, s, d);       \
     } while (0)
 #define KORE_COMMA ,
     if (d.a.cache_type == kF32) KORE_DECODE(decode32_kernel);
@@ -693,8 +693,8 @@ hipError_t launch_attend(const AttendArgs &a, hipStream_t s) {
     const dim3 merge((unsigned)joined, (unsigned)std::clamp(8 * a.num_cu / joined, 1, a.hd / 4));
 #define KORE_MERGE(A)                                                                    \
     do {                                                                                 \
-        if (chunk) return launch(merge_kernel<A, kChunkRows>, merge, kThreads, s, d, hdp / 4);   \
-        else return launch(merge_kernel<A, kRows>, merge, kThreads, s, d, hdp / 4);              \
+        if (chunk) return launch(merge_kernel<A, kChunkRows>, merge, kThreads, 0, s, d, hdp / 4);   \
+        else return launch(merge_kernel<A, kRows>, merge, kThreads, 0, s, d, hdp / 4);              \
     } while (0)
     if (a.type == kF32) KORE_MERGE(float);
     else if (a.type == kF16) KORE_MERGE(half_t);

@@ -2,21 +2,15 @@
 // paged-attention kernels.  Internal to libkore_paged.so.
 #pragma once
 
+#include "kore_launch.h"
 #include "kore_paged_kernels.h"
 
 #include <climits>
-#include <type_traits>
 
 namespace kore_paged_gpu {
 namespace {
 
-// Launches kernel(args...) and returns what that launch says: hipGetLastError() would
-// also report an error that another call of the thread has left, and take it away.
-template <class... P>
-inline hipError_t launch(void (*kernel)(P...), dim3 grid, unsigned threads, hipStream_t s, std::type_identity_t<P>... args) {
-    void *at[] = {static_cast<void *>(&args)...};
-    return hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, dim3(threads), at, 0, s);
-}
+using kore_gpu::launch;
 
 typedef _Float16 half_t;
 typedef __bf16 bhalf_t;

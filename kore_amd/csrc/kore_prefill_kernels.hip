@@ -44,11 +44,14 @@
 
 #include "kore_attn_kernels.h"
 #include "kore_attn_device.h"
+#include "kore_launch.h"
 
 #include <algorithm>
 #include <vector>
 
 namespace kore_attn_gpu {
+
+using kore_gpu::launch;
 namespace {
 
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
@@ -1012,12 +1015,10 @@ bool exact(const PrefillArgs &a) { return (a.hd == 64 || a.hd == 128) && a.pos0 
 template <int HDP, bool EXACT>
 hipError_t launch_t(const PrefillArgs &a, hipStream_t s) {
     const dim3 grid(a.n_split > 0 ? a.n_units * a.n_head_kv : a.n_items * a.n_head_kv * a.n_kseg);
-    hipLaunchKernelGGL((prefill_kernel<HDP, EXACT>), grid, dim3(kThreads), 0, s, a);
-    if (a.n_split > 0 || a.n_kseg > 1) {
-        const dim3 cgrid(a.n_head_kv * (a.n_split > 0 ? a.n_split : a.n_items) * 4);
-        hipLaunchKernelGGL((prefill_combine_kernel<HDP, EXACT>), cgrid, dim3(256), 0, s, a);
-    }
-    return hipGetLastError();
+    if (hipError_t e = launch(prefill_kernel<HDP, EXACT>, grid, dim3(kThreads), 0, s, a)) return e;
+    if (a.n_split <= 0 && a.n_kseg <= 1) return hipSuccess;
+    const dim3 cgrid(a.n_head_kv * (a.n_split > 0 ? a.n_split : a.n_items) * 4);
+    return launch(prefill_combine_kernel<HDP, EXACT>, cgrid, dim3(256), 0, s, a);
 }
 
 }  // namespace

@@ -14,6 +14,7 @@
 // be spread over all lanes without changing a single rounding.
 #include "kore_qmv_kernels.h"
 #include "kore_g16_split.h"
+#include "kore_launch.h"
 #include "kore_swiglu.h"
 
 #include <algorithm>
@@ -22,6 +23,8 @@
 #include <type_traits>
 
 namespace kore_qmv_gpu {
+
+using kore_gpu::launch;
 namespace {
 
 constexpr int kThreads = 256;
@@ -891,9 +894,8 @@ hipError_t launch_group_r(const GroupArgs &a, int grid, int num_cu, hipStream_t 
         return e ? atoi(e) : -1;
     }();
     const int pipe = forced >= 0 ? forced : (num_cu > 0 && grid > 4 * num_cu ? 0 : 1);
-    if (pipe == 0) hipLaunchKernelGGL((matvec_group_kernel<AVX2, RW, FUSED, 2, 0>), dim3(grid), dim3(kThreads), lds, s, a);
-    else hipLaunchKernelGGL((matvec_group_kernel<AVX2, RW, FUSED, 1, 1>), dim3(grid), dim3(kThreads), lds, s, a);
-    return hipGetLastError();
+    const auto kernel = pipe == 0 ? matvec_group_kernel<AVX2, RW, FUSED, 2, 0> : matvec_group_kernel<AVX2, RW, FUSED, 1, 1>;
+    return launch(kernel, dim3(grid), dim3(kThreads), lds, s, a);
 }
 
 template <bool AVX2, bool FUSED>
@@ -968,14 +970,12 @@ hipError_t launch_quantize_q8k(const float *x, int64_t n, uint8_t *xq, bool imag
     if (pre.norm_w && n > INT32_MAX) return hipErrorInvalidValue;
     if (pre.up) {
         if (nb > INT32_MAX) return hipErrorInvalidValue;
-        if (image) hipLaunchKernelGGL(swiglu_quantize_kernel<true>, dim3((unsigned)nb), dim3(kThreads), 0, s, x, pre.up, xq, nb);
-        else hipLaunchKernelGGL(swiglu_quantize_kernel<false>, dim3((unsigned)nb), dim3(kThreads), 0, s, x, pre.up, xq, nb);
-        return hipGetLastError();
+        return launch(image ? swiglu_quantize_kernel<true> : swiglu_quantize_kernel<false>, dim3((unsigned)nb), dim3(kThreads), 0,
+                      s, x, pre.up, xq, nb);
     }
     const int64_t grid = (nb + kThreads / 16 - 1) / (kThreads / 16);
-    if (image) hipLaunchKernelGGL(quantize_q8k_kernel<true>, dim3((unsigned)grid), dim3(kThreads), 0, s, x, xq, nb, pre);
-    else hipLaunchKernelGGL(quantize_q8k_kernel<false>, dim3((unsigned)grid), dim3(kThreads), 0, s, x, xq, nb, pre);
-    return hipGetLastError();
+    return launch(image ? quantize_q8k_kernel<true> : quantize_q8k_kernel<false>, dim3((unsigned)grid), dim3(kThreads), 0, s, x, xq,
+                  nb, pre);
 }
 
 hipError_t launch_synth_blocks(int type, int64_t nblocks, uint64_t seed, uint8_t *dst, hipStream_t s) {
@@ -983,17 +983,15 @@ hipError_t launch_synth_blocks(int type, int64_t nblocks, uint64_t seed, uint8_t
     const int wpb = (type == kQ4K ? kQ4Bytes : kQ6Bytes) / 2;
     const int64_t n16 = nblocks * wpb;
     const int64_t grid = (n16 + kThreads - 1) / kThreads;
-    hipLaunchKernelGGL(synth_blocks_kernel, dim3((unsigned)grid), dim3(kThreads), 0, s, (uint16_t *)dst, n16, wpb,
-                       type == kQ4K ? 0 : 104, type == kQ4K ? 1 : -1, splitmix64_host(seed));
-    return hipGetLastError();
+    return launch(synth_blocks_kernel, dim3((unsigned)grid), dim3(kThreads), 0, s, (uint16_t *)dst, n16, wpb,
+                  type == kQ4K ? 0 : 104, type == kQ4K ? 1 : -1, splitmix64_host(seed));
 }
 
 hipError_t launch_q6k_split(const uint8_t *raw, int64_t nblocks, uint8_t *body, uint16_t *d, hipStream_t s) {
     if (nblocks <= 0) return hipSuccess;
     const int64_t grid = (nblocks * 53 + kThreads - 1) / kThreads;
-    hipLaunchKernelGGL(q6k_split_kernel, dim3((unsigned)grid), dim3(kThreads), 0, s, (const uint16_t *)raw,
-                       nblocks, (uint32_t *)body, d);
-    return hipGetLastError();
+    return launch(q6k_split_kernel, dim3((unsigned)grid), dim3(kThreads), 0, s, (const uint16_t *)raw, nblocks, (uint32_t *)body,
+                  d);
 }
 
 }  // namespace kore_qmv_gpu
@@ -1113,14 +1111,12 @@ hipError_t launch_rmsnorm_rows(const float *x, const float *w, int n, int n_rows
     if (x16 && (n % 256 || n > 16 * kThreads || n_rows > kGemmMaxB ||
                 (((uintptr_t)x | (uintptr_t)w | (uintptr_t)out | (uintptr_t)x16) & 15)))
         return hipErrorInvalidValue;
-    hipLaunchKernelGGL(rmsnorm_rows_kernel, dim3((unsigned)n_rows), dim3(kThreads), 0, s, x, w, n, eps, out, x16);
-    return hipGetLastError();
+    return launch(rmsnorm_rows_kernel, dim3((unsigned)n_rows), dim3(kThreads), 0, s, x, w, n, eps, out, x16);
 }
 
 hipError_t launch_swiglu(float *g, const float *u, int64_t n, hipStream_t s) {
     if (n <= 0 || !g || !u) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(swiglu_kernel, dim3((unsigned)((n + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, g, u, n);
-    return hipGetLastError();
+    return launch(swiglu_kernel, dim3((unsigned)((n + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, g, u, n);
 }
 
 }  // namespace kore_qmv_gpu
@@ -1191,9 +1187,8 @@ hipError_t launch_get_rows(int type, const uint8_t *data, const int64_t *rows, i
         if (rows[z] < 0) return hipErrorInvalidValue;
         list.row[z] = rows[z];
     }
-    hipLaunchKernelGGL(get_rows_kernel, dim3((unsigned)((n + kThreads - 1) / kThreads), n_rows), dim3(kThreads), 0, s,
-                       type, data, n / per * bytes, n, out, list);
-    return hipGetLastError();
+    return launch(get_rows_kernel, dim3((unsigned)((n + kThreads - 1) / kThreads), n_rows), dim3(kThreads), 0, s, type, data,
+                  n / per * bytes, n, out, list);
 }
 
 }  // namespace kore_qmv_gpu

@@ -230,10 +230,10 @@ hipError_t launch_rope(const RopeArgs &a, hipStream_t s) {
     const dim3 grid = row_grid(a.n_tok, a.hd / (v4 ? 8 : 2) * a.n_head);
 #define KORE_ROPE_CASE(T)                                                                         \
     do {                                                                                          \
-        if (v4 && a.turn.interleaved) return launch(rope_kernel<T, 4, true>, grid, kThreads, s, a);       \
-        else if (v4) return launch(rope_kernel<T, 4, false>, grid, kThreads, s, a);                       \
-        else if (a.turn.interleaved) return launch(rope_kernel<T, 1, true>, grid, kThreads, s, a);        \
-        else return launch(rope_kernel<T, 1, false>, grid, kThreads, s, a);                               \
+        if (v4 && a.turn.interleaved) return launch(rope_kernel<T, 4, true>, grid, kThreads, 0, s, a);       \
+        else if (v4) return launch(rope_kernel<T, 4, false>, grid, kThreads, 0, s, a);                       \
+        else if (a.turn.interleaved) return launch(rope_kernel<T, 1, true>, grid, kThreads, 0, s, a);        \
+        else return launch(rope_kernel<T, 1, false>, grid, kThreads, 0, s, a);                               \
     } while (0)
     if (a.type == kF32) KORE_ROPE_CASE(float);
     else if (a.type == kF16) KORE_ROPE_CASE(half_t);
@@ -249,10 +249,10 @@ hipError_t launch_append(const AppendArgs &a, hipStream_t s) {
     const dim3 grid = row_grid(a.b.n_tok, a.hd / (v4 ? 8 : 2) * ((a.q ? a.n_head : 0) + 2 * a.n_head_kv));
 #define KORE_APPEND_CASE(T, C)                                                                    \
     do {                                                                                          \
-        if (v4 && a.turn.interleaved) return launch(append_kernel<T, C, 4, true>, grid, kThreads, s, a);  \
-        else if (v4) return launch(append_kernel<T, C, 4, false>, grid, kThreads, s, a);                  \
-        else if (a.turn.interleaved) return launch(append_kernel<T, C, 1, true>, grid, kThreads, s, a);   \
-        else return launch(append_kernel<T, C, 1, false>, grid, kThreads, s, a);                          \
+        if (v4 && a.turn.interleaved) return launch(append_kernel<T, C, 4, true>, grid, kThreads, 0, s, a);  \
+        else if (v4) return launch(append_kernel<T, C, 4, false>, grid, kThreads, 0, s, a);                  \
+        else if (a.turn.interleaved) return launch(append_kernel<T, C, 1, true>, grid, kThreads, 0, s, a);   \
+        else return launch(append_kernel<T, C, 1, false>, grid, kThreads, 0, s, a);                          \
     } while (0)
     if (a.type == kF32 && a.cache_type == kF32) KORE_APPEND_CASE(float, float);
     else if (a.type == kF32 && a.cache_type == kF16) KORE_APPEND_CASE(float, half_t);

@@ -101,3 +101,43 @@ def test_rotated_q_in_the_place_of_k_or_v():
         call(q=c.ptr("q"), qs=E, q_out=c.ptr("out"), qo=E)      # apart
         kv.sync()
     assert torch.equal(wide[:, E:], before[:, E:]) and not torch.equal(wide[:, :E], before[:, :E])
+
+
+def test_a_layers_step_after_an_error_of_another_call():
+    """As above for the layer's steps over either cache, and the attention, matvec and matmul calls that they are made of."""
+    from kore_amd import KoreAttn, hip, paged, qmv, rope
+    from kore_amd.layer import Layer
+    from tests.test_gpu_layer_paged import E, FF, HD, KVD, NH, NKV, _weights
+    L = hip.lib()
+    L.hipPeekAtLastError.restype = L.hipGetLastError.restype = C.c_int
+    n, w = 5, _weights(1)[0]
+    x = torch.randn(n, E, device="cuda")
+    q, k, v, out = (torch.randn(n, c, device="cuda") for c in (E, KVD, KVD, E))
+    p = {m: t.data_ptr() for m, t in (("x", x), ("q", q), ("k", k), ("v", v), ("out", out))}
+    starts, lens, pages = (torch.tensor(t, dtype=torch.int32, device="cuda") for t in ([0, n], [n], [0]))
+    torch.cuda.synchronize()
+    try:
+        with paged.PagedKV(1, 2, 16, NH, NKV, HD, "f32", rope.Config(HD)) as kv, Layer(E, FF, NH, NKV, 1e-6) as layer, \
+                KoreAttn(1, 32, NH, NKV, HD, 1e6) as a, KoreAttn(1, 32, 6, 3, 36, 1e6) as generic:
+            b = paged.Batch(1, n, starts.data_ptr(), lens.data_ptr(), pages.data_ptr(), 1, n)
+            calls = [lambda: layer.paged_dev(w, kv, 0, b, p["x"]),
+                     lambda: layer.prefill_dev(w, a, 0, 0, n, p["x"]),
+                     lambda: layer.decode_dev(w, a, 0, n, p["x"]),
+                     lambda: a.prefill_dev(0, 0, n, p["q"], p["k"], p["v"], p["out"]),
+                     lambda: a.append_dev(0, n, 1, p["k"], p["v"]),
+                     lambda: a.decode_dev(0, n, p["q"], p["k"], p["v"], p["out"]),
+                     lambda: generic.decode_dev(0, 0, p["q"], p["k"], p["v"], p["out"]),
+                     lambda: qmv.rmsnorm_rows_dev(p["x"], w.bufs["attn_norm"].ptr, E, n, 1e-6, p["out"]),
+                     lambda: w.mats[0].mv_dev(p["x"], p["out"]),
+                     lambda: w.mats[0].matmul_batch_dev(p["x"], n, p["out"])]
+            for i, call in enumerate(calls):
+                assert L.hipSetDevice(1 << 20) != 0      # no such device
+                left = L.hipPeekAtLastError()
+                try:
+                    call()
+                    assert L.hipPeekAtLastError() == left, i
+                finally:
+                    L.hipGetLastError()
+            torch.cuda.synchronize()
+    finally:
+        w.close()
