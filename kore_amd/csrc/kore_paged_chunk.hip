@@ -516,12 +516,13 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
                 // (2048 fp16 rows of 28/4/128: 50.2 us with every reference under 2^11, 51.9 with every one over it.)
                 if constexpr (PP == 1) {
                     const float base = ref == kNone ? 0.f : ref;
-                    far = __any(fabsf(base * s2) >= 0x1p11f);
-                    if (far) {
+                    far = fabsf(base * s2) >= 0x1p11f;
+                    if (__any(far)) {
+                        const float off = far ? base : 0.f;   // (a row's bits are not its neighbours' business)
 #pragma unroll
                         for (int m = 0; m < MT; ++m)
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) s[m][i] -= base;
+                            for (int i = 0; i < 16; ++i) s[m][i] -= off;
                     }
                 }
             }

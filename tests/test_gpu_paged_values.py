@@ -177,6 +177,26 @@ def test_an_infinity_at_the_other_end_of_the_scores(dtype, cache, max_q):
             assert (np.abs(row - want) <= e).all()
 
 
+@pytest.mark.parametrize("dtype,cache", PAIRS)
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("max_q", [1, 64])
+def test_other_rows_do_not_notice_a_q_that_is_not_finite(dtype, cache, bad, max_q):
+    """A row, a head and a single value of q are not finite: the others' bits are those of a finite q."""
+    c = Case([(30, 200), (1, 2500), (2, 40)], 6, 2, 64, 16, dtype, cache, seed=11).up()
+    with c.handle() as kv:
+        c.attend(kv, max_q=max_q)
+        want = c.rows("out", 6)[0].clone()
+        odd = torch.zeros(c.n_tok, 6, dtype=torch.bool)
+        odd[4], odd[11, 2], odd[31, 5], odd[20, 0] = True, True, True, True
+        c.q[4], c.q[11, 2], c.q[31, 5] = bad, bad, bad
+        c.q[20, 0, 17] = bad
+        c.d["q"].copy_(c.wide(c.q))
+        torch.cuda.synchronize()
+        c.attend(kv, max_q=max_q)
+    got = c.rows("out", 6)[0]
+    assert torch.equal(got[~odd].view(torch.uint8), want[~odd].view(torch.uint8))
+
+
 # ---- units of q and K ----------------------------------------------------------------
 
 @pytest.mark.parametrize("cache", ["f32", "f16", "bf16"])
