@@ -11,7 +11,7 @@
 // workgroups of four took 56 where this took 51, an earlier pair of variants).
 //
 // us, and TFLOP/s of products made (a large bf16 product: 1154 to 1207): 2048 fp16 rows of
-// 28/4/128 50 to 60 over boxes, 500 to 600; 512 fp32 rows over 32749 bf16 keys, three
+// 28/4/128 50 to 60 over several cards, 500 to 600; 512 fp32 rows over 32749 bf16 keys, three
 // products each, 589 to 656, 1090 to 1210; 2048 fp32 rows over an fp32 cache, three and
 // six, 154 to 180, 750 to 880.  The rest is vector instructions (weights, parts), which
 // matrix instructions of another wave hardly overlap, a workgroup's start, and waits at
