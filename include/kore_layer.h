@@ -97,6 +97,24 @@ KORE_LAYER_API int kore_layer_prefill_dev(kore_layer_t L, const kore_layer_weigh
 KORE_LAYER_API int kore_layer_paged_dev(kore_layer_t L, const kore_layer_weights *w, kore_paged_t kv, int layer,
                                         const kore_paged_batch *b, float *x, void *workspace, void *stream);
 
+/* What a step of drafted tokens, or a model that normalises its heads, has beside a
+ * batch: the rows' positions and slots as kore_paged_plan_dev leaves them, norms of
+ * q's and k's heads (with the layer's rms_eps), a tree, a window. */
+typedef struct kore_layer_paged_opts {
+    const int *pos;                  /* device [n_tok] */
+    const int64_t *slot;             /* device [n_tok], aligned to 8 bytes */
+    const float *q_norm, *k_norm;    /* device, head_dim weights each, or NULL */
+    const kore_paged_tree *tree;     /* NULL: each row attends up to its own position */
+    int window;                      /* 0: none */
+} kore_layer_paged_opts;
+
+/* kore_layer_paged_dev with the rows stored by their slots (kore_paged_append_rows_dev)
+ * and, with a tree, attended by it (kore_paged_attend_tree_dev).  Rows whose position
+ * is negative hold nothing of use afterwards. */
+KORE_LAYER_API int kore_layer_paged_ex_dev(kore_layer_t L, const kore_layer_weights *w, kore_paged_t kv, int layer,
+                                           const kore_paged_batch *b, const kore_layer_paged_opts *o, float *x,
+                                           void *workspace, void *stream);
+
 /* Wait for the layer's own stream. */
 KORE_LAYER_API int kore_layer_sync(kore_layer_t L);
 

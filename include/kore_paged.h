@@ -123,6 +123,113 @@ KORE_PAGED_API int kore_paged_attend_dev(kore_paged_t h, int layer, const kore_p
                                          int64_t q_stride, void *out, int64_t out_stride, float scale, int window,
                                          void *workspace, void *stream);
 
+/* ---- steps of drafted tokens -------------------------------------------------
+ *
+ * A server that drafts lets a sequence's new rows be a tree: several guesses at the
+ * next tokens, checked at once.  The calls below make a step's tables on the
+ * device (plan), store its rows by them (append_rows, with the norms of models that
+ * have them), attend the tree (attend_tree) and keep its accepted path (keep), so
+ * that a step needs nothing of the host but the drafted tokens and can be captured:
+ *     plan (held -> kv_len) ... layers ... keep (kv_len -> held). */
+
+/* What a step's tables are made of: the requests, and the pages that are free.
+ * All arrays are device memory, ints aligned to 4 bytes, slot and mask to 8. */
+typedef struct kore_paged_plan {
+    int n_seq, n_tok;            /* sequences; rows that the step's buffers hold */
+    const int *n_new;            /* [n_seq] new rows of each sequence, 0 or more */
+    const int *kv_held;          /* [n_seq] positions that each holds */
+    int *kv_len;                 /* [n_seq] out: with the new rows (may be kv_held) */
+    int *pages;                  /* [n_seq][pages_stride]: entries that the new rows need are added */
+    int pages_stride;
+    const int *free_pages;       /* [n_pages]: the first n_free[0] are free, the last of them taken first */
+    const int *n_free;           /* [1] */
+    int *n_free_out;             /* [1] out: less those taken (may be n_free) */
+    const int *parent;           /* [n_tok], or NULL: rows one behind the other.  Entry of a sequence's i-th new row: the
+                                    row, 0 .. i - 1 of the same, that it follows, or -1 (what is held; so is any other) */
+    int *q_start;                /* [n_seq + 1] out: the batch's */
+    int *pos;                    /* [n_tok] out: each row's position, kv_held and its depth in the tree; -1: no row */
+    int64_t *slot;               /* [n_tok] out: where it is stored, page * page_size + slot of it; -1: nowhere */
+    uint64_t *mask;              /* [n_tok][mask_words] out with parent, else NULL: bit j % 64 of word j / 64 is set where
+                                    the j-th new row of the sequence is the row itself or before it in the tree */
+    int mask_words;              /* 1 .. 16 with parent, else 0 */
+    int *status;                 /* [1] out */
+} kore_paged_plan;
+
+/* Makes the step's tables.  Sequence s gets rows q_start[s] .. and, where they pass
+ * the pages that it holds, new ones: the pages of all sequences, one after the
+ * other, are taken from the end of the free ones.  The i-th new row lies at position
+ * kv_held + i of the sequence's pages, whatever its depth.
+ * status 0: done.  Over 0: so many pages are missing; -1: a request is malformed (a
+ * negative number, more positions than the table's row, more rows than n_tok or
+ * than the mask's bits, an n_free outside 0 .. n_pages).  Then nothing is taken:
+ * kv_len is kv_held, n_free_out is n_free, pages are as they were, and q_start, pos,
+ * slot and mask are those of a step without rows, which the other calls take.
+ * A page that the table names is taken to be the sequence's own behind its full
+ * ones: rows go into the last, where it has room.  At most 2^16 sequences and 2^23
+ * rows.  But for the pairs named above no two arrays overlap.  Pointers on the
+ * handle's device; stream as in the append. */
+KORE_PAGED_API int kore_paged_plan_dev(kore_paged_t h, const kore_paged_plan *p, void *stream);
+
+/* Rows as a plan leaves them, and the norms of their heads. */
+typedef struct kore_paged_rows {
+    int n_tok;
+    const int *pos;              /* device [n_tok]: turned to this position; negative: the row is left as it is */
+    const int64_t *slot;         /* device [n_tok]: page * page_size + slot; outside the pool: not stored */
+    const float *q_norm, *k_norm;/* device, head_dim weights each, or NULL: that one is turned only */
+    float norm_eps;              /* over 0 where there is a norm */
+} kore_paged_rows;
+
+/* kore_paged_append_dev by the rows' own positions and slots: q and k normalised
+ * as by kore_rope_norm_dev, turned, rounded and stored (q into q_out), v rounded
+ * and stored.  No two rows have the same slot.  Everything else as there. */
+KORE_PAGED_API int kore_paged_append_rows_dev(kore_paged_t h, int layer, const kore_paged_rows *r, int type, const void *k,
+                                              int64_t k_stride, const void *v, int64_t v_stride, const void *q,
+                                              int64_t q_stride, void *q_out, int64_t q_out_stride, void *stream);
+
+/* Which of its sequence's new rows a row attends. */
+typedef struct kore_paged_tree {
+    const uint64_t *mask;        /* device [n_tok][mask_words], aligned to 8 bytes: bit j % 64 of word j / 64 of a row is
+                                    the j-th new row of its sequence */
+    int mask_words;              /* 1 .. 16; new rows past the mask's bits are not attended */
+    const int *pos;              /* device [n_tok] positions of the rows; NULL allowed without a window */
+} kore_paged_tree;
+
+/* kore_paged_attend_dev for new rows that are a tree, or any set: a row of a
+ * sequence with n of them attends the kv_len - n positions before them, in a
+ * window w those over pos - w alone (pos is taken within kv_len - n .. kv_len - 1),
+ * and of the new ones those that its mask names, itself only if it does; the
+ * window does not touch these.  Everything else as there. */
+KORE_PAGED_API int kore_paged_attend_tree_dev(kore_paged_t h, int layer, const kore_paged_batch *b, const kore_paged_tree *t,
+                                              int type, const void *q, int64_t q_stride, void *out, int64_t out_stride,
+                                              float scale, int window, void *workspace, void *stream);
+
+/* What is kept of a step's rows.  Device memory, ints aligned to 4 bytes. */
+typedef struct kore_paged_keep {
+    int n_seq, n_tok;
+    const int *q_start;          /* [n_seq + 1] of the step */
+    const int *n_keep;           /* [n_seq]: so many of the sequence's n new rows (over n: all); negative: the sequence ends */
+    const int *rows;             /* [n_tok]: entries from q_start[s] on, ascending: which of them, 0 .. n - 1; or NULL: the
+                                    first ones */
+    const int *kv_len;           /* [n_seq], with the step's rows */
+    int *kv_out;                 /* [n_seq] out: with those kept (may be kv_len); 0 for a sequence that ends */
+    const int *pages;            /* [n_seq][pages_stride] */
+    int pages_stride;
+    int *free_pages;             /* [n_pages], with n_free and n_free_out; or all NULL: no page is given back */
+    const int *n_free;           /* [1] */
+    int *n_free_out;             /* [1] out (may be n_free) */
+} kore_paged_keep;
+
+/* Moves the kept rows' K and V in every layer so that the i-th lies behind what the
+ * sequence held before the step and the i - 1 before it, and gives the pages that no
+ * position needs any more back: each sequence's, in the table's order, to the end
+ * of the free ones.  The table keeps its entries.  Entries of it that are no page are
+ * not given back, nor pages past n_pages free ones.  A sequence that ends gives all
+ * its pages back (so it must share none).  Entries of `rows` outside 0 .. n - 1 move
+ * nothing; entries that do not ascend leave nothing of use in the rows kept.  At most
+ * 2^16 sequences.  But for the pairs named above no two arrays overlap.  Pointers on
+ * the handle's device; stream as in the append. */
+KORE_PAGED_API int kore_paged_keep_dev(kore_paged_t h, const kore_paged_keep *k, void *stream);
+
 /* Bytes of an attention workspace of this handle, for any batch. */
 KORE_PAGED_API size_t kore_paged_workspace_bytes(kore_paged_t h);
 

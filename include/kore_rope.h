@@ -89,6 +89,28 @@ KORE_PAGED_API int kore_rope_apply_dev(kore_rope_t r, int type, int n_tok, int n
                                        int64_t x_stride, const int *pos, void *out, int64_t out_stride,
                                        int transpose, void *stream);
 
+/* Heads of rows that are normalised and turned in one pass (models that take the
+ * root mean square off the heads of q and k before the rotation). */
+typedef struct kore_rope_heads {
+    const void *x;              /* [n_tok] rows of n_head heads */
+    void *out;                  /* likewise; may be x itself with the same stride */
+    int64_t x_stride, out_stride;
+    int n_head;
+    const float *norm;          /* device, head_dim weights, or NULL: turned only */
+} kore_rope_heads;
+
+/* n_sets (1 or 2: q's heads, q's and k's) of n_tok rows, in one launch: each head
+ * is first x w / sqrt(mean(x^2) + eps), then turned as by kore_rope_apply_dev.
+ * The sum of squares and the root are in double, 1 / root is rounded to float, and
+ * so is either product; then as there, so that each value is rounded to its type
+ * once.  (kore's rmsnorm, kore.cpp:1367-1372, head by head, but for the root's
+ * rounding.)  eps over 0.  Sizes, strides, alignment and stream as there; norm
+ * aligned to a float.  A row whose position is negative is left as it is.  The
+ * rows of a set overlap no other's.  A head with values that are not finite holds
+ * nothing of use; no other notices. */
+KORE_PAGED_API int kore_rope_norm_dev(kore_rope_t r, int type, int n_tok, int head_dim, const kore_rope_heads *sets,
+                                      int n_sets, const int *pos, float eps, void *stream);
+
 /* The plan's rot_dim / 2 frequencies (host copy) and m. */
 KORE_PAGED_API int kore_rope_get_freqs(kore_rope_t r, float *freqs, float *magnitude);
 

@@ -5,6 +5,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <cmath>
 #include <new>
 #include <string>
 
@@ -238,9 +239,13 @@ KORE_LAYER_API int kore_layer_prefill_dev(kore_layer_t L, const kore_layer_weigh
     });
 }
 
-KORE_LAYER_API int kore_layer_paged_dev(kore_layer_t L, const kore_layer_weights *w, kore_paged_t kv, int layer,
-                                        const kore_paged_batch *b, float *x, void *workspace, void *stream) {
-    if (!L) return fail(nullptr, KORE_LAYER_E_INVALID, "layer handle is NULL");
+extern "C++" {
+namespace {
+
+// What the paged steps check before anything is launched: all that the append and the attention would refuse (what
+// else the append refuses leaves x and the cache as they were).
+int check_paged(kore_layer *L, const kore_layer_weights *w, kore_paged_t kv, int layer, const kore_paged_batch *b, const float *x,
+                const void *workspace) {
     if (!w || !kv || !b || !x || ((uintptr_t)x & 15))
         return fail(L, KORE_LAYER_E_INVALID, "w, kv, batch or x missing or x unaligned");
     if (int rc = check_weights(L, w)) return rc;
@@ -251,10 +256,22 @@ KORE_LAYER_API int kore_layer_paged_dev(kore_layer_t L, const kore_layer_weights
     if (pi.device != L->device) return fail(L, KORE_LAYER_E_INVALID, "the paged cache and the layer are on different devices");
     if (b->n_tok < 1 || b->n_tok > kMaxBatch || b->n_seq < 1)
         return fail(L, KORE_LAYER_E_INVALID, "n_tok must be 1..64 (kore's KORE_BMAX), of one sequence or more");
-    // before anything is launched: what the append and the attention would refuse (what else the append refuses
-    // leaves x and the cache as they were)
     if (layer < 0 || layer >= pi.config.n_layer || !b->q_start || !b->kv_len || !b->pages || ((uintptr_t)workspace & 15))
         return fail(L, KORE_LAYER_E_INVALID, "layer outside the cache, a batch array missing or the workspace unaligned");
+    return KORE_LAYER_OK;
+}
+
+int paged_error(kore_layer *L, kore_paged_t kv) {
+    return fail(L, KORE_LAYER_E_STEP, std::string("paged attention: ") + kore_paged_last_error(kv));
+}
+
+}  // namespace
+}  // extern "C++"
+
+KORE_LAYER_API int kore_layer_paged_dev(kore_layer_t L, const kore_layer_weights *w, kore_paged_t kv, int layer,
+                                        const kore_paged_batch *b, float *x, void *workspace, void *stream) {
+    if (!L) return fail(nullptr, KORE_LAYER_E_INVALID, "layer handle is NULL");
+    if (int rc = check_paged(L, w, kv, layer, b, x, workspace)) return rc;
     void *s = stream ? stream : (void *)L->stream;
     const int64_t E = L->E, kvd = L->kvd;
     return rows_step(L, w, b->n_tok, x, s, [&] {
@@ -262,8 +279,39 @@ KORE_LAYER_API int kore_layer_paged_dev(kore_layer_t L, const kore_layer_weights
                 KORE_PAGED_OK ||
             kore_paged_attend_dev(kv, layer, b, KORE_PAGED_F32, L->bq, E, L->batt, E, 0.0f, 0, workspace, s) !=
                 KORE_PAGED_OK)
-            return fail(L, KORE_LAYER_E_STEP, std::string("paged attention: ") + kore_paged_last_error(kv));
+            return paged_error(L, kv);
         return KORE_LAYER_OK;
+    });
+}
+
+KORE_LAYER_API int kore_layer_paged_ex_dev(kore_layer_t L, const kore_layer_weights *w, kore_paged_t kv, int layer,
+                                           const kore_paged_batch *b, const kore_layer_paged_opts *o, float *x,
+                                           void *workspace, void *stream) {
+    if (!L) return fail(nullptr, KORE_LAYER_E_INVALID, "layer handle is NULL");
+    if (int rc = check_paged(L, w, kv, layer, b, x, workspace)) return rc;
+    if (!o || !o->pos || !o->slot || ((uintptr_t)o->pos & 3) || ((uintptr_t)o->slot & 7))
+        return fail(L, KORE_LAYER_E_INVALID, "opts, pos or slot missing or unaligned");
+    if (((uintptr_t)o->q_norm & 3) || ((uintptr_t)o->k_norm & 3))
+        return fail(L, KORE_LAYER_E_INVALID, "q_norm or k_norm unaligned");
+    if ((o->q_norm || o->k_norm) && !(L->eps > 0 && std::isfinite(L->eps)))
+        return fail(L, KORE_LAYER_E_INVALID, "norms of heads need a layer whose rms_eps is positive");
+    if (o->window < 0) return fail(L, KORE_LAYER_E_INVALID, "negative window");
+    if (const kore_paged_tree *t = o->tree)
+        if (!t->mask || ((uintptr_t)t->mask & 7) || t->mask_words < 1 || t->mask_words > 16 || ((uintptr_t)t->pos & 3) ||
+            (o->window && !t->pos))
+            return fail(L, KORE_LAYER_E_INVALID, "the tree's mask or pos missing or unaligned, or mask_words outside 1..16");
+    void *s = stream ? stream : (void *)L->stream;
+    const int64_t E = L->E, kvd = L->kvd;
+    const kore_paged_rows rows{b->n_tok, o->pos, o->slot, o->q_norm, o->k_norm, L->eps};
+    return rows_step(L, w, b->n_tok, x, s, [&] {
+        if (kore_paged_append_rows_dev(kv, layer, &rows, KORE_PAGED_F32, L->bk, kvd, L->bv, kvd, L->bq, E, L->bq, E, s) !=
+            KORE_PAGED_OK)
+            return paged_error(L, kv);
+        const int rc = o->tree ? kore_paged_attend_tree_dev(kv, layer, b, o->tree, KORE_PAGED_F32, L->bq, E, L->batt, E, 0.0f,
+                                                            o->window, workspace, s)
+                               : kore_paged_attend_dev(kv, layer, b, KORE_PAGED_F32, L->bq, E, L->batt, E, 0.0f, o->window,
+                                                       workspace, s);
+        return rc == KORE_PAGED_OK ? KORE_LAYER_OK : paged_error(L, kv);
     });
 }
 

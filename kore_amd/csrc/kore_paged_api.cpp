@@ -231,26 +231,79 @@ int check_overlap(H *h, const void *x, int64_t xs, const void *y, int64_t ys, in
     return check_apart(h, "input and output", x, xs, n, y, ys, n, n_tok, type);
 }
 
-int check_batch(kore_paged *h, int layer, const kore_paged_batch *b, int type) {
-    if (!b) return fail(h, KORE_PAGED_E_INVALID, "null batch");
+// The limits of a row of heads that is turned.
+int check_heads(kore_rope *r, int n_tok, int n_head, int head_dim) {
+    if (n_tok < 0 || n_head <= 0) return fail(r, KORE_PAGED_E_INVALID, "bad n_tok %d or n_head %d", n_tok, n_head);
+    if (head_dim < r->cfg.rot_dim || head_dim % 2 != 0)
+        return fail(r, KORE_PAGED_E_INVALID, "head_dim %d is odd or under rot_dim %d", head_dim, r->cfg.rot_dim);
+    if (n_tok > kMaxRows) return fail(r, KORE_PAGED_E_UNSUPPORTED, "n_tok %d is over %d", n_tok, kMaxRows);
+    if (head_dim > kMaxRopeHeadDim)
+        return fail(r, KORE_PAGED_E_UNSUPPORTED, "head_dim %d over %d", head_dim, kMaxRopeHeadDim);
+    if ((int64_t)n_head * head_dim > 1 << 24)
+        return fail(r, KORE_PAGED_E_UNSUPPORTED, "%d heads of %d are too large a row", n_head, head_dim);
+    return KORE_PAGED_OK;
+}
+
+// Arrays of a step's tables: there, and aligned to their elements.
+template <class H>
+int check_array(H *h, const char *what, const void *p, size_t size) {
+    if (!p) return fail(h, KORE_PAGED_E_INVALID, "null %s", what);
+    if ((uintptr_t)p % size) return fail(h, KORE_PAGED_E_INVALID, "%s is not aligned to %zu bytes", what, size);
+    return KORE_PAGED_OK;
+}
+
+int check_layer(kore_paged *h, int layer, int type) {
     if (layer < 0 || layer >= h->cfg.n_layer)
         return fail(h, KORE_PAGED_E_INVALID, "layer %d outside [0, %d)", layer, h->cfg.n_layer);
     if (!type_ok(type)) return fail(h, KORE_PAGED_E_INVALID, "unknown type %d", type);
     if (type != KORE_PAGED_F32 && type != h->cfg.cache_type)
         return fail(h, KORE_PAGED_E_INVALID, "rows of type %d with a cache of type %d (rows are fp32 or of the cache's type)",
                     type, h->cfg.cache_type);
+    return KORE_PAGED_OK;
+}
+
+int check_table(kore_paged *h, int n_seq, int pages_stride) {
+    if (pages_stride <= 0 || pages_stride > kMaxKeys / h->cfg.page_size)
+        return fail(h, KORE_PAGED_E_INVALID, "pages_stride %d outside 1..%d", pages_stride, kMaxKeys / h->cfg.page_size);
+    if (n_seq > kMaxSeq)
+        return fail(h, KORE_PAGED_E_UNSUPPORTED, "n_seq %d is too large (over %d)", n_seq, kMaxSeq);
+    return KORE_PAGED_OK;
+}
+
+bool eps_ok(float eps) { return eps > 0 && std::isfinite(eps); }
+
+int check_batch(kore_paged *h, int layer, const kore_paged_batch *b, int type) {
+    if (!b) return fail(h, KORE_PAGED_E_INVALID, "null batch");
+    if (int rc = check_layer(h, layer, type)) return rc;
     if (b->n_seq < 0 || b->n_tok < 0 || b->max_q < 0)
         return fail(h, KORE_PAGED_E_INVALID, "negative n_seq, n_tok or max_q");
     if (b->n_seq == 0 || b->n_tok == 0) return KORE_PAGED_OK;
     if (!b->q_start || !b->kv_len || !b->pages) return fail(h, KORE_PAGED_E_INVALID, "null q_start, kv_len or pages");
-    if (b->pages_stride <= 0 || b->pages_stride > kMaxKeys / h->cfg.page_size)
-        return fail(h, KORE_PAGED_E_INVALID, "pages_stride %d outside 1..%d", b->pages_stride, kMaxKeys / h->cfg.page_size);
-    if (b->n_seq > kMaxSeq)
-        return fail(h, KORE_PAGED_E_UNSUPPORTED, "n_seq %d is too large (over %d)", b->n_seq, kMaxSeq);
+    if (int rc = check_table(h, b->n_seq, b->pages_stride)) return rc;
     if (b->n_tok > kMaxRows || (int64_t)b->n_tok * h->cfg.n_head > kMaxRowHeads ||
         (int64_t)b->n_seq * h->cfg.n_head_kv > kMaxSeqHeads)
         return fail(h, KORE_PAGED_E_UNSUPPORTED, "n_tok %d x %d heads or n_seq %d x %d kv-heads is too large", b->n_tok,
                     h->cfg.n_head, b->n_seq, h->cfg.n_head_kv);
+    return KORE_PAGED_OK;
+}
+
+// The rows of an append (n_tok over 0).
+int check_qkv(kore_paged *h, int n_tok, int type, const void *k, int64_t k_stride, const void *v, int64_t v_stride, const void *q,
+              int64_t q_stride, const void *q_out, int64_t q_out_stride) {
+    const int64_t kvd = (int64_t)h->cfg.n_head_kv * h->cfg.head_dim, E = (int64_t)h->cfg.n_head * h->cfg.head_dim;
+    if (!k || !v) return fail(h, KORE_PAGED_E_INVALID, "null buffer");
+    if ((q == nullptr) != (q_out == nullptr)) return fail(h, KORE_PAGED_E_INVALID, "q without q_out, or q_out without q");
+    if (int rc = check_aligned(h, "k", k, type)) return rc;
+    if (int rc = check_aligned(h, "v", v, type)) return rc;
+    if (q) {
+        if (int rc = check_stride(h, "q", q_stride, E, n_tok)) return rc;
+        if (int rc = check_stride(h, "q_out", q_out_stride, E, n_tok)) return rc;
+        if (int rc = check_aligned(h, "q", q, type)) return rc;
+        if (int rc = check_aligned(h, "q_out", q_out, type)) return rc;
+        if (int rc = check_overlap(h, q, q_stride, q_out, q_out_stride, E, n_tok, type)) return rc;
+        if (int rc = check_apart(h, "k and q_out", k, k_stride, kvd, q_out, q_out_stride, E, n_tok, type)) return rc;
+        if (int rc = check_apart(h, "v and q_out", v, v_stride, kvd, q_out, q_out_stride, E, n_tok, type)) return rc;
+    }
     return KORE_PAGED_OK;
 }
 
@@ -305,14 +358,7 @@ int kore_rope_apply_dev(kore_rope_t r, int type, int n_tok, int n_head, int head
                         const int *pos, void *out, int64_t out_stride, int transpose, void *stream) {
     if (!r) return FAIL0(KORE_PAGED_E_INVALID, "null handle");
     if (!type_ok(type)) return fail(r, KORE_PAGED_E_INVALID, "unknown type %d", type);
-    if (n_tok < 0 || n_head <= 0) return fail(r, KORE_PAGED_E_INVALID, "bad n_tok %d or n_head %d", n_tok, n_head);
-    if (head_dim < r->cfg.rot_dim || head_dim % 2 != 0)
-        return fail(r, KORE_PAGED_E_INVALID, "head_dim %d is odd or under rot_dim %d", head_dim, r->cfg.rot_dim);
-    if (n_tok > kMaxRows) return fail(r, KORE_PAGED_E_UNSUPPORTED, "n_tok %d is over %d", n_tok, kMaxRows);
-    if (head_dim > kMaxRopeHeadDim)
-        return fail(r, KORE_PAGED_E_UNSUPPORTED, "head_dim %d over %d", head_dim, kMaxRopeHeadDim);
-    if ((int64_t)n_head * head_dim > 1 << 24)
-        return fail(r, KORE_PAGED_E_UNSUPPORTED, "%d heads of %d are too large a row", n_head, head_dim);
+    if (int rc = check_heads(r, n_tok, n_head, head_dim)) return rc;
     const int64_t n = (int64_t)n_head * head_dim;
     if (int rc = check_stride(r, "x", x_stride, n, n_tok)) return rc;
     if (int rc = check_stride(r, "out", out_stride, n, n_tok)) return rc;
@@ -325,6 +371,50 @@ int kore_rope_apply_dev(kore_rope_t r, int type, int n_tok, int n_head, int head
     if (int rc = on_device(r, on)) return rc;
     const RopeArgs a{r->turn(), x, out, pos, x_stride, out_stride, n_tok, n_head, head_dim, transpose ? -1 : 1, type};
     HIP_TRY(r, launch_rope(a, pick_stream(r, stream)));
+    return KORE_PAGED_OK;
+}
+
+int kore_rope_norm_dev(kore_rope_t r, int type, int n_tok, int head_dim, const kore_rope_heads *sets, int n_sets, const int *pos,
+                       float eps, void *stream) {
+    if (!r) return FAIL0(KORE_PAGED_E_INVALID, "null handle");
+    if (!type_ok(type)) return fail(r, KORE_PAGED_E_INVALID, "unknown type %d", type);
+    if (!sets || n_sets < 1 || n_sets > 2) return fail(r, KORE_PAGED_E_INVALID, "no sets, or %d of them (1 or 2)", n_sets);
+    if (!eps_ok(eps)) return fail(r, KORE_PAGED_E_INVALID, "eps must be positive and finite");
+    HeadsArgs a{};
+    for (int i = 0; i < n_sets; ++i) {
+        const kore_rope_heads &t = sets[i];
+        if (int rc = check_heads(r, n_tok, t.n_head, head_dim)) return rc;
+        const int64_t n = (int64_t)t.n_head * head_dim;
+        if (int rc = check_stride(r, "x", t.x_stride, n, n_tok)) return rc;
+        if (int rc = check_stride(r, "out", t.out_stride, n, n_tok)) return rc;
+        a.set[i] = HeadSet{t.x, t.out, t.x_stride, t.out_stride, t.n_head, t.norm};
+    }
+    if (n_tok == 0) return KORE_PAGED_OK;
+    if (int rc = check_array(r, "pos", pos, 4)) return rc;
+    for (int i = 0; i < n_sets; ++i) {
+        const HeadSet &t = a.set[i];
+        const int64_t n = (int64_t)t.n_head * head_dim;
+        if (!t.x || !t.out) return fail(r, KORE_PAGED_E_INVALID, "null buffer");
+        if (int rc = check_aligned(r, "x", t.x, type)) return rc;
+        if (int rc = check_aligned(r, "out", t.out, type)) return rc;
+        if (int rc = check_aligned(r, "norm", t.norm, KORE_PAGED_F32)) return rc;
+        if (int rc = check_overlap(r, t.x, t.x_stride, t.out, t.out_stride, n, n_tok, type)) return rc;
+        if (i == 0) continue;
+        const HeadSet &o = a.set[0];
+        const int64_t on = (int64_t)o.n_head * head_dim;
+        if (int rc = check_apart(r, "the sets' output", o.out, o.out_stride, on, t.out, t.out_stride, n, n_tok, type)) return rc;
+        if (int rc = check_apart(r, "one set's input and the other's output", o.x, o.x_stride, on, t.out, t.out_stride, n, n_tok, type)) return rc;
+        if (int rc = check_apart(r, "one set's output and the other's input", o.out, o.out_stride, on, t.x, t.x_stride, n, n_tok, type)) return rc;
+    }
+    OnDevice on(r->device);
+    if (int rc = on_device(r, on)) return rc;
+    a.turn = r->turn();
+    a.pos = pos;
+    a.eps = eps;
+    a.n_tok = n_tok;
+    a.hd = head_dim;
+    a.type = type;
+    HIP_TRY(r, launch_heads(a, pick_stream(r, stream)));
     return KORE_PAGED_OK;
 }
 
@@ -421,23 +511,11 @@ int kore_paged_append_dev(kore_paged_t h, int layer, const kore_paged_batch *b, 
     if (!h) return FAIL0(KORE_PAGED_E_INVALID, "null handle");
     if (int rc = check_batch(h, layer, b, type)) return rc;
     const kore_paged_config &c = h->cfg;
-    const int64_t kvd = (int64_t)c.n_head_kv * c.head_dim, E = (int64_t)c.n_head * c.head_dim;
+    const int64_t kvd = (int64_t)c.n_head_kv * c.head_dim;
     if (int rc = check_stride(h, "k", k_stride, kvd, b->n_tok)) return rc;
     if (int rc = check_stride(h, "v", v_stride, kvd, b->n_tok)) return rc;
     if (b->n_seq == 0 || b->n_tok == 0) return KORE_PAGED_OK;
-    if (!k || !v) return fail(h, KORE_PAGED_E_INVALID, "null buffer");
-    if ((q == nullptr) != (q_out == nullptr)) return fail(h, KORE_PAGED_E_INVALID, "q without q_out, or q_out without q");
-    if (int rc = check_aligned(h, "k", k, type)) return rc;
-    if (int rc = check_aligned(h, "v", v, type)) return rc;
-    if (q) {
-        if (int rc = check_stride(h, "q", q_stride, E, b->n_tok)) return rc;
-        if (int rc = check_stride(h, "q_out", q_out_stride, E, b->n_tok)) return rc;
-        if (int rc = check_aligned(h, "q", q, type)) return rc;
-        if (int rc = check_aligned(h, "q_out", q_out, type)) return rc;
-        if (int rc = check_overlap(h, q, q_stride, q_out, q_out_stride, E, b->n_tok, type)) return rc;
-        if (int rc = check_apart(h, "k and q_out", k, k_stride, kvd, q_out, q_out_stride, E, b->n_tok, type)) return rc;
-        if (int rc = check_apart(h, "v and q_out", v, v_stride, kvd, q_out, q_out_stride, E, b->n_tok, type)) return rc;
-    }
+    if (int rc = check_qkv(h, b->n_tok, type, k, k_stride, v, v_stride, q, q_stride, q_out, q_out_stride)) return rc;
     OnDevice on(h->device);
     if (int rc = on_device(h, on)) return rc;
     AppendArgs a{};
@@ -465,10 +543,12 @@ int kore_paged_append_dev(kore_paged_t h, int layer, const kore_paged_batch *b, 
     return KORE_PAGED_OK;
 }
 
-int kore_paged_attend_dev(kore_paged_t h, int layer, const kore_paged_batch *b, int type, const void *q,
-                          int64_t q_stride, void *out, int64_t out_stride, float scale, int window, void *workspace,
-                          void *stream) {
-    if (!h) return FAIL0(KORE_PAGED_E_INVALID, "null handle");
+extern "C++" {
+namespace {
+
+// Attention of the batch's rows; t NULL: each up to its own position.
+int attend(kore_paged_t h, int layer, const kore_paged_batch *b, const kore_paged_tree *t, int type, const void *q,
+           int64_t q_stride, void *out, int64_t out_stride, float scale, int window, void *workspace, void *stream) {
     if (int rc = check_batch(h, layer, b, type)) return rc;
     const kore_paged_config &c = h->cfg;
     const int64_t E = (int64_t)c.n_head * c.head_dim;
@@ -478,7 +558,14 @@ int kore_paged_attend_dev(kore_paged_t h, int layer, const kore_paged_batch *b, 
     if (scale != 0 && !(scale >= 1e-30f && scale <= 1e30f))
         return fail(h, KORE_PAGED_E_INVALID, "scale is neither 0 nor within 1e-30 .. 1e30");
     if ((uintptr_t)workspace % 16) return fail(h, KORE_PAGED_E_INVALID, "the workspace is not 16-byte aligned");
+    if (t && (t->mask_words < 1 || t->mask_words > kMaxWords))
+        return fail(h, KORE_PAGED_E_INVALID, "mask_words %d outside 1..%d", t->mask_words, kMaxWords);
     if (b->n_seq == 0 || b->n_tok == 0) return KORE_PAGED_OK;
+    if (t) {
+        if (int rc = check_array(h, "mask", t->mask, 8)) return rc;
+        if (t->pos || window)
+            if (int rc = check_array(h, "pos", t->pos, 4)) return rc;
+    }
     if (!q || !out) return fail(h, KORE_PAGED_E_INVALID, "null buffer");
     if (int rc = check_aligned(h, "q", q, type)) return rc;
     if (int rc = check_aligned(h, "out", out, type)) return rc;
@@ -506,7 +593,171 @@ int kore_paged_attend_dev(kore_paged_t h, int layer, const kore_paged_batch *b, 
     a.max_q = b->max_q;
     a.num_cu = h->num_cu;
     a.part = workspace ? (float *)workspace : h->part;
+    if (t) a.tree = Tree{(const unsigned long long *)t->mask, t->pos, t->mask_words};
     HIP_TRY(h, launch_attend(a, pick_stream(h, stream)));
+    return KORE_PAGED_OK;
+}
+
+}  // namespace
+}  // extern "C++"
+
+int kore_paged_attend_dev(kore_paged_t h, int layer, const kore_paged_batch *b, int type, const void *q,
+                          int64_t q_stride, void *out, int64_t out_stride, float scale, int window, void *workspace,
+                          void *stream) {
+    if (!h) return FAIL0(KORE_PAGED_E_INVALID, "null handle");
+    return attend(h, layer, b, nullptr, type, q, q_stride, out, out_stride, scale, window, workspace, stream);
+}
+
+int kore_paged_attend_tree_dev(kore_paged_t h, int layer, const kore_paged_batch *b, const kore_paged_tree *t, int type,
+                               const void *q, int64_t q_stride, void *out, int64_t out_stride, float scale, int window,
+                               void *workspace, void *stream) {
+    if (!h) return FAIL0(KORE_PAGED_E_INVALID, "null handle");
+    if (!t) return fail(h, KORE_PAGED_E_INVALID, "null tree");
+    return attend(h, layer, b, t, type, q, q_stride, out, out_stride, scale, window, workspace, stream);
+}
+
+int kore_paged_plan_dev(kore_paged_t h, const kore_paged_plan *p, void *stream) {
+    if (!h) return FAIL0(KORE_PAGED_E_INVALID, "null handle");
+    if (!p) return fail(h, KORE_PAGED_E_INVALID, "null plan");
+    if (p->n_seq < 0 || p->n_tok < 0) return fail(h, KORE_PAGED_E_INVALID, "negative n_seq or n_tok");
+    if (int rc = check_table(h, p->n_seq, p->pages_stride)) return rc;
+    if (p->n_tok > kMaxRows) return fail(h, KORE_PAGED_E_UNSUPPORTED, "n_tok %d is over %d", p->n_tok, kMaxRows);
+    if (p->parent || p->mask) {
+        if (p->mask_words < 1 || p->mask_words > kMaxWords)
+            return fail(h, KORE_PAGED_E_INVALID, "mask_words %d outside 1..%d", p->mask_words, kMaxWords);
+        if (int rc = check_array(h, "parent", p->parent, 4)) return rc;
+        if (int rc = check_array(h, "mask", p->mask, 8)) return rc;
+    } else if (p->mask_words != 0) {
+        return fail(h, KORE_PAGED_E_INVALID, "mask_words %d without parent and mask", p->mask_words);
+    }
+    if (p->n_seq) {
+        if (int rc = check_array(h, "n_new", p->n_new, 4)) return rc;
+        if (int rc = check_array(h, "kv_held", p->kv_held, 4)) return rc;
+        if (int rc = check_array(h, "kv_len", p->kv_len, 4)) return rc;
+        if (int rc = check_array(h, "pages", p->pages, 4)) return rc;
+        if (int rc = check_array(h, "free_pages", p->free_pages, 4)) return rc;
+    }
+    if (int rc = check_array(h, "n_free", p->n_free, 4)) return rc;
+    if (int rc = check_array(h, "n_free_out", p->n_free_out, 4)) return rc;
+    if (int rc = check_array(h, "q_start", p->q_start, 4)) return rc;
+    if (int rc = check_array(h, "status", p->status, 4)) return rc;
+    if (p->n_tok) {
+        if (int rc = check_array(h, "pos", p->pos, 4)) return rc;
+        if (int rc = check_array(h, "slot", p->slot, 8)) return rc;
+    }
+    OnDevice on(h->device);
+    if (int rc = on_device(h, on)) return rc;
+    PlanArgs a{};
+    a.n_seq = p->n_seq;
+    a.n_tok = p->n_tok;
+    a.n_pages = h->cfg.n_pages;
+    a.page_shift = h->page_shift;
+    a.pages_stride = p->pages_stride;
+    a.words = p->mask_words;
+    a.n_new = p->n_new;
+    a.kv_held = p->kv_held;
+    a.free_pages = p->free_pages;
+    a.n_free = p->n_free;
+    a.parent = p->parent;
+    a.kv_len = p->kv_len;
+    a.pages = p->pages;
+    a.n_free_out = p->n_free_out;
+    a.q_start = p->q_start;
+    a.pos = p->pos;
+    a.status = p->status;
+    a.slot = p->slot;
+    a.mask = (unsigned long long *)p->mask;
+    HIP_TRY(h, launch_plan(a, pick_stream(h, stream)));
+    return KORE_PAGED_OK;
+}
+
+int kore_paged_append_rows_dev(kore_paged_t h, int layer, const kore_paged_rows *r, int type, const void *k,
+                               int64_t k_stride, const void *v, int64_t v_stride, const void *q, int64_t q_stride,
+                               void *q_out, int64_t q_out_stride, void *stream) {
+    if (!h) return FAIL0(KORE_PAGED_E_INVALID, "null handle");
+    if (!r) return fail(h, KORE_PAGED_E_INVALID, "null rows");
+    if (int rc = check_layer(h, layer, type)) return rc;
+    const kore_paged_config &c = h->cfg;
+    if (r->n_tok < 0) return fail(h, KORE_PAGED_E_INVALID, "negative n_tok");
+    if (r->n_tok > kMaxRows || (int64_t)r->n_tok * c.n_head > kMaxRowHeads)
+        return fail(h, KORE_PAGED_E_UNSUPPORTED, "n_tok %d x %d heads is too large", r->n_tok, c.n_head);
+    if ((r->q_norm || r->k_norm) && !eps_ok(r->norm_eps))
+        return fail(h, KORE_PAGED_E_INVALID, "norm_eps must be positive and finite");
+    const int64_t kvd = (int64_t)c.n_head_kv * c.head_dim;
+    if (int rc = check_stride(h, "k", k_stride, kvd, r->n_tok)) return rc;
+    if (int rc = check_stride(h, "v", v_stride, kvd, r->n_tok)) return rc;
+    if (r->n_tok == 0) return KORE_PAGED_OK;
+    if (int rc = check_array(h, "pos", r->pos, 4)) return rc;
+    if (int rc = check_array(h, "slot", r->slot, 8)) return rc;
+    if (int rc = check_qkv(h, r->n_tok, type, k, k_stride, v, v_stride, q, q_stride, q_out, q_out_stride)) return rc;
+    if (int rc = check_aligned(h, "q_norm", r->q_norm, KORE_PAGED_F32)) return rc;
+    if (int rc = check_aligned(h, "k_norm", r->k_norm, KORE_PAGED_F32)) return rc;
+    OnDevice on(h->device);
+    if (int rc = on_device(h, on)) return rc;
+    const size_t at = (size_t)layer * h->layer_elems() * type_bytes(c.cache_type);
+    HeadsArgs a{};
+    if (h->rope) a.turn = h->rope->turn();
+    if (q) a.set[0] = HeadSet{q, q_out, q_stride, q_out_stride, c.n_head, r->q_norm};
+    a.set[1] = HeadSet{k, (char *)h->k_pool + at, k_stride, 0, c.n_head_kv, r->k_norm};
+    a.pos = r->pos;
+    a.eps = r->q_norm || r->k_norm ? r->norm_eps : 1.0f;
+    a.n_tok = r->n_tok;
+    a.hd = c.head_dim;
+    a.type = type;
+    a.slot = r->slot;
+    a.v = v;
+    a.v_stride = v_stride;
+    a.v_pool = (char *)h->v_pool + at;
+    a.n_pages = c.n_pages;
+    a.page_shift = h->page_shift;
+    a.cache_type = c.cache_type;
+    HIP_TRY(h, launch_heads(a, pick_stream(h, stream)));
+    return KORE_PAGED_OK;
+}
+
+int kore_paged_keep_dev(kore_paged_t h, const kore_paged_keep *k, void *stream) {
+    if (!h) return FAIL0(KORE_PAGED_E_INVALID, "null handle");
+    if (!k) return fail(h, KORE_PAGED_E_INVALID, "null keep");
+    if (k->n_seq < 0 || k->n_tok < 0) return fail(h, KORE_PAGED_E_INVALID, "negative n_seq or n_tok");
+    if (int rc = check_table(h, k->n_seq, k->pages_stride)) return rc;
+    if (k->n_seq) {
+        if (int rc = check_array(h, "q_start", k->q_start, 4)) return rc;
+        if (int rc = check_array(h, "n_keep", k->n_keep, 4)) return rc;
+        if (int rc = check_array(h, "kv_len", k->kv_len, 4)) return rc;
+        if (int rc = check_array(h, "kv_out", k->kv_out, 4)) return rc;
+        if (int rc = check_array(h, "pages", k->pages, 4)) return rc;
+        if ((uintptr_t)k->rows % 4) return fail(h, KORE_PAGED_E_INVALID, "rows is not aligned to 4 bytes");
+    }
+    if (k->free_pages || k->n_free || k->n_free_out) {
+        if (int rc = check_array(h, "free_pages", k->free_pages, 4)) return rc;
+        if (int rc = check_array(h, "n_free", k->n_free, 4)) return rc;
+        if (int rc = check_array(h, "n_free_out", k->n_free_out, 4)) return rc;
+    }
+    OnDevice on(h->device);
+    if (int rc = on_device(h, on)) return rc;
+    const kore_paged_config &c = h->cfg;
+    KeepArgs a{};
+    a.n_seq = k->n_seq;
+    a.n_tok = k->n_tok;
+    a.n_layer = c.n_layer;
+    a.n_pages = c.n_pages;
+    a.page_shift = h->page_shift;
+    a.pages_stride = k->pages_stride;
+    a.n_head_kv = c.n_head_kv;
+    a.hd = c.head_dim;
+    a.cache_type = c.cache_type;
+    a.q_start = k->q_start;
+    a.n_keep = k->n_keep;
+    a.rows = k->rows;
+    a.kv_len = k->kv_len;
+    a.pages = k->pages;
+    a.n_free = k->n_free;
+    a.kv_out = k->kv_out;
+    a.free_pages = k->free_pages;
+    a.n_free_out = k->n_free_out;
+    a.k_pool = h->k_pool;
+    a.v_pool = h->v_pool;
+    HIP_TRY(h, launch_keep(a, pick_stream(h, stream)));
     return KORE_PAGED_OK;
 }
 

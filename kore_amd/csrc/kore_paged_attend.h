@@ -120,7 +120,9 @@ struct Share {
     int keys;       // that a tile can span
 };
 
-template <int TILE>
+// Trees: a row sees the keys before the new rows, and any of those; tiles and cuts are
+// made as if it saw all.
+template <int TILE, bool TREE>
 __device__ __forceinline__ Share share_of(const Batch &b, int s, int rep, int cap, int window, int &q0, int &n, int &kv) {
     q0 = min(max(b.q_start[s], 0), b.n_tok);
     n = min(max(b.q_start[s + 1], q0), b.n_tok) - q0;
@@ -128,7 +130,7 @@ __device__ __forceinline__ Share share_of(const Batch &b, int s, int rep, int ca
     Share r;
     r.tiles = (n * rep + TILE - 1) / TILE;
     // the rows of a tile span (TILE - 1) / rep + 2 tokens at most, and its first key is rounded down by up to 63
-    const int held = max(0, min(kv, cap)), wide = (TILE - 1) / rep + 65;
+    const int held = max(0, min(kv, cap)), wide = TREE ? n + 65 : (TILE - 1) / rep + 65;
     r.keys = window < held - wide ? window + wide : held;
     return r;
 }
@@ -166,13 +168,13 @@ __device__ __forceinline__ T last_lane(T x) {
 // sequences, then a sequence's tiles from the last (which has the most keys),
 // then its splits, then the kv-heads.  by_tile (the merge): over the split tiles
 // alone, one number for all splits.
-template <int TILE>
+template <int TILE, bool TREE>
 __device__ __forceinline__ bool place_of(const Batch &b, const Cut &c, int id, int nkv, int cap, int window, bool by_tile,
                                          Place &p) {
     const int lane = threadIdx.x & 63;
     int len = INT_MAX, q0 = 0, n = 0, kv = 0;
     const auto share = [&](int s0) {
-        return s0 + lane < b.n_seq ? share_of<TILE>(b, s0 + lane, c.rep, cap, window, q0, n, kv) : Share{0, 0};
+        return s0 + lane < b.n_seq ? share_of<TILE, TREE>(b, s0 + lane, c.rep, cap, window, q0, n, kv) : Share{0, 0};
     };
     Share r = share(0);
     if (c.target) {
@@ -230,10 +232,11 @@ struct Keys {
     int lo, hi, seen_lo, all_lo, all_hi;
 };
 
-template <int TILE>
+template <int TILE, bool TREE>
 __device__ __forceinline__ Keys keys_of(const Place &p, const Cut &c, int cap, int window) {
-    const int t0 = c.by_rep.of(p.tile * TILE), t1 = min(p.n - 1, c.by_rep.of(p.tile * TILE + TILE - 1));
-    const int p0 = p.kv - p.n + t0, p1 = p.kv - p.n + t1;   // positions of the first and last row
+    // positions of the first and last row; of a tree, the lowest and the highest that its rows may have
+    const int t0 = TREE ? 0 : c.by_rep.of(p.tile * TILE), t1 = TREE ? p.n - 1 : min(p.n - 1, c.by_rep.of(p.tile * TILE + TILE - 1));
+    const int p0 = p.kv - p.n + t0, p1 = p.kv - p.n + t1;
     Keys k;
     k.seen_lo = window <= p0 ? p0 - window + 1 : 0;
     const int first = k.seen_lo & ~63, end = min(p1 + 1, cap);
@@ -248,7 +251,7 @@ __device__ __forceinline__ Keys keys_of(const Place &p, const Cut &c, int cap, i
     k.hi = scalar(k.hi);
     k.seen_lo = scalar(k.seen_lo);
     k.all_lo = scalar(window <= p1 ? p1 - window + 1 : 0);
-    k.all_hi = scalar(min(p0 + 1, cap));
+    k.all_hi = scalar(min(TREE ? max(p0, 0) : p0 + 1, cap));
     return k;
 }
 
@@ -418,15 +421,30 @@ struct Row {
     int token, head;
 };
 
-__device__ __forceinline__ Row row_of(const Place &p, int r, const Cut &c, int cap, int window) {
+template <bool TREE>
+__device__ __forceinline__ Row row_of(const Place &p, int r, const TileArgs &d, int cap) {
+    const Cut &c = d.cut;
+    const int window = d.a.window;
     Row x;
     x.real = r < p.n * c.rep;
     x.token = c.by_rep.of(r);
     x.head = p.head * c.rep + (r - x.token * c.rep);
-    const int pos = p.kv - p.n + x.token;
+    int pos = p.kv - p.n + x.token;
+    if (TREE && window != INT_MAX && x.real) pos = min(max(d.a.tree.pos[p.q0 + x.token], p.kv - p.n), p.kv - 1);
     x.lo = window <= pos ? pos - window + 1 : 0;
-    x.hi = x.real ? min(pos + 1, cap) : 0;
+    if (TREE) x.lo = min(x.lo, max(p.kv - p.n, 0));   // (the new rows are the mask's)
+    x.hi = x.real ? min(TREE ? p.kv : pos + 1, cap) : 0;
     return x;
+}
+
+// Trees: bit j of the result says whether the row may see the key key0 + j, as far as its
+// mask goes: all those before the new rows, and of the new ones those whose bits are set.
+__device__ __forceinline__ unsigned long long mask_of(const AttendArgs &a, const Place &p, const Row &row, int key0) {
+    const unsigned long long *const mask = a.tree.mask + (size_t)(p.q0 + (row.real ? row.token : 0)) * a.tree.words;
+    const int from = key0 - (p.kv - p.n), w = from >> 6, shift = from & 63;
+    const auto word = [&](int i) { return i < 0 ? ~0ULL : i < a.tree.words ? mask[i] : 0ULL; };
+    const unsigned long long lo = word(w);
+    return shift ? lo >> shift | word(w + 1) << (64 - shift) : lo;
 }
 
 // N pieces of a row of q, 8 values each, piece t from dim first + step t: all requested

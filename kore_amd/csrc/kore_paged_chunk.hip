@@ -102,7 +102,7 @@ __device__ __forceinline__ void weights(const float (&x)[8], V (&part)[N]) {
     }
 }
 
-template <class A, class S, int HDP>
+template <class A, class S, int HDP, bool TREE>
 __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(TileArgs d) {
     typedef typename Form<A, S>::C C;
     typedef typename Form<A, S>::CV CV;
@@ -150,10 +150,10 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
     auto &kinds = all_kinds[team];
     auto &odd_of = all_odd[team];
     Place p;
-    if (!place_of<kRows>(a.b, d.cut, blockIdx.x, a.n_head_kv, cap, a.window, false, p)) return;
-    const Keys k = keys_of<kRows>(p, d.cut, cap, a.window);
+    if (!place_of<kRows, TREE>(a.b, d.cut, blockIdx.x, a.n_head_kv, cap, a.window, false, p)) return;
+    const Keys k = keys_of<kRows, TREE>(p, d.cut, cap, a.window);
     const int col = lane & 31, half = lane >> 5;
-    const Row row = row_of(p, p.tile * kRows + wave * 32 + col, d.cut, cap, a.window);
+    const Row row = row_of<TREE>(p, p.tile * kRows + wave * 32 + col, d, cap);
     const int *table = a.b.pages + (size_t)p.seq * a.b.pages_stride;
     const int slot_mask = (1 << a.page_shift) - 1;
     const bool padded = a.hd != HDP;
@@ -163,10 +163,10 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
     {
         const int r0 = p.tile * kRows + wave * 32, r1 = min(r0 + 31, p.n * rep - 1);
         const int p0 = p.kv - p.n + d.cut.by_rep.of(r0), p1 = p.kv - p.n + d.cut.by_rep.of(max(r1, 0));
-        see_lo = a.window <= p0 ? p0 - a.window + 1 : 0;
-        see_hi = r0 <= r1 ? min(p1 + 1, k.hi) : 0;
-        all_lo = a.window <= p1 ? p1 - a.window + 1 : 0;
-        all_hi = min(p0 + 1, k.hi);
+        see_lo = TREE ? k.seen_lo : a.window <= p0 ? p0 - a.window + 1 : 0;
+        see_hi = r0 <= r1 ? min(TREE ? p.kv : p1 + 1, k.hi) : 0;
+        all_lo = TREE ? k.all_lo : a.window <= p1 ? p1 - a.window + 1 : 0;
+        all_hi = min(TREE ? k.all_hi : p0 + 1, k.hi);
         see_lo = scalar(see_lo);
         see_hi = scalar(see_hi);
         all_lo = scalar(all_lo);
@@ -200,7 +200,7 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
         const A *src[kQLoads];
 #pragma unroll
         for (int i = 0; i < kQLoads; ++i) {
-            const Row r = row_of(p, p.tile * kRows + i * kQPass + q_first, d.cut, cap, a.window);
+            const Row r = row_of<TREE>(p, p.tile * kRows + i * kQPass + q_first, d, cap);
             q_real[i] = r.real && my_dim < a.hd;
             src[i] = q_row_of<A>(a, p, r) + min(my_dim, a.hd - 8);
         }
@@ -450,6 +450,8 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
             bool far = false;
             unsigned has_weight[MT];   // CAREFUL: of the step's keys, for the lane's row
             if (any) {
+                unsigned long long seen = ~0ULL;   // keys 32 m + 8 (i / 4) + i % 4 of the lane's 4 half ..
+                if (TREE && !whole) seen = mask_of(a, p, row, key0) >> (4 * half);
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
                     s[m] = floatx16{};
@@ -491,7 +493,8 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             const int at = 32 * m + 8 * (i / 4) + 4 * half + i % 4, key = key0 + at;
-                            if (!(key >= row.lo && key < min(row.hi, k.hi) && (has >> (2 * m + i / 8) & 1))) s[m][i] = kNone;
+                            const bool in = key >= row.lo && key < min(row.hi, k.hi) && (has >> (2 * m + i / 8) & 1);
+                            if (!(in && (!TREE || (seen >> (32 * m + 8 * (i / 4) + i % 4) & 1)))) s[m][i] = kNone;
                         }
                 }
                 float top = kNone;
@@ -689,16 +692,15 @@ __global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(T
         }
 }
 
-}  // namespace
-
+template <bool TREE>
 hipError_t launch_chunk(const TileArgs &d, hipStream_t s) {
     const int hdp = padded_dim(d.a.hd);
     const dim3 grid((unsigned)d.places);
 #define KORE_CHUNK(A, S)                                                        \
     do {                                                                        \
-        if (hdp == 64) return launch(chunk_kernel<A, S, 64>, grid, Shape<A, S, 64>::threads, 0, s, d);     \
-        else if (hdp == 128) return launch(chunk_kernel<A, S, 128>, grid, Shape<A, S, 128>::threads, 0, s, d); \
-        else return launch(chunk_kernel<A, S, 256>, grid, Shape<A, S, 256>::threads, 0, s, d);              \
+        if (hdp == 64) return launch(chunk_kernel<A, S, 64, TREE>, grid, Shape<A, S, 64>::threads, 0, s, d);     \
+        else if (hdp == 128) return launch(chunk_kernel<A, S, 128, TREE>, grid, Shape<A, S, 128>::threads, 0, s, d); \
+        else return launch(chunk_kernel<A, S, 256, TREE>, grid, Shape<A, S, 256>::threads, 0, s, d);              \
     } while (0)
     if (d.a.cache_type == kF32) KORE_CHUNK(float, float);
     else if (d.a.type == kF32 && d.a.cache_type == kF16) KORE_CHUNK(float, half_t);
@@ -706,6 +708,12 @@ hipError_t launch_chunk(const TileArgs &d, hipStream_t s) {
     else if (d.a.type == kF16) KORE_CHUNK(half_t, half_t);
     else KORE_CHUNK(bhalf_t, bhalf_t);
 #undef KORE_CHUNK
+}
+
+}  // namespace
+
+hipError_t launch_chunk(const TileArgs &d, hipStream_t s) {
+    return d.a.tree.mask ? launch_chunk<true>(d, s) : launch_chunk<false>(d, s);
 }
 
 }  // namespace kore_paged_gpu

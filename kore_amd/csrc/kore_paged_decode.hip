@@ -72,7 +72,7 @@ __device__ __forceinline__ void finish(const TileArgs &d, const Place &p, const 
 // 32 sequences of 1k to 8k keys, 28/4/128, fp32 rows over an fp16 cache: 63 us for 282
 // MB, 4.5 TB/s (a large copy: 5.1); one bf16 token over 131072 keys of 16/2/128: 29.6
 // us for 134 MB, 4.5 TB/s.
-template <class A, class C, int HDP, int W>
+template <class A, class C, int HDP, int W, bool TREE>
 __global__ __launch_bounds__(64 * W, HDP <= 128 && W == 4 ? 2 : 1) void decode16_kernel(TileArgs d) {
     // 16-bit rows could have their weights in one part; the second costs nothing beside the loads, and leaves the result
     // no rounding but its own (bf16, one token over 131072 keys: error 1.7e-3 instead of 2.3e-3 of the result)
@@ -90,10 +90,10 @@ __global__ __launch_bounds__(64 * W, HDP <= 128 && W == 4 ? 2 : 1) void decode16
     const AttendArgs &a = d.a;
     const int cap = a.b.pages_stride << a.page_shift, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Place p;
-    if (!place_of<kRows>(a.b, d.cut, blockIdx.x, a.n_head_kv, cap, a.window, false, p)) return;
-    const Keys k = keys_of<kRows>(p, d.cut, cap, a.window);
+    if (!place_of<kRows, TREE>(a.b, d.cut, blockIdx.x, a.n_head_kv, cap, a.window, false, p)) return;
+    const Keys k = keys_of<kRows, TREE>(p, d.cut, cap, a.window);
     const int col = lane & 15, g = lane >> 4;
-    const Row row = row_of(p, p.tile * kRows + col, d.cut, cap, a.window);
+    const Row row = row_of<TREE>(p, p.tile * kRows + col, d, cap);
     const int *table = a.b.pages + (size_t)p.seq * a.b.pages_stride;
     const int slot_mask = (1 << a.page_shift) - 1;
     const bool padded = a.hd != HDP;
@@ -212,6 +212,8 @@ __global__ __launch_bounds__(64 * W, HDP <= 128 && W == 4 ? 2 : 1) void decode16
                         kr[1][t] = vec8{};
                     }
             }
+            unsigned seen = ~0u;   // keys 16 m + i of the lane's 4 g ..
+            if (TREE && !whole) seen = (unsigned)(mask_of(a, p, row, key0) >> (4 * g));
             floatx4 s[2];
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
@@ -254,7 +256,8 @@ __global__ __launch_bounds__(64 * W, HDP <= 128 && W == 4 ? 2 : 1) void decode16
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int key = key0 + 16 * m + 4 * g + i;
-                        if (!(key >= row.lo && key < min(row.hi, k.hi) && (m ? has1 : has0))) s[m][i] = kNone;
+                        const bool in = key >= row.lo && key < min(row.hi, k.hi) && (m ? has1 : has0);
+                        if (!(in && (!TREE || (seen >> (16 * m + i) & 1)))) s[m][i] = kNone;
                     }
             }
             float top = kNone;
@@ -338,7 +341,7 @@ __global__ __launch_bounds__(64 * W, HDP <= 128 && W == 4 ? 2 : 1) void decode16
 // One token over 512 keys of 14/2/64: 6.1 us (a launch's own time is some 2; then three
 // rounds of memory); 24 of uneven length, 28/4/128: 100 us for
 // 455 MB, 4.5 TB/s.
-template <int HDP, int W>
+template <int HDP, int W, bool TREE>
 __global__ __launch_bounds__(64 * W, HDP <= 128 && W == 4 ? 2 : 1) void decode32_kernel(TileArgs d) {
     constexpr int KU = HDP / 16, DJ = HDP / 64, kBlock = 16;
     __shared__ float4 states[W][HDP / 4][kRows];
@@ -346,10 +349,10 @@ __global__ __launch_bounds__(64 * W, HDP <= 128 && W == 4 ? 2 : 1) void decode32
     const AttendArgs &a = d.a;
     const int cap = a.b.pages_stride << a.page_shift, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Place p;
-    if (!place_of<kRows>(a.b, d.cut, blockIdx.x, a.n_head_kv, cap, a.window, false, p)) return;
-    const Keys k = keys_of<kRows>(p, d.cut, cap, a.window);
+    if (!place_of<kRows, TREE>(a.b, d.cut, blockIdx.x, a.n_head_kv, cap, a.window, false, p)) return;
+    const Keys k = keys_of<kRows, TREE>(p, d.cut, cap, a.window);
     const int col = lane & 15, g = lane >> 4;
-    const Row row = row_of(p, p.tile * kRows + col, d.cut, cap, a.window);
+    const Row row = row_of<TREE>(p, p.tile * kRows + col, d, cap);
     const int *table = a.b.pages + (size_t)p.seq * a.b.pages_stride;
     const int slot_mask = (1 << a.page_shift) - 1;
     const bool padded = a.hd != HDP;
@@ -426,6 +429,8 @@ __global__ __launch_bounds__(64 * W, HDP <= 128 && W == 4 ? 2 : 1) void decode32
                 for (int u = 0; u < KU; ++u)
                     if (16 * u + 4 * g >= a.hd) kr[u] = floatx4{0, 0, 0, 0};
             }
+            unsigned seen = ~0u;   // keys of the lane's 4 g ..
+            if (TREE && !whole) seen = (unsigned)(mask_of(a, p, row, key0) >> (4 * g));
             floatx4 s = floatx4{0, 0, 0, 0}, s2 = floatx4{0, 0, 0, 0};   // two chains
 #pragma unroll
             for (int u = 0; u < KU; ++u)
@@ -442,7 +447,7 @@ __global__ __launch_bounds__(64 * W, HDP <= 128 && W == 4 ? 2 : 1) void decode32
                 for (int i = 0; i < 4; ++i) {
                     const int key = key0 + 4 * g + i;
                     const bool in = key < k.hi && key >= k.seen_lo && has;
-                    if (!(in && key >= row.lo && key < row.hi)) s[i] = kNone;
+                    if (!(in && key >= row.lo && key < row.hi && (!TREE || (seen >> i & 1)))) s[i] = kNone;
 #pragma unroll
                     for (int x = 0; x < DJ; ++x)
                         if (!in) vr[i][x] = floatx4{0, 0, 0, 0};
@@ -534,7 +539,7 @@ __global__ __launch_bounds__(64 * W, HDP <= 128 && W == 4 ? 2 : 1) void decode32
 // tile's dims.  (Few tiles may have hundreds of splits, many tiles two each.)  Bound by
 // its launch and two rounds of memory: 4.7 us for two tiles of eight splits, 7.5 for 128
 // of three, 12.4 for 112 of 128 rows.
-template <class A, int TILE>
+template <class A, int TILE, bool TREE>
 __global__ __launch_bounds__(kThreads) void merge_kernel(TileArgs d, int hd4) {
     constexpr int kLanes = kThreads / TILE, kFlight = 8;
     __shared__ float4 so[kLanes][TILE];
@@ -542,7 +547,7 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(TileArgs d, int hd4) {
     const AttendArgs &a = d.a;
     const int cap = a.b.pages_stride << a.page_shift;
     Place p;
-    if (!place_of<TILE>(a.b, d.cut, blockIdx.x, a.n_head_kv, cap, a.window, true, p)) return;
+    if (!place_of<TILE, TREE>(a.b, d.cut, blockIdx.x, a.n_head_kv, cap, a.window, true, p)) return;
     if ((unsigned)p.part + (unsigned)(p.n_split - 1) * (unsigned)a.n_head_kv >= (unsigned)d.parts) return;   // as there
     int parts = 1;
     while (parts < kLanes && parts < p.n_split) parts *= 2;
@@ -606,15 +611,15 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(TileArgs d, int hd4) {
     }
 }
 
-template <int W>
+template <int W, bool TREE>
 hipError_t launch_decode(const TileArgs &d, hipStream_t s) {
     const int hdp = padded_dim(d.a.hd);
     const dim3 grid((unsigned)d.places);
 #define KORE_DECODE(KERNEL, ...)                                                                \
     do {                                                                                        \
-        if (hdp == 64) return launch(KERNEL<__VA_ARGS__ 64, W>, grid, 64 * W, 0, s, d);                    \
-        else if (hdp == 128) return launch(KERNEL<__VA_ARGS__ 128, W>, grid, 64 * W, 0, s, d);             \
-        else if constexpr (W == 4) return launch(KERNEL<__VA_ARGS__ 256, W>, grid, 64 * W, 0, s, d);       \
+        if (hdp == 64) return launch(KERNEL<__VA_ARGS__ 64, W, TREE>, grid, 64 * W, 0, s, d);                    \
+        else if (hdp == 128) return launch(KERNEL<__VA_ARGS__ 128, W, TREE>, grid, 64 * W, 0, s, d);             \
+        else if constexpr (W == 4) return launch(KERNEL<__VA_ARGS__ 256, W, TREE>, grid, 64 * W, 0, s, d);       \
     } while (0)
 #define KORE_COMMA ,
     if (d.a.cache_type == kF32) KORE_DECODE(decode32_kernel);
@@ -630,12 +635,7 @@ hipError_t launch_decode(const TileArgs &d, hipStream_t s) {
 constexpr int kPerCu = 2;                              // workgroups of a CU, of the 16-row kernels
 constexpr int kShort = 1280;                           // keys that a tile among many is not split for
 
-}  // namespace
-
-size_t attend_workspace_bytes(int hd, int num_cu) {
-    return 2 * (size_t)num_cu * kChunkRows * ((size_t)padded_dim(hd) + 2) * sizeof(float);
-}
-
+template <bool TREE>
 hipError_t launch_attend(const AttendArgs &a, hipStream_t s) {
     TileArgs d{};
     d.a = a;
@@ -664,7 +664,8 @@ hipError_t launch_attend(const AttendArgs &a, hipStream_t s) {
     //   100 tokens over 300 keys, one over 1024, 2048, 65536: 23.0 / 20.6, 24.8 / 29.5, 60 / 645;
     //   300 tokens over 1000 keys, one over 65536: 186 / 776; 300 over 1100: 137 / 124 (the price of being ready for it).
     const int at_once = chunk ? a.num_cu : kPerCu * a.num_cu;
-    const long long most = std::min((long long)a.b.pages_stride << a.page_shift, (long long)a.window + (rows - 1) / d.cut.rep + 65);
+    const long long most = std::min((long long)a.b.pages_stride << a.page_shift,
+                                    (long long)a.window + (TREE ? a.b.n_tok : (rows - 1) / d.cut.rep) + 65);
     // A split's fewest keys, of 64, 128 and 256: 64 fp32 rows over 512 keys 22.6, 25.1, 32.4 us; 64 fp16 rows 15.5, 15.3,
     // 16.8; one token over 512 keys 9.6, 10.1, 11.2.
     d.cut.min_len = chunk && size == 2 ? 128 : 64;
@@ -685,7 +686,7 @@ hipError_t launch_attend(const AttendArgs &a, hipStream_t s) {
     d.part_o = a.part;
     d.parts = d.cut.target + (int)std::min<long long>(d.cut.target, tiles);
     d.part_ml = a.part + (size_t)d.parts * rows * hdp;
-    const hipError_t e = chunk ? launch_chunk(d, s) : wide ? launch_decode<8>(d, s) : launch_decode<4>(d, s);
+    const hipError_t e = chunk ? launch_chunk(d, s) : wide ? launch_decode<8, TREE>(d, s) : launch_decode<4, TREE>(d, s);
     if (e != hipSuccess || !d.cut.target) return e;
     // some eight workgroups a CU, where there are dims enough (32 sequences, fp16 cache: 57.8 us from cache, with one a CU
     // 78.3, with 32 59.9)
@@ -693,13 +694,23 @@ hipError_t launch_attend(const AttendArgs &a, hipStream_t s) {
     const dim3 merge((unsigned)joined, (unsigned)std::clamp(8 * a.num_cu / joined, 1, a.hd / 4));
 #define KORE_MERGE(A)                                                                    \
     do {                                                                                 \
-        if (chunk) return launch(merge_kernel<A, kChunkRows>, merge, kThreads, 0, s, d, hdp / 4);   \
-        else return launch(merge_kernel<A, kRows>, merge, kThreads, 0, s, d, hdp / 4);              \
+        if (chunk) return launch(merge_kernel<A, kChunkRows, TREE>, merge, kThreads, 0, s, d, hdp / 4);   \
+        else return launch(merge_kernel<A, kRows, TREE>, merge, kThreads, 0, s, d, hdp / 4);              \
     } while (0)
     if (a.type == kF32) KORE_MERGE(float);
     else if (a.type == kF16) KORE_MERGE(half_t);
     else KORE_MERGE(bhalf_t);
 #undef KORE_MERGE
+}
+
+}  // namespace
+
+size_t attend_workspace_bytes(int hd, int num_cu) {
+    return 2 * (size_t)num_cu * kChunkRows * ((size_t)padded_dim(hd) + 2) * sizeof(float);
+}
+
+hipError_t launch_attend(const AttendArgs &a, hipStream_t s) {
+    return a.tree.mask ? launch_attend<true>(a, s) : launch_attend<false>(a, s);
 }
 
 }  // namespace kore_paged_gpu

@@ -205,6 +205,108 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a) {
     }
 }
 
+// ---- heads that are normalised ---------------------------------------------------
+//
+// A head is a group's of G lanes, G the power of two that holds its units (at most 64:
+// then U units a lane), so that its sum of squares stays among them.  In double, so that no value's
+// square is too large or too small.
+
+template <int CTRL>
+__device__ __forceinline__ double from_dpp(double x) {
+    const long long b = __builtin_bit_cast(long long, x);
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)b, CTRL, 0xf, 0xf, true);
+    const int hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, 0xf, 0xf, true);
+    return __builtin_bit_cast(double, (long long)(unsigned)lo | (long long)hi << 32);
+}
+// The sum over a group of G = 1, 2, 4, .. 64 lanes, the same in all.
+__device__ __forceinline__ double group_sum(double x, int G) {
+    if (G > 1) x += from_dpp<0xb1>(x);     // lane i ^ 1
+    if (G > 2) x += from_dpp<0x4e>(x);     // i ^ 2
+    if (G > 4) x += from_dpp<0x141>(x);    // 7 - i of 8
+    if (G > 8) x += from_dpp<0x140>(x);    // 15 - i of 16
+    if (G > 16) x += __shfl_xor(x, 16);
+    if (G > 32) x += __shfl_xor(x, 32);
+    return x;
+}
+// 1 / sqrt(x): the hardware's 26 bits or so, and one step of Newton's.
+__device__ __forceinline__ float rsqrt_(double x) {
+    const double y = __builtin_amdgcn_rsq(x);
+    return (float)(y * (1.5 - 0.5 * x * y * y));
+}
+
+// A block takes a row's heads of both sets, then, where it stores, those of v; or a
+// gridDim.y-th of them.
+template <class T, class C, int V, int U, bool INTER, bool STORE>
+__global__ __launch_bounds__(kThreads) void heads_kernel(HeadsArgs a, int G) {
+    __shared__ float2 cs[kMaxRot / 2];
+    const int row = blockIdx.x, pos = a.pos[row];
+    if (pos < 0) return;
+    const int units = a.hd / (2 * V), lane = threadIdx.x & (G - 1), per = kThreads / G;
+    const int nq = a.set[0].n_head, nk = a.set[1].n_head, n_v = STORE ? nk : 0, total = nq + nk + n_v;
+    size_t at = 0;   // of the slot's first head in a pool
+    bool stored = false;
+    if (STORE) {
+        const int64_t slot = a.slot[row];
+        stored = slot >= 0 && slot < (int64_t)a.n_pages << a.page_shift;
+        const int64_t page = slot >> a.page_shift;
+        at = (((size_t)page * nk << a.page_shift) + (size_t)(slot - (page << a.page_shift))) * a.hd;
+    }
+    const size_t pool_step = (size_t)a.hd << a.page_shift;
+    stage_turn(a.turn, pos, cs);
+    for (int h0 = blockIdx.y * per; h0 < total; h0 += per * gridDim.y) {
+        const int h = h0 + threadIdx.x / G;
+        const bool real = h < total, is_v = STORE && h >= nq + nk;
+        const int which = h >= nq, head = h - (is_v ? nq + nk : which ? nq : 0);
+        const HeadSet &set = a.set[which];
+        const T *const x = (real ? is_v ? (const T *)a.v + (size_t)row * a.v_stride : (const T *)set.x + (size_t)row * set.x_stride : (const T *)a.set[0].x) +
+                           (real ? (size_t)head * a.hd : 0);
+        T va[U][V], vb[U][V];
+        float wa[U][V], wb[U][V];
+        const float *const w = real && !is_v ? set.norm : nullptr;
+        double sum = 0;
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const int unit = lane + j * G;
+            if (!real || unit >= units) continue;
+            const Unit<V> u(unit, is_v ? 0 : a.turn.rot, INTER);
+            load_n<V>(x + u.at0, va[j]);
+            load_n<V>(x + u.at1, vb[j]);
+            if (w) {
+                load_n<V>(w + u.at0, wa[j]);
+                load_n<V>(w + u.at1, wb[j]);
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const double p = to_f32(va[j][i]), q = to_f32(vb[j][i]);
+                sum += p * p + q * q;
+            }
+        }
+        const float scale = rsqrt_(group_sum(sum, G) / a.hd + a.eps);
+        if (!real) continue;
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const int unit = lane + j * G;
+            if (unit >= units) continue;
+            float fa[V], fb[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                fa[i] = to_f32(va[j][i]);
+                fb[i] = to_f32(vb[j][i]);
+                if (w) {
+                    fa[i] = fa[i] * scale * wa[j][i];
+                    fb[i] = fb[i] * scale * wb[j][i];
+                }
+            }
+            const Unit<V> u(unit, is_v ? 0 : a.turn.rot, INTER);
+            if (STORE && which) {
+                if (stored) turn_unit<V>(u, fa, fb, (C *)(is_v ? a.v_pool : set.out) + at + head * pool_step, unit, INTER, cs, 1.0f);
+            } else {
+                turn_unit<V>(u, fa, fb, (T *)set.out + (size_t)row * set.out_stride + (size_t)head * a.hd, unit, INTER, cs, 1.0f);
+            }
+        }
+    }
+}
+
 // Workgroups that share a row: as many as give a thread one unit while the launch has
 // less than four a CU or so (us, with them / one a row, 32 heads of 128: 1 row 2.39 /
 // 2.61, 16 rows 3.07 / 3.50, 333 rows 3.90 / 4.23; an append of 16 rows 3.39 / 4.54).
@@ -239,6 +341,41 @@ hipError_t launch_rope(const RopeArgs &a, hipStream_t s) {
     else if (a.type == kF16) KORE_ROPE_CASE(half_t);
     else KORE_ROPE_CASE(bhalf_t);
 #undef KORE_ROPE_CASE
+}
+
+hipError_t launch_heads(const HeadsArgs &a, hipStream_t s) {
+    const int tb = type_bytes(a.type);
+    bool v4 = fours(a.turn.rot, a.hd);
+    for (const HeadSet &t : a.set) {
+        v4 = v4 && t.x_stride % 4 == 0 && aligned(tb, t.x) && aligned(4, t.norm);
+        const bool pool = a.slot && &t == &a.set[1];
+        v4 = v4 && (pool ? aligned(type_bytes(a.cache_type), t.out, a.v_pool) : t.out_stride % 4 == 0 && aligned(tb, t.out));
+    }
+    if (a.slot) v4 = v4 && a.v_stride % 4 == 0 && aligned(tb, a.v);
+    const int units = a.hd / (v4 ? 8 : 2);
+    int G = 1;
+    while (G < units && G < 64) G *= 2;
+    const dim3 grid = row_grid(a.n_tok, (a.set[0].n_head + a.set[1].n_head * (a.slot ? 2 : 1)) * G);
+#define KORE_HEADS_CASE(T, C, STORE)                                                                              \
+    do {                                                                                                          \
+        if (v4 && units > 64 && a.turn.interleaved) return launch(heads_kernel<T, C, 4, 2, true, STORE>, grid, kThreads, 0, s, a, G);  \
+        else if (v4 && units > 64) return launch(heads_kernel<T, C, 4, 2, false, STORE>, grid, kThreads, 0, s, a, G);                  \
+        else if (v4 && a.turn.interleaved) return launch(heads_kernel<T, C, 4, 1, true, STORE>, grid, kThreads, 0, s, a, G);           \
+        else if (v4) return launch(heads_kernel<T, C, 4, 1, false, STORE>, grid, kThreads, 0, s, a, G);                                \
+        else if (a.turn.interleaved) return launch(heads_kernel<T, C, 1, 8, true, STORE>, grid, kThreads, 0, s, a, G);                 \
+        else return launch(heads_kernel<T, C, 1, 8, false, STORE>, grid, kThreads, 0, s, a, G);                                        \
+    } while (0)
+    if (!a.slot) {
+        if (a.type == kF32) KORE_HEADS_CASE(float, float, false);
+        else if (a.type == kF16) KORE_HEADS_CASE(half_t, half_t, false);
+        else KORE_HEADS_CASE(bhalf_t, bhalf_t, false);
+    }
+    if (a.type == kF32 && a.cache_type == kF32) KORE_HEADS_CASE(float, float, true);
+    else if (a.type == kF32 && a.cache_type == kF16) KORE_HEADS_CASE(float, half_t, true);
+    else if (a.type == kF32) KORE_HEADS_CASE(float, bhalf_t, true);
+    else if (a.type == kF16) KORE_HEADS_CASE(half_t, half_t, true);
+    else KORE_HEADS_CASE(bhalf_t, bhalf_t, true);
+#undef KORE_HEADS_CASE
 }
 
 hipError_t launch_append(const AppendArgs &a, hipStream_t s) {

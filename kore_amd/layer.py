@@ -7,6 +7,7 @@ libkore_attn's decode on one stream.
     w = LayerWeights.upload(types, mats, attn_norm, ffn_norm, bq, bk, bv, n_embd, n_ff, kv_dim)
     L.decode_dev(w, attn, layer, pos, x_ptr)       # x (device) updated in place
     L.paged_dev(w, kv, layer, batch, x_ptr)        # rows of several sequences over a paged.PagedKV
+    L.paged_ex_dev(w, kv, layer, batch, x_ptr, pos, slot, q_norm, k_norm, tree)   # drafted trees, normalised heads
 
 No CPU fallback: without the built library or a GPU every call raises.
 """
@@ -36,12 +37,20 @@ class _Weights(C.Structure):
                                    "attn_norm", "ffn_norm", "bq", "bk", "bv")]
 
 
+class _PagedOpts(C.Structure):
+    """kore_layer_paged_opts"""
+    _fields_ = [("pos", _vp), ("slot", _vp), ("q_norm", _vp), ("k_norm", _vp), ("tree", C.POINTER(paged.TreeStruct)),
+                ("window", _i)]
+
+
 SYMBOLS = [
     ("kore_layer_create", _i, [C.POINTER(_vp), _i, _i, _i, _i, _f]),
     ("kore_layer_destroy", None, [_vp]),
     ("kore_layer_decode_dev", _i, [_vp, C.POINTER(_Weights), _vp, _i, _i, _vp, _i, _vp]),
     ("kore_layer_prefill_dev", _i, [_vp, C.POINTER(_Weights), _vp, _i, _i, _i, _vp, _vp]),
     ("kore_layer_paged_dev", _i, [_vp, C.POINTER(_Weights), _vp, _i, C.POINTER(paged.BatchStruct), _vp, _vp, _vp]),
+    ("kore_layer_paged_ex_dev", _i, [_vp, C.POINTER(_Weights), _vp, _i, C.POINTER(paged.BatchStruct), C.POINTER(_PagedOpts),
+                                     _vp, _vp, _vp]),
     ("kore_layer_sync", _i, [_vp]),
     ("kore_layer_last_error", C.c_char_p, [_vp]),
 ]
@@ -143,6 +152,16 @@ class Layer:
         s = w.struct()
         self._check(lib().kore_layer_paged_dev(self._h, C.byref(s), kv.handle, layer, C.byref(batch.struct), x_ptr,
                                                workspace, stream))
+
+    def paged_ex_dev(self, w: LayerWeights, kv: "paged.PagedKV", layer: int, batch: "paged.Batch", x_ptr: int, pos: int,
+                     slot: int, q_norm: int | None = None, k_norm: int | None = None, tree: "paged.Tree | None" = None,
+                     window: int = 0, workspace: int | None = None, stream=None) -> None:
+        """paged_dev with the rows' positions and slots (device, as PagedKV.plan_dev leaves them), norms of q's and k's heads
+        (device, head_dim weights), and the rows of a sequence as a tree."""
+        s = w.struct()
+        o = _PagedOpts(pos, slot, q_norm, k_norm, None if tree is None else C.pointer(tree.struct), window)
+        self._check(lib().kore_layer_paged_ex_dev(self._h, C.byref(s), kv.handle, layer, C.byref(batch.struct), C.byref(o),
+                                                  x_ptr, workspace, stream))
 
     def sync(self):
         self._check(lib().kore_layer_sync(self._h))

@@ -4,6 +4,8 @@ scaled for contexts past the trained one.
 
     r = Rope(Config(rot_dim=128, scaling="yarn", factor=4.0, orig_ctx=32768))
     r.apply_dev("f32", n_tok, n_head, head_dim, x_ptr, pos_ptr, out_ptr, stream=s)
+    r.norm_dev("bf16", n_tok, head_dim, [Heads(q_ptr, q_ptr, n_head, head_dim, norm=q_norm_ptr),
+                                         Heads(k_ptr, k_ptr, n_head_kv, head_dim, norm=k_norm_ptr)], pos_ptr, stream=s)
 
 Device pointers are plain integers.  There is no CPU fallback: without the built
 library or a GPU every call raises.
@@ -35,10 +37,16 @@ class RopeConfig(C.Structure):
                 ("beta_fast", _f), ("beta_slow", _f), ("magnitude", _f), ("freq_factors", _vp)]
 
 
+class HeadsStruct(C.Structure):
+    """kore_rope_heads"""
+    _fields_ = [("x", _vp), ("out", _vp), ("x_stride", _i64), ("out_stride", _i64), ("n_head", _i), ("norm", _vp)]
+
+
 SYMBOLS = [
     ("kore_rope_create", _i, [C.POINTER(_vp), C.POINTER(RopeConfig)]),
     ("kore_rope_destroy", None, [_vp]),
     ("kore_rope_apply_dev", _i, [_vp, _i, _i, _i, _i, _vp, _i64, _vp, _vp, _i64, _i, _vp]),
+    ("kore_rope_norm_dev", _i, [_vp, _i, _i, _i, C.POINTER(HeadsStruct), _i, _vp, _f, _vp]),
     ("kore_rope_get_freqs", _i, [_vp, _vp, C.POINTER(_f)]),
     ("kore_rope_sync", _i, [_vp]),
     ("kore_rope_last_error", C.c_char_p, [_vp]),
@@ -96,6 +104,18 @@ class Config:
                                  beta_slow, magnitude, None if self.factors is None else self.factors.ctypes.data)
 
 
+class Heads:
+    """A set of rows of n_head heads of head_dim values (kore_rope_heads): device pointers of the rows, of those that they
+    become and of the norm's weights (None: the heads are turned only).  Strides in elements, None: rows one behind the
+    other."""
+
+    def __init__(self, x: int, out: int, n_head: int, head_dim: int, norm: int | None = None, x_stride: int | None = None,
+                 out_stride: int | None = None):
+        n = n_head * head_dim
+        self.struct = HeadsStruct(x, out, n if x_stride is None else x_stride, n if out_stride is None else out_stride, n_head,
+                                  norm)
+
+
 class Rope:
     """kore_rope_t: a rotary plan on the current HIP device."""
 
@@ -121,6 +141,12 @@ class Rope:
         self._check(lib().kore_rope_apply_dev(self._h, type_code(dtype), n_tok, n_head, head_dim, x,
                                               n if x_stride is None else x_stride, pos, out,
                                               n if out_stride is None else out_stride, int(transpose), stream))
+
+    def norm_dev(self, dtype: str, n_tok: int, head_dim: int, sets, pos: int, eps: float = 1e-6, stream=None) -> None:
+        """One or two sets (Heads) of n_tok rows: each head over its root mean square, times its set's weights, then turned
+        to the row's position (pos: device, int32; rows with a negative one are left as they are)."""
+        a = (HeadsStruct * len(sets))(*[s.struct for s in sets])
+        self._check(lib().kore_rope_norm_dev(self._h, type_code(dtype), n_tok, head_dim, a, len(sets), pos, eps, stream))
 
     def freqs(self):
         """(frequencies [rot_dim / 2], magnitude)"""
