@@ -35,6 +35,7 @@ struct Cut {
     Divisor by_rep, by_heads;   // by rep, and by the kv-heads
     int target;      // a split has all work / target, in tiles x keys, or more; 0: nothing is split
     int min_len;     // a split's fewest keys
+    int at_once;     // trees: workgroups that the card holds at once, to be filled by splits; 0: by target
 };
 
 // A launch over tiles; part_o [part][dim / 4][row] float4 and part_ml [part][row]
@@ -164,6 +165,23 @@ __device__ __forceinline__ T last_lane(T x) {
     return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
 }
 
+// The length of a tree's splits.  Trees of one step are much alike, their tiles few and
+// long: what counts is that the workgroups fill the card once.  Of n workgroups' work
+// cut into pieces of one length, a tile's last piece is half as long in the mean, so that
+// all / (n - tiles / 2) makes some n of them; where it makes more, the length grows by
+// eighths until it does not.  (Lane s has sequence s's share; 64 sequences at most.)
+__device__ __forceinline__ int fitting_len(const Cut &c, const Share &r, float all, float tiles, int nkv) {
+    const float n = (float)c.at_once;
+    float want = fmaxf(all / (n - 0.5f * tiles), (float)c.min_len);
+    for (int i = 0; i < 16; ++i) {   // (to six times the first: two pieces of a tile are long one by then)
+        const int len = ((int)fminf(want, 1e9f) + 63) & ~63;
+        const unsigned pieces = max(((unsigned)r.keys + (unsigned)len - 1) / (unsigned)len, 1u);
+        if (last_lane(prefix_sum((float)r.tiles * (float)nkv * (float)pieces)) <= n) return len;
+        want = (float)len * 1.125f;
+    }
+    return 1 << 30;
+}
+
 // The place of number `id`, false where there is none.  Numbers run over the
 // sequences, then a sequence's tiles from the last (which has the most keys),
 // then its splits, then the kv-heads.  by_tile (the merge): over the split tiles
@@ -185,8 +203,14 @@ __device__ __forceinline__ bool place_of(const Batch &b, const Cut &c, int id, i
             const Share t = share(s0);
             w += (float)t.tiles * (float)t.keys;
         }
-        const float each = ceilf(last_lane(prefix_sum(w)) * (float)nkv / (float)c.target);
-        len = max(c.min_len, ((int)fminf(each, 1e9f) + 63) & ~63);
+        const float all = last_lane(prefix_sum(w)) * (float)nkv;
+        const float tiles = TREE && c.at_once ? last_lane(prefix_sum((float)r.tiles)) * (float)nkv : 0.f;
+        if (TREE && c.at_once && tiles <= (float)c.at_once) {
+            len = fitting_len(c, r, all, tiles, nkv);
+        } else {
+            const float each = ceilf(all / (float)c.target);
+            len = max(c.min_len, ((int)fminf(each, 1e9f) + 63) & ~63);
+        }
     }
     int at = 0, part_at = 0;
     for (int s0 = 0; s0 < b.n_seq; s0 += 64) {

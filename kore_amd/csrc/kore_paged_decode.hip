@@ -650,7 +650,25 @@ hipError_t launch_attend(const AttendArgs &a, hipStream_t s) {
     // 128 rows a tile, 28/4/128 at 32768 keys, new rows 2, 6, 9, 18: fp16 20.7 / 26.6, 27.5 / 26.7, 42.3 / 26.7, 53.3 /
     // 28.8; fp32 rows and cache 32 / 55, 56 / 57, 80 / 56, 124 / 61; 16 sequences of 2048, fp16: 23.4 / 27.8, 30.9 / 27.9,
     // 30.0 / 28.3, 47.5 / 36.5.
-    const bool chunk = (long long)max_q * d.cut.rep > 3 * kRows;
+    bool chunk = (long long)max_q * d.cut.rep > 3 * kRows;
+    // Trees have up to some hundred rows a kv-head, and every tile reads all keys of its sequence: which tiles take less time
+    // goes by both.  A launch of either takes a start, the merge in it (more of it for wide heads in tiles of 16, and for many
+    // tiles of 128), and so much for each key of each tile: us, heads of 128, fitted to 1 to 16 trees of 8 to 32 tokens over
+    // 500 to 8000 keys, run with both.  Over 171 such cases and other heads it takes 1.02 times the better tiles' time (1.42
+    // at most).  us, 16 / 128 rows a tile, 28/4/128, 1 tree of 8 over 500, of 32 over 8000, 16 of 32 over 2000: fp16 10.5 /
+    // 14.3, 32.4 / 20.8, 82 / 44; fp32 rows over fp16 12.2 / 18.3, 34.0 / 28.4, 86 / 62; fp32 cache 12.4 / 23.1, 58 / 42, 199 / 118.
+    if (TREE) {
+        const bool f32 = a.cache_type == kF32, parts = a.type == kF32;
+        const auto us = [&](int tile, double start, double each, double full) {
+            const long long of_all = (long long)a.b.n_tok * d.cut.rep / tile + a.b.n_seq;
+            const long long of_each = ((long long)max_q * d.cut.rep + tile - 1) / tile * a.b.n_seq;
+            const double tiles = (double)std::min(of_all, of_each) * a.n_head_kv;
+            const double keys = (double)std::min((long long)a.b.pages_stride << a.page_shift, (long long)a.window + a.b.n_tok);
+            return start + full * std::min(tiles / 64, 1.0) + each * tiles * keys * padded_dim(a.hd) / 128;
+        };
+        chunk = us(kChunkRows, f32 ? 24 : parts ? 18 : 16, f32 ? 36e-5 : parts ? 15e-5 : 9e-5, 4) <
+                us(kRows, a.hd > 128 ? 22 : f32 ? 12 : 10, f32 ? 10.5e-5 : 4e-5, 0);
+    }
     const int rows = chunk ? kChunkRows : kRows;
     // the most (tile, kv-head)s that n_tok rows of n_seq sequences can be
     const long long tiles = ((long long)a.b.n_tok * d.cut.rep / rows + std::min(a.b.n_seq, a.b.n_tok)) * a.n_head_kv;
@@ -680,17 +698,21 @@ hipError_t launch_attend(const AttendArgs &a, hipStream_t s) {
     else if (few) d.cut.target = most > d.cut.min_len ? (int)(at_once - tiles) : 0;
     else if (a.b.n_seq == 1 || most <= kShort) d.cut.target = 0;
     else d.cut.target = (int)(chunk ? std::min<long long>(tiles / 2, at_once) : std::min<long long>(tiles, at_once / 2));
+    // Trees that are split at all fill the card once, where a lane has each sequence (fitting_len).  us, by target / so,
+    // 28/4/128: 16 of up to 32 over up to 8000 fp16 keys, fp32 rows 200 / 91; 8 of 32 over 4000, fp16 41 / 37; 32 of up to 16
+    // over up to 2000 fp32 keys 132 / 89; one of 63 over 131000 bf16 keys of 16/2/128 97 / 91.
+    if (TREE && d.cut.target && a.b.n_seq <= 64) d.cut.at_once = at_once;
     d.scale_log2 = (float)((double)a.scale * 1.4426950408889634074);
     const int hdp = padded_dim(a.hd);
-    d.places = (int)tiles + d.cut.target;
+    d.places = std::max((int)tiles + d.cut.target, d.cut.at_once);
     d.part_o = a.part;
-    d.parts = d.cut.target + (int)std::min<long long>(d.cut.target, tiles);
+    d.parts = std::max(d.cut.target + (int)std::min<long long>(d.cut.target, tiles), d.cut.at_once);
     d.part_ml = a.part + (size_t)d.parts * rows * hdp;
     const hipError_t e = chunk ? launch_chunk(d, s) : wide ? launch_decode<8, TREE>(d, s) : launch_decode<4, TREE>(d, s);
     if (e != hipSuccess || !d.cut.target) return e;
     // some eight workgroups a CU, where there are dims enough (32 sequences, fp16 cache: 57.8 us from cache, with one a CU
     // 78.3, with 32 59.9)
-    const int joined = (int)std::min<long long>(d.cut.target, tiles);   // the most tiles that can be split
+    const int joined = (int)std::min<long long>(std::max(d.cut.target, d.cut.at_once / 2), tiles);   // the most tiles that can be split
     const dim3 merge((unsigned)joined, (unsigned)std::clamp(8 * a.num_cu / joined, 1, a.hd / 4));
 #define KORE_MERGE(A)                                                                    \
     do {                                                                                 \
