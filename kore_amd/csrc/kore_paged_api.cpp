@@ -413,6 +413,7 @@ int kore_rope_norm_dev(kore_rope_t r, int type, int n_tok, int head_dim, const k
     a.eps = eps;
     a.n_tok = n_tok;
     a.hd = head_dim;
+    a.per_dim = 1.0 / head_dim;
     a.type = type;
     HIP_TRY(r, launch_heads(a, pick_stream(r, stream)));
     return KORE_PAGED_OK;
@@ -703,6 +704,7 @@ int kore_paged_append_rows_dev(kore_paged_t h, int layer, const kore_paged_rows 
     a.eps = r->q_norm || r->k_norm ? r->norm_eps : 1.0f;
     a.n_tok = r->n_tok;
     a.hd = c.head_dim;
+    a.per_dim = 1.0 / c.head_dim;
     a.type = type;
     a.slot = r->slot;
     a.v = v;

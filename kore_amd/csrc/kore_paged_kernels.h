@@ -58,6 +58,7 @@ struct HeadsArgs {
     HeadSet set[2];          // q, k; sets without rows have no heads
     const int *pos;          // negative: the row is left
     float eps;
+    double per_dim;          // 1 / hd
     int n_tok, hd, type;
     // the store: v's rows, and where k's and v's go
     const int64_t *slot;     // NULL: no store

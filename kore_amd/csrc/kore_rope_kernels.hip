@@ -1,7 +1,7 @@
 // kore_rope_kernels.hip - rotary positions of rows, and the append of rotated
 // rows to a paged cache (gfx950).
 //
-// Both are bound by memory: 6 flops a pair beside 16 bytes (fp32) of traffic,
+// Rotation and append are bound by memory: 6 flops a pair beside 16 bytes (fp32) of traffic,
 // and a cosine and sine for each pair of a row, shared by its heads.  4096 bf16 rows of
 // 36 heads of 96: 11.8 us, 4.8 TB/s (a large copy: 5.1); three prompts' 1777 rows of
 // 28/4/128 into a bf16 cache: 15.1 us, 5.2 TB/s.  Few rows are a launch and three
@@ -231,18 +231,44 @@ __device__ __forceinline__ double group_sum(double x, int G) {
 // 1 / sqrt(x): the hardware's 26 bits or so, and one step of Newton's.
 __device__ __forceinline__ float rsqrt_(double x) {
     const double y = __builtin_amdgcn_rsq(x);
-    return (float)(y * (1.5 - 0.5 * x * y * y));
+    return (float)(y * __builtin_fma(-0.5 * x * y, y, 1.5));
 }
 
 // A block takes a row's heads of both sets, then, where it stores, those of v; or a
-// gridDim.y-th of them.
-template <class T, class C, int V, int U, bool INTER, bool STORE>
-__global__ __launch_bounds__(kThreads) void heads_kernel(HeadsArgs a, int G) {
+// gridDim.y-th of them.  G0: G, where it is known.  Instructions bound it as much as
+// memory: 16-bit rows are taken eight pairs a lane where they allow it (4000 bf16 rows of
+// 28 + 4 heads of 128: 12.6 us, 5.2 TB/s; four pairs a lane 15.3), and nothing is
+// requested before the turn, which would cost waves (18.4 with three heads ahead).  32
+// trees of up to 48 fp32 rows of 28/4/128 stored in bf16: 8.9 us, 4.5 TB/s.
+template <class T, class C, int V, int U, int G0, bool INTER, bool STORE>
+__global__ __launch_bounds__(kThreads) void heads_kernel(HeadsArgs a, int group) {
     __shared__ float2 cs[kMaxRot / 2];
-    const int row = blockIdx.x, pos = a.pos[row];
+    const int G = G0 ? G0 : group, row = blockIdx.x, pos = a.pos[row];
     if (pos < 0) return;
-    const int units = a.hd / (2 * V), lane = threadIdx.x & (G - 1), per = kThreads / G;
-    const int nq = a.set[0].n_head, nk = a.set[1].n_head, n_v = STORE ? nk : 0, total = nq + nk + n_v;
+    const int units = a.hd / (2 * V), in = threadIdx.x & (G - 1), per = (int)blockDim.x / G;
+    const int nq = a.set[0].n_head, nk = a.set[1].n_head, total = nq + nk + (STORE ? nk : 0), step = per * gridDim.y;
+    const int first = blockIdx.y * per + (int)threadIdx.x / G;
+    T xa[U][V], xb[U][V];
+    float wa[U][V], wb[U][V];
+    const auto request = [&](int h) {
+        const bool is_k = h >= nq, is_v = STORE && h >= nq + nk;
+        const T *const x = is_v   ? (const T *)a.v + (size_t)row * a.v_stride + (size_t)(h - nq - nk) * a.hd
+                           : is_k ? (const T *)a.set[1].x + (size_t)row * a.set[1].x_stride + (size_t)(h - nq) * a.hd
+                                  : (const T *)a.set[0].x + (size_t)row * a.set[0].x_stride + (size_t)h * a.hd;
+        const float *const w = is_v ? nullptr : is_k ? a.set[1].norm : a.set[0].norm;
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int unit = in + i * G;
+            if (h >= total || unit >= units) continue;
+            const Unit<V> u(unit, is_v ? 0 : a.turn.rot, INTER);
+            load_n<V>(x + u.at0, xa[i]);
+            load_n<V>(x + u.at1, xb[i]);
+            if (w) {
+                load_n<V>(w + u.at0, wa[i]);
+                load_n<V>(w + u.at1, wb[i]);
+            }
+        }
+    };
     size_t at = 0;   // of the slot's first head in a pool
     bool stored = false;
     if (STORE) {
@@ -251,57 +277,43 @@ __global__ __launch_bounds__(kThreads) void heads_kernel(HeadsArgs a, int G) {
         const int64_t page = slot >> a.page_shift;
         at = (((size_t)page * nk << a.page_shift) + (size_t)(slot - (page << a.page_shift))) * a.hd;
     }
-    const size_t pool_step = (size_t)a.hd << a.page_shift;
-    stage_turn(a.turn, pos, cs);
-    for (int h0 = blockIdx.y * per; h0 < total; h0 += per * gridDim.y) {
-        const int h = h0 + threadIdx.x / G;
-        const bool real = h < total, is_v = STORE && h >= nq + nk;
-        const int which = h >= nq, head = h - (is_v ? nq + nk : which ? nq : 0);
-        const HeadSet &set = a.set[which];
-        const T *const x = (real ? is_v ? (const T *)a.v + (size_t)row * a.v_stride : (const T *)set.x + (size_t)row * set.x_stride : (const T *)a.set[0].x) +
-                           (real ? (size_t)head * a.hd : 0);
-        T va[U][V], vb[U][V];
-        float wa[U][V], wb[U][V];
-        const float *const w = real && !is_v ? set.norm : nullptr;
+    for (int i = threadIdx.x; i < a.turn.rot / 2; i += blockDim.x) cs[i] = cos_sin(pos, a.turn.freq[i], a.turn.size);
+    __syncthreads();
+    for (int h = first; h - (int)threadIdx.x / G < total; h += step) {   // (the same rounds in every lane)
+        request(h);
+        const bool is_k = h >= nq, is_v = STORE && h >= nq + nk, normed = !is_v && (is_k ? a.set[1].norm : a.set[0].norm);
+        float fa[U][V], fb[U][V];
         double sum = 0;
 #pragma unroll
-        for (int j = 0; j < U; ++j) {
-            const int unit = lane + j * G;
-            if (!real || unit >= units) continue;
-            const Unit<V> u(unit, is_v ? 0 : a.turn.rot, INTER);
-            load_n<V>(x + u.at0, va[j]);
-            load_n<V>(x + u.at1, vb[j]);
-            if (w) {
-                load_n<V>(w + u.at0, wa[j]);
-                load_n<V>(w + u.at1, wb[j]);
+        for (int i = 0; i < U; ++i)
+#pragma unroll
+            for (int x = 0; x < V; ++x) {
+                const bool there = U * G0 == 0 ? in + i * G < units : in < units;
+                fa[i][x] = there ? to_f32(xa[i][x]) : 0.f;
+                fb[i][x] = there ? to_f32(xb[i][x]) : 0.f;
+                sum = __builtin_fma((double)fa[i][x], (double)fa[i][x], sum);
+                sum = __builtin_fma((double)fb[i][x], (double)fb[i][x], sum);
             }
+        const float scale = rsqrt_(group_sum(sum, G) * a.per_dim + a.eps);
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const double p = to_f32(va[j][i]), q = to_f32(vb[j][i]);
-                sum += p * p + q * q;
-            }
-        }
-        const float scale = rsqrt_(group_sum(sum, G) / a.hd + a.eps);
-        if (!real) continue;
+        for (int i = 0; i < U; ++i) {
+            const int unit = in + i * G;
+            if (h >= total || unit >= units) continue;
+            if (normed) {
 #pragma unroll
-        for (int j = 0; j < U; ++j) {
-            const int unit = lane + j * G;
-            if (unit >= units) continue;
-            float fa[V], fb[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                fa[i] = to_f32(va[j][i]);
-                fb[i] = to_f32(vb[j][i]);
-                if (w) {
-                    fa[i] = fa[i] * scale * wa[j][i];
-                    fb[i] = fb[i] * scale * wb[j][i];
+                for (int x = 0; x < V; ++x) {
+                    fa[i][x] = fa[i][x] * scale * wa[i][x];
+                    fb[i][x] = fb[i][x] * scale * wb[i][x];
                 }
             }
             const Unit<V> u(unit, is_v ? 0 : a.turn.rot, INTER);
-            if (STORE && which) {
-                if (stored) turn_unit<V>(u, fa, fb, (C *)(is_v ? a.v_pool : set.out) + at + head * pool_step, unit, INTER, cs, 1.0f);
+            if (STORE && is_k) {
+                C *const to = (C *)(is_v ? a.v_pool : a.set[1].out) + at + ((size_t)(is_v ? h - nq - nk : h - nq) << a.page_shift) * a.hd;
+                if (stored) turn_unit<V>(u, fa[i], fb[i], to, unit, INTER, cs, 1.0f);
             } else {
-                turn_unit<V>(u, fa, fb, (T *)set.out + (size_t)row * set.out_stride + (size_t)head * a.hd, unit, INTER, cs, 1.0f);
+                T *const to = is_k ? (T *)a.set[1].out + (size_t)row * a.set[1].out_stride + (size_t)(h - nq) * a.hd
+                                   : (T *)a.set[0].out + (size_t)row * a.set[0].out_stride + (size_t)h * a.hd;
+                turn_unit<V>(u, fa[i], fb[i], to, unit, INTER, cs, 1.0f);
             }
         }
     }
@@ -344,26 +356,41 @@ hipError_t launch_rope(const RopeArgs &a, hipStream_t s) {
 }
 
 hipError_t launch_heads(const HeadsArgs &a, hipStream_t s) {
-    const int tb = type_bytes(a.type);
-    bool v4 = fours(a.turn.rot, a.hd);
-    for (const HeadSet &t : a.set) {
-        v4 = v4 && t.x_stride % 4 == 0 && aligned(tb, t.x) && aligned(4, t.norm);
-        const bool pool = a.slot && &t == &a.set[1];
-        v4 = v4 && (pool ? aligned(type_bytes(a.cache_type), t.out, a.v_pool) : t.out_stride % 4 == 0 && aligned(tb, t.out));
-    }
-    if (a.slot) v4 = v4 && a.v_stride % 4 == 0 && aligned(tb, a.v);
-    const int units = a.hd / (v4 ? 8 : 2);
+    // Units of n pairs where heads, their parts, rows and buffers start at multiples of N values.
+    const auto wide = [&](int n) {
+        const auto fits = [n](const void *p, int type) { return (uintptr_t)p % (size_t)(n * type_bytes(type)) == 0; };
+        bool ok = a.turn.rot % (2 * n) == 0 && (a.hd - a.turn.rot) % (2 * n) == 0;
+        for (const HeadSet &t : a.set) {
+            const bool pool = a.slot && &t == &a.set[1];
+            ok = ok && t.x_stride % n == 0 && fits(t.x, a.type) && fits(t.norm, kF32) && (pool || t.out_stride % n == 0) &&
+                 fits(t.out, pool ? a.cache_type : a.type);
+        }
+        return ok && (!a.slot || (a.v_stride % n == 0 && fits(a.v, a.type) && fits(a.v_pool, a.cache_type)));
+    };
+    const int V = a.type != kF32 && wide(8) ? 8 : wide(4) ? 4 : 1, units = a.hd / (2 * V);
     int G = 1;
     while (G < units && G < 64) G *= 2;
-    const dim3 grid = row_grid(a.n_tok, (a.set[0].n_head + a.set[1].n_head * (a.slot ? 2 : 1)) * G);
-#define KORE_HEADS_CASE(T, C, STORE)                                                                              \
-    do {                                                                                                          \
-        if (v4 && units > 64 && a.turn.interleaved) return launch(heads_kernel<T, C, 4, 2, true, STORE>, grid, kThreads, 0, s, a, G);  \
-        else if (v4 && units > 64) return launch(heads_kernel<T, C, 4, 2, false, STORE>, grid, kThreads, 0, s, a, G);                  \
-        else if (v4 && a.turn.interleaved) return launch(heads_kernel<T, C, 4, 1, true, STORE>, grid, kThreads, 0, s, a, G);           \
-        else if (v4) return launch(heads_kernel<T, C, 4, 1, false, STORE>, grid, kThreads, 0, s, a, G);                                \
-        else if (a.turn.interleaved) return launch(heads_kernel<T, C, 1, 8, true, STORE>, grid, kThreads, 0, s, a, G);                 \
-        else return launch(heads_kernel<T, C, 1, 8, false, STORE>, grid, kThreads, 0, s, a, G);                                        \
+    const int lanes = (a.set[0].n_head + a.set[1].n_head * (a.slot ? 2 : 1)) * G;
+    // A workgroup's threads go round the row's heads a few times, so that the turn's start is a small part of its work (us, of
+    // 64 / 128 / 256 / 512 threads: 3000 fp16 rows of 14 + 2 heads of 64 5.1 / 5.7 / 7.4 / 11.5; 4000 bf16 rows of 28 + 4 of 128
+    // 13.2 / 12.5 / 13.9 / 17.0; 1000 fp32 rows of those 11.0 / 8.2 / 7.7 / 7.7).
+    const int threads = lanes <= 64 ? 64 : lanes <= 384 ? 128 : 256;
+    const dim3 grid((unsigned)a.n_tok, (unsigned)std::clamp(1024 / a.n_tok, 1, (lanes + threads - 1) / threads));
+#define KORE_HEADS_LAUNCH(T, C, V, U, G0, STORE)                                                                          \
+    return a.turn.interleaved ? launch(heads_kernel<T, C, V, U, G0, true, STORE>, grid, threads, 0, s, a, G)             \
+                              : launch(heads_kernel<T, C, V, U, G0, false, STORE>, grid, threads, 0, s, a, G)
+#define KORE_HEADS_CASE(T, C, STORE)                                                            \
+    do {                                                                                        \
+        if constexpr (sizeof(T) == 2) {                                                         \
+            if (V == 8 && G == 8) KORE_HEADS_LAUNCH(T, C, 8, 1, 8, STORE);                      \
+            if (V == 8) KORE_HEADS_LAUNCH(T, C, 8, 1, 0, STORE);                                \
+        } else {                                                                                \
+            if (V == 4 && G == 16) KORE_HEADS_LAUNCH(T, C, 4, 1, 16, STORE);                    \
+        }                                                                                       \
+        if (V == 4 && units <= 64) KORE_HEADS_LAUNCH(T, C, 4, 1, 0, STORE);                     \
+        if (V == 4) KORE_HEADS_LAUNCH(T, C, 4, 2, 0, STORE);                                    \
+        if (units <= 64) KORE_HEADS_LAUNCH(T, C, 1, 1, 0, STORE);                               \
+        KORE_HEADS_LAUNCH(T, C, 1, 8, 0, STORE);                                                \
     } while (0)
     if (!a.slot) {
         if (a.type == kF32) KORE_HEADS_CASE(float, float, false);
@@ -376,6 +403,7 @@ hipError_t launch_heads(const HeadsArgs &a, hipStream_t s) {
     else if (a.type == kF16) KORE_HEADS_CASE(half_t, half_t, true);
     else KORE_HEADS_CASE(bhalf_t, bhalf_t, true);
 #undef KORE_HEADS_CASE
+#undef KORE_HEADS_LAUNCH
 }
 
 hipError_t launch_append(const AppendArgs &a, hipStream_t s) {

@@ -42,6 +42,8 @@ class HeadsStruct(C.Structure):
     _fields_ = [("x", _vp), ("out", _vp), ("x_stride", _i64), ("out_stride", _i64), ("n_head", _i), ("norm", _vp)]
 
 
+_ONE_OR_TWO = (None, HeadsStruct * 1, HeadsStruct * 2)
+
 SYMBOLS = [
     ("kore_rope_create", _i, [C.POINTER(_vp), C.POINTER(RopeConfig)]),
     ("kore_rope_destroy", None, [_vp]),
@@ -145,8 +147,9 @@ class Rope:
     def norm_dev(self, dtype: str, n_tok: int, head_dim: int, sets, pos: int, eps: float = 1e-6, stream=None) -> None:
         """One or two sets (Heads) of n_tok rows: each head over its root mean square, times its set's weights, then turned
         to the row's position (pos: device, int32; rows with a negative one are left as they are)."""
-        a = (HeadsStruct * len(sets))(*[s.struct for s in sets])
-        self._check(lib().kore_rope_norm_dev(self._h, type_code(dtype), n_tok, head_dim, a, len(sets), pos, eps, stream))
+        n = len(sets)
+        a = _ONE_OR_TWO[n](*[s.struct for s in sets]) if 1 <= n <= 2 else None
+        self._check(lib().kore_rope_norm_dev(self._h, type_code(dtype), n_tok, head_dim, a, n, pos, eps, stream))
 
     def freqs(self):
         """(frequencies [rot_dim / 2], magnitude)"""
