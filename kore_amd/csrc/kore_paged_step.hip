@@ -31,12 +31,13 @@ __device__ __forceinline__ long long wave_prefix(long long x) {
     return x;
 }
 
-// Two numbers a thread: what the threads before it have, and all of them.
+// Two numbers a thread: what the threads before it have, and all of them.  (One barrier:
+// `waves` is not used again before another.)
 struct Sums {
     long long before[2], all[2];
 };
 __device__ __forceinline__ Sums block_sums(long long x, long long y, long long (*waves)[2]) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = blockDim.x >> 6;
     const long long px = wave_prefix(x), py = wave_prefix(y);
     if (lane == 63) {
         waves[wave][0] = px;
@@ -44,51 +45,55 @@ __device__ __forceinline__ Sums block_sums(long long x, long long y, long long (
     }
     __syncthreads();
     Sums s{{px - x, py - y}, {0, 0}};
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w)
+    for (int w = 0; w < n; ++w)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            if (w < wave) s.before[i] += waves[w][i];
-            s.all[i] += waves[w][i];
+            const long long of = waves[w][i];
+            if (w < wave) s.before[i] += of;
+            s.all[i] += of;
         }
-    __syncthreads();
     return s;
 }
 
 // ---- the plan ---------------------------------------------------------------------
 
 // A request: its rows, what it holds, the pages it has and those it needs.  One that no
-// table holds is bad and asks for nothing.
+// table holds asks for more rows than any step has.
+constexpr long long kBad = 1LL << 40;
 struct Request {
-    long long held;
-    int n, had, need;
+    int held, n, had, need;
     bool bad;
+    __device__ __forceinline__ long long rows() const { return bad ? kBad : n; }
 };
 __device__ __forceinline__ Request request(const PlanArgs &a, int s) {
     Request r{0, 0, 0, 0, false};
     if (s >= a.n_seq) return r;
-    const int n = a.n_new[s], held = a.kv_held[s];
-    const int mask = (1 << a.page_shift) - 1;
-    r.bad = n < 0 || held < 0 || (long long)n + held > (long long)a.pages_stride << a.page_shift || n > a.n_tok ||
-            (a.words && n > 64 * a.words);
-    r.held = held;
+    const int n = a.n_new[s], mask = (1 << a.page_shift) - 1;
+    r.held = a.kv_held[s];
+    r.bad = n < 0 || r.held < 0 || (long long)n + r.held > (long long)a.pages_stride << a.page_shift || (a.words && n > 64 * a.words);
     if (r.bad) return r;
     r.n = n;
-    r.had = (int)(((long long)held + mask) >> a.page_shift);
-    r.need = (int)(((long long)held + n + mask) >> a.page_shift) - r.had;
+    r.had = (int)(((long long)r.held + mask) >> a.page_shift);
+    r.need = (int)(((long long)r.held + n + mask) >> a.page_shift) - r.had;
     return r;
 }
 
+// What comes of the sums of all: 0, or why there is no step.
+__device__ __forceinline__ int status_of(const PlanArgs &a, const Sums &all, int n_free) {
+    if (n_free < 0 || n_free > a.n_pages || all.all[0] > a.n_tok) return -1;
+    return (int)min(max(all.all[1] - n_free, 0LL), (long long)INT_MAX);
+}
+
 // A row's depth in its tree and its mask: a walk from parent to parent, each before the
-// row, so that it ends.
-__device__ __forceinline__ int ancestors(const PlanArgs &a, int first, int i, unsigned long long *mask) {
-    const int *const parent = a.parent + first;
+// row, so that it ends.  parent_of(i): entry i of the sequence.
+template <class F>
+__device__ __forceinline__ int ancestors(const PlanArgs &a, int i, const F &parent_of, unsigned long long *mask) {
     int at = i, depth = 0;
     for (int w = a.words - 1; w >= 0; --w) {
         unsigned long long bits = 0;
         while (at >= 64 * w) {
             bits |= 1ULL << (at & 63);
-            const int up = parent[at];
+            const int up = parent_of(at);
             const bool root = up < 0 || up >= at;
             at = root ? -1 : up;
             if (!root) ++depth;
@@ -98,138 +103,154 @@ __device__ __forceinline__ int ancestors(const PlanArgs &a, int first, int i, un
     return depth;
 }
 
-// What a row gets: sequence s, its i-th new row (s < 0: no row).  page: of the row's slot.
-__device__ __forceinline__ void put_row(const PlanArgs &a, int row, bool real, int first, int i, int held, int page) {
+// A row's entries: the i-th new one of a sequence that held `held`, its slot on `page`.
+template <class F>
+__device__ __forceinline__ void put_row(const PlanArgs &a, int row, bool real, int i, int held, int page, const F &parent_of) {
+    unsigned long long *const mask = a.mask + (size_t)row * a.words;
     const int at = held + i;
     int pos = -1;
     long long slot = -1;
     if (real) {
-        pos = a.words ? held + ancestors(a, first, i, a.mask + (size_t)row * a.words) : at;
+        pos = a.words ? held + ancestors(a, i, parent_of, mask) : at;
         if (page >= 0 && page < a.n_pages) slot = ((long long)page << a.page_shift) + (at & ((1 << a.page_shift) - 1));
     } else {
-        for (int w = 0; w < a.words; ++w) a.mask[(size_t)row * a.words + w] = 0;
+        for (int w = 0; w < a.words; ++w) mask[w] = 0;
     }
     a.pos[row] = pos;
     a.slot[row] = slot;
 }
 
-// One workgroup: the requests' sums, what comes of them, and the tables of the sequences;
-// ROWS: also those of the rows (at most kThreads sequences).
-template <bool ROWS>
+// The last of n numbers, ascending from one that is x or less, that is x or less.
+template <class F>
+__device__ __forceinline__ int last_upto(const F &number, int n, int x) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int m = (lo + hi) >> 1;
+        if (number(m) <= x) lo = m;
+        else hi = m;
+    }
+    return lo;
+}
+
+// A step whose sequences have a thread each: every workgroup sums them all and takes
+// some of the rows, the first one also writes what is the sequences'.  Two rounds of
+// memory: the requests, the parents of the workgroup's rows and the number of free
+// pages; then the pages that rows go into, a sequence's last and those at the end of the
+// free ones.  (Workgroups but the first need inputs that the first does not overwrite.)
 __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
     __shared__ long long waves[kWaves][2];
-    __shared__ int any_bad;
-    __shared__ int starts[kThreads + 1], firsts[kThreads + 1], helds[kThreads];   // of a round's sequences
-    const int tid = threadIdx.x, n_free = a.n_free[0];
-    if (tid == 0) any_bad = n_free < 0 || n_free > a.n_pages;
-    __syncthreads();
-    // the sums of all
-    long long rows = 0, need = 0;
-    bool bad = false;
-    Request r = request(a, tid);
-    for (int s = tid; s < a.n_seq; s += kThreads) {
-        if (s != tid) r = request(a, s);
-        rows += r.n;
-        need += r.need;
-        bad |= r.bad;
+    __shared__ int starts[kThreads + 1], firsts[kThreads], helds[kThreads], lasts[kThreads], tops[kThreads], parents[kThreads];
+    const int tid = threadIdx.x, T = blockDim.x, page_mask = (1 << a.page_shift) - 1;
+    int base = blockIdx.x * T;
+    const int my_parent = a.words && base + tid < a.n_tok ? a.parent[base + tid] : -1;
+    const int n_free = a.n_free[0];
+    const Request r = request(a, tid);
+    if (tid < n_free && n_free <= a.n_pages) tops[tid] = a.free_pages[n_free - 1 - tid];
+    // of the pages that a sequence holds only the last has room
+    lasts[tid] = !r.bad && r.held & page_mask ? a.pages[(size_t)tid * a.pages_stride + (r.held >> a.page_shift)] : -1;
+    parents[tid] = my_parent;
+    helds[tid] = r.held;
+    const Sums sum = block_sums(r.rows(), r.need, waves);
+    const int status = status_of(a, sum, n_free);
+    const int start = status ? 0 : (int)sum.before[0], n_rows = status ? 0 : (int)sum.all[0];
+    starts[tid + 1] = status ? 0 : start + r.n;   // (behind the last sequence: all rows)
+    firsts[tid] = status ? 0 : (int)sum.before[1] - r.had;   // page j of the sequence is new page firsts + j of all
+    if (tid == 0) starts[0] = 0;
+    if (blockIdx.x == 0) {
+        if (tid == 0) {
+            a.status[0] = status;
+            a.n_free_out[0] = status ? n_free : n_free - (int)sum.all[1];
+            a.q_start[0] = 0;
+        }
+        if (tid < a.n_seq) {
+            a.q_start[tid + 1] = starts[tid + 1];
+            a.kv_len[tid] = status ? r.held : r.held + r.n;
+        }
     }
-    if (bad) any_bad = 1;
+    __syncthreads();
+    for (bool again = false; base < a.n_tok; base += gridDim.x * T, again = true) {
+        if (a.words && again) {
+            __syncthreads();
+            if (base + tid < a.n_tok) parents[tid] = a.parent[base + tid];
+            __syncthreads();
+        }
+        const int row = base + tid;
+        if (row >= a.n_tok) continue;
+        const bool real = row < n_rows;
+        int first = 0, i = 0, held = 0, page = -1;
+        if (real) {
+            const int l = last_upto([&](int m) { return starts[m]; }, a.n_seq, row);
+            first = starts[l];
+            i = row - first;
+            held = helds[l];
+            const int j = (held + i) >> a.page_shift;
+            if (j << a.page_shift >= held) {
+                const int number = firsts[l] + j;
+                page = number < T ? tops[number] : a.free_pages[n_free - 1 - number];
+                if (((held + i) & page_mask) == 0) a.pages[(size_t)l * a.pages_stride + j] = page;
+            } else {
+                page = lasts[l];
+            }
+        }
+        put_row(a, row, real, i, held, page, [&](int x) { return first + x >= base ? parents[first + x - base] : a.parent[first + x]; });
+    }
+}
+
+// Steps of more sequences, or of many rows whose outputs take the place of the inputs: one
+// workgroup for what is the sequences', kThreads of them at a time, then the rows.
+__global__ __launch_bounds__(kThreads) void plan_sequences_kernel(PlanArgs a) {
+    __shared__ long long waves[kWaves][2];
+    __shared__ int firsts[kThreads], hads[kThreads];   // of a round's sequences
+    const int tid = threadIdx.x, n_free = a.n_free[0];
+    long long rows = 0, need = 0;
+    for (int s = tid; s < a.n_seq; s += kThreads) {
+        const Request r = request(a, s);
+        rows += r.rows();
+        need += r.need;
+    }
     const Sums all = block_sums(rows, need, waves);
-    const long long missing = all.all[1] - n_free;
-    const int status = any_bad || all.all[0] > a.n_tok ? -1 : missing > 0 ? (int)min(missing, (long long)INT_MAX) : 0;
+    const int status = status_of(a, all, n_free);
     if (tid == 0) {
         a.status[0] = status;
         a.n_free_out[0] = status ? n_free : n_free - (int)all.all[1];
         a.q_start[0] = 0;
     }
-    // the sequences, a round of them at a time
     long long row_at = 0, need_at = 0;
     for (int s0 = 0; s0 < a.n_seq; s0 += kThreads) {
         const int s = s0 + tid;
-        if (a.n_seq > kThreads) r = request(a, s);
+        Request r = request(a, s);
         if (status) r.n = r.need = 0;
+        __syncthreads();
         const Sums sum = block_sums(r.n, r.need, waves);
         if (s < a.n_seq) {
             a.q_start[s + 1] = (int)(row_at + sum.before[0]) + r.n;
-            a.kv_len[s] = (int)r.held + r.n;
+            a.kv_len[s] = r.held + r.n;
         }
-        starts[tid + 1] = (int)(row_at + sum.before[0]) + r.n;   // (behind the last sequence: all rows)
-        firsts[tid] = (int)(need_at + sum.before[1]) - r.had;    // the j-th page of the sequence is number firsts + j
-        helds[tid] = (int)r.held;
-        if (tid == 0) starts[0] = (int)row_at;
+        firsts[tid] = (int)(need_at + sum.before[1]);
+        hads[tid] = r.had;
         __syncthreads();
-        // whose the number x is: the last sequence of the round that begins no later
-        const auto owner = [&](const auto &begins, int x) {
-            int lo = 0, hi = min(kThreads, a.n_seq - s0);   // begins(lo) <= x < begins(hi)
-            while (hi - lo > 1) {
-                const int m = (lo + hi) >> 1;
-                if (begins(m) <= x) lo = m;
-                else hi = m;
-            }
-            return lo;
-        };
-        if constexpr (ROWS) {
-            const int n_rows = (int)all.all[0];
-            for (int row = tid; row < a.n_tok; row += kThreads) {
-                const bool real = !status && row < n_rows;
-                int first = 0, i = 0, held = 0, page = -1;
-                if (real) {
-                    const int l = owner([&](int m) { return starts[m]; }, row);
-                    first = starts[l];
-                    i = row - first;
-                    held = helds[l];
-                    const int j = (held + i) >> a.page_shift;
-                    int *const entry = a.pages + (size_t)l * a.pages_stride + j;
-                    if (j << a.page_shift >= held) {   // a page that is new
-                        page = a.free_pages[n_free - 1 - (firsts[l] + j)];
-                        if (((held + i) & ((1 << a.page_shift) - 1)) == 0) *entry = page;
-                    } else {
-                        page = *entry;
-                    }
-                }
-                put_row(a, row, real, first, i, held, page);
-            }
-        } else {
-            // the round's new pages
-            const int n_need = (int)sum.all[1];
-            const int had = r.had;
-            __syncthreads();
-            firsts[tid] += had;
-            starts[tid] = had;   // (not needed any more)
-            __syncthreads();
-            for (int x = tid; x < n_need; x += kThreads) {
-                const int number = (int)need_at + x;
-                const int l = owner([&](int m) { return firsts[m]; }, number);
-                a.pages[(size_t)(s0 + l) * a.pages_stride + starts[l] + number - firsts[l]] = a.free_pages[n_free - 1 - number];
-            }
+        for (int x = tid; x < (int)sum.all[1]; x += kThreads) {   // the round's new pages
+            const int number = (int)need_at + x;
+            const int l = last_upto([&](int m) { return firsts[m]; }, min(kThreads, a.n_seq - s0), number);
+            a.pages[(size_t)(s0 + l) * a.pages_stride + hads[l] + number - firsts[l]] = a.free_pages[n_free - 1 - number];
         }
         row_at += sum.all[0];
         need_at += sum.all[1];
-        __syncthreads();
     }
-    if (ROWS && a.n_seq == 0)
-        for (int row = tid; row < a.n_tok; row += kThreads) put_row(a, row, false, 0, 0, 0, -1);
 }
-
-// The rows of a plan whose sequences are done, a thread each.
 __global__ __launch_bounds__(256) void plan_rows_kernel(PlanArgs a) {
     const int row = blockIdx.x * 256 + threadIdx.x;
     if (row >= a.n_tok) return;
     const bool real = row < a.q_start[a.n_seq];
     int first = 0, i = 0, held = 0, page = -1;
     if (real) {
-        int lo = 0, hi = a.n_seq;   // q_start[lo] <= row < q_start[hi]
-        while (hi - lo > 1) {
-            const int m = (lo + hi) >> 1;
-            if (a.q_start[m] <= row) lo = m;
-            else hi = m;
-        }
-        first = a.q_start[lo];
+        const int s = last_upto([&](int m) { return a.q_start[m]; }, a.n_seq, row);
+        first = a.q_start[s];
         i = row - first;
-        held = a.kv_len[lo] - (a.q_start[lo + 1] - first);
-        page = a.pages[(size_t)lo * a.pages_stride + ((held + i) >> a.page_shift)];
+        held = a.kv_len[s] - (a.q_start[s + 1] - first);
+        page = a.pages[(size_t)s * a.pages_stride + ((held + i) >> a.page_shift)];
     }
-    put_row(a, row, real, first, i, held, page);
+    put_row(a, row, real, i, held, page, [&](int x) { return a.parent[first + x]; });
 }
 
 // ---- what is kept -------------------------------------------------------------------
@@ -249,44 +270,49 @@ __device__ __forceinline__ End end_of(const KeepArgs &a, int s) {
     return e;
 }
 
-// A thread has 16 bytes of a position's K or V, of one kv-head of a layer, and moves them
-// from row to row, eight rows in flight: what it overwrites lies before all that it has
-// still to read, since the rows ascend.
-constexpr int kMoves = 256, kFlight = 8;
+// The moves of a sequence, by workgroup `part` of `share`.  A thread has 16 bytes of a
+// position's K or V, of one kv-head of a layer, and moves them from row to row, eight rows
+// in flight: what it overwrites lies before all that it has still to read, since the rows
+// ascend.
+constexpr int kMoveThreads = 256, kMoves = kMoveThreads, kFlight = 8;
 
-// Workgroups seq * share .. of a sequence share its pieces.
-__global__ __launch_bounds__(256) void move_kernel(KeepArgs a, int share) {
+__device__ __forceinline__ void move_rows(const KeepArgs &a, int seq, int part, int share) {
     __shared__ long long from[kMoves], to[kMoves];   // 16-byte pieces, from the head's first; from -1: nothing moves
-    const int seq = blockIdx.x / share, part = blockIdx.x - seq * share;
+    __shared__ int near[kMoveThreads];               // the first pages of the new rows
     const End e = end_of(a, seq);
     if (e.keep <= 0) return;
-    const int row_pieces = a.hd * type_bytes(a.cache_type) / 16;
+    const int row_pieces = a.hd * type_bytes(a.cache_type) / 16, held = e.kv - e.n;
     const long long head_pieces = (long long)row_pieces << a.page_shift, page_pieces = head_pieces * a.n_head_kv;
     const int per_pool = a.n_head_kv * row_pieces;   // pieces of a position's K or V
     const long long pieces = 2LL * per_pool * a.n_layer;
     const int *const table = a.pages + (size_t)seq * a.pages_stride;
+    const int first_page = max(held, 0) >> a.page_shift;
+    {
+        const int at = first_page + (int)threadIdx.x;
+        near[threadIdx.x] = at < a.pages_stride && at <= (e.kv - 1) >> a.page_shift ? table[at] : -1;
+    }
     const auto piece_of = [&](int pos) -> long long {
         const int at = pos >> a.page_shift;
         if (pos < 0 || at >= a.pages_stride) return -1;
-        const int page = table[at];
+        const int page = at - first_page < kMoveThreads ? near[at - first_page] : table[at];
         if (page < 0 || page >= a.n_pages) return -1;
         return page * page_pieces + (long long)(pos & ((1 << a.page_shift) - 1)) * row_pieces;
     };
     for (int i0 = 0; i0 < e.keep; i0 += kMoves) {
-        const int n = min(kMoves, e.keep - i0);
+        const int n = min(kMoves, e.keep - i0), i = i0 + threadIdx.x;
+        const int row = (int)threadIdx.x < n ? a.rows[e.start + i] : -1;
         __syncthreads();
         if ((int)threadIdx.x < n) {
-            const int i = i0 + threadIdx.x, row = a.rows[e.start + i];
             long long f = -1, t = -1;
             if (row >= 0 && row < e.n && row != i) {
-                f = piece_of(e.kv - e.n + row);
-                t = piece_of(e.kv - e.n + i);
+                f = piece_of(held + row);
+                t = piece_of(held + i);
             }
             from[threadIdx.x] = t < 0 ? -1 : f;
             to[threadIdx.x] = t;
         }
         __syncthreads();
-        for (long long id = (long long)part * 256 + threadIdx.x; id < pieces; id += share * 256) {
+        for (long long id = (long long)part * kMoveThreads + threadIdx.x; id < pieces; id += share * kMoveThreads) {
             const int pool = (int)(id / per_pool), in_pos = (int)(id - (long long)pool * per_pool);   // K and V of a layer side by side
             const int head = in_pos / row_pieces, piece = in_pos - head * row_pieces;
             uint4 *const base = (uint4 *)(pool & 1 ? a.v_pool : a.k_pool) + (long long)(pool >> 1) * a.n_pages * page_pieces +
@@ -304,59 +330,116 @@ __global__ __launch_bounds__(256) void move_kernel(KeepArgs a, int share) {
     }
 }
 
-// The lengths, and the pages that no position needs any more, by one workgroup: a wave
-// has a run of the sequences, 64 at a time in its lanes; it counts their pages, the waves
-// add up, and it goes through them again and writes.
-__global__ __launch_bounds__(kThreads) void ends_kernel(KeepArgs a) {
+// The lengths, and the pages that no position needs any more, by one workgroup.  A wave
+// has a run of the sequences, 64 at a time in its lanes; a lane takes a few pages of its
+// sequence, the wave together a sequence's many.  The pages are counted, the waves add
+// up, and each writes its own.
+constexpr int kFew = 4;
+struct Given {
+    int lo, hi, count;      // of the lane's sequence: entries of the table, those that are pages
+    int page[kFew];         // where they are few
+    __device__ __forceinline__ bool many() const { return hi - lo > kFew; }
+};
+__device__ __forceinline__ void give_back(const KeepArgs &a) {
     __shared__ long long waves[kWaves][2];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int each = (a.n_seq + kWaves - 1) / kWaves, s_first = wave * each, s_end = min(a.n_seq, s_first + each);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n_wave = blockDim.x >> 6;
+    const int each = (a.n_seq + n_wave - 1) / n_wave, s_first = wave * each, s_end = min(a.n_seq, s_first + each);
     const int mask = (1 << a.page_shift) - 1;
     const int n_free = a.n_free ? min(max(a.n_free[0], 0), a.n_pages) : 0;
+    const auto is_page = [&](int page) { return page >= 0 && page < a.n_pages; };
     const auto pages_of = [&](int kv) { return (int)min(((long long)kv + mask) >> a.page_shift, (long long)a.pages_stride); };
-    // every page of the run's sequences: visit(valid in this lane, page, lanes before it)
-    const auto each_page = [&](const auto &visit) {
-        for (int s0 = s_first; s0 < s_end; s0 += 64) {
-            int lo = 0, hi = 0;
-            if (s0 + lane < s_end) {
-                const End e = end_of(a, s0 + lane);
-                lo = pages_of(e.after);
-                hi = pages_of(e.kv);
-            }
-            for (unsigned long long left = __ballot(hi > lo); left; left &= left - 1) {
-                const int l = __builtin_ctzll(left), from = __builtin_amdgcn_readlane(lo, l), to = __builtin_amdgcn_readlane(hi, l);
-                const int *const table = a.pages + (size_t)(s0 + l) * a.pages_stride;
-                for (int j = from; j < to; j += 64) {
-                    const int page = j + lane < to ? table[j + lane] : -1;
-                    visit(page >= 0 && page < a.n_pages, page);
-                }
-            }
+    // the pages of lane l's sequence, which has many: visit(a page, or not, in each lane)
+    const auto each_page = [&](const Given &g, int s0, int l, const auto &visit) {
+        const int from = __builtin_amdgcn_readlane(g.lo, l), to = __builtin_amdgcn_readlane(g.hi, l);
+        const int *const table = a.pages + (size_t)(s0 + l) * a.pages_stride;
+        for (int j = from; j < to; j += 64) {
+            const int page = j + lane < to ? table[j + lane] : -1;
+            visit(is_page(page), page);
         }
     };
-    long long count = 0;
-    if (a.free_pages) each_page([&](bool valid, int) { count += __popcll(__ballot(valid)); });
-    const Sums sum = block_sums(lane == 0 ? count : 0, 0, waves);
-    long long at = n_free + __shfl(sum.before[0], 0);
-    if (a.free_pages)
-        each_page([&](bool valid, int page) {
-            const unsigned long long here = __ballot(valid);
-            const long long to = at + __popcll(here & ((1ULL << lane) - 1));
-            if (valid && to < a.n_pages) a.free_pages[to] = page;
-            at += __popcll(here);
-        });
-    if (a.n_free && threadIdx.x == 0) a.n_free_out[0] = (int)min(n_free + sum.all[0], (long long)a.n_pages);
+    const auto find = [&](int s0) {
+        Given g{0, 0, 0, {}};
+        if (s0 + lane < s_end) {
+            const End e = end_of(a, s0 + lane);
+            g.lo = pages_of(e.after);
+            g.hi = pages_of(e.kv);
+        }
+        const int *const table = a.pages + (size_t)min(s0 + lane, a.n_seq - 1) * a.pages_stride;
+#pragma unroll
+        for (int j = 0; j < kFew; ++j) {
+            g.page[j] = !g.many() && g.lo + j < g.hi ? table[g.lo + j] : -1;
+            g.count += is_page(g.page[j]);
+        }
+        for (unsigned long long left = __ballot(g.many()); left; left &= left - 1) {
+            const int l = __builtin_ctzll(left);
+            int count = 0;
+            each_page(g, s0, l, [&](bool real, int) { count += __popcll(__ballot(real)); });
+            if (lane == l) g.count = count;
+        }
+        return g;
+    };
+    // the first page of the batch becomes free page number `at`; the number behind its last
+    const auto put = [&](const Given &g, int s0, long long at) {
+        const long long upto = wave_prefix(g.count);
+        long long to = at + upto - g.count;
+#pragma unroll
+        for (int j = 0; j < kFew; ++j)
+            if (is_page(g.page[j])) {
+                if (to < a.n_pages) a.free_pages[to] = g.page[j];
+                ++to;
+            }
+        for (unsigned long long left = __ballot(g.many()); left; left &= left - 1) {
+            const int l = __builtin_ctzll(left);
+            long long next = at + __shfl(upto - g.count, l);
+            each_page(g, s0, l, [&](bool real, int page) {
+                const unsigned long long here = __ballot(real);
+                const long long mine = next + __popcll(here & ((1ULL << lane) - 1));
+                if (real && mine < a.n_pages) a.free_pages[mine] = page;
+                next += __popcll(here);
+            });
+        }
+        return at + __shfl(upto, 63);
+    };
+    if (a.n_free) {
+        Given g = find(s_first);
+        long long count = g.count;
+        for (int s0 = s_first + 64; s0 < s_end; s0 += 64) count += find(s0).count;
+        const Sums sum = block_sums(count, 0, waves);
+        long long at = put(g, s_first, n_free + __shfl(sum.before[0], 0));
+        for (int s0 = s_first + 64; s0 < s_end; s0 += 64) at = put(find(s0), s0, at);
+        if (threadIdx.x == 0) a.n_free_out[0] = (int)min(n_free + sum.all[0], (long long)a.n_pages);
+    }
     __syncthreads();
-    for (int s = threadIdx.x; s < a.n_seq; s += kThreads) a.kv_out[s] = end_of(a, s).after;
+    for (int s = threadIdx.x; s < a.n_seq; s += blockDim.x) a.kv_out[s] = end_of(a, s).after;
 }
 
-// Steps of up to so many rows and sequences are one workgroup's, rows and all.
+// One launch for both, where the lengths that the moves read are not those that are written.
+__global__ __launch_bounds__(kMoveThreads) void keep_kernel(KeepArgs a, int share) {
+    if (blockIdx.x == 0) return give_back(a);
+    const int id = blockIdx.x - 1, seq = id / share;
+    move_rows(a, seq, id - seq * share, share);
+}
+__global__ __launch_bounds__(kMoveThreads) void move_kernel(KeepArgs a, int share) {
+    const int seq = blockIdx.x / share;
+    move_rows(a, seq, blockIdx.x - seq * share, share);
+}
+__global__ __launch_bounds__(kThreads) void ends_kernel(KeepArgs a) { give_back(a); }
+
+// Rows that one workgroup takes where others must not be.
 constexpr int kOneRows = 4096;
+// Sequences whose pages four waves give back beside the moves.
+constexpr int kOneSeqs = 1024;
 
 }  // namespace
 
 hipError_t launch_plan(const PlanArgs &a, hipStream_t s) {
-    if (a.n_tok <= kOneRows && a.n_seq <= kThreads) return launch(plan_kernel<true>, dim3(1), kThreads, 0, s, a);
-    const hipError_t e = launch(plan_kernel<false>, dim3(1), kThreads, 0, s, a);
+    const bool in_place = a.kv_len == a.kv_held || a.n_free_out == a.n_free;
+    if (a.n_seq <= kThreads && (!in_place || a.n_tok <= kOneRows)) {
+        const int threads = (std::clamp(std::max(a.n_seq, a.n_tok), 1, kThreads) + 63) & ~63;
+        const int blocks = in_place ? 1 : std::max(1, (a.n_tok + threads - 1) / threads);
+        return launch(plan_kernel, dim3((unsigned)blocks), threads, 0, s, a);
+    }
+    const hipError_t e = launch(plan_sequences_kernel, dim3(1), kThreads, 0, s, a);
     if (e != hipSuccess || a.n_tok == 0) return e;
     return launch(plan_rows_kernel, dim3((unsigned)((a.n_tok + 255) / 256)), 256, 0, s, a);
 }
@@ -366,8 +449,10 @@ hipError_t launch_keep(const KeepArgs &a, hipStream_t s) {
     if (a.rows && a.n_seq && a.n_tok) {
         // (a launch has fewer than 2^32 threads)
         const long long pieces = 2LL * a.n_layer * a.n_head_kv * a.hd * type_bytes(a.cache_type) / 16;
-        const int share = (int)std::min<long long>((pieces + 255) / 256, (1 << 23) / a.n_seq);
-        const hipError_t e = launch(move_kernel, dim3((unsigned)(share * a.n_seq)), 256, 0, s, a, share);
+        const int share = (int)std::min<long long>((pieces + kMoveThreads - 1) / kMoveThreads, (1 << 23) / a.n_seq);
+        if (a.n_seq <= kOneSeqs && a.kv_out != a.kv_len)
+            return launch(keep_kernel, dim3((unsigned)(1 + share * a.n_seq)), kMoveThreads, 0, s, a, share);
+        const hipError_t e = launch(move_kernel, dim3((unsigned)(share * a.n_seq)), kMoveThreads, 0, s, a, share);
         if (e != hipSuccess) return e;
     }
     return launch(ends_kernel, dim3(1), kThreads, 0, s, a);

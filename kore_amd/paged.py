@@ -168,6 +168,9 @@ class PagedKV:
         if rc != KORE_PAGED_OK:
             raise PagedError(rc, lib().kore_paged_last_error(None).decode())
         self._h = h
+        L = lib()
+        self._plan, self._rows, self._tree, self._keep = (L.kore_paged_plan_dev, L.kore_paged_append_rows_dev,
+                                                          L.kore_paged_attend_tree_dev, L.kore_paged_keep_dev)
         self.kv_dim, self.E = n_head_kv * head_dim, n_head * head_dim
 
     def _check(self, rc: int) -> None:
@@ -197,28 +200,34 @@ class PagedKV:
 
     def plan_dev(self, plan: Plan, stream=None) -> None:
         """Makes a step's tables of the requests' lengths, and takes the pages that it needs."""
-        self._check(lib().kore_paged_plan_dev(self._h, plan._ref, stream))
+        rc = self._plan(self._h, plan._ref, stream)
+        if rc:
+            self._check(rc)
 
     def append_rows_dev(self, layer: int, rows: Rows, dtype: str, k: int, v: int, q: int | None = None, q_out: int | None = None,
                         k_stride: int | None = None, v_stride: int | None = None, q_stride: int | None = None,
                         q_out_stride: int | None = None, stream=None) -> None:
         """append_dev by the rows' own positions and slots, with the norms of q's and k's heads."""
-        self._check(lib().kore_paged_append_rows_dev(
-            self._h, layer, rows._ref, type_code(dtype), k, self.kv_dim if k_stride is None else k_stride, v,
-            self.kv_dim if v_stride is None else v_stride, q, self.E if q_stride is None else q_stride, q_out,
-            self.E if q_out_stride is None else q_out_stride, stream))
+        rc = self._rows(self._h, layer, rows._ref, type_code(dtype), k, self.kv_dim if k_stride is None else k_stride, v,
+                        self.kv_dim if v_stride is None else v_stride, q, self.E if q_stride is None else q_stride, q_out,
+                        self.E if q_out_stride is None else q_out_stride, stream)
+        if rc:
+            self._check(rc)
 
     def attend_tree_dev(self, layer: int, batch: Batch, tree: Tree, dtype: str, q: int, out: int, q_stride: int | None = None,
                         out_stride: int | None = None, scale: float = 0.0, window: int = 0, workspace: int | None = None,
                         stream=None) -> None:
         """attend_dev for new rows that are a tree: each attends what its sequence held before, and the new ones of its mask."""
-        self._check(lib().kore_paged_attend_tree_dev(
-            self._h, layer, batch._ref, tree._ref, type_code(dtype), q, self.E if q_stride is None else q_stride, out,
-            self.E if out_stride is None else out_stride, scale, window, workspace, stream))
+        rc = self._tree(self._h, layer, batch._ref, tree._ref, type_code(dtype), q, self.E if q_stride is None else q_stride, out,
+                        self.E if out_stride is None else out_stride, scale, window, workspace, stream)
+        if rc:
+            self._check(rc)
 
     def keep_dev(self, keep: Keep, stream=None) -> None:
         """Moves the kept rows together in every layer, and gives back lengths and pages."""
-        self._check(lib().kore_paged_keep_dev(self._h, keep._ref, stream))
+        rc = self._keep(self._h, keep._ref, stream)
+        if rc:
+            self._check(rc)
 
     def workspace_bytes(self) -> int:
         return int(lib().kore_paged_workspace_bytes(self._h))

@@ -42,7 +42,7 @@ class HeadsStruct(C.Structure):
     _fields_ = [("x", _vp), ("out", _vp), ("x_stride", _i64), ("out_stride", _i64), ("n_head", _i), ("norm", _vp)]
 
 
-_ONE_OR_TWO = (None, HeadsStruct * 1, HeadsStruct * 2)
+_SETS = {1: HeadsStruct * 1, 2: HeadsStruct * 2}
 
 SYMBOLS = [
     ("kore_rope_create", _i, [C.POINTER(_vp), C.POINTER(RopeConfig)]),
@@ -81,9 +81,10 @@ class PagedError(RuntimeError):
 
 
 def type_code(name: str) -> int:
-    if name not in TYPES:
+    code = TYPES.get(name)
+    if code is None:
         raise ValueError(f"type {name!r} is not one of {sorted(TYPES)}")
-    return TYPES[name]
+    return code
 
 
 class Config:
@@ -106,7 +107,7 @@ class Config:
                                  beta_slow, magnitude, None if self.factors is None else self.factors.ctypes.data)
 
 
-class Heads:
+class Heads(HeadsStruct):
     """A set of rows of n_head heads of head_dim values (kore_rope_heads): device pointers of the rows, of those that they
     become and of the norm's weights (None: the heads are turned only).  Strides in elements, None: rows one behind the
     other."""
@@ -114,8 +115,7 @@ class Heads:
     def __init__(self, x: int, out: int, n_head: int, head_dim: int, norm: int | None = None, x_stride: int | None = None,
                  out_stride: int | None = None):
         n = n_head * head_dim
-        self.struct = HeadsStruct(x, out, n if x_stride is None else x_stride, n if out_stride is None else out_stride, n_head,
-                                  norm)
+        super().__init__(x, out, n if x_stride is None else x_stride, n if out_stride is None else out_stride, n_head, norm)
 
 
 class Rope:
@@ -128,6 +128,7 @@ class Rope:
         if rc != KORE_PAGED_OK:
             raise PagedError(rc, lib().kore_rope_last_error(None).decode())
         self._h = h
+        self._norm = lib().kore_rope_norm_dev
         self.rot_dim = config.rot_dim
 
     def _check(self, rc: int) -> None:
@@ -148,8 +149,10 @@ class Rope:
         """One or two sets (Heads) of n_tok rows: each head over its root mean square, times its set's weights, then turned
         to the row's position (pos: device, int32; rows with a negative one are left as they are)."""
         n = len(sets)
-        a = _ONE_OR_TWO[n](*[s.struct for s in sets]) if 1 <= n <= 2 else None
-        self._check(lib().kore_rope_norm_dev(self._h, type_code(dtype), n_tok, head_dim, a, n, pos, eps, stream))
+        a = _SETS[n](*sets) if n in _SETS else None   # (another number is refused by the call)
+        rc = self._norm(self._h, type_code(dtype), n_tok, head_dim, a, n, pos, eps, stream)
+        if rc:
+            self._check(rc)
 
     def freqs(self):
         """(frequencies [rot_dim / 2], magnitude)"""
