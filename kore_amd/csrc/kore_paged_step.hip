@@ -274,11 +274,12 @@ __device__ __forceinline__ End end_of(const KeepArgs &a, int s) {
 // position's K or V, of one kv-head of a layer, and moves them from row to row, eight rows
 // in flight: what it overwrites lies before all that it has still to read, since the rows
 // ascend.
-constexpr int kMoveThreads = 256, kMoves = kMoveThreads, kFlight = 8;
+constexpr int kMoveThreads = 256, kFlight = 8;   // (at most)
 
 __device__ __forceinline__ void move_rows(const KeepArgs &a, int seq, int part, int share) {
-    __shared__ long long from[kMoves], to[kMoves];   // 16-byte pieces, from the head's first; from -1: nothing moves
+    __shared__ long long from[kMoveThreads], to[kMoveThreads];   // 16-byte pieces, from the head's first; from -1: nothing moves
     __shared__ int near[kMoveThreads];               // the first pages of the new rows
+    const int T = blockDim.x;
     const End e = end_of(a, seq);
     if (e.keep <= 0) return;
     const int row_pieces = a.hd * type_bytes(a.cache_type) / 16, held = e.kv - e.n;
@@ -287,20 +288,21 @@ __device__ __forceinline__ void move_rows(const KeepArgs &a, int seq, int part, 
     const long long pieces = 2LL * per_pool * a.n_layer;
     const int *const table = a.pages + (size_t)seq * a.pages_stride;
     const int first_page = max(held, 0) >> a.page_shift;
-    {
-        const int at = first_page + (int)threadIdx.x;
-        near[threadIdx.x] = at < a.pages_stride && at <= (e.kv - 1) >> a.page_shift ? table[at] : -1;
-    }
+    const int at_page = first_page + (int)threadIdx.x;
+    const int my_page = at_page < a.pages_stride && at_page <= (e.kv - 1) >> a.page_shift ? table[at_page] : -1;
+    int next_row = (int)threadIdx.x < e.keep ? a.rows[e.start + threadIdx.x] : -1;
+    near[threadIdx.x] = my_page;
     const auto piece_of = [&](int pos) -> long long {
         const int at = pos >> a.page_shift;
         if (pos < 0 || at >= a.pages_stride) return -1;
-        const int page = at - first_page < kMoveThreads ? near[at - first_page] : table[at];
+        const int page = at - first_page < T ? near[at - first_page] : table[at];
         if (page < 0 || page >= a.n_pages) return -1;
         return page * page_pieces + (long long)(pos & ((1 << a.page_shift) - 1)) * row_pieces;
     };
-    for (int i0 = 0; i0 < e.keep; i0 += kMoves) {
-        const int n = min(kMoves, e.keep - i0), i = i0 + threadIdx.x;
-        const int row = (int)threadIdx.x < n ? a.rows[e.start + i] : -1;
+    for (int i0 = 0; i0 < e.keep; i0 += T) {
+        const int n = min(T, e.keep - i0), i = i0 + threadIdx.x;
+        const int row = next_row;
+        next_row = i + T < e.keep ? a.rows[e.start + i + T] : -1;
         __syncthreads();
         if ((int)threadIdx.x < n) {
             long long f = -1, t = -1;
@@ -312,9 +314,11 @@ __device__ __forceinline__ void move_rows(const KeepArgs &a, int seq, int part, 
             to[threadIdx.x] = t;
         }
         __syncthreads();
-        for (long long id = (long long)part * kMoveThreads + threadIdx.x; id < pieces; id += share * kMoveThreads) {
-            const int pool = (int)(id / per_pool), in_pos = (int)(id - (long long)pool * per_pool);   // K and V of a layer side by side
-            const int head = in_pos / row_pieces, piece = in_pos - head * row_pieces;
+        for (long long id = (long long)part * T + threadIdx.x; id < pieces; id += share * T) {
+            // K and V of a layer side by side (a division of 32 bits where it does)
+            const int pool = id >> 32 ? (int)(id / per_pool) : (int)((unsigned)id / (unsigned)per_pool);
+            const unsigned in_pos = (unsigned)(id - (long long)pool * per_pool), head = in_pos / (unsigned)row_pieces;
+            const unsigned piece = in_pos - head * row_pieces;
             uint4 *const base = (uint4 *)(pool & 1 ? a.v_pool : a.k_pool) + (long long)(pool >> 1) * a.n_pages * page_pieces +
                                 head * head_pieces + piece;
             for (int i = 0; i < n; i += kFlight) {
@@ -352,9 +356,16 @@ __device__ __forceinline__ void give_back(const KeepArgs &a) {
     const auto each_page = [&](const Given &g, int s0, int l, const auto &visit) {
         const int from = __builtin_amdgcn_readlane(g.lo, l), to = __builtin_amdgcn_readlane(g.hi, l);
         const int *const table = a.pages + (size_t)(s0 + l) * a.pages_stride;
-        for (int j = from; j < to; j += 64) {
-            const int page = j + lane < to ? table[j + lane] : -1;
-            visit(is_page(page), page);
+        for (int j0 = from; j0 < to; j0 += 64 * kFlight) {
+            int page[kFlight];
+#pragma unroll
+            for (int x = 0; x < kFlight; ++x) {
+                const int j = j0 + 64 * x + lane;
+                page[x] = j < to ? table[j] : -1;
+            }
+#pragma unroll
+            for (int x = 0; x < kFlight; ++x)
+                if (j0 + 64 * x < to) visit(is_page(page[x]), page[x]);
         }
     };
     const auto find = [&](int s0) {
@@ -449,10 +460,14 @@ hipError_t launch_keep(const KeepArgs &a, hipStream_t s) {
     if (a.rows && a.n_seq && a.n_tok) {
         // (a launch has fewer than 2^32 threads)
         const long long pieces = 2LL * a.n_layer * a.n_head_kv * a.hd * type_bytes(a.cache_type) / 16;
-        const int share = (int)std::min<long long>((pieces + kMoveThreads - 1) / kMoveThreads, (1 << 23) / a.n_seq);
+        // One wave a workgroup waits for no other; it also has a lane for each of 64 sequences' pages, and more take four (us, of
+        // 64 / 128 / 256 threads: 2 sequences' 20 rows of 28 layers 8.6 / 9.4 / 10.8; 32 sequences' 7 rows 6.9 / 7.3 / 8.3; 300
+        // sequences in 2 layers 9.4 / 7.3 / 5.1).
+        const int threads = a.n_seq <= 64 ? 64 : kMoveThreads;
+        const int share = (int)std::min<long long>((pieces + threads - 1) / threads, (1 << 23) / a.n_seq);
         if (a.n_seq <= kOneSeqs && a.kv_out != a.kv_len)
-            return launch(keep_kernel, dim3((unsigned)(1 + share * a.n_seq)), kMoveThreads, 0, s, a, share);
-        const hipError_t e = launch(move_kernel, dim3((unsigned)(share * a.n_seq)), kMoveThreads, 0, s, a, share);
+            return launch(keep_kernel, dim3((unsigned)(1 + share * a.n_seq)), threads, 0, s, a, share);
+        const hipError_t e = launch(move_kernel, dim3((unsigned)(share * a.n_seq)), threads, 0, s, a, share);
         if (e != hipSuccess) return e;
     }
     return launch(ends_kernel, dim3(1), kThreads, 0, s, a);
