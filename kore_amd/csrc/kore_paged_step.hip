@@ -36,22 +36,25 @@ __device__ __forceinline__ long long wave_prefix(long long x) {
 struct Sums {
     long long before[2], all[2];
 };
+__device__ __forceinline__ long long of_lane(long long x, int lane) {
+    return (long long)(unsigned)__builtin_amdgcn_readlane((int)x, lane) | (long long)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32;
+}
 __device__ __forceinline__ Sums block_sums(long long x, long long y, long long (*waves)[2]) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = blockDim.x >> 6;
     const long long px = wave_prefix(x), py = wave_prefix(y);
+    Sums s{{px - x, py - y}, {of_lane(px, 63), of_lane(py, 63)}};
+    if (n == 1) return s;
     if (lane == 63) {
         waves[wave][0] = px;
         waves[wave][1] = py;
     }
     __syncthreads();
-    Sums s{{px - x, py - y}, {0, 0}};
-    for (int w = 0; w < n; ++w)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const long long of = waves[w][i];
-            if (w < wave) s.before[i] += of;
-            s.all[i] += of;
-        }
+    for (int i = 0; i < 2; ++i) {   // the waves' sums, one a lane
+        const long long of = wave_prefix(lane < n ? waves[lane][i] : 0);
+        if (wave) s.before[i] += of_lane(of, wave - 1);
+        s.all[i] = of_lane(of, 63);
+    }
     return s;
 }
 
@@ -85,33 +88,31 @@ __device__ __forceinline__ int status_of(const PlanArgs &a, const Sums &all, int
 }
 
 // A row's depth in its tree and its mask: a walk from parent to parent, each before the
-// row, so that it ends.  parent_of(i): entry i of the sequence.
-template <class F>
-__device__ __forceinline__ int ancestors(const PlanArgs &a, int i, const F &parent_of, unsigned long long *mask) {
-    int at = i, depth = 0;
+// row, so that it ends.  parent: of the sequence's rows.  A row holds one bit for itself
+// and each row before it.
+__device__ __forceinline__ int ancestors(const PlanArgs &a, int i, const int *parent, unsigned long long *mask) {
+    int at = i, depth = -1;
     for (int w = a.words - 1; w >= 0; --w) {
         unsigned long long bits = 0;
         while (at >= 64 * w) {
             bits |= 1ULL << (at & 63);
-            const int up = parent_of(at);
-            const bool root = up < 0 || up >= at;
-            at = root ? -1 : up;
-            if (!root) ++depth;
+            const int up = parent[at];
+            at = (unsigned)up < (unsigned)at ? up : -1;   // (a negative one is a large one)
         }
         mask[w] = bits;
+        depth += __popcll(bits);
     }
     return depth;
 }
 
 // A row's entries: the i-th new one of a sequence that held `held`, its slot on `page`.
-template <class F>
-__device__ __forceinline__ void put_row(const PlanArgs &a, int row, bool real, int i, int held, int page, const F &parent_of) {
+__device__ __forceinline__ void put_row(const PlanArgs &a, int row, bool real, int i, int held, int page, const int *parent) {
     unsigned long long *const mask = a.mask + (size_t)row * a.words;
     const int at = held + i;
     int pos = -1;
     long long slot = -1;
     if (real) {
-        pos = a.words ? held + ancestors(a, i, parent_of, mask) : at;
+        pos = a.words ? held + ancestors(a, i, parent, mask) : at;
         if (page >= 0 && page < a.n_pages) slot = ((long long)page << a.page_shift) + (at & ((1 << a.page_shift) - 1));
     } else {
         for (int w = 0; w < a.words; ++w) mask[w] = 0;
@@ -133,29 +134,37 @@ __device__ __forceinline__ int last_upto(const F &number, int n, int x) {
 }
 
 // A step whose sequences have a thread each: every workgroup sums them all and takes
-// some of the rows, the first one also writes what is the sequences'.  Two rounds of
-// memory: the requests, the parents of the workgroup's rows and the number of free
+// some of the rows; the first one also writes what is the sequences'.  Two rounds
+// of memory: the requests, the parents of the workgroup's rows and the number of free
 // pages; then the pages that rows go into, a sequence's last and those at the end of the
-// free ones.  (Workgroups but the first need inputs that the first does not overwrite.)
+// free ones.  The rest is in LDS: a row's sequence by halves, its ancestors one after the
+// other.  (Workgroups but the first need inputs that the first does not overwrite.)
+//
+// A token of one sequence 3.0 us, 64 trees of up to 32 4.6, 24 thousand rows of 1000
+// sequences 5.8: a launch of some 2 and the rounds.
 __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
     __shared__ long long waves[kWaves][2];
-    __shared__ int starts[kThreads + 1], firsts[kThreads], helds[kThreads], lasts[kThreads], tops[kThreads], parents[kThreads];
+    __shared__ int starts[kThreads], firsts[kThreads], helds[kThreads], lasts[kThreads], tops[kThreads];
+    __shared__ int parents[kThreads + 64 * kMaxWords];   // of the rows before the workgroup's that their trees may have, and of its own
     const int tid = threadIdx.x, T = blockDim.x, page_mask = (1 << a.page_shift) - 1;
     int base = blockIdx.x * T;
-    const int my_parent = a.words && base + tid < a.n_tok ? a.parent[base + tid] : -1;
-    const int n_free = a.n_free[0];
+    const int before = 64 * a.words, n_free = a.n_free[0];
+    const auto stage_parents = [&] {
+        for (int x = tid; x < before + T; x += T) {
+            const int row = base - before + x;
+            parents[x] = row >= 0 && row < a.n_tok ? a.parent[row] : -1;
+        }
+    };
+    if (a.words) stage_parents();
     const Request r = request(a, tid);
     if (tid < n_free && n_free <= a.n_pages) tops[tid] = a.free_pages[n_free - 1 - tid];
     // of the pages that a sequence holds only the last has room
     lasts[tid] = !r.bad && r.held & page_mask ? a.pages[(size_t)tid * a.pages_stride + (r.held >> a.page_shift)] : -1;
-    parents[tid] = my_parent;
     helds[tid] = r.held;
     const Sums sum = block_sums(r.rows(), r.need, waves);
-    const int status = status_of(a, sum, n_free);
-    const int start = status ? 0 : (int)sum.before[0], n_rows = status ? 0 : (int)sum.all[0];
-    starts[tid + 1] = status ? 0 : start + r.n;   // (behind the last sequence: all rows)
+    const int status = status_of(a, sum, n_free), n_rows = status ? 0 : (int)sum.all[0], start = status ? 0 : (int)sum.before[0];
+    starts[tid] = start;
     firsts[tid] = status ? 0 : (int)sum.before[1] - r.had;   // page j of the sequence is new page firsts + j of all
-    if (tid == 0) starts[0] = 0;
     if (blockIdx.x == 0) {
         if (tid == 0) {
             a.status[0] = status;
@@ -163,7 +172,7 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
             a.q_start[0] = 0;
         }
         if (tid < a.n_seq) {
-            a.q_start[tid + 1] = starts[tid + 1];
+            a.q_start[tid + 1] = status ? 0 : start + r.n;
             a.kv_len[tid] = status ? r.held : r.held + r.n;
         }
     }
@@ -171,7 +180,7 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
     for (bool again = false; base < a.n_tok; base += gridDim.x * T, again = true) {
         if (a.words && again) {
             __syncthreads();
-            if (base + tid < a.n_tok) parents[tid] = a.parent[base + tid];
+            stage_parents();
             __syncthreads();
         }
         const int row = base + tid;
@@ -192,7 +201,7 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
                 page = lasts[l];
             }
         }
-        put_row(a, row, real, i, held, page, [&](int x) { return first + x >= base ? parents[first + x - base] : a.parent[first + x]; });
+        put_row(a, row, real, i, held, page, parents + (first - base + before));
     }
 }
 
@@ -250,7 +259,7 @@ __global__ __launch_bounds__(256) void plan_rows_kernel(PlanArgs a) {
         held = a.kv_len[s] - (a.q_start[s + 1] - first);
         page = a.pages[(size_t)s * a.pages_stride + ((held + i) >> a.page_shift)];
     }
-    put_row(a, row, real, i, held, page, [&](int x) { return a.parent[first + x]; });
+    put_row(a, row, real, i, held, page, a.parent + first);
 }
 
 // ---- what is kept -------------------------------------------------------------------
@@ -446,7 +455,9 @@ constexpr int kOneSeqs = 1024;
 hipError_t launch_plan(const PlanArgs &a, hipStream_t s) {
     const bool in_place = a.kv_len == a.kv_held || a.n_free_out == a.n_free;
     if (a.n_seq <= kThreads && (!in_place || a.n_tok <= kOneRows)) {
-        const int threads = (std::clamp(std::max(a.n_seq, a.n_tok), 1, kThreads) + 63) & ~63;
+        // No more threads than sequences, where other workgroups take the rest of the rows (us, 64 / 256 / 1024 threads: 64 trees
+        // 4.6 / 5.0 / 5.4; 8000 rows of 4 prompts 3.4 / 3.8 / 4.3).
+        const int threads = (std::clamp(in_place ? std::max(a.n_seq, a.n_tok) : a.n_seq, 1, kThreads) + 63) & ~63;
         const int blocks = in_place ? 1 : std::max(1, (a.n_tok + threads - 1) / threads);
         return launch(plan_kernel, dim3((unsigned)blocks), threads, 0, s, a);
     }
