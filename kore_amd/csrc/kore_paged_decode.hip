@@ -663,7 +663,7 @@ hipError_t launch_attend(const AttendArgs &a, hipStream_t s) {
             const long long of_all = (long long)a.b.n_tok * d.cut.rep / tile + a.b.n_seq;
             const long long of_each = ((long long)max_q * d.cut.rep + tile - 1) / tile * a.b.n_seq;
             const double tiles = (double)std::min(of_all, of_each) * a.n_head_kv;
-            const double keys = (double)std::min((long long)a.b.pages_stride << a.page_shift, (long long)a.window + a.b.n_tok);
+            const double keys = (double)std::min((long long)a.b.pages_stride << a.page_shift, (long long)a.window + max_q);
             return start + full * std::min(tiles / 64, 1.0) + each * tiles * keys * padded_dim(a.hd) / 128;
         };
         chunk = us(kChunkRows, f32 ? 24 : parts ? 18 : 16, f32 ? 36e-5 : parts ? 15e-5 : 9e-5, 4) <

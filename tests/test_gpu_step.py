@@ -133,6 +133,17 @@ def test_plan_of_trees(words, n_seq, width):
     assert Tables(n_new, [int(x) for x in rng.integers(0, 90, n_seq)], 16, words=words, parent=parent, seed=n_seq).run() == 0
 
 
+@pytest.mark.parametrize("words,n_seq,most", [(1, 1500, 9), (2, 40, 128), (16, 9, 1024)])
+def test_plan_of_trees_in_place(words, n_seq, most):
+    """More sequences than one workgroup's threads, or many rows whose outputs take the inputs' place: two launches."""
+    rng = np.random.default_rng(words)
+    n_new = [int(x) for x in rng.integers(most // 2, most + 1, n_seq)]
+    n_new[-1] = min(most, 64 * words)
+    parent = [q for n in n_new for q in step_ref.tree(rng, n, max(1, n // 7))]
+    held = [int(x) for x in rng.integers(0, 70, n_seq)]
+    assert Tables(n_new, held, 16, words=words, parent=parent, seed=n_seq, alias=True).run() == 0
+
+
 def test_plan_without_slack():
     """The last page and the last row of the buffers; a table's row that is full; a page of the table that is none."""
     assert Tables([16, 0, 5], [16, 33, 11], 16, n_tok=21, extra=0).run() == 0
@@ -633,7 +644,7 @@ def test_keep(cache, nkv, hd, ps, n_layer, rows, free):
 def test_keep_of_many_rows_and_sequences():
     Kept([(700, 1000), (300, 300)], [650, 257], 1, 64, 32, "f16", seed=1).run()
     rng = np.random.default_rng(2)
-    for n_seq in (16, 17, 1030, 3000):
+    for n_seq in (16, 17, 64, 65, 300, 1030, 3000):
         lens = [(int(n), int(n + h)) for n, h in zip(rng.integers(0, 20, n_seq), rng.integers(0, 200, n_seq))]
         Kept(lens, [int(x) for x in rng.integers(-1, 9, n_seq)], 1, 8, 16, "f32", seed=n_seq).run()
     Kept([(3, 20000), (1, 9000), (0, 5)], [-1, -1, -1], 1, 8, 16, "f16", seed=4).run()
@@ -651,6 +662,110 @@ def test_keep_of_what_is_not_there():
     k.pages[0, 1], k.pages[1, 2] = -1, k.n_pages + 7
     k.run()
     Kept([(9, 40), (6, 60)], [-1, -1], 2, 64, 16, "f16", seed=3, n_free=8).run()
+
+
+# ---- places and streams ---------------------------------------------------------------------
+
+def test_store_into_pools_at_16_bytes():
+    """Pools, rows and weights that start at 16 bytes, at an element, or at any: the same bits."""
+    from kore_amd import paged, rope
+    w = [np.linspace(0.5, 2, 128, dtype=np.float32), np.linspace(2, 0.5, 128, dtype=np.float32)]
+    for dtype, cache in (("f32", "f32"), ("bf16", "bf16"), ("f32", "f16")):
+        got = []
+        for off, row_off in ((0, 0), (16, 0), (16, 4), (0, 1)):
+            c = Case([(3, 9), (1, 17), (40, 40)], 6, 2, 128, 16, dtype, cache, seed=3, row_off=row_off, row_pad=8 - row_off).up()
+            n = c.d["k_pool"].numel() * c.d["k_pool"].element_size()
+            raw = [torch.zeros(n + 64, dtype=torch.uint8, device="cuda") for _ in range(2)]
+            torch.cuda.synchronize()
+            with paged.PagedKV(1, c.n_pages, 16, 6, 2, 128, cache, rope.Config(128), *[r.data_ptr() + off for r in raw]) as kv:
+                _store(c, kv, *_slots(c), w)
+            got.append([r[off:off + n].cpu() for r in raw] + [c.rows("out", 6)[0]])
+        for other in got[1:]:
+            for a, b in zip(got[0], other):
+                assert _bits(a, b)
+
+
+def test_steps_past_32_bits():
+    """Slots whose offset in the pool passes 2^32 bytes and 2^31 elements: rows stored there, a tree attended, a path kept."""
+    from kore_amd import paged
+    nkv, hd, ps = 8, 128, 256
+    n_pages = (2 ** 31 + 2 ** 28) // (nkv * hd * ps)
+    c = Case([(9, 300), (40, 280)], 16, nkv, hd, ps, "f16", "f16", seed=4)
+    mask, _ = _masks(c, np.random.default_rng(4), "tree", 1)
+    far = {int(p): n_pages - 1 - i for i, p in enumerate(sorted(set(c.pages[c.pages >= 0].tolist())))}
+    table = np.vectorize(lambda x: far.get(int(x), -1))(c.pages).astype(np.int32)
+    with paged.PagedKV(1, n_pages, ps, 16, nkv, hd, "f16") as kv:
+        assert kv.info().pool_bytes > 2 ** 32
+        # the whole of either sequence through the store, which keeps rows as they are
+        w = Case([(k, k) for _, k in c.lens], 16, nkv, hd, ps, "f16", "f16", seed=5)
+        slot = []
+        for s, (n, _) in enumerate(w.lens):
+            p, at = np.arange(n), int(w.starts[s])
+            w.k[at:at + n] = c.k_pool[0, c.pages[s, p // ps], :, p % ps]
+            w.v[at:at + n] = c.v_pool[0, c.pages[s, p // ps], :, p % ps]
+            slot += (table[s, p // ps].astype(np.int64) * ps + p % ps).tolist()
+        assert max(slot) * nkv * hd > 2 ** 31
+        c.up()
+        w.up()
+        _store(w, kv, np.zeros(w.n_tok, np.int32), np.asarray(slot))
+        t = _dev(table)
+        m = _dev(mask.view(np.int64), torch.int64)
+        torch.cuda.synchronize()
+        b = paged.Batch(2, c.n_tok, c.d["starts"].data_ptr(), c.d["kv_len"].data_ptr(), t.data_ptr(), c.stride, 40)
+        kv.attend_tree_dev(0, b, paged.Tree(m.data_ptr()), "f16", c.ptr("q"), c.ptr("out"))
+        kv.sync()
+        check_rows(c, c.rows("out", 16)[0], *step_ref.tree_exact(c, mask))
+        # the second sequence keeps rows 3, 20 and 39 of its 40
+        keep, rows, ends = _dev([0, 3]), _dev([0] * 9 + [3, 20, 39] + [0] * 37), torch.zeros(2, dtype=torch.int32, device="cuda")
+        torch.cuda.synchronize()
+        kv.keep_dev(paged.Keep(2, c.n_tok, c.d["starts"].data_ptr(), keep.data_ptr(), c.d["kv_len"].data_ptr(), ends.data_ptr(), t.data_ptr(),
+                               c.stride, rows=rows.data_ptr()))
+        kv.sync()
+        assert ends.tolist() == [291, 243]
+        # what lies there now, by a token that attends one position at a time
+        one = Case([(1, 1)], 16, nkv, hd, ps, "f16", "f16", seed=6).up()
+        for i, row in enumerate((3, 20, 39)):
+            n = torch.tensor([241 + i], dtype=torch.int32, device="cuda")
+            t2 = t[1:].contiguous()
+            torch.cuda.synchronize()
+            kv.attend_dev(0, paged.Batch(1, 1, one.d["starts"].data_ptr(), n.data_ptr(), t2.data_ptr(), c.stride, 1), "f16", one.ptr("q"),
+                          one.ptr("out"), window=1)
+            kv.sync()
+            p = 240 + row
+            want = c.v_pool[0, c.pages[1, p // ps], :, p % ps]
+            got = one.rows("out", 16)[0][0].view(nkv, 2, hd)
+            assert torch.equal(got[:, 0], want) and torch.equal(got[:, 1], want)
+
+
+def test_two_streams_at_once():
+    """Trees of two caches, each call with a workspace of its own, on two streams at once: the bits of one after the other."""
+    cs = [Case([(20, 3000), (5, 700)], 16, 2, 128, 64, "f32", "f16", seed=i).up() for i in range(2)]
+    masks = [_masks(c, np.random.default_rng(i), "tree", 1)[0] for i, c in enumerate(cs)]
+    from kore_amd import paged
+    with cs[0].handle() as kv:
+        dev = [(_dev(m.view(np.int64), torch.int64), torch.empty(kv.workspace_bytes(), dtype=torch.uint8, device="cuda"), torch.cuda.Stream())
+               for m in masks]
+
+        def attend(c, m, ws, st, handle):
+            handle.attend_tree_dev(0, c.batch(), paged.Tree(m.data_ptr()), "f32", c.ptr("q"), c.ptr("out"), workspace=ws.data_ptr(),
+                                   stream=st.cuda_stream)
+
+        with cs[1].handle() as kv2:
+            want = []
+            for c, (m, ws, st), h in zip(cs, dev, (kv, kv2)):
+                torch.cuda.synchronize()
+                attend(c, m, ws, st, h)
+                torch.cuda.synchronize()
+                want.append(c.d["out"].clone())
+            for _ in range(10):
+                for c in cs:
+                    c.d["out"].fill_(77.0)
+                torch.cuda.synchronize()
+                for c, (m, ws, st), h in zip(cs, dev, (kv, kv2)):
+                    attend(c, m, ws, st, h)
+                torch.cuda.synchronize()
+                for c, w in zip(cs, want):
+                    assert _bits(c.d["out"], w)
 
 
 # ---- refusals ----------------------------------------------------------------------------
