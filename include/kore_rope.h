@@ -99,7 +99,7 @@ typedef struct kore_rope_heads {
     const float *norm;          /* device, head_dim weights, or NULL: turned only */
 } kore_rope_heads;
 
-/* n_sets (1 or 2: q's heads, q's and k's) of n_tok rows, in one launch: each head
+/* One set (k NULL) or two (q's heads and k's) of n_tok rows, in one launch: each head
  * is first x w / sqrt(mean(x^2) + eps), then turned as by kore_rope_apply_dev.
  * The sum of squares and the root are in double, 1 / root is rounded to float, and
  * so is either product; then as there, so that each value is rounded to its type
@@ -108,8 +108,8 @@ typedef struct kore_rope_heads {
  * aligned to a float.  A row whose position is negative is left as it is.  The
  * rows of a set overlap no other's.  A head with values that are not finite holds
  * nothing of use; no other notices. */
-KORE_PAGED_API int kore_rope_norm_dev(kore_rope_t r, int type, int n_tok, int head_dim, const kore_rope_heads *sets,
-                                      int n_sets, const int *pos, float eps, void *stream);
+KORE_PAGED_API int kore_rope_norm_dev(kore_rope_t r, int type, int n_tok, int head_dim, const kore_rope_heads *q,
+                                      const kore_rope_heads *k, const int *pos, float eps, void *stream);
 
 /* The plan's rot_dim / 2 frequencies (host copy) and m. */
 KORE_PAGED_API int kore_rope_get_freqs(kore_rope_t r, float *freqs, float *magnitude);

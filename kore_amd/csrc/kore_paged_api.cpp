@@ -374,15 +374,16 @@ int kore_rope_apply_dev(kore_rope_t r, int type, int n_tok, int n_head, int head
     return KORE_PAGED_OK;
 }
 
-int kore_rope_norm_dev(kore_rope_t r, int type, int n_tok, int head_dim, const kore_rope_heads *sets, int n_sets, const int *pos,
-                       float eps, void *stream) {
+int kore_rope_norm_dev(kore_rope_t r, int type, int n_tok, int head_dim, const kore_rope_heads *q, const kore_rope_heads *k,
+                       const int *pos, float eps, void *stream) {
     if (!r) return FAIL0(KORE_PAGED_E_INVALID, "null handle");
     if (!type_ok(type)) return fail(r, KORE_PAGED_E_INVALID, "unknown type %d", type);
-    if (!sets || n_sets < 1 || n_sets > 2) return fail(r, KORE_PAGED_E_INVALID, "no sets, or %d of them (1 or 2)", n_sets);
+    if (!q) return fail(r, KORE_PAGED_E_INVALID, "null set");
     if (!eps_ok(eps)) return fail(r, KORE_PAGED_E_INVALID, "eps must be positive and finite");
     HeadsArgs a{};
+    const int n_sets = k ? 2 : 1;
     for (int i = 0; i < n_sets; ++i) {
-        const kore_rope_heads &t = sets[i];
+        const kore_rope_heads &t = i ? *k : *q;
         if (int rc = check_heads(r, n_tok, t.n_head, head_dim)) return rc;
         const int64_t n = (int64_t)t.n_head * head_dim;
         if (int rc = check_stride(r, "x", t.x_stride, n, n_tok)) return rc;

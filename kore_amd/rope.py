@@ -42,13 +42,11 @@ class HeadsStruct(C.Structure):
     _fields_ = [("x", _vp), ("out", _vp), ("x_stride", _i64), ("out_stride", _i64), ("n_head", _i), ("norm", _vp)]
 
 
-_SETS = {1: HeadsStruct * 1, 2: HeadsStruct * 2}
-
 SYMBOLS = [
     ("kore_rope_create", _i, [C.POINTER(_vp), C.POINTER(RopeConfig)]),
     ("kore_rope_destroy", None, [_vp]),
     ("kore_rope_apply_dev", _i, [_vp, _i, _i, _i, _i, _vp, _i64, _vp, _vp, _i64, _i, _vp]),
-    ("kore_rope_norm_dev", _i, [_vp, _i, _i, _i, C.POINTER(HeadsStruct), _i, _vp, _f, _vp]),
+    ("kore_rope_norm_dev", _i, [_vp, _i, _i, _i, C.POINTER(HeadsStruct), C.POINTER(HeadsStruct), _vp, _f, _vp]),
     ("kore_rope_get_freqs", _i, [_vp, _vp, C.POINTER(_f)]),
     ("kore_rope_sync", _i, [_vp]),
     ("kore_rope_last_error", C.c_char_p, [_vp]),
@@ -107,7 +105,7 @@ class Config:
                                  beta_slow, magnitude, None if self.factors is None else self.factors.ctypes.data)
 
 
-class Heads(HeadsStruct):
+class Heads:
     """A set of rows of n_head heads of head_dim values (kore_rope_heads): device pointers of the rows, of those that they
     become and of the norm's weights (None: the heads are turned only).  Strides in elements, None: rows one behind the
     other."""
@@ -115,7 +113,9 @@ class Heads(HeadsStruct):
     def __init__(self, x: int, out: int, n_head: int, head_dim: int, norm: int | None = None, x_stride: int | None = None,
                  out_stride: int | None = None):
         n = n_head * head_dim
-        super().__init__(x, out, n if x_stride is None else x_stride, n if out_stride is None else out_stride, n_head, norm)
+        self.struct = HeadsStruct(x, out, n if x_stride is None else x_stride, n if out_stride is None else out_stride, n_head,
+                                  norm)
+        self._ref = C.byref(self.struct)
 
 
 class Rope:
@@ -148,9 +148,10 @@ class Rope:
     def norm_dev(self, dtype: str, n_tok: int, head_dim: int, sets, pos: int, eps: float = 1e-6, stream=None) -> None:
         """One or two sets (Heads) of n_tok rows: each head over its root mean square, times its set's weights, then turned
         to the row's position (pos: device, int32; rows with a negative one are left as they are)."""
-        n = len(sets)
-        a = _SETS[n](*sets) if n in _SETS else None   # (another number is refused by the call)
-        rc = self._norm(self._h, type_code(dtype), n_tok, head_dim, a, n, pos, eps, stream)
+        if len(sets) > 2:
+            raise ValueError(f"{len(sets)} sets of heads (1 or 2)")
+        q, k = sets[0]._ref if sets else None, sets[1]._ref if len(sets) == 2 else None
+        rc = self._norm(self._h, type_code(dtype), n_tok, head_dim, q, k, pos, eps, stream)
         if rc:
             self._check(rc)
 

@@ -28,7 +28,7 @@ def test_struct_layouts(tmp_path):
 def test_null_handles():
     from kore_amd import layer, paged, rope
     L, bad = paged.lib(), rope.KORE_PAGED_E_INVALID
-    assert L.kore_rope_norm_dev(None, 0, 1, 8, None, 1, None, 1e-6, None) == bad
+    assert L.kore_rope_norm_dev(None, 0, 1, 8, None, None, None, 1e-6, None) == bad
     assert L.kore_paged_plan_dev(None, None, None) == bad and L.kore_paged_keep_dev(None, None, None) == bad
     assert L.kore_paged_append_rows_dev(None, 0, None, 0, None, 0, None, 0, None, 0, None, 0, None) == bad
     assert L.kore_paged_attend_tree_dev(None, 0, None, None, 0, None, 0, None, 0, 0.0, 0, None, None) == bad

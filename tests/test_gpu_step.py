@@ -287,7 +287,7 @@ def test_norm_refuses():
     good = [H(X, Y, 4, 64, x_stride=384, out_stride=384), H(X + 1024, Y + 1024, 2, 64, x_stride=384, out_stride=384)]
     with rope.Rope(rope.Config(64)) as r:
         for kw, code, text in [
-                (dict(sets=[]), -1, "sets"), (dict(sets=good * 2), -1, "sets"), (dict(eps=0.0), -1, "eps"), (dict(eps=math.nan), -1, "eps"),
+                (dict(sets=[]), -1, "null set"), (dict(eps=0.0), -1, "eps"), (dict(eps=math.nan), -1, "eps"),
                 (dict(eps=math.inf), -1, "eps"), (dict(pos=None), -1, "pos"), (dict(pos=P + 2), -1, "pos"), (dict(hd=62), -1, "head_dim"),
                 (dict(hd=65), -1, "head_dim"), (dict(hd=1026), -3, "head_dim"), (dict(n=-1), -1, "n_tok"), (dict(n=2 ** 23 + 1), -3, "n_tok"),
                 (dict(sets=[H(X, Y, 0, 64)]), -1, "n_head"), (dict(sets=[H(X, Y, 4, 64, x_stride=255)]), -1, "stride"),
@@ -300,6 +300,8 @@ def test_norm_refuses():
             with pytest.raises(rope.PagedError, match=text) as e:
                 r.norm_dev("f32", kw.get("n", 4), kw.get("hd", 64), kw.get("sets", good), kw.get("pos", P), kw.get("eps", 1e-6))
             assert e.value.code == code
+        with pytest.raises(ValueError, match="sets"):
+            r.norm_dev("f32", 4, 64, good * 2, P)
         r.norm_dev("f32", 0, 64, good, None)
         r.sync()
         assert (y == 7.0).all()
