@@ -666,7 +666,7 @@ hipError_t launch_attend(const AttendArgs &a, hipStream_t s) {
             const double keys = (double)std::min((long long)a.b.pages_stride << a.page_shift, (long long)a.window + max_q);
             return start + full * std::min(tiles / 64, 1.0) + each * tiles * keys * padded_dim(a.hd) / 128;
         };
-        chunk = us(kChunkRows, f32 ? 24 : parts ? 18 : 16, f32 ? 36e-5 : parts ? 15e-5 : 9e-5, 4) <
+        chunk = us(kChunkRows, f32 ? 24 : parts ? 18 : 16, f32 ? 33e-5 : parts ? 15e-5 : 9e-5, 4) <
                 us(kRows, a.hd > 128 ? 22 : f32 ? 12 : 10, f32 ? 10.5e-5 : 4e-5, 0);
     }
     const int rows = chunk ? kChunkRows : kRows;
