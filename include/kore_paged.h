@@ -166,8 +166,9 @@ typedef struct kore_paged_plan {
  * slot and mask are those of a step without rows, which the other calls take.
  * A page that the table names is taken to be the sequence's own behind its full
  * ones: rows go into the last, where it has room.  At most 2^16 sequences and 2^23
- * rows.  But for the pairs named above no two arrays overlap.  Pointers on the
- * handle's device; stream as in the append. */
+ * rows.  Without sequences their arrays and free_pages may be NULL, without rows
+ * pos and slot.  But for the pairs named above no two arrays overlap.  Pointers on
+ * the handle's device; stream as in the append. */
 KORE_PAGED_API int kore_paged_plan_dev(kore_paged_t h, const kore_paged_plan *p, void *stream);
 
 /* Rows as a plan leaves them, and the norms of their heads. */

@@ -157,7 +157,7 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
     };
     if (a.words) stage_parents();
     const Request r = request(a, tid);
-    if (tid < n_free && n_free <= a.n_pages) tops[tid] = a.free_pages[n_free - 1 - tid];
+    if (a.n_seq && tid < n_free && n_free <= a.n_pages) tops[tid] = a.free_pages[n_free - 1 - tid];
     // of the pages that a sequence holds only the last has room
     lasts[tid] = !r.bad && r.held & page_mask ? a.pages[(size_t)tid * a.pages_stride + (r.held >> a.page_shift)] : -1;
     helds[tid] = r.held;

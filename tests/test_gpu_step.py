@@ -92,7 +92,7 @@ class Tables:
             assert np.array_equal(self.get(out), want[name]), name
         assert np.array_equal(self.get("pages").reshape(len(self.held), -1) if self.held else want["pages"], want["pages"])
         if self.words:
-            assert np.array_equal(self.get("mask").view(np.uint64).reshape(self.n_tok, -1), want["mask"])
+            assert np.array_equal(self.get("mask").view(np.uint64).reshape(self.n_tok, self.words), want["mask"])
         assert np.array_equal(self.get("free"), self.free) and np.array_equal(self.get("n_new"), self.n_new)
         return int(want["status"][0])
 
@@ -165,6 +165,28 @@ def test_plan_refused_on_the_device(kw, status, big):
         kw["n_tok"] = 5000
     t = Tables(kw.pop("n_new"), kw.pop("held"), 16, **kw)
     assert t.run() == status
+
+
+@pytest.mark.parametrize("n_tok", [0, 3])
+@pytest.mark.parametrize("words", [0, 1])
+@pytest.mark.parametrize("alias", [False, True])
+def test_steps_without_sequences(n_tok, words, alias):
+    """Arrays that hold nothing may be NULL, with free pages beside them."""
+    from kore_amd import paged
+    t = Tables([], [], 16, n_tok=n_tok, words=words, parent=[], alias=alias).up()
+    p = t.ptr
+    with t.handle() as kv:
+        kv.plan_dev(paged.Plan(0, n_tok, None, None, None, None, 1, None, p("n_free"), p("n_free_out"), p("q_start"),
+                               p("pos") if n_tok else None, p("slot") if n_tok else None, p("status"),
+                               *((p("parent"), p("mask"), words) if words else ())))
+        kv.sync()
+        assert t.check() == 0
+        assert t.get("n_free_out")[0] == t.n_free > 0
+        kv.keep_dev(paged.Keep(0, n_tok, None, None, None, None, None, 1, free_pages=p("free"), n_free=p("n_free"),
+                               n_free_out=p("n_free_out")))
+        kv.keep_dev(paged.Keep(0, n_tok, None, None, None, None, None, 1))
+        kv.sync()
+    assert t.check() == 0
 
 
 def test_plan_missing_is_whole():
