@@ -199,7 +199,8 @@ typedef struct kore_paged_tree {
  * sequence with n of them attends the kv_len - n positions before them, in a
  * window w those over pos - w alone (pos is taken within kv_len - n .. kv_len - 1),
  * and of the new ones those that its mask names, itself only if it does; the
- * window does not touch these.  Everything else as there. */
+ * window does not touch these.  Whether a step takes 16-row tiles or chunks goes by
+ * its size, and with it what is rounded on the way (above).  Everything else as there. */
 KORE_PAGED_API int kore_paged_attend_tree_dev(kore_paged_t h, int layer, const kore_paged_batch *b, const kore_paged_tree *t,
                                               int type, const void *q, int64_t q_stride, void *out, int64_t out_stride,
                                               float scale, int window, void *workspace, void *stream);

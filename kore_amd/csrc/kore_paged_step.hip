@@ -434,6 +434,9 @@ __device__ __forceinline__ void give_back(const KeepArgs &a) {
 }
 
 // One launch for both, where the lengths that the moves read are not those that are written.
+// 16 drafted tokens of which four stay, 24 layers: 3.7 us, a launch and three rounds (ends and
+// rows, pages, the rows themselves); 32 sequences' seven rows, 28 layers of 4 kv-heads of 128:
+// 7.0, since rows of a head are 256 bytes each, and lie apart.
 __global__ __launch_bounds__(kMoveThreads) void keep_kernel(KeepArgs a, int share) {
     if (blockIdx.x == 0) return give_back(a);
     const int id = blockIdx.x - 1, seq = id / share;

@@ -358,7 +358,7 @@ hipError_t launch_rope(const RopeArgs &a, hipStream_t s) {
 }
 
 hipError_t launch_heads(const HeadsArgs &a, hipStream_t s) {
-    // Units of n pairs where heads, their parts, rows and buffers start at multiples of N values.
+    // Units of n pairs where heads, their parts, rows and buffers start at multiples of n values.
     const auto wide = [&](int n) {
         const auto fits = [n](const void *p, int type) { return (uintptr_t)p % (size_t)(n * type_bytes(type)) == 0; };
         bool ok = a.turn.rot % (2 * n) == 0 && (a.hd - a.turn.rot) % (2 * n) == 0;
