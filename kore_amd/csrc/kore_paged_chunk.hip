@@ -41,10 +41,13 @@ template <> struct Form<float, float> {
 };
 
 // What a tile's shape asks of LDS and registers: keys of a step; teams of a
-// workgroup (a CU holds one workgroup).
-template <class A, class S, int HDP> struct Shape {
+// workgroup (a CU holds one workgroup).  Values in parts are taken 32 keys at a time, which
+// leaves the loop its registers; trees with heads up to 64, which have them, 64 (us, 32 / 64
+// keys, 14/2/64, fp32 rows: 16 trees of 32 over up to 8000 fp16 keys 40.8 / 39.9, 100 over up to
+// 3000 130 / 113, one of 64 over 32000 fp32 keys 60.0 / 57.5; heads of 128 99 / 120, they spill).
+template <class A, class S, int HDP, bool TREE> struct Shape {
     static constexpr bool parts = Form<A, S>::qp > 1;
-    static constexpr int keys = parts ? 32 : 64;
+    static constexpr int keys = parts && !(TREE && HDP == 64) ? 32 : 64;
     static constexpr int teams = HDP <= 128 ? 2 : 1, threads = 64 * kWaves * teams;
     static constexpr bool lag = parts && teams == 2;   // the second team a phase behind
 };
@@ -103,15 +106,15 @@ __device__ __forceinline__ void weights(const float (&x)[8], V (&part)[N]) {
 }
 
 template <class A, class S, int HDP, bool TREE>
-__global__ __launch_bounds__((Shape<A, S, HDP>::threads), 1) void chunk_kernel(TileArgs d) {
+__global__ __launch_bounds__((Shape<A, S, HDP, TREE>::threads), 1) void chunk_kernel(TileArgs d) {
     typedef typename Form<A, S>::C C;
     typedef typename Form<A, S>::CV CV;
     typedef typename Mma<C>::vec8 vec8;
     typedef typename Mma<CV>::vec8 vvec8;
     typedef CV vec4 __attribute__((ext_vector_type(4)));
     constexpr int QP = Form<A, S>::qp, KP = Form<A, S>::kp, VP = Form<A, S>::vp, PP = Form<A, S>::pp;
-    constexpr int kKeys = Shape<A, S, HDP>::keys, kTeams = Shape<A, S, HDP>::teams;
-    constexpr bool kLag = Shape<A, S, HDP>::lag;
+    constexpr int kKeys = Shape<A, S, HDP, TREE>::keys, kTeams = Shape<A, S, HDP, TREE>::teams;
+    constexpr bool kLag = Shape<A, S, HDP, TREE>::lag;
     constexpr int KS = HDP / 16, DT = HDP / 32, MT = kKeys / 32;         // k-steps, dim tiles, key tiles
     // Rows of LDS: 16 rows' 16-byte pieces of K, and four rows' 64 bytes of V, lie on
     // different banks
@@ -698,9 +701,9 @@ hipError_t launch_chunk(const TileArgs &d, hipStream_t s) {
     const dim3 grid((unsigned)d.places);
 #define KORE_CHUNK(A, S)                                                        \
     do {                                                                        \
-        if (hdp == 64) return launch(chunk_kernel<A, S, 64, TREE>, grid, Shape<A, S, 64>::threads, 0, s, d);     \
-        else if (hdp == 128) return launch(chunk_kernel<A, S, 128, TREE>, grid, Shape<A, S, 128>::threads, 0, s, d); \
-        else return launch(chunk_kernel<A, S, 256, TREE>, grid, Shape<A, S, 256>::threads, 0, s, d);              \
+        if (hdp == 64) return launch(chunk_kernel<A, S, 64, TREE>, grid, Shape<A, S, 64, TREE>::threads, 0, s, d);     \
+        else if (hdp == 128) return launch(chunk_kernel<A, S, 128, TREE>, grid, Shape<A, S, 128, TREE>::threads, 0, s, d); \
+        else return launch(chunk_kernel<A, S, 256, TREE>, grid, Shape<A, S, 256, TREE>::threads, 0, s, d);              \
     } while (0)
     if (d.a.cache_type == kF32) KORE_CHUNK(float, float);
     else if (d.a.type == kF32 && d.a.cache_type == kF16) KORE_CHUNK(float, half_t);
