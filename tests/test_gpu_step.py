@@ -561,6 +561,60 @@ def test_new_rows_that_are_not_attended(dtype, cache, max_q, bad):
     assert _bits(got[~hit], other[~hit])
 
 
+def _tall(c, keys=131072):
+    """The case with a table of so many keys, more than any sequence has: a step that may be as long as that takes tiles of
+    128 rows, where a few of 16 would do for what it is (16 heads share a kv-head)."""
+    c.pages = np.ascontiguousarray(np.pad(c.pages, ((0, 0), (0, keys // c.ps - c.stride)), constant_values=-1))
+    c.stride = keys // c.ps
+    return c
+
+
+@pytest.mark.parametrize("kind", ["tree", "any"])
+@pytest.mark.parametrize("dtype,cache", PAIRS)
+@pytest.mark.parametrize("nh,nkv,hd,ps", [(32, 2, 64, 16), (16, 1, 64, 32), (16, 1, 40, 128), (16, 1, 128, 16), (32, 2, 96, 64), (16, 1, 256, 16)])
+@pytest.mark.parametrize("lens", ["few", "trees", "before_the_first"])
+def test_trees_in_tall_tiles(dtype, cache, nh, nkv, hd, ps, lens, kind):
+    c = _tall(Case(TREES[lens], nh, nkv, hd, ps, dtype, cache, seed=hd + ps, extra_rows=3)).up()
+    mask, pos = _masks(c, np.random.default_rng(hd), kind, 1)
+    with c.handle() as kv:
+        _attend_tree(c, kv, mask)
+        got, clean = c.rows("out", nh)
+        assert clean and (got[c.used:] == 77.0).all()
+        check_rows(c, got, *step_ref.tree_exact(c, mask))
+        if lens != "before_the_first" and kind == "tree":
+            for window in (1, 100):
+                _attend_tree(c, kv, mask, pos, window=window)
+                check_rows(c, c.rows("out", nh)[0], *step_ref.tree_exact(c, mask, pos, window=window), name=str(window))
+
+
+@pytest.mark.parametrize("dtype,cache", PAIRS)
+@pytest.mark.parametrize("hd", [48, 64, 128, 256])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_bad_values_in_tall_tiles(dtype, cache, hd, bad):
+    """Infinities and NaN in V of what is held, which all rows attend, and of new rows that some masks name; pages that are
+    none; then in K of a new row that no other attends."""
+    c = _tall(Case([(40, 700), (33, 33), (5, 100)], 16, 1, hd, 16, dtype, cache, seed=hd))
+    mask, _ = _masks(c, np.random.default_rng(6), "tree", 1)
+    for s, p, dim in ((0, 300, 3), (0, 680, hd - 1), (1, 9, 5), (2, 96, 8)):
+        c.v_pool[0, int(c.pages[s, p // 16]), :, p % 16, dim] = bad
+    c.pages[0, 4], c.pages[0, 30] = -1, c.n_pages
+    mask[40 + 32, 0] |= np.uint64(1 << 32)
+    for i in range(40, 40 + 32):
+        mask[i, 0] &= ~np.uint64(1 << 32)      # (row 32 of the second sequence is attended by itself alone)
+    c.up()
+    with c.handle() as kv:
+        _attend_tree(c, kv, mask)
+        got = c.rows("out", 16)[0]
+        check_rows(c, got, *step_ref.tree_exact(c, mask))
+        page = int(c.pages[1, 2])
+        c.k_pool[0, page, :, 0, 3] = bad       # position 32
+        c.d["k_pool"].copy_(c.k_pool)
+        _attend_tree(c, kv, mask)
+    other = c.rows("out", 16)[0]
+    keep = np.arange(c.n_tok) != 72
+    assert _bits(got[keep], other[keep])
+
+
 @pytest.mark.parametrize("dtype,cache", [("f32", "f32"), ("f32", "f16"), ("bf16", "bf16")])
 @pytest.mark.parametrize("pad,off", [(0, 0), (8, 8), (3, 1)])
 def test_tree_strides_and_places(dtype, cache, pad, off):
