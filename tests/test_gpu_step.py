@@ -420,6 +420,40 @@ def test_store_in_place_and_without_q():
         assert _bits(c.d[n], d.d[n]) and _bits(c.d[n], e.d[n])
 
 
+@pytest.mark.parametrize("dtype,cache", PAIRS)
+@pytest.mark.parametrize("nh,nkv,hd", [(6, 2, 64), (5, 1, 72), (3, 3, 40)])
+def test_rows_of_q_k_and_v_side_by_side(dtype, cache, nh, nkv, hd):
+    """One wide row holds all three, as one product leaves them: normalised and stored in place, the bits of rows of their own."""
+    from kore_amd import paged, rope
+    w = [np.linspace(0.5, 2, hd, dtype=np.float32)] * 2
+    c, d = (Case([(3, 9), (20, 37), (1, 64)], nh, nkv, hd, 16, dtype, cache, seed=hd).up() for _ in range(2))
+    pos, slot = _slots(c)
+    E, kvd, n = nh * hd, nkv * hd, c.n_tok
+    wide = torch.cat([x.reshape(n, -1) for x in (c.q, c.k, c.v)], 1).cuda()
+    two = wide.clone()
+    step, size = wide.shape[1], wide.element_size()
+    at = lambda t, i: t.data_ptr() + i * size  # noqa: E731
+    g, p, t = torch.from_numpy(w[0]).cuda(), _dev(pos), _dev(slot, torch.int64)
+    torch.cuda.synchronize()
+    with c.handle(rope.Config(hd)) as a, d.handle(rope.Config(hd)) as b, rope.Rope(rope.Config(hd)) as r:
+        _store(c, a, pos, slot, w)
+        rows = paged.Rows(n, p.data_ptr(), t.data_ptr(), g.data_ptr(), g.data_ptr(), norm_eps=1e-6)
+        b.append_rows_dev(0, rows, dtype, at(wide, E), at(wide, E + kvd), q=at(wide, 0), q_out=at(wide, 0), k_stride=step, v_stride=step,
+                          q_stride=step, q_out_stride=step)
+        b.sync()
+        r.norm_dev(dtype, n, hd, [rope.Heads(at(two, 0), at(two, 0), nh, hd, g.data_ptr(), step, step),
+                                  rope.Heads(at(two, E), at(two, E), nkv, hd, g.data_ptr(), step, step)], p.data_ptr(), 1e-6)
+        r.sync()
+    for k in ("k_pool", "v_pool"):
+        assert _bits(c.d[k], d.d[k])
+    k_v = torch.cat([c.k.reshape(n, -1), c.v.reshape(n, -1)], 1)
+    assert _bits(wide[:, :E].cpu(), c.rows("out", nh)[0].reshape(n, E)) and _bits(wide[:, E:].cpu(), k_v)
+    assert _bits(two[:, :E], wide[:, :E]) and _bits(two[:, E + kvd:].cpu(), c.v.reshape(n, -1))
+    got = two[:, E:E + kvd].cpu().reshape(n, nkv, hd)
+    want, most = step_ref.heads(to64(c.k), pos, *rope_freqs(hd), "half", w[1], 1e-6)
+    assert (np.abs(to64(got) - want) <= step_ref.heads_bound(want, most, dtype, True)).all()
+
+
 # ---- attention of trees -------------------------------------------------------------
 
 def _masks(c, rng, kind, words):
