@@ -2,6 +2,7 @@
 // forward() chained from libkore_qmv's fused matvec launches and libkore_attn's
 // decode, all on one stream.
 #include "kore_layer.h"
+#include "kore_paged_kernels.h"
 
 #include <hip/hip_runtime.h>
 
@@ -242,14 +243,13 @@ KORE_LAYER_API int kore_layer_prefill_dev(kore_layer_t L, const kore_layer_weigh
 extern "C++" {
 namespace {
 
-// What the paged steps check before anything is launched: all that the append and the attention would refuse (what
-// else the append refuses leaves x and the cache as they were).
+// What the paged steps check before anything is launched.  With check_batch all that the attention would refuse; the
+// append comes first, and what that refuses leaves x and the cache as they were.  pi: the cache's.
 int check_paged(kore_layer *L, const kore_layer_weights *w, kore_paged_t kv, int layer, const kore_paged_batch *b, const float *x,
-                const void *workspace) {
+                const void *workspace, kore_paged_info &pi) {
     if (!w || !kv || !b || !x || ((uintptr_t)x & 15))
         return fail(L, KORE_LAYER_E_INVALID, "w, kv, batch or x missing or x unaligned");
     if (int rc = check_weights(L, w)) return rc;
-    kore_paged_info pi{};
     if (kore_paged_get_info(kv, &pi) != KORE_PAGED_OK || pi.config.n_head != L->n_head ||
         pi.config.n_head_kv != L->n_head_kv || pi.config.head_dim != L->head_dim)
         return fail(L, KORE_LAYER_E_INVALID, "the paged cache's geometry differs from the layer's");
@@ -258,6 +258,14 @@ int check_paged(kore_layer *L, const kore_layer_weights *w, kore_paged_t kv, int
         return fail(L, KORE_LAYER_E_INVALID, "n_tok must be 1..64 (kore's KORE_BMAX), of one sequence or more");
     if (layer < 0 || layer >= pi.config.n_layer || !b->q_start || !b->kv_len || !b->pages || ((uintptr_t)workspace & 15))
         return fail(L, KORE_LAYER_E_INVALID, "layer outside the cache, a batch array missing or the workspace unaligned");
+    return KORE_LAYER_OK;
+}
+
+// The limits of a batch: the store by slots, which takes no batch, would be done by the time the attention sees them.
+int check_batch(kore_layer *L, const kore_paged_batch *b, const kore_paged_config &c) {
+    if (b->max_q < 0 || b->pages_stride < 1 || b->pages_stride > kore_paged_gpu::kMaxKeys / c.page_size ||
+        b->n_seq > kore_paged_gpu::kMaxSeq || (int64_t)b->n_seq * c.n_head_kv > kore_paged_gpu::kMaxSeqHeads)
+        return fail(L, KORE_LAYER_E_INVALID, "batch: max_q negative, or pages_stride or n_seq outside the cache's limits");
     return KORE_LAYER_OK;
 }
 
@@ -271,7 +279,8 @@ int paged_error(kore_layer *L, kore_paged_t kv) {
 KORE_LAYER_API int kore_layer_paged_dev(kore_layer_t L, const kore_layer_weights *w, kore_paged_t kv, int layer,
                                         const kore_paged_batch *b, float *x, void *workspace, void *stream) {
     if (!L) return fail(nullptr, KORE_LAYER_E_INVALID, "layer handle is NULL");
-    if (int rc = check_paged(L, w, kv, layer, b, x, workspace)) return rc;
+    kore_paged_info pi{};
+    if (int rc = check_paged(L, w, kv, layer, b, x, workspace, pi)) return rc;
     void *s = stream ? stream : (void *)L->stream;
     const int64_t E = L->E, kvd = L->kvd;
     return rows_step(L, w, b->n_tok, x, s, [&] {
@@ -288,7 +297,9 @@ KORE_LAYER_API int kore_layer_paged_ex_dev(kore_layer_t L, const kore_layer_weig
                                            const kore_paged_batch *b, const kore_layer_paged_opts *o, float *x,
                                            void *workspace, void *stream) {
     if (!L) return fail(nullptr, KORE_LAYER_E_INVALID, "layer handle is NULL");
-    if (int rc = check_paged(L, w, kv, layer, b, x, workspace)) return rc;
+    kore_paged_info pi{};
+    if (int rc = check_paged(L, w, kv, layer, b, x, workspace, pi)) return rc;
+    if (int rc = check_batch(L, b, pi.config)) return rc;
     if (!o || !o->pos || !o->slot || ((uintptr_t)o->pos & 3) || ((uintptr_t)o->slot & 7))
         return fail(L, KORE_LAYER_E_INVALID, "opts, pos or slot missing or unaligned");
     if (((uintptr_t)o->q_norm & 3) || ((uintptr_t)o->k_norm & 3))
