@@ -105,7 +105,7 @@ typedef struct kore_layer_paged_opts {
     const int64_t *slot;             /* device [n_tok], aligned to 8 bytes */
     const float *q_norm, *k_norm;    /* device, head_dim weights each, or NULL */
     const kore_paged_tree *tree;     /* NULL: each row attends up to its own position */
-    int window;                      /* 0: none */
+    int window;                      /* 0: none; with a tree it is the plan's too (kore_paged_plan) */
 } kore_layer_paged_opts;
 
 /* kore_layer_paged_dev with the rows stored by their slots (kore_paged_append_rows_dev)

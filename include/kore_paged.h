@@ -150,9 +150,11 @@ typedef struct kore_paged_plan {
     int *pos;                    /* [n_tok] out: each row's position, kv_held and its depth in the tree; -1: no row */
     int64_t *slot;               /* [n_tok] out: where it is stored, page * page_size + slot of it; -1: nowhere */
     uint64_t *mask;              /* [n_tok][mask_words] out with parent, else NULL: bit j % 64 of word j / 64 is set where
-                                    the j-th new row of the sequence is the row itself or before it in the tree */
+                                    the j-th new row of the sequence is the row itself or before it in the tree (in `window`) */
     int mask_words;              /* 1 .. 16 with parent, else 0 */
     int *status;                 /* [1] out */
+    int window;                  /* with parent: rows this many positions or more before a row are not in its mask; 0: all
+                                    before it are (layers of several windows: a plan, with a mask, for each) */
 } kore_paged_plan;
 
 /* Makes the step's tables.  Sequence s gets rows q_start[s] .. and, where they pass
@@ -199,7 +201,7 @@ typedef struct kore_paged_tree {
  * sequence with n of them attends the kv_len - n positions before them, in a
  * window w those over pos - w alone (pos is taken within kv_len - n .. kv_len - 1),
  * and of the new ones those that its mask names, itself only if it does; the
- * window does not touch these.  Whether a step takes 16-row tiles or chunks goes by
+ * window does not touch these, so that a model's window is also its plan's.  Whether a step takes 16-row tiles or chunks goes by
  * its size, and with it what is rounded on the way (above).  Everything else as there. */
 KORE_PAGED_API int kore_paged_attend_tree_dev(kore_paged_t h, int layer, const kore_paged_batch *b, const kore_paged_tree *t,
                                               int type, const void *q, int64_t q_stride, void *out, int64_t out_stride,

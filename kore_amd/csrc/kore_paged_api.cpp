@@ -632,6 +632,7 @@ int kore_paged_plan_dev(kore_paged_t h, const kore_paged_plan *p, void *stream) 
     } else if (p->mask_words != 0) {
         return fail(h, KORE_PAGED_E_INVALID, "mask_words %d without parent and mask", p->mask_words);
     }
+    if (p->window < 0) return fail(h, KORE_PAGED_E_INVALID, "negative window %d", p->window);
     if (p->n_seq) {
         if (int rc = check_array(h, "n_new", p->n_new, 4)) return rc;
         if (int rc = check_array(h, "kv_held", p->kv_held, 4)) return rc;
@@ -656,6 +657,7 @@ int kore_paged_plan_dev(kore_paged_t h, const kore_paged_plan *p, void *stream) 
     a.page_shift = h->page_shift;
     a.pages_stride = p->pages_stride;
     a.words = p->mask_words;
+    a.window = p->window ? p->window : INT_MAX;
     a.n_new = p->n_new;
     a.kv_held = p->kv_held;
     a.free_pages = p->free_pages;

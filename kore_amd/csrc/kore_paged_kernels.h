@@ -109,6 +109,7 @@ struct AttendArgs {
 
 struct PlanArgs {
     int n_seq, n_tok, n_pages, page_shift, pages_stride, words;   // words 0: no trees
+    int window;              // of the masks; INT_MAX: none
     const int *n_new, *kv_held, *free_pages, *n_free, *parent;
     int *kv_len, *pages, *n_free_out, *q_start, *pos, *status;
     int64_t *slot;

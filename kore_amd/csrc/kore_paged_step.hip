@@ -89,7 +89,7 @@ __device__ __forceinline__ int status_of(const PlanArgs &a, const Sums &all, int
 
 // A row's depth in its tree and its mask: a walk from parent to parent, each before the
 // row, so that it ends.  parent: of the sequence's rows.  A row holds one bit for itself
-// and each row before it.
+// and each row before it, or the last `window` of them, which are the highest.
 __device__ __forceinline__ int ancestors(const PlanArgs &a, int i, const int *parent, unsigned long long *mask) {
     int at = i, depth = -1;
     for (int w = a.words - 1; w >= 0; --w) {
@@ -101,6 +101,18 @@ __device__ __forceinline__ int ancestors(const PlanArgs &a, int i, const int *pa
         }
         mask[w] = bits;
         depth += __popcll(bits);
+    }
+    // (taken off afterwards, by the rows that are so deep alone: the walk itself is what a plan of deep trees takes)
+    for (int w = 0, off = depth + 1 - a.window; off > 0; ++w) {
+        unsigned long long bits = mask[w];
+        const int n = __popcll(bits);
+        if (n <= off) {
+            bits = 0;
+            off -= n;
+        } else {
+            for (; off > 0; --off) bits &= bits - 1;
+        }
+        mask[w] = bits;
     }
     return depth;
 }

@@ -50,7 +50,7 @@ class PlanStruct(C.Structure):
     """kore_paged_plan"""
     _fields_ = [("n_seq", _i), ("n_tok", _i), ("n_new", _vp), ("kv_held", _vp), ("kv_len", _vp), ("pages", _vp),
                 ("pages_stride", _i), ("free_pages", _vp), ("n_free", _vp), ("n_free_out", _vp), ("parent", _vp),
-                ("q_start", _vp), ("pos", _vp), ("slot", _vp), ("mask", _vp), ("mask_words", _i), ("status", _vp)]
+                ("q_start", _vp), ("pos", _vp), ("slot", _vp), ("mask", _vp), ("mask_words", _i), ("status", _vp), ("window", _i)]
 
 
 class RowsStruct(C.Structure):
@@ -112,13 +112,13 @@ class Batch:
 class Plan:
     """The requests of a step and the tables that are made of them (kore_paged_plan): device pointers, int32 but for slot
     [n_tok] and mask [n_tok][mask_words], which are 64-bit.  kv_len and n_free_out may be kv_held and n_free; parent and mask
-    go together (None: every sequence's rows one behind the other)."""
+    go together (None: every sequence's rows one behind the other); window: of the masks, as the attention's."""
 
     def __init__(self, n_seq: int, n_tok: int, n_new: int, kv_held: int, kv_len: int, pages: int, pages_stride: int,
                  free_pages: int, n_free: int, n_free_out: int, q_start: int, pos: int, slot: int, status: int,
-                 parent: int | None = None, mask: int | None = None, mask_words: int = 0):
+                 parent: int | None = None, mask: int | None = None, mask_words: int = 0, window: int = 0):
         self.struct = PlanStruct(n_seq, n_tok, n_new, kv_held, kv_len, pages, pages_stride, free_pages, n_free, n_free_out, parent,
-                                 q_start, pos, slot, mask, mask_words, status)
+                                 q_start, pos, slot, mask, mask_words, status, window)
         self._ref = C.byref(self.struct)
 
 

@@ -1,0 +1,120 @@
+"""Steps of drafted tokens where they could go wrong and tests/test_gpu_step.py does not look: windows that a path is as deep as."""
+import numpy as np
+import pytest
+
+from tests import step_ref
+from tests.paged_ref import PAIRS, Case, check_rows
+from tests.test_gpu_step import Tables, _attend_tree
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- windows of masks ------------------------------------------------------------------
+
+def _windowed(parents, window, words):
+    """Masks of trees, [sum of rows][words]: each row and those above it in its tree that are fewer than `window` rows up."""
+    mask = []
+    for parent in parents:
+        for i in range(len(parent)):
+            bits, at, up = 0, i, 0
+            while at >= 0 and up < (window or 1 << 30):
+                bits |= 1 << at
+                at, up = parent[at], up + 1
+            mask.append([bits >> (64 * w) & (1 << 64) - 1 for w in range(words)])
+    return np.asarray(mask, np.uint64).reshape(-1, words)
+
+
+class Windowed(Tables):
+    """Tables of a plan with a window, which its masks alone are to show."""
+
+    def __init__(self, n_new, held, ps, parents, words, window, **kw):
+        super().__init__(n_new, held, ps, words=words, parent=[q for p in parents for q in p], **kw)
+        self.parents, self.window = parents, window
+
+    def plan(self):
+        p = super().plan()
+        p.struct.window = self.window
+        return p
+
+    def get(self, name):
+        got = super().get(name)
+        if name != "mask":
+            return got
+        n = sum(self.n_new)
+        mask = got.view(np.uint64).reshape(self.n_tok, self.words)
+        assert np.array_equal(mask[:n], _windowed(self.parents, self.window, self.words))
+        return np.concatenate([_windowed(self.parents, 0, self.words), mask[n:]]).view(np.int64)
+
+
+@pytest.mark.parametrize("window", [1, 2, 7, 63, 64, 65, 130, 2 ** 31 - 1])
+@pytest.mark.parametrize("words,n_seq,alias", [(1, 9, False), (2, 9, False), (5, 9, False), (16, 9, False), (1, 9, True), (16, 9, True),
+                                               (1, 1100, False), (2, 1100, True)])
+def test_masks_in_a_window(words, window, n_seq, alias):
+    """A mask is the window's last of a row's path, positions and slots are as without one: in one launch and in two."""
+    rng = np.random.default_rng(words * 1000 + window % 1000)
+    n_new = [int(x) for x in rng.integers(0, 64 * words + 1 if n_seq < 10 else 20, n_seq)]
+    n_new[0] = 64 * words
+    parents = [list(range(-1, n - 1)) if i % 3 == 0 else step_ref.tree(rng, n, 1 + i % 3) for i, n in enumerate(n_new)]
+    assert Windowed(n_new, [int(x) for x in rng.integers(0, 90, n_seq)], 16, parents, words, window, alias=alias).run() == 0
+
+
+def _plan_masks(c, parents, words, window):
+    """(masks, positions) that a plan makes of a Case's new rows."""
+    held = [int(kv) - n for n, kv in c.lens]
+    t = Windowed([n for n, _ in c.lens], held, c.ps, parents, words, window, n_tok=c.n_tok)
+    assert t.run() == 0
+    mask = Tables.get(t, "mask").view(np.uint64).reshape(c.n_tok, words)
+    return mask, t.get("pos").astype(np.int32)
+
+
+@pytest.mark.parametrize("dtype,cache", PAIRS)
+@pytest.mark.parametrize("window", [1, 5, 12, 64, 100])
+@pytest.mark.parametrize("max_q", [1, None])
+def test_a_planned_chain_in_a_window_is_causal(dtype, cache, window, max_q):
+    """Plan and attention with the window of a model: kore_paged_attend_dev's rows, paths deeper than the window among them."""
+    c = Case([(12, 300), (5, 5), (1, 77), (90, 100), (64, 64)], 12, 2, 96, 16, dtype, cache, seed=window).up()
+    mask, pos = _plan_masks(c, [list(range(-1, n - 1)) for n, _ in c.lens], 2, window)
+    with c.handle() as kv:
+        _attend_tree(c, kv, mask, pos, window=window, max_q=max_q)
+    check_rows(c, c.rows("out", 12)[0], *c.exact(window=window))
+
+
+@pytest.mark.parametrize("window", [2, 4])
+def test_a_planned_tree_in_a_window_is_its_paths(window):
+    """Each row of a tree is the last of its path, decoded as a chain of its own in the same window."""
+    rng = np.random.default_rng(window)
+    n, held = 24, 30
+    parent = step_ref.tree(rng, n, 1)
+    c = Case([(n, held + n)], 4, 2, 64, 16, "f32", "f32", seed=window).up()
+    mask, pos = _plan_masks(c, [parent], 1, window)
+    with c.handle() as kv:
+        _attend_tree(c, kv, mask, pos, window=window)
+    got = c.rows("out", 4)[0].double().numpy()
+    deepest = 0
+    for i in range(n):
+        path = [i]
+        while parent[path[0]] >= 0:
+            path.insert(0, parent[path[0]])
+        deepest = max(deepest, len(path))
+        one = Case([(len(path), held + len(path))], 4, 2, 64, 16, "f32", "f32")
+        at = lambda p: (c.pages[0, p // 16], slice(None), p % 16)  # noqa: E731
+        for p, src in enumerate(list(range(held)) + [held + r for r in path]):
+            for a, b in ((one.k_pool, c.k_pool), (one.v_pool, c.v_pool)):
+                a[0, one.pages[0, p // 16], :, p % 16] = b[0][at(src)]
+        one.q[:] = c.q[path]
+        want, bound = one.exact(window=window)
+        assert (np.abs(got[i] - want[-1]) <= bound[-1]).all(), i
+    assert deepest > window
+
+
+def test_a_window_below_zero_is_refused():
+    from kore_amd import paged
+    t = Tables([2], [3], 16, words=1, parent=[-1, 0]).up()
+    p = t.ptr
+    with t.handle() as kv:
+        with pytest.raises(paged.PagedError, match="window") as e:
+            kv.plan_dev(paged.Plan(1, t.n_tok, p("n_new"), p("held"), p("kv_len"), p("pages"), t.stride, p("free"), p("n_free"),
+                                   p("n_free_out"), p("q_start"), p("pos"), p("slot"), p("status"), p("parent"), p("mask"), 1, window=-1))
+        assert e.value.code == -1
+        kv.sync()
+    assert (t.get("status") == 99).all() and (t.get("pos") == 99).all() and (t.get("mask") == 99).all()
