@@ -101,8 +101,8 @@ typedef struct kore_rope_heads {
 
 /* One set (k NULL) or two (q's heads and k's) of n_tok rows, in one launch: each head
  * is first x w / sqrt(mean(x^2) + eps), then turned as by kore_rope_apply_dev.
- * The sum of squares and the root are in double, 1 / root is rounded to float, and
- * so is either product; then as there, so that each value is rounded to its type
+ * The sum of squares and the root are in double, 1 / root is rounded to float's 24
+ * bits, however large the root, and so is either product; then as there, so that each value is rounded to its type
  * once.  (kore's rmsnorm, kore.cpp:1367-1372, head by head, but for the root's
  * rounding.)  eps over 0.  Sizes, strides, alignment and stream as there; norm
  * aligned to a float.  A row whose position is negative is left as it is.  The

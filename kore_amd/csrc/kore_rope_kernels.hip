@@ -296,7 +296,20 @@ __global__ __launch_bounds__(kThreads) void heads_kernel(HeadsArgs a, int group)
                 sum = __builtin_fma((double)fa[i][x], (double)fa[i][x], sum);
                 sum = __builtin_fma((double)fb[i][x], (double)fb[i][x], sum);
             }
-        const float scale = rsqrt_(group_sum(sum, G) * a.per_dim + a.eps);
+        const double mean = group_sum(sum, G) * a.per_dim + a.eps;
+        float scale = rsqrt_(mean);
+        const bool far = mean > 0x1p252;   // 1 / root is no normal float: 2^4 are moved from the values to it
+        if (__any(far)) {
+            const float down = far ? 0x1p-4f : 1.f;
+            scale = rsqrt_(mean * (double)(down * down));
+#pragma unroll
+            for (int i = 0; i < U; ++i)
+#pragma unroll
+                for (int x = 0; x < V; ++x) {
+                    fa[i][x] *= normed ? down : 1.f;
+                    fb[i][x] *= normed ? down : 1.f;
+                }
+        }
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             const int unit = in + i * G;

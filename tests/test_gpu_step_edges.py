@@ -1,10 +1,12 @@
-"""Steps of drafted tokens where they could go wrong and tests/test_gpu_step.py does not look: windows that a path is as deep as."""
+"""Steps of drafted tokens where they could go wrong and tests/test_gpu_step.py does not look: windows that a path is as deep as,
+heads next to the largest float."""
 import numpy as np
 import pytest
+import torch
 
 from tests import step_ref
-from tests.paged_ref import PAIRS, Case, check_rows
-from tests.test_gpu_step import Tables, _attend_tree
+from tests.paged_ref import PAIRS, Case, check_rows, to64
+from tests.test_gpu_step import Tables, _attend_tree, _bits, _norm
 
 pytestmark = pytest.mark.gpu
 
@@ -118,3 +120,31 @@ def test_a_window_below_zero_is_refused():
         assert e.value.code == -1
         kv.sync()
     assert (t.get("status") == 99).all() and (t.get("pos") == 99).all() and (t.get("mask") == 99).all()
+
+
+# ---- heads next to the largest float --------------------------------------------------------
+
+@pytest.mark.parametrize("hd", [2, 64, 66, 128, 640, 1022])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_norm_next_to_the_largest_float(hd, dtype):
+    """Heads whose root mean square passes 2^126, beside ordinary ones and one without weights.  Position 0 turns by 1 and 0,
+    exactly, so that 1 / root, its product and the weights' (powers of two, exact) leave two half steps of fp32 and the rounding
+    to the type."""
+    from kore_amd import rope
+    rng = np.random.default_rng(hd)
+    x = np.sign(rng.standard_normal((12, 5, hd))) * (0.5 + 0.5 * rng.random((12, 5, hd)))
+    x[:, :3] *= np.float64(2.0) ** rng.uniform(126.5, 127.9, (12, 3, 1))
+    x[:, 3] *= 1e-3
+    x[3, 1, 1:] *= 2.0 ** -200
+    x = torch.from_numpy(x).to(torch.bfloat16 if dtype == "bf16" else torch.float32)
+    assert torch.isfinite(x).all()
+    w = 2.0 ** rng.integers(-2, 3, hd)
+    cfg = rope.Config(min(hd, 512))
+    got, bare = _norm(dtype, [x, x], np.zeros(12, int), [w, None], cfg)
+    v = to64(x)
+    want = v / np.sqrt(np.mean(v * v, -1, keepdims=True) + float(np.float32(1e-6))) * w
+    bound = 2 * 2.0 ** -24 * (1 + 2.0 ** -20) * np.abs(want) + 2.0 ** -149
+    if dtype == "bf16":
+        bound += 2.0 ** -8 * (np.abs(want) + bound)
+    assert (np.abs(to64(got) - want) <= bound).all()
+    assert _bits(bare, x)
