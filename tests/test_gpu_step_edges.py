@@ -1,12 +1,12 @@
 """Steps of drafted tokens where they could go wrong and tests/test_gpu_step.py does not look: windows that a path is as deep as,
-heads next to the largest float."""
+heads next to the largest float, masks of many words in tiles of 128 rows, many sequences."""
 import numpy as np
 import pytest
 import torch
 
 from tests import step_ref
 from tests.paged_ref import PAIRS, Case, check_rows, to64
-from tests.test_gpu_step import Tables, _attend_tree, _bits, _norm
+from tests.test_gpu_step import Tables, _attend_tree, _bits, _masks, _norm, _tall
 
 pytestmark = pytest.mark.gpu
 
@@ -148,3 +148,71 @@ def test_norm_next_to_the_largest_float(hd, dtype):
         bound += 2.0 ** -8 * (np.abs(want) + bound)
     assert (np.abs(to64(got) - want) <= bound).all()
     assert _bits(bare, x)
+
+
+# ---- trees of many rows, and of many sequences -------------------------------------------------
+#
+# A table of many keys lets a step take tiles of 128 rows (_tall); in a window it is the hint of the most rows, which may be any.
+TALL_Q = 1 << 17
+
+
+@pytest.mark.parametrize("dtype,cache", PAIRS)
+@pytest.mark.parametrize("hd,ps,words", [(64, 16, 2), (128, 64, 5), (128, 16, 16), (48, 32, 3), (256, 128, 2)])
+def test_wide_trees_in_tall_tiles(dtype, cache, hd, ps, words):
+    """Masks of several words in tiles of 128 rows: fewer bits than rows and more, what is held no multiple of a word, windows."""
+    c = _tall(Case([(150, 150 + 61), (65, 65), (333, 333 + 100), (1, 40), (129, 129 + 7)], 8, 1, hd, ps, dtype, cache, seed=hd + words,
+                   extra_rows=2)).up()
+    with c.handle() as kv:
+        for kind, window in (("tree", 0), ("tree", 70), ("any", 0)):
+            mask, pos = _masks(c, np.random.default_rng(words), kind, words)
+            c.d["out"].fill_(55.0)
+            _attend_tree(c, kv, mask, pos, window=window, max_q=TALL_Q)
+            got, clean = c.rows("out", 8)
+            assert clean and (got[c.used:] == 55.0).all()
+            check_rows(c, got, *step_ref.tree_exact(c, mask, pos, window=window), name="%s, window %d" % (kind, window))
+
+
+@pytest.mark.parametrize("dtype,cache", PAIRS)
+@pytest.mark.parametrize("hd", [64, 128])
+def test_planned_chains_in_tall_tiles_are_causal(dtype, cache, hd):
+    """Chains of up to some hundred rows in tiles of 128 rows, with a window and without: kore_paged_attend_dev's rows."""
+    c = _tall(Case([(12, 300), (5, 5), (1, 77), (200, 230), (128, 128), (64, 131)], 8, 1, hd, 16, dtype, cache, seed=hd)).up()
+    with c.handle() as kv:
+        for window in (0, 5, 64, 100):
+            mask, pos = _plan_masks(c, [list(range(-1, n - 1)) for n, _ in c.lens], 4, window)
+            _attend_tree(c, kv, mask, pos, window=window, max_q=TALL_Q)
+            check_rows(c, c.rows("out", 8)[0], *c.exact(window=window), name=str(window))
+
+
+@pytest.mark.parametrize("dtype,cache", [("f32", "f32"), ("f32", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("n_seq", [64, 65, 130])
+@pytest.mark.parametrize("tall", [False, True])
+def test_trees_of_many_sequences(dtype, cache, n_seq, tall):
+    """As many sequences as a wave has lanes, and more: some without rows, a few long enough to be split, with a window and without."""
+    rng = np.random.default_rng(n_seq)
+    lens = [(int(n), int(n + h)) for n, h in zip(rng.integers(0, 40 if tall else 9, n_seq), rng.integers(0, 120, n_seq))]
+    for s in (0, 40, 63, n_seq - 1):
+        lens[s] = (int(rng.integers(2, 20)), int(rng.integers(2500, 4000)))
+    c = Case(lens, 8, 1, 64, 64, dtype, cache, seed=n_seq, extra_rows=1)
+    c = (_tall(c) if tall else c).up()
+    mask, pos = _masks(c, np.random.default_rng(1), "tree", 1)
+    with c.handle() as kv:
+        for window in (0, 700):
+            _attend_tree(c, kv, mask, pos, window=window, max_q=TALL_Q if tall else 1)
+            check_rows(c, c.rows("out", 8)[0], *step_ref.tree_exact(c, mask, pos, window=window), name=str(window))
+
+
+@pytest.mark.parametrize("dtype,cache", [("f32", "f32"), ("f16", "f16")])
+@pytest.mark.parametrize("n,max_q", [(30, 1), (100, TALL_Q)])
+def test_more_tiles_than_the_card_holds_at_once(dtype, cache, n, max_q):
+    """Forty trees whose tiles are over twice the CUs (16 rows) or over them (128 rows), beside a long sequence that is split."""
+    rng = np.random.default_rng(n)
+    lens = [(n, n + int(h)) for h in rng.integers(0, 60, 40)]
+    lens[7] = (n, 3000)
+    c = Case(lens, 8, 1, 64, 16, dtype, cache, seed=n)
+    c = (c if max_q == 1 else _tall(c)).up()
+    mask, pos = _masks(c, np.random.default_rng(1), "tree", 2)
+    with c.handle() as kv:
+        for window in (0, 1500):
+            _attend_tree(c, kv, mask, pos, window=window, max_q=max_q)
+            check_rows(c, c.rows("out", 8)[0], *step_ref.tree_exact(c, mask, pos, window=window), name=str(window))
