@@ -216,3 +216,20 @@ def test_more_tiles_than_the_card_holds_at_once(dtype, cache, n, max_q):
         for window in (0, 1500):
             _attend_tree(c, kv, mask, pos, window=window, max_q=max_q)
             check_rows(c, c.rows("out", 8)[0], *step_ref.tree_exact(c, mask, pos, window=window), name=str(window))
+
+
+@pytest.mark.parametrize("dtype,cache", PAIRS)
+@pytest.mark.parametrize("lens,tall", [([(8, 60), (3, 40), (1, 1)], False), ([(20, 3000), (5, 700)], False), ([(64, 3000), (40, 90)], True)])
+def test_trees_in_place(dtype, cache, lens, tall):
+    """The result in q's own rows, in one launch and with splits joined: the bits of rows of its own."""
+    from kore_amd import paged
+    c = Case(lens, 8, 2, 64, 64, dtype, cache, seed=3, extra_rows=2)
+    c = (_tall(c) if tall else c).up()
+    mask, _ = _masks(c, np.random.default_rng(3), "tree", 1)
+    m = torch.from_numpy(mask.view(np.int64)).cuda()
+    with c.handle() as kv:
+        _attend_tree(c, kv, mask)
+        want, behind = c.d["out"][:c.used].clone(), c.d["q"][c.used:].clone()
+        kv.attend_tree_dev(0, c.batch(), paged.Tree(m.data_ptr()), dtype, c.ptr("q"), c.ptr("q"), q_stride=c.step("q"), out_stride=c.step("q"))
+        kv.sync()
+    assert _bits(c.d["q"][:c.used], want) and _bits(c.d["q"][c.used:], behind)
