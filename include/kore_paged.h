@@ -54,7 +54,7 @@
  *   largest, 24 of V and of the weights.
  * fp16 and bf16 rows hold q as it is; their weights are two parts of the type in
  * 16-row tiles and one, rounded to the type, in chunks (many new rows of a
- * sequence).  A sum is split over workgroups by a rule on the whole batch, in a
+ * sequence; trees by a rule of their own, below).  A sum is split over workgroups by a rule on the whole batch, in a
  * fixed order: the same call gives the same bits, another batch around a
  * sequence may differ in the last ones.
  *
@@ -201,8 +201,11 @@ typedef struct kore_paged_tree {
  * sequence with n of them attends the kv_len - n positions before them, in a
  * window w those over pos - w alone (pos is taken within kv_len - n .. kv_len - 1),
  * and of the new ones those that its mask names, itself only if it does; the
- * window does not touch these, so that a model's window is also its plan's.  Whether a step takes 16-row tiles or chunks goes by
- * its size, and with it what is rounded on the way (above).  Everything else as there. */
+ * window does not touch these, so that a model's window is also its plan's.
+ * Whether a step takes 16-row tiles or chunks goes by its rows and by the positions
+ * that pages_stride and the window allow (not by kv_len, which is the device's), and
+ * with it what is rounded on the way (above): a few rows suffice where the table is
+ * wide.  Everything else as there. */
 KORE_PAGED_API int kore_paged_attend_tree_dev(kore_paged_t h, int layer, const kore_paged_batch *b, const kore_paged_tree *t,
                                               int type, const void *q, int64_t q_stride, void *out, int64_t out_stride,
                                               float scale, int window, void *workspace, void *stream);

@@ -654,8 +654,11 @@ hipError_t launch_attend(const AttendArgs &a, hipStream_t s) {
     // Trees have up to some hundred rows a kv-head, and every tile reads all keys of its sequence: which tiles take less time
     // goes by both.  A launch of either takes a start, the merge in it (more of it for wide heads in tiles of 16, and for many
     // tiles of 128), and so much for each key of each tile: us, heads of 128, fitted to 1 to 16 trees of 8 to 32 tokens over
-    // 500 to 8000 keys, run with both.  Over 171 such cases and other heads it takes 1.02 times the better tiles' time (1.42
-    // at most).  us, 16 / 128 rows a tile, 28/4/128, 1 tree of 8 over 500, of 32 over 8000, 16 of 32 over 2000: fp16 10.5 /
+    // 500 to 8000 keys, run with both.  The keys are those that the table's width and the window allow, since the host knows no
+    // lengths: over 171 such cases and other heads, with tables as wide as the longest sequence, it takes 1.02 times the better
+    // tiles' time (1.42 at most); behind wide tables it may take 128 rows where 16 would do (us, tight / 4096 / 32768 positions:
+    // 1 tree of 8 over 500 fp16 keys 10.7 / 11.4 / 14.7, of 32 10.7 / 18.0 / 14.5, fp32 rows 12.2 / 20.2 / 18.3, fp32 cache 20.2 /
+    // 23.2 / 23.2; 16 trees of 32 over 1000 29.5 / 31.4 / 31.2, 43.8 / 41.6 / 41.6, 96.9 / 70.9 / 70.9).  us, 16 / 128 rows a tile, 28/4/128, 1 tree of 8 over 500, of 32 over 8000, 16 of 32 over 2000: fp16 10.5 /
     // 14.3, 32.4 / 20.8, 82 / 44; fp32 rows over fp16 12.2 / 18.3, 34.0 / 28.4, 86 / 62; fp32 cache 12.4 / 23.1, 58 / 42, 199 / 118.
     if (TREE) {
         const bool f32 = a.cache_type == kF32, parts = a.type == kF32;

@@ -152,8 +152,9 @@ __device__ __forceinline__ int last_upto(const F &number, int n, int x) {
 // free ones.  The rest is in LDS: a row's sequence by halves, its ancestors one after the
 // other.  (Workgroups but the first need inputs that the first does not overwrite.)
 //
-// A token of one sequence 3.0 us, 64 trees of up to 32 4.6, 24 thousand rows of 1000
-// sequences 5.8: a launch of some 2 and the rounds.
+// A token of one sequence 3.1 us (up to 3.9 where the host issues more slowly), 64 trees of
+// up to 32 4.3, 24 thousand rows of 1000 sequences 5.4: a launch of some 2 and the rounds.
+// Deep trees walk an LDS latency a row above: 8 of up to 320 rows, half as deep, 12 us.
 __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
     __shared__ long long waves[kWaves][2];
     __shared__ int starts[kThreads], firsts[kThreads], helds[kThreads], lasts[kThreads], tops[kThreads];
@@ -218,7 +219,8 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
 }
 
 // Steps of more sequences, or of many rows whose outputs take the place of the inputs: one
-// workgroup for what is the sequences', kThreads of them at a time, then the rows.
+// workgroup for what is the sequences', kThreads of them at a time, then the rows.  2500
+// sequences of four rows 14 us.
 __global__ __launch_bounds__(kThreads) void plan_sequences_kernel(PlanArgs a) {
     __shared__ long long waves[kWaves][2];
     __shared__ int firsts[kThreads], hads[kThreads];   // of a round's sequences
@@ -446,7 +448,7 @@ __device__ __forceinline__ void give_back(const KeepArgs &a) {
 }
 
 // One launch for both, where the lengths that the moves read are not those that are written.
-// 16 drafted tokens of which four stay, 24 layers: 3.7 us, a launch and three rounds (ends and
+// 16 drafted tokens of which four stay, 24 layers: 3.7 to 4.5 us, a launch and three rounds (ends and
 // rows, pages, the rows themselves); 32 sequences' seven rows, 28 layers of 4 kv-heads of 128:
 // 7.0, since rows of a head are 256 bytes each, and lie apart.
 __global__ __launch_bounds__(kMoveThreads) void keep_kernel(KeepArgs a, int share) {

@@ -157,7 +157,7 @@ class Layer:
                      slot: int, q_norm: int | None = None, k_norm: int | None = None, tree: "paged.Tree | None" = None,
                      window: int = 0, workspace: int | None = None, stream=None) -> None:
         """paged_dev with the rows' positions and slots (device, as PagedKV.plan_dev leaves them), norms of q's and k's heads
-        (device, head_dim weights), and the rows of a sequence as a tree."""
+        (device, head_dim weights), the rows of a sequence as a tree, a window (of a tree, the plan's too)."""
         s = w.struct()
         o = _PagedOpts(pos, slot, q_norm, k_norm, None if tree is None else C.pointer(tree.struct), window)
         self._check(lib().kore_layer_paged_ex_dev(self._h, C.byref(s), kv.handle, layer, C.byref(batch.struct), C.byref(o),
