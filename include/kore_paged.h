@@ -154,7 +154,7 @@ typedef struct kore_paged_plan {
     int mask_words;              /* 1 .. 16 with parent, else 0 */
     int *status;                 /* [1] out */
     int window;                  /* with parent: rows this many positions or more before a row are not in its mask; 0: all
-                                    before it are (layers of several windows: a plan, with a mask, for each) */
+                                    before it are (layers of several windows: a plan for each, not in place, alike but for mask) */
 } kore_paged_plan;
 
 /* Makes the step's tables.  Sequence s gets rows q_start[s] .. and, where they pass
